@@ -145,6 +145,74 @@ int qs_quantize(int ggml_type, int src_type, const void *src, int64_t n_rows, in
 /* Message describing the last failure on the calling thread ("" if none). */
 const char *qs_last_error(void);
 
+/* ---- a layer on packed weights ----
+ *
+ * What a program does with the blocks that qs_quantize() writes: rows of
+ * activations go to 8 bits (after their RMS norm, or as they are) and are
+ * multiplied with packed weights, with low-rank adapters beside the product.
+ * The reference ends at the file and has none of this. Serving forms: there is
+ * no gradient through codes. Every call is asynchronous and stream-ordered on
+ * hip_stream, allocates nothing and never synchronises; the launch status is
+ * the return value. Safe to call from several threads.
+ *
+ * 8-bit rows: t rows of k codes (int8, -127..127) and k/32 f32 scales; row r
+ * stands for code[r][i] * scale[r][i / 32]. */
+
+/* RMS norm of rows (their sum with a residual, if one is given) to 8-bit rows:
+ *   h = x + residual;  u = h * weight;  a = max |u| / 127 per 32 values
+ *   code = rint(u / a) (0 where a is 0);  scale = a / sqrt(mean(h^2) + eps)
+ * all in f32, the mean over the row. weight NULL: no norm (u = h, scale = a).
+ *   src_type:  type of x, residual and sum (QS_SRC_*)
+ *   x, residual: rows with unit stride along k; 16-byte aligned, row strides
+ *              multiples of 16 bytes; residual may be NULL
+ *   weight:    k f32 values, 16-byte aligned, or NULL
+ *   sum:       receives h, rounded to src_type, contiguous; NULL if not wanted;
+ *              may be x or residual itself if that is contiguous
+ *   q, scales: contiguous; q 16-byte aligned
+ * k is a multiple of 32 up to 2^17. A NaN or an infinity in a group makes its
+ * scale NaN; one in a row makes the row's mean, and so all its scales, NaN or
+ * (for an infinity, in the other groups) 0. */
+int qs_rms_norm_q8(int src_type, const void *x, int64_t rows, int64_t k, int64_t x_row_stride_bytes,
+                   const void *residual, int64_t residual_row_stride_bytes, const float *weight, float eps,
+                   void *sum, int8_t *q, float *scales, void *hip_stream);
+
+/* The values of 8-bit rows, code * scale, rounded to dst_type (QS_SRC_*).
+ * Contiguous; q and dst 16-byte aligned. */
+int qs_q8_values(const int8_t *q, const float *scales, int64_t rows, int64_t k, int dst_type, void *dst,
+                 void *hip_stream);
+
+/* Low-rank adapters of one weight, side by side. Adapter i has the rank
+ * offsets[i+1] - offsets[i], a multiple of 8 up to max_rank (pad with zero
+ * rows of a and zero columns of b). All pointers are device pointers. */
+typedef struct qs_adapters {
+    int32_t count;          /* adapters */
+    int32_t type;           /* QS_SRC_F16 or QS_SRC_BF16 */
+    int32_t max_rank;       /* of any adapter; a multiple of 8, at most 4096 */
+    const void *a;          /* offsets[count] rows of k */
+    const void *b;          /* adapter i: n rows of its rank, from value n * offsets[i] */
+    const int32_t *offsets; /* count + 1, from 0 */
+    const float *scales;    /* count */
+} qs_adapters;
+
+/* Bytes of workspace a call with adapters needs for t rows. */
+int64_t qs_packed_linear_workspace(int64_t t, int max_rank);
+
+/* y = x W^T for t 8-bit rows x and a packed weight W of n rows of k values (as
+ * qs_quantize() writes them: n contiguous rows of qs_row_bytes(k)), and for
+ * rows with an adapter  y += scale * B (A x).
+ *   dst:       t contiguous rows of n values of dst_type (QS_SRC_*)
+ *   adapters, ids: both or neither; ids[r] (device) is the adapter of row r,
+ *              any value outside 0..count-1 means none
+ *   workspace: qs_packed_linear_workspace() bytes, 16-byte aligned, used by
+ *              this call alone until it is done; may be NULL without adapters
+ * Codes are multiplied exactly, scales applied in f32, y rounded once. The
+ * result of a row does not depend on timing; it may differ in the last bits
+ * of f32 with t (another split of the sum). t is at most 2^24, each of n*k,
+ * t*k and n*t at most 2^34. */
+int qs_packed_linear(int ggml_type, const void *weight, int64_t n, int64_t k, const int8_t *q, const float *scales,
+                     int64_t t, int dst_type, void *dst, int64_t dst_bytes, const qs_adapters *adapters,
+                     const int32_t *ids, void *workspace, int64_t workspace_bytes, void *hip_stream);
+
 /* ---- host pipeline of the command line ----
  *
  * Replaces the reference's CudaPipeline (quant-studio.py:148-213), its

@@ -133,6 +133,20 @@ def _load_library() -> ctypes.CDLL:
         L.qs_pipeline_finish.argtypes = [ctypes.c_void_p]
         L.qs_pipeline_destroy.restype = None
         L.qs_pipeline_destroy.argtypes = [ctypes.c_void_p]
+        L.qs_rms_norm_q8.restype = ctypes.c_int
+        L.qs_rms_norm_q8.argtypes = [ctypes.c_int, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
+                                     ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_float,
+                                     ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]
+        L.qs_q8_values.restype = ctypes.c_int
+        L.qs_q8_values.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_int,
+                                   ctypes.c_void_p, ctypes.c_void_p]
+        L.qs_packed_linear_workspace.restype = ctypes.c_int64
+        L.qs_packed_linear_workspace.argtypes = [ctypes.c_int64, ctypes.c_int]
+        L.qs_packed_linear.restype = ctypes.c_int
+        L.qs_packed_linear.argtypes = [ctypes.c_int, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64,
+                                       ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int,
+                                       ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p,
+                                       ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p]
         if L.qs_abi_version() != ABI_VERSION:
             raise ImportError(f"{LIB_PATH}: ABI version {L.qs_abi_version()} != {ABI_VERSION}")
         _lib = L
@@ -337,6 +351,11 @@ def _registry() -> dict[str, QuantSpec]:
 
 QUANT_TYPES: dict[str, QuantSpec] = _registry()
 
-__all__ = ["QUANT_TYPES", "ALL_SPECS", "QuantSpec", "QuantSpecError", "TORCH_DTYPES",
+# a layer on packed weights (torch is imported when one of them is called)
+from .packed import (AdapterBank, PackedWeight, Q8Rows, packed_linear, q8_rows,  # noqa: E402
+                     rms_norm_q8)
+
+__all__ = ["AdapterBank", "PackedWeight", "Q8Rows", "packed_linear", "q8_rows", "rms_norm_q8",
+           "QUANT_TYPES", "ALL_SPECS", "QuantSpec", "QuantSpecError", "TORCH_DTYPES",
            "GGMLQuantizationType", "LlamaFileType", "library", "quantize", "row_bytes", "init",
            "set_sqrt_rounding", "sqrt_rounding"]

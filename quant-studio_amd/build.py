@@ -38,6 +38,10 @@ UNITS = [
     ("qs_launch.hip", ["-DQS_LAUNCH_SRC=0"]),
     ("qs_launch.hip", ["-DQS_LAUNCH_SRC=1"]),
     ("qs_launch.hip", ["-DQS_LAUNCH_SRC=30"]),
+    # a layer on packed weights; qs_linear.hip holds the formats in six sets
+    ("qs_norm.hip", []),
+    ("qs_linear_api.hip", []),
+    *[("qs_linear.hip", [f"-DQS_LINEAR_SET={i}"]) for i in range(6)],
 ]
 
 
