@@ -194,17 +194,19 @@ typedef struct qs_adapters {
     const float *scales;    /* count */
 } qs_adapters;
 
-/* Bytes of workspace a call with adapters needs for t rows. */
-int64_t qs_packed_linear_workspace(int64_t t, int max_rank);
+/* Bytes of workspace that a qs_packed_linear call of these sizes needs
+ * (max_rank 0: without adapters); 0 where it needs none. */
+int64_t qs_packed_linear_workspace(int ggml_type, int64_t n, int64_t k, int64_t t, int max_rank);
 
 /* y = x W^T for t 8-bit rows x and a packed weight W of n rows of k values (as
  * qs_quantize() writes them: n contiguous rows of qs_row_bytes(k)), and for
  * rows with an adapter  y += scale * B (A x).
+ *   weight:    4-byte aligned, 2-byte where the type's blocks are not whole words
  *   dst:       t contiguous rows of n values of dst_type (QS_SRC_*)
  *   adapters, ids: both or neither; ids[r] (device) is the adapter of row r,
  *              any value outside 0..count-1 means none
- *   workspace: qs_packed_linear_workspace() bytes, 16-byte aligned, used by
- *              this call alone until it is done; may be NULL without adapters
+ *   workspace: qs_packed_linear_workspace() bytes, 256-byte aligned, used by
+ *              this call alone until it is done; may be NULL where that is 0
  * Codes are multiplied exactly, scales applied in f32, y rounded once. The
  * result of a row does not depend on timing; it may differ in the last bits
  * of f32 with t (another split of the sum). t is at most 2^24, each of n*k,

@@ -41,6 +41,7 @@ UNITS = [
     # a layer on packed weights; qs_linear.hip holds the formats in six sets
     ("qs_norm.hip", []),
     ("qs_linear_api.hip", []),
+    ("qs_matrix.hip", []),
     *[("qs_linear.hip", [f"-DQS_LINEAR_SET={i}"]) for i in range(6)],
 ]
 

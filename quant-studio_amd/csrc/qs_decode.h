@@ -20,32 +20,33 @@
 namespace qsd {
 
 // BLK values in BYTES bytes; SUB groups of 32 / SUB values with a scale of
-// their own in each 32; MIN: there is an m.
+// their own in each 32; MIN: there is an m; GRID: entries of the type's grid;
+// RAW: words that hold a group's bytes and its block's scales.
 template <int TYPE>
 struct Format;
-#define QS_FORMAT(T, blk, bytes, sub, min, grid)                                          \
+#define QS_FORMAT(T, blk, bytes, sub, min, grid, raw)                                     \
     template <>                                                                           \
     struct Format<T> {                                                                    \
-        static constexpr int BLK = blk, BYTES = bytes, SUB = sub, GRID = grid;            \
+        static constexpr int BLK = blk, BYTES = bytes, SUB = sub, GRID = grid, RAW = raw; \
         static constexpr bool MIN = min;                                                  \
     };
-QS_FORMAT(QS_TYPE_Q4_0, 32, 18, 1, false, 0)
-QS_FORMAT(QS_TYPE_Q4_1, 32, 20, 1, true, 0)
-QS_FORMAT(QS_TYPE_Q5_0, 32, 22, 1, false, 0)
-QS_FORMAT(QS_TYPE_Q5_1, 32, 24, 1, true, 0)
-QS_FORMAT(QS_TYPE_Q8_0, 32, 34, 1, false, 0)
-QS_FORMAT(QS_TYPE_IQ4_NL, 32, 18, 1, false, 0)
-QS_FORMAT(QS_TYPE_Q2_K, 256, 84, 2, true, 0)
-QS_FORMAT(QS_TYPE_Q3_K, 256, 110, 2, false, 0)
-QS_FORMAT(QS_TYPE_Q4_K, 256, 144, 1, true, 0)
-QS_FORMAT(QS_TYPE_Q5_K, 256, 176, 1, true, 0)
-QS_FORMAT(QS_TYPE_Q6_K, 256, 210, 2, false, 0)
-QS_FORMAT(QS_TYPE_IQ4_XS, 256, 136, 1, false, 0)
-QS_FORMAT(QS_TYPE_IQ2_XXS, 256, 66, 1, false, 256)
-QS_FORMAT(QS_TYPE_IQ2_XS, 256, 74, 2, false, 512)
-QS_FORMAT(QS_TYPE_IQ2_S, 256, 82, 2, false, 1024)
-QS_FORMAT(QS_TYPE_IQ3_XXS, 256, 98, 1, false, 256)
-QS_FORMAT(QS_TYPE_IQ3_S, 256, 110, 1, false, 512)
+QS_FORMAT(QS_TYPE_Q4_0, 32, 18, 1, false, 0, 5)
+QS_FORMAT(QS_TYPE_Q4_1, 32, 20, 1, true, 0, 5)
+QS_FORMAT(QS_TYPE_Q5_0, 32, 22, 1, false, 0, 6)
+QS_FORMAT(QS_TYPE_Q5_1, 32, 24, 1, true, 0, 6)
+QS_FORMAT(QS_TYPE_Q8_0, 32, 34, 1, false, 0, 9)
+QS_FORMAT(QS_TYPE_IQ4_NL, 32, 18, 1, false, 0, 5)
+QS_FORMAT(QS_TYPE_Q2_K, 256, 84, 2, true, 0, 10)
+QS_FORMAT(QS_TYPE_Q3_K, 256, 110, 2, false, 0, 20)
+QS_FORMAT(QS_TYPE_Q4_K, 256, 144, 1, true, 0, 12)
+QS_FORMAT(QS_TYPE_Q5_K, 256, 176, 1, true, 0, 20)
+QS_FORMAT(QS_TYPE_Q6_K, 256, 210, 2, false, 0, 18)
+QS_FORMAT(QS_TYPE_IQ4_XS, 256, 136, 1, false, 0, 6)
+QS_FORMAT(QS_TYPE_IQ2_XXS, 256, 66, 1, false, 256, 3)
+QS_FORMAT(QS_TYPE_IQ2_XS, 256, 74, 2, false, 512, 4)
+QS_FORMAT(QS_TYPE_IQ2_S, 256, 82, 2, false, 1024, 5)
+QS_FORMAT(QS_TYPE_IQ3_XXS, 256, 98, 1, false, 256, 4)
+QS_FORMAT(QS_TYPE_IQ3_S, 256, 110, 1, false, 512, 6)
 #undef QS_FORMAT
 
 // The grids of the IQ types as device constants; a kernel copies the one it
@@ -77,23 +78,55 @@ struct Group {
 
 // ---- bytes ----
 
-// Blocks start at any even address; the hardware takes such loads.
+// Blocks start at any even address; the hardware takes such loads from memory.
 template <int WORDS>
 QS_DEV void load_words(const uint8_t* p, uint32_t (&w)[WORDS]) {
     __builtin_memcpy(w, p, 4 * WORDS);
-}
-QS_DEV uint32_t load_u32(const uint8_t* p) {
-    uint32_t v;
-    __builtin_memcpy(&v, p, 4);
-    return v;
 }
 QS_DEV uint32_t load_u16(const uint8_t* p) {
     uint16_t v;
     __builtin_memcpy(&v, p, 2);
     return v;
 }
+
+// A place in bytes copied to LDS (on whose boundaries the copy keeps memory's).
+// An LDS read off its boundary takes several times as long (of Q6_K's 210-byte
+// blocks it made four fifths of the LDS time), so where blocks are not whole
+// words (SHIFT) the words around are read and shifted together.
+template <bool SHIFT>
+struct LdsBytes {
+    const uint8_t* base;
+    int at;
+    QS_DEV LdsBytes operator+(int o) const { return {base, at + o}; }
+    QS_DEV uint8_t operator[](int o) const { return base[at + o]; }
+};
+template <int WORDS, bool SHIFT>
+QS_DEV void load_words(LdsBytes<SHIFT> p, uint32_t (&w)[WORDS]) {
+    if constexpr (!SHIFT) {
+        __builtin_memcpy(w, __builtin_assume_aligned(p.base + p.at, 4), 4 * WORDS);
+    } else {
+        const uint32_t* d = reinterpret_cast<const uint32_t*>(p.base + (p.at & ~3));
+        const uint32_t sh = (uint32_t)(p.at & 2) * 8;
+        uint32_t lo = d[0];
+#pragma unroll
+        for (int i = 0; i < WORDS; i++) {
+            const uint32_t hi = d[i + 1];
+            w[i] = __builtin_amdgcn_alignbit(hi, lo, sh);
+            lo = hi;
+        }
+    }
+}
+template <bool SHIFT>
+QS_DEV uint32_t load_u16(LdsBytes<SHIFT> p) {
+    return *reinterpret_cast<const uint16_t*>(p.base + p.at);
+}
+template <typename P>
+QS_DEV uint32_t load_u32(P p) {
+    uint32_t w[1];
+    load_words(p, w);
+    return w[0];
+}
 QS_DEV float half_bits(uint32_t b) { return __half2float(__ushort_as_half((unsigned short)b)); }
-QS_DEV float load_f16(const uint8_t* p) { return half_bits(load_u16(p)); }
 
 // ---- four bytes at a time ----
 
@@ -146,121 +179,190 @@ QS_DEV void scale_min(const uint32_t (&s)[3], int j, uint32_t& sc, uint32_t& mn)
     mn = low ? (b & 63u) : (((c >> 4) & 15u) | ((b >> 2) & 0x30u));
 }
 
-// Group g (0 .. BLK/32 - 1) of the block at b. `grid` is the staged table of
-// the IQ types.
+// The bytes of group g (0 .. BLK/32 - 1) of the block at b, as loaded: what a
+// kernel holds between issuing the loads and using them.
 template <int TYPE>
-QS_DEV void decode_group(const uint8_t* b, int g, const uint16_t* grid, Group<TYPE>& o) {
-    o.m[0] = 0.0f;
+struct Raw {
+    uint32_t w[Format<TYPE>::RAW];
+};
+
+template <int N, int WORDS, typename P>
+QS_DEV void load_at(uint32_t (&w)[WORDS], int at, P p) {
+    uint32_t v[N];
+    load_words(p, v);
+#pragma unroll
+    for (int i = 0; i < N; i++) w[at + i] = v[i];
+}
+
+template <int TYPE, typename P>
+QS_DEV void load_group(P b, int g, Raw<TYPE>& o) {
+    if constexpr (TYPE == QS_TYPE_Q4_0 || TYPE == QS_TYPE_IQ4_NL) {
+        load_at<4>(o.w, 0, b + 2);
+        o.w[4] = load_u16(b);
+    } else if constexpr (TYPE == QS_TYPE_Q4_1) {
+        load_at<4>(o.w, 0, b + 4);
+        o.w[4] = load_u32(b);
+    } else if constexpr (TYPE == QS_TYPE_Q5_0) {
+        load_at<5>(o.w, 0, b + 2);      // the fifth bits, then 16 bytes of nibbles
+        o.w[5] = load_u16(b);
+    } else if constexpr (TYPE == QS_TYPE_Q5_1) {
+        load_at<5>(o.w, 0, b + 4);
+        o.w[5] = load_u32(b);
+    } else if constexpr (TYPE == QS_TYPE_Q8_0) {
+        load_at<8>(o.w, 0, b + 2);
+        o.w[8] = load_u16(b);
+    } else if constexpr (TYPE == QS_TYPE_Q2_K) {
+        load_at<8>(o.w, 0, b + 16 + 32 * (g >> 2));
+        o.w[8] = load_u32(b + 80);
+        o.w[9] = load_u16(b + 2 * g);
+    } else if constexpr (TYPE == QS_TYPE_Q3_K) {
+        load_at<8>(o.w, 0, b + 32 + 32 * (g >> 2));
+        load_at<8>(o.w, 8, b);
+        load_at<3>(o.w, 16, b + 96);
+        o.w[19] = load_u16(b + 108);
+    } else if constexpr (TYPE == QS_TYPE_Q4_K) {
+        load_at<8>(o.w, 0, b + 16 + 32 * (g >> 1));
+        load_at<4>(o.w, 8, b);          // d, dmin, 12 bytes of scales
+    } else if constexpr (TYPE == QS_TYPE_Q5_K) {
+        load_at<8>(o.w, 0, b + 48 + 32 * (g >> 1));
+        load_at<4>(o.w, 8, b);
+        load_at<8>(o.w, 12, b + 16);
+    } else if constexpr (TYPE == QS_TYPE_Q6_K) {
+        load_at<8>(o.w, 0, b + 64 * (g >> 2) + 32 * (g & 1));
+        load_at<8>(o.w, 8, b + 128 + 32 * (g >> 2));
+        o.w[16] = load_u16(b + 192 + 2 * g);
+        o.w[17] = load_u16(b + 208);
+    } else if constexpr (TYPE == QS_TYPE_IQ4_XS) {
+        load_at<4>(o.w, 0, b + 8 + 16 * g);
+        load_at<2>(o.w, 4, b);
+    } else if constexpr (TYPE == QS_TYPE_IQ2_XXS) {
+        load_at<2>(o.w, 0, b + 2 + 8 * g);      // four grid indices; four times seven signs and the scale
+        o.w[2] = load_u16(b);
+    } else if constexpr (TYPE == QS_TYPE_IQ2_XS) {
+        load_at<2>(o.w, 0, b + 2 + 8 * g);      // four entries: grid index (9 bits), seven signs
+        o.w[2] = load_u16(b);
+        o.w[3] = b[66 + g];
+    } else if constexpr (TYPE == QS_TYPE_IQ2_S) {
+        o.w[0] = load_u32(b + 2 + 4 * g);
+        o.w[1] = load_u32(b + 34 + 4 * g);
+        o.w[2] = load_u16(b);
+        o.w[3] = b[66 + g];
+        o.w[4] = b[74 + g];
+    } else if constexpr (TYPE == QS_TYPE_IQ3_XXS) {
+        load_at<2>(o.w, 0, b + 2 + 8 * g);      // eight grid indices
+        o.w[2] = load_u32(b + 66 + 4 * g);
+        o.w[3] = load_u16(b);
+    } else {
+        static_assert(TYPE == QS_TYPE_IQ3_S, "format");
+        load_at<2>(o.w, 0, b + 2 + 8 * g);
+        o.w[2] = load_u32(b + 74 + 4 * g);
+        o.w[3] = load_u16(b);
+        o.w[4] = b[66 + g];
+        o.w[5] = b[106 + (g >> 1)];
+    }
+}
+
+// scale k (of 16) of a Q3_K block: the low nibbles of bytes 0..7, then their
+// high ones; two more bits from bytes 8..11
+template <int TYPE>
+QS_DEV int q3_scale(const Raw<TYPE>& r, int k) {
+    const int by = 8 * (k & 3);
+    const uint32_t lo = ((((k >> 2) & 1) ? r.w[17] : r.w[16]) >> (by + 4 * (k >> 3))) & 15u;
+    const uint32_t hi = (r.w[18] >> (by + 2 * (k >> 2))) & 3u;
+    return (int)(lo | (hi << 4)) - 32;
+}
+
+// What the codes of a format are less than the bits that store them (they have
+// a minimum, are signed, or come from a table: 0).
+template <int TYPE>
+constexpr int offset() {
+    return TYPE == QS_TYPE_Q4_0 ? 8 : TYPE == QS_TYPE_Q5_0 ? 16 : TYPE == QS_TYPE_Q3_K ? 4 : TYPE == QS_TYPE_Q6_K ? 32 : 0;
+}
+template <int TYPE, bool STORED>
+QS_DEV uint32_t codes(uint32_t stored) {
+    if constexpr (STORED || offset<TYPE>() == 0) return stored;
+    else return sub_bytes<offset<TYPE>()>(stored);
+}
+
+// Group g of a block from its bytes. `grid` is the staged table of the IQ
+// types. STORED: the codes as stored, offset() too large.
+template <int TYPE, bool STORED = false>
+QS_DEV void decode_group(const Raw<TYPE>& r, int g, const uint16_t* grid, Group<TYPE>& o) {
+    const uint32_t(&w)[Format<TYPE>::RAW] = r.w;
+    o.m[0] = o.m[Format<TYPE>::SUB - 1] = 0.0f;
     if constexpr (TYPE == QS_TYPE_Q4_0 || TYPE == QS_TYPE_Q4_1 || TYPE == QS_TYPE_IQ4_NL) {
-        uint32_t w[4];
-        load_words(b + (TYPE == QS_TYPE_Q4_1 ? 4 : 2), w);
-        o.d[0] = load_f16(b);
-        if constexpr (TYPE == QS_TYPE_Q4_1) o.m[0] = -load_f16(b + 2);
+        o.d[0] = half_bits(w[4] & 0xffffu);
+        if constexpr (TYPE == QS_TYPE_Q4_1) o.m[0] = -half_bits(w[4] >> 16);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const uint32_t lo = w[i] & 0x0f0f0f0fu, hi = (w[i] >> 4) & 0x0f0f0f0fu;
-            if constexpr (TYPE == QS_TYPE_Q4_0) o.c[i] = sub_bytes<8>(lo), o.c[4 + i] = sub_bytes<8>(hi);
-            else if constexpr (TYPE == QS_TYPE_Q4_1) o.c[i] = lo, o.c[4 + i] = hi;
-            else o.c[i] = iq4_levels(lo), o.c[4 + i] = iq4_levels(hi);
+            if constexpr (TYPE == QS_TYPE_IQ4_NL) o.c[i] = iq4_levels(lo), o.c[4 + i] = iq4_levels(hi);
+            else o.c[i] = codes<TYPE, STORED>(lo), o.c[4 + i] = codes<TYPE, STORED>(hi);
         }
     } else if constexpr (TYPE == QS_TYPE_Q5_0 || TYPE == QS_TYPE_Q5_1) {
-        constexpr int AT = TYPE == QS_TYPE_Q5_0 ? 2 : 4;
-        uint32_t w[5];
-        load_words(b + AT, w);      // the fifth bits, then 16 bytes of nibbles
-        o.d[0] = load_f16(b);
-        if constexpr (TYPE == QS_TYPE_Q5_1) o.m[0] = -load_f16(b + 2);
+        o.d[0] = half_bits(w[5] & 0xffffu);
+        if constexpr (TYPE == QS_TYPE_Q5_1) o.m[0] = -half_bits(w[5] >> 16);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const uint32_t lo = (w[1 + i] & 0x0f0f0f0fu) | (spread4(w[0] >> (4 * i)) << 4);
             const uint32_t hi = ((w[1 + i] >> 4) & 0x0f0f0f0fu) | (spread4(w[0] >> (16 + 4 * i)) << 4);
-            o.c[i] = TYPE == QS_TYPE_Q5_0 ? sub_bytes<16>(lo) : lo;
-            o.c[4 + i] = TYPE == QS_TYPE_Q5_0 ? sub_bytes<16>(hi) : hi;
+            o.c[i] = codes<TYPE, STORED>(lo), o.c[4 + i] = codes<TYPE, STORED>(hi);
         }
     } else if constexpr (TYPE == QS_TYPE_Q8_0) {
-        load_words(b + 2, o.c);
-        o.d[0] = load_f16(b);
+#pragma unroll
+        for (int i = 0; i < 8; i++) o.c[i] = w[i];
+        o.d[0] = half_bits(w[8]);
     } else if constexpr (TYPE == QS_TYPE_Q2_K) {
-        uint32_t w[8];
-        load_words(b + 16 + 32 * (g >> 2), w);
-        const uint32_t sc = load_u16(b + 2 * g), dd = load_u32(b + 80);
-        const float d = half_bits(dd & 0xffffu), dmin = half_bits(dd >> 16);
+        const uint32_t sc = w[9];
+        const float d = half_bits(w[8] & 0xffffu), dmin = half_bits(w[8] >> 16);
         o.d[0] = d * (float)(sc & 15u), o.m[0] = dmin * (float)((sc >> 4) & 15u);
         o.d[1] = d * (float)((sc >> 8) & 15u), o.m[1] = dmin * (float)(sc >> 12);
         const int sh = 2 * (g & 3);
 #pragma unroll
         for (int i = 0; i < 8; i++) o.c[i] = (w[i] >> sh) & 0x03030303u;
     } else if constexpr (TYPE == QS_TYPE_Q3_K) {
-        uint32_t w[8], h[8], s[3];
-        load_words(b + 32 + 32 * (g >> 2), w);
-        load_words(b, h);
-        load_words(b + 96, s);
-        const float d = load_f16(b + 108);
+        const float d = half_bits(w[19]);
         const int sh = 2 * (g & 3);
 #pragma unroll
         for (int i = 0; i < 8; i++)
-            o.c[i] = sub_bytes<4>(((w[i] >> sh) & 0x03030303u) | (((h[i] >> g) & ONES) << 2));
+            o.c[i] = codes<TYPE, STORED>(((w[i] >> sh) & 0x03030303u) | (((w[8 + i] >> g) & ONES) << 2));
 #pragma unroll
-        for (int j = 0; j < 2; j++) {
-            const int k = 2 * g + j, by = 8 * (k & 3);
-            // scale k: the low nibbles of bytes 0..7, then their high ones; two more bits from bytes 8..11
-            const uint32_t lo = ((((k >> 2) & 1) ? s[1] : s[0]) >> (by + 4 * (k >> 3))) & 15u;
-            const uint32_t hi = (s[2] >> (by + 2 * (k >> 2))) & 3u;
-            o.d[j] = d * (float)((int)(lo | (hi << 4)) - 32);
-        }
-        o.m[1] = 0.0f;
+        for (int j = 0; j < 2; j++) o.d[j] = d * (float)q3_scale(r, 2 * g + j);
     } else if constexpr (TYPE == QS_TYPE_Q4_K || TYPE == QS_TYPE_Q5_K) {
-        uint32_t head[4], w[8], h[8], sc, mn;
-        load_words(b, head);        // d, dmin, 12 bytes of scales
-        load_words(b + (TYPE == QS_TYPE_Q4_K ? 16 : 48) + 32 * (g >> 1), w);
-        if constexpr (TYPE == QS_TYPE_Q5_K) load_words(b + 16, h);
-        const uint32_t s[3] = {head[1], head[2], head[3]};
+        uint32_t sc, mn;
+        const uint32_t s[3] = {w[9], w[10], w[11]};
         scale_min(s, g, sc, mn);
-        o.d[0] = half_bits(head[0] & 0xffffu) * (float)sc;
-        o.m[0] = half_bits(head[0] >> 16) * (float)mn;
+        o.d[0] = half_bits(w[8] & 0xffffu) * (float)sc;
+        o.m[0] = half_bits(w[8] >> 16) * (float)mn;
         const int sh = 4 * (g & 1);
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             o.c[i] = (w[i] >> sh) & 0x0f0f0f0fu;
-            if constexpr (TYPE == QS_TYPE_Q5_K) o.c[i] |= ((h[i] >> g) & ONES) << 4;
+            if constexpr (TYPE == QS_TYPE_Q5_K) o.c[i] |= ((w[12 + i] >> g) & ONES) << 4;
         }
     } else if constexpr (TYPE == QS_TYPE_Q6_K) {
-        const int n = g >> 2, quad = g & 3;
-        uint32_t w[8], h[8];
-        load_words(b + 64 * n + 32 * (quad & 1), w);
-        load_words(b + 128 + 32 * n, h);
-        const uint32_t sc = load_u16(b + 192 + 2 * g);
-        const float d = load_f16(b + 208);
-        o.d[0] = d * (float)(int8_t)(sc & 0xffu), o.d[1] = d * (float)(int8_t)(sc >> 8);
-        o.m[1] = 0.0f;
-        const int sl = 4 * (quad >> 1), sh = 2 * quad;
+        const float d = half_bits(w[17]);
+        o.d[0] = d * (float)(int8_t)(w[16] & 0xffu), o.d[1] = d * (float)(int8_t)(w[16] >> 8);
+        const int sl = 4 * ((g >> 1) & 1), sh = 2 * (g & 3);
 #pragma unroll
         for (int i = 0; i < 8; i++)
-            o.c[i] = sub_bytes<32>(((w[i] >> sl) & 0x0f0f0f0fu) | (((h[i] >> sh) & 0x03030303u) << 4));
+            o.c[i] = codes<TYPE, STORED>(((w[i] >> sl) & 0x0f0f0f0fu) | (((w[8 + i] >> sh) & 0x03030303u) << 4));
     } else if constexpr (TYPE == QS_TYPE_IQ4_XS) {
-        uint32_t w[4];
-        load_words(b + 8 + 16 * g, w);
-        const uint32_t head = load_u32(b), sl = load_u32(b + 4);
-        const uint32_t ls = ((sl >> (4 * g)) & 15u) | (((head >> (16 + 2 * g)) & 3u) << 4);
-        o.d[0] = half_bits(head & 0xffffu) * (float)((int)ls - 32);
+        const uint32_t ls = ((w[5] >> (4 * g)) & 15u) | (((w[4] >> (16 + 2 * g)) & 3u) << 4);
+        o.d[0] = half_bits(w[4] & 0xffffu) * (float)((int)ls - 32);
 #pragma unroll
         for (int i = 0; i < 4; i++)
             o.c[i] = iq4_levels(w[i] & 0x0f0f0f0fu), o.c[4 + i] = iq4_levels((w[i] >> 4) & 0x0f0f0f0fu);
     } else if constexpr (TYPE == QS_TYPE_IQ2_XXS) {
-        uint32_t w[2];              // four grid indices; four times seven signs and the scale
-        load_words(b + 2 + 8 * g, w);
-        o.d[0] = load_f16(b) * (0.5f + (float)(w[1] >> 28)) * 0.25f;
+        o.d[0] = half_bits(w[2]) * (0.5f + (float)(w[1] >> 28)) * 0.25f;
 #pragma unroll
         for (int l = 0; l < 4; l++) {
             const uint32_t e = grid[(w[0] >> (8 * l)) & 255u], s = signs8((w[1] >> (7 * l)) & 127u);
             o.c[2 * l] = sign4(iq2_levels(e), s), o.c[2 * l + 1] = sign4(iq2_levels(e >> 8), s >> 4);
         }
     } else if constexpr (TYPE == QS_TYPE_IQ2_XS) {
-        uint32_t w[2];              // four entries: grid index (9 bits), seven signs
-        load_words(b + 2 + 8 * g, w);
-        const float d = load_f16(b);
-        const uint32_t sc = b[66 + g];
-        o.d[0] = d * (0.5f + (float)(sc & 15u)) * 0.25f, o.d[1] = d * (0.5f + (float)(sc >> 4)) * 0.25f;
-        o.m[1] = 0.0f;
+        const float d = half_bits(w[2]);
+        o.d[0] = d * (0.5f + (float)(w[3] & 15u)) * 0.25f, o.d[1] = d * (0.5f + (float)(w[3] >> 4)) * 0.25f;
 #pragma unroll
         for (int l = 0; l < 4; l++) {
             const uint32_t v = (w[l >> 1] >> (16 * (l & 1))) & 0xffffu;
@@ -268,37 +370,28 @@ QS_DEV void decode_group(const uint8_t* b, int g, const uint16_t* grid, Group<TY
             o.c[2 * l] = sign4(iq2_levels(e), s), o.c[2 * l + 1] = sign4(iq2_levels(e >> 8), s >> 4);
         }
     } else if constexpr (TYPE == QS_TYPE_IQ2_S) {
-        const uint32_t idx = load_u32(b + 2 + 4 * g), sg = load_u32(b + 34 + 4 * g);
-        const uint32_t qh = b[66 + g], sc = b[74 + g];
-        const float d = load_f16(b);
-        o.d[0] = d * (0.5f + (float)(sc & 15u)) * 0.25f, o.d[1] = d * (0.5f + (float)(sc >> 4)) * 0.25f;
-        o.m[1] = 0.0f;
+        const float d = half_bits(w[2]);
+        o.d[0] = d * (0.5f + (float)(w[4] & 15u)) * 0.25f, o.d[1] = d * (0.5f + (float)(w[4] >> 4)) * 0.25f;
 #pragma unroll
         for (int l = 0; l < 4; l++) {
-            const uint32_t e = grid[((idx >> (8 * l)) & 255u) | (((qh >> (2 * l)) & 3u) << 8)], s = sg >> (8 * l);
+            const uint32_t e = grid[((w[0] >> (8 * l)) & 255u) | (((w[3] >> (2 * l)) & 3u) << 8)], s = w[1] >> (8 * l);
             o.c[2 * l] = sign4(iq2_levels(e), s), o.c[2 * l + 1] = sign4(iq2_levels(e >> 8), s >> 4);
         }
     } else if constexpr (TYPE == QS_TYPE_IQ3_XXS) {
-        uint32_t w[2];              // eight grid indices
-        load_words(b + 2 + 8 * g, w);
-        const uint32_t aux = load_u32(b + 66 + 4 * g);
-        o.d[0] = load_f16(b) * (0.5f + (float)(aux >> 28)) * 0.5f;
+        o.d[0] = half_bits(w[3]) * (0.5f + (float)(w[2] >> 28)) * 0.5f;
 #pragma unroll
         for (int l = 0; l < 4; l++) {
-            const uint32_t s = signs8((aux >> (7 * l)) & 127u), i2 = w[l >> 1] >> (16 * (l & 1));
+            const uint32_t s = signs8((w[2] >> (7 * l)) & 127u), i2 = w[l >> 1] >> (16 * (l & 1));
             // levels 4 12 20 28 36 44 52 62
             o.c[2 * l] = sign4(iq3_levels(grid[i2 & 255u], 0x3e342c24u, 0x1c140c04u), s);
             o.c[2 * l + 1] = sign4(iq3_levels(grid[(i2 >> 8) & 255u], 0x3e342c24u, 0x1c140c04u), s >> 4);
         }
     } else {
         static_assert(TYPE == QS_TYPE_IQ3_S, "format");
-        uint32_t w[2];
-        load_words(b + 2 + 8 * g, w);
-        const uint32_t sg = load_u32(b + 74 + 4 * g), qh = b[66 + g], sc = b[106 + (g >> 1)];
-        o.d[0] = load_f16(b) * (float)(1 + 2 * ((sc >> (4 * (g & 1))) & 15u));
+        o.d[0] = half_bits(w[3]) * (float)(1 + 2 * ((w[5] >> (4 * (g & 1))) & 15u));
 #pragma unroll
         for (int l = 0; l < 4; l++) {
-            const uint32_t s = sg >> (8 * l), i2 = w[l >> 1] >> (16 * (l & 1)), h = qh >> (2 * l);
+            const uint32_t s = w[2] >> (8 * l), i2 = w[l >> 1] >> (16 * (l & 1)), h = w[4] >> (2 * l);
             // levels 1 3 5 ... 15
             o.c[2 * l] = sign4(iq3_levels(grid[(i2 & 255u) | ((h & 1u) << 8)], 0x0f0d0b09u, 0x07050301u), s);
             o.c[2 * l + 1] =
@@ -307,11 +400,15 @@ QS_DEV void decode_group(const uint8_t* b, int g, const uint16_t* grid, Group<TY
     }
 }
 
-// the group of 32 values number `gi` of a row
-template <int TYPE>
-QS_DEV void decode_row_group(const uint8_t* row, int gi, const uint16_t* grid, Group<TYPE>& o) {
+// the group of 32 values number `gi` of a row, and its number in its block
+template <int TYPE, typename P>
+QS_DEV void load_row_group(P row, int gi, Raw<TYPE>& o) {
     constexpr int PER = Format<TYPE>::BLK / 32;
-    decode_group<TYPE>(row + (int64_t)(gi / PER) * Format<TYPE>::BYTES, gi % PER, grid, o);
+    load_group<TYPE>(row + gi / PER * Format<TYPE>::BYTES, gi % PER, o);    // a row is under 2^31 bytes
+}
+template <int TYPE>
+QS_DEV int group_in_block(int gi) {
+    return gi % (Format<TYPE>::BLK / 32);
 }
 
 }  // namespace qsd

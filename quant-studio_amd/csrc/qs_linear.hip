@@ -4,6 +4,7 @@
 
 #include "qs_launch_kernel.h"
 #include "qs_linear_kernels.h"
+#include "qs_matrix.h"
 
 namespace qsl {
 
@@ -11,34 +12,85 @@ using qs_host::launch_kernel;
 
 namespace {
 
-template <int TYPE, int T, int L, int R>
-hipError_t few(const LinearArgs& a, hipStream_t st) {
-    constexpr int ROWS = 256 / L * R;
-    return launch_kernel(k_linear_few<TYPE, T, L, R>, dim3((unsigned)((a.n + ROWS - 1) / ROWS)), dim3(256), 0, st, a);
+template <int TYPE, int L>
+FewPlan few_plan(const LinearArgs& a) {
+    const int64_t rows = 256 / L, w = (rows * a.row_bytes + 15 + 4 + 15) / 16 * 16;    // a shifted read takes the word after its last
+    return {(int)(w < 1 << 20 ? w : 1 << 20), (a.n + rows - 1) / rows};
+}
+template <int TYPE>
+size_t few_lds(const FewPlan& p, int t, int64_t k) {
+    return (size_t)(p.w_bytes + k / 32 * few_record(t) * 16 + Format<TYPE>::GRID * 2);
 }
 
-template <int TYPE, int BM, int BN, int WM, int WN, int WK, int G>
+template <int TYPE, int T, int L>
+hipError_t few(const LinearArgs& a, const FewPlan& p, hipStream_t st) {
+    const size_t lds = few_lds<TYPE>(p, T, a.k);
+    // as many workgroups as the 256 CUs hold at a time: x is staged once by each
+    const int64_t held = 256 * (int64_t)(160 * 1024 / lds < 8 ? 160 * 1024 / lds : 8);
+    return launch_kernel(k_linear_few<TYPE, T, L>, dim3((unsigned)(p.blocks < held ? p.blocks : held)), dim3(256), lds,
+                         st, a, p);
+}
+
+template <int TYPE, int L>
+hipError_t few_rows(int t, const LinearArgs& a, const FewPlan& p, hipStream_t st) {
+    switch (t) {
+    case 1: return few<TYPE, 1, L>(a, p, st);
+    case 2: return few<TYPE, 2, L>(a, p, st);
+    case 3: return few<TYPE, 3, L>(a, p, st);
+    case 4: return few<TYPE, 4, L>(a, p, st);
+    case 5: return few<TYPE, 5, L>(a, p, st);
+    case 6: return few<TYPE, 6, L>(a, p, st);
+    default: return few<TYPE, 8, L>(a, p, st);
+    }
+}
+
+template <int TYPE, int BM, int BN, int WM, int WN, int WK, int G, int D>
 hipError_t tile(const LinearArgs& a, hipStream_t st) {
     const int64_t tiles = ((a.t + BM - 1) / BM) * ((a.n + BN - 1) / BN);
-    return launch_kernel(k_linear_tile<TYPE, BM, BN, WM, WN, WK, G>, dim3((unsigned)tiles),
+    // a multiple of the 8 XCDs: each takes a run of tiles
+    return launch_kernel(k_linear_tile<TYPE, BM, BN, WM, WN, WK, G, D>, dim3((unsigned)((tiles + 7) / 8 * 8)),
                          dim3(64 * WM * WN * WK), 0, st, a);
+}
+
+template <int TYPE>
+hipError_t matrix(const LinearArgs& a, void* work, hipStream_t st) {
+    const MatrixPlan plan = matrix_plan(TYPE, a.n, a.k, a.t);
+    uint8_t *xl = static_cast<uint8_t*>(work), *wl = xl + plan.x_bytes;
+    const int64_t per = (plan.groups + 7) / 8;
+    for (int64_t first = 0; first < a.n; first += plan.slice) {
+        const int64_t count = a.n - first < plan.slice ? a.n - first : plan.slice;
+        LayoutArgs lay{a.w + first * a.row_bytes, wl, a.q, a.s, xl, a.row_bytes, count, a.t, a.k,
+                       (count + 31) / 32 * per, plan.groups};
+        const int64_t blocks = lay.w_blocks + (first ? 0 : (a.t + 31) / 32 * per);      // the rows once
+        hipError_t e = launch_kernel(k_lay_out<TYPE>, dim3((unsigned)blocks), dim3(256), 0, st, lay);
+        if (e != hipSuccess) return e;
+        using M = MatrixFormat<TYPE>;
+        e = launch_matrix(M::PLANES, M::MINS, MatrixArgs{a, xl, wl, first, count, plan.groups}, st);
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 }  // namespace
 
 template <int TYPE>
-hipError_t launch_linear(const LinearArgs& a, hipStream_t st) {
-    if (a.t == 1) return few<TYPE, 1, 16, 1>(a, st);
-    if (a.t == 2) return few<TYPE, 2, 16, 1>(a, st);
-    if (a.t <= 4) return few<TYPE, 4, 16, 1>(a, st);
-    // 128 x 128 tiles where they fill the 256 CUs, else 32 x 32 ones whose
-    // eight waves share the groups
-    const int64_t large = ((a.t + 127) / 128) * ((a.n + 127) / 128);
-    if (a.t > 64 && large >= 192) return tile<TYPE, 128, 128, 2, 2, 1, 4>(a, st);
-    return tile<TYPE, 32, 32, 1, 1, 8, 16>(a, st);
+hipError_t launch_linear(const LinearArgs& a, void* work, hipStream_t st) {
+    // Up to 8 rows: dot products. 16 lanes to a weight row, or a wave where
+    // that leaves too few workgroups or rows too long for LDS.
+    if (a.t <= 8) {
+        const int t = a.t <= 6 ? (int)a.t : 8;
+        const FewPlan p16 = few_plan<TYPE, 16>(a), p64 = few_plan<TYPE, 64>(a);
+        if (p16.blocks >= 512 && few_lds<TYPE>(p16, t, a.k) <= 80 * 1024) return few_rows<TYPE, 16>(t, a, p16, st);
+        if (few_lds<TYPE>(p64, t, a.k) <= 160 * 1024) return few_rows<TYPE, 64>(t, a, p64, st);
+    }
+    if (takes_matrix(a.t)) return matrix<TYPE>(a, work, st);
+    // the rows in one tile, so that the weight is read and decoded once; four
+    // waves share its groups
+    if (a.t <= 32) return tile<TYPE, 32, 32, 1, 1, 4, 8, 3>(a, st);
+    return tile<TYPE, 64, 32, 1, 1, 4, 8, 2>(a, st);
 }
 
-#define QS_LINEAR(T) template hipError_t launch_linear<T>(const LinearArgs&, hipStream_t);
+#define QS_LINEAR(T) template hipError_t launch_linear<T>(const LinearArgs&, void*, hipStream_t);
 #if QS_LINEAR_SET == 0
 QS_LINEAR(QS_TYPE_Q4_0) QS_LINEAR(QS_TYPE_Q4_1) QS_LINEAR(QS_TYPE_Q8_0)
 #elif QS_LINEAR_SET == 1

@@ -197,7 +197,9 @@ class PackedWeight:
             raise ValueError(f"PackedWeight: rows of {data.shape[1]} bytes are not blocks of {size} ({name})")
         self.name = name
         self.ggml_type = int(QUANT_TYPES[name].ggml_type)
-        self.data = data if data.is_contiguous() and data.data_ptr() % 2 == 0 else _dense(data)
+        # what the C call takes: blocks of whole words on 4-byte boundaries, others on 2-byte ones
+        align = 2 if size % 4 else 4
+        self.data = data if data.is_contiguous() and data.data_ptr() % align == 0 else _dense(data)
         self.n, self.k = data.shape[0], data.shape[1] // size * blk
 
 
@@ -274,7 +276,7 @@ def packed_linear(rows, weight: PackedWeight, dtype=None, adapters: AdapterBank 
     _same_device(q, "packed_linear", weight=weight.data)
     if (adapters is None) != (ids is None):
         raise ValueError("packed_linear: adapters and ids go together")
-    bank, work = None, None
+    bank = None
     if adapters is not None:
         if adapters.n != weight.n or adapters.k != k:
             raise ValueError(f"packed_linear: adapters of a ({adapters.n}, {adapters.k}) weight, "
@@ -283,10 +285,11 @@ def packed_linear(rows, weight: PackedWeight, dtype=None, adapters: AdapterBank 
             raise ValueError(f"packed_linear: ids must be int32 ({t},), got {ids.dtype} {tuple(ids.shape)}")
         _same_device(q, "packed_linear", adapters=adapters.a, ids=ids)
         ids = ids.contiguous()
-        need = library().qs_packed_linear_workspace(t, adapters._c.max_rank)
-        if need < 0:
-            _fail()
-        bank, work = ctypes.byref(adapters._c), torch.empty((need,), dtype=torch.uint8, device=q.device)
+        bank = ctypes.byref(adapters._c)
+    need = library().qs_packed_linear_workspace(weight.ggml_type, weight.n, k, t, 0 if bank is None else adapters._c.max_rank)
+    if need < 0:
+        _fail()
+    work = torch.empty((need,), dtype=torch.uint8, device=q.device) if need else None
     if out is None:
         out = torch.empty((t, weight.n), dtype=dtype, device=q.device)
     elif out.dtype != dtype or tuple(out.shape) != (t, weight.n) or not out.is_contiguous() or out.device != q.device:
@@ -296,7 +299,7 @@ def packed_linear(rows, weight: PackedWeight, dtype=None, adapters: AdapterBank 
                                         scale.data_ptr(), t, dst, out.data_ptr(), out.numel() * out.element_size(),
                                         bank, None if ids is None else ids.data_ptr(),
                                         None if work is None else work.data_ptr(),
-                                        0 if work is None else work.numel(), _stream(q))
+                                        need, _stream(q))
     if rc != 0:
         _fail()
     return out

@@ -74,8 +74,10 @@ def test_linear_refuses_adapters(qs):
                       (dict(max_rank=8192), b"multiple of 8"), (dict(a=None), b"null adapter"), (dict(b=72), b"aligned"),
                       (dict(offsets=None), b"null adapter"), (dict(work=None), b"workspace"), (dict(wsize=100), b"workspace")):
         assert call(**bad) == -22 and word in L.qs_last_error(), (bad, L.qs_last_error())
-    assert L.qs_packed_linear_workspace(10, 16) >= 640
-    assert L.qs_packed_linear_workspace(-1, 16) == -22 and L.qs_packed_linear_workspace(1, 3) == -22
+    assert L.qs_packed_linear_workspace(12, 4, 256, 10, 16) >= 640
+    assert L.qs_packed_linear_workspace(12, 4, 256, -1, 16) == -22 and L.qs_packed_linear_workspace(12, 4, 256, 1, 3) == -22
+    assert L.qs_packed_linear_workspace(99, 4, 256, 1, 0) == -95 and L.qs_packed_linear_workspace(12, 4, 100, 1, 0) == -22
+    assert L.qs_packed_linear_workspace(12, 4, 256, 1, 0) == 0
 
 
 def test_python_refuses_what_it_can_see(qs):
