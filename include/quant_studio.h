@@ -196,7 +196,7 @@ typedef struct qs_adapters {
 
 /* Bytes of workspace that a qs_packed_linear call of these sizes needs
  * (max_rank 0: without adapters); 0 where it needs none. */
-int64_t qs_packed_linear_workspace(int ggml_type, int64_t n, int64_t k, int64_t t, int max_rank);
+int64_t qs_packed_linear_workspace(int ggml_type, int64_t n, int64_t k, int64_t t, int dst_type, int max_rank);
 
 /* y = x W^T for t 8-bit rows x and a packed weight W of n rows of k values (as
  * qs_quantize() writes them: n contiguous rows of qs_row_bytes(k)), and for
@@ -207,9 +207,12 @@ int64_t qs_packed_linear_workspace(int ggml_type, int64_t n, int64_t k, int64_t 
  *              any value outside 0..count-1 means none
  *   workspace: qs_packed_linear_workspace() bytes, 256-byte aligned, used by
  *              this call alone until it is done; may be NULL where that is 0
- * Codes are multiplied exactly, scales applied in f32, y rounded once. The
- * result of a row does not depend on timing; it may differ in the last bits
- * of f32 with t (another split of the sum). t is at most 2^24, each of n*k,
+ * Codes are multiplied exactly, scales applied in f32, y rounded once; but a
+ * bf16 result of more than 128 rows, with k >= 1024 and t*n*k >= 2^31, takes
+ * both factors' values rounded to f16 (11 bits; rows scaled by powers of two
+ * first, so that nothing overflows), whose error is some 1% of that of the
+ * result's own rounding. The result of a row does not depend on timing; it may
+ * differ in the last bits of f32 with t and n (another split of the sum). t is at most 2^24, each of n*k,
  * t*k and n*t at most 2^34. */
 int qs_packed_linear(int ggml_type, const void *weight, int64_t n, int64_t k, const int8_t *q, const float *scales,
                      int64_t t, int dst_type, void *dst, int64_t dst_bytes, const qs_adapters *adapters,

@@ -142,7 +142,7 @@ def _load_library() -> ctypes.CDLL:
                                    ctypes.c_void_p, ctypes.c_void_p]
         L.qs_packed_linear_workspace.restype = ctypes.c_int64
         L.qs_packed_linear_workspace.argtypes = [ctypes.c_int, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
-                                                 ctypes.c_int]
+                                                 ctypes.c_int, ctypes.c_int]
         L.qs_packed_linear.restype = ctypes.c_int
         L.qs_packed_linear.argtypes = [ctypes.c_int, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64,
                                        ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int,

@@ -9,6 +9,10 @@
 
 namespace qsl {
 
+// rows up to which a product takes dot products, and tiles that decode the
+// weight themselves; above, both factors are laid out for the matrix units
+constexpr int64_t FEW_ROWS = 8, TILE_ROWS = 128;
+
 struct LinearArgs {
     const uint8_t* w;       // n rows of row_bytes
     const int8_t* q;        // t rows of k codes
@@ -20,17 +24,20 @@ struct LinearArgs {
     const int32_t* ids;     // adapter of each row; outside 0..adapters-1: none
     const int32_t* off;     // adapters + 1 rank offsets, multiples of 8
     const uint16_t* b;      // adapter i: n rows of its rank, from n * off[i]
-    const float* v;         // t rows of ldv: scale * A x
     int64_t ldv;
     int32_t adapters;
     int b_type;             // QS_SRC_F16 / QS_SRC_BF16
+    const float* v;         // to FEW_ROWS rows: scale * A x, t rows of ldv
+    const float* delta;     // to TILE_ROWS rows: B v, t rows of n
+    const uint16_t *v_hi, *v_lo;    // above: scale * A x as hi + lo, t rows of ldv
+    const float* v_unit;            // and what that is to be multiplied by (F16), t rows of ldv / 32
 };
 
 // Many rows: both factors are laid out for the matrix units first, in `work`.
 // A weight is taken in slices of at most SLICE values, whose layout the 256 MB
 // cache behind the L2s holds.
 constexpr int64_t SLICE = INT64_C(1) << 26;
-constexpr int STAGE_GROUPS = 2, TILE = 128;
+constexpr int STAGE_GROUPS = 2, STAGE_GROUPS16 = 8, TILE = 256;
 
 constexpr bool two_planes(int type) { return type == QS_TYPE_Q6_K || type == QS_TYPE_IQ2_XS || type == QS_TYPE_IQ2_S; }
 constexpr int minima(int type) {
@@ -44,19 +51,31 @@ constexpr int panel_group_bytes(int planes, int mins) { return planes * 1024 + (
 struct MatrixPlan {
     int64_t slice;              // weight rows of a slice, a multiple of TILE
     int groups;                 // of a row, rounded up to whole stages
+    int64_t scale_bytes;        // of the factors' row scales (F16)
     int64_t x_bytes, w_bytes;   // of the layouts
+    int64_t bytes() const { return scale_bytes + x_bytes + w_bytes; }
 };
-inline MatrixPlan matrix_plan(int type, int64_t n, int64_t k, int64_t t) {
+inline int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+// f16: the layout of qs_matrix16.h, else that of qs_matrix.h
+inline MatrixPlan matrix_plan(int type, bool f16, int64_t n, int64_t k, int64_t t) {
     MatrixPlan p;
-    p.groups = (int)((k / 32 + STAGE_GROUPS - 1) / STAGE_GROUPS * STAGE_GROUPS);
-    const int64_t rows = SLICE / k / TILE * TILE, all = (n + TILE - 1) / TILE * TILE;
+    p.groups = (int)round_up(k / 32, f16 ? STAGE_GROUPS16 : STAGE_GROUPS);
+    const int64_t rows = SLICE / k / TILE * TILE, all = round_up(n, TILE), panels = round_up(t, TILE) / 32;
     p.slice = rows < TILE ? TILE : rows < all ? rows : all;
-    p.x_bytes = (t + TILE - 1) / TILE * (TILE / 32) * p.groups * panel_group_bytes(1, minima(type));
-    p.w_bytes = p.slice / 32 * p.groups * panel_group_bytes(two_planes(type) ? 2 : 1, minima(type));
+    p.scale_bytes = f16 ? round_up((t + p.slice) * 4, 256) : 0;
+    p.x_bytes = panels * p.groups * (f16 ? 2048 : panel_group_bytes(1, minima(type)));
+    p.w_bytes = p.slice / 32 * p.groups * (f16 ? 2048 : panel_group_bytes(two_planes(type) ? 2 : 1, minima(type)));
     return p;
 }
-// whether a product takes that way
-inline bool takes_matrix(int64_t t) { return t > 128; }
+inline bool takes_matrix(int64_t t) { return t > TILE_ROWS; }
+// Large products whose result is bf16 (8 bits) take factors of f16 (11 bits);
+// everything else exact codes. Rows of 256 values and products of 2^30 take as
+// long either way (q4_k, 2,000 rows, 3,000 x 256: 19 us f16, 20 us exact; 513
+// rows, 1,025 x 768: 17 and 16); 512 rows with 2,560 x 2,560 37 and 48, 4,096
+// with 9,728 x 2,560 248 and 418.
+inline bool takes_f16(int dst_type, int64_t t, int64_t n, int64_t k) {
+    return dst_type == QS_SRC_BF16 && takes_matrix(t) && k >= 1024 && t * n >= (INT64_C(1) << 31) / k;
+}
 
 template <int TYPE>
 hipError_t launch_linear(const LinearArgs& a, void* work, hipStream_t st);
@@ -68,5 +87,29 @@ struct MatrixArgs {
     int groups;                 // as laid out
 };
 hipError_t launch_matrix(int planes, int mins, const MatrixArgs& a, hipStream_t st);
+
+struct Matrix16Args {
+    LinearArgs l;
+    const uint8_t *xl, *wl;
+    const float *ws, *xs;       // row scales
+    int64_t first, count;       // the weight's rows of this slice
+    int groups;                 // as laid out
+};
+hipError_t launch_matrix16(const Matrix16Args& a, hipStream_t st);
+
+struct AdapterArgs {
+    const int8_t* q;
+    const float* s;
+    const uint16_t *a, *b;      // adapter i: rows off[i] .. off[i + 1] of k; n rows of its rank from n * off[i]
+    const int32_t *ids, *off;
+    const float* scales;
+    float* v;                   // [t][ldv]
+    uint16_t *hi, *lo;          // v as hi + lo in the adapters' type: [t][ldv]
+    float* unit;                // what that is to be multiplied by (F16): [t][ldv / 32]
+    float* delta;               // [t][n]
+    int64_t k, n, t, ldv;
+    int32_t adapters;
+};
+hipError_t launch_adapters(int type, const AdapterArgs& a, hipStream_t st);
 
 }  // namespace qsl

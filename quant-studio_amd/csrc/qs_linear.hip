@@ -4,7 +4,7 @@
 
 #include "qs_launch_kernel.h"
 #include "qs_linear_kernels.h"
-#include "qs_matrix.h"
+#include "qs_matrix16.h"
 
 namespace qsl {
 
@@ -54,18 +54,39 @@ hipError_t tile(const LinearArgs& a, hipStream_t st) {
 
 template <int TYPE>
 hipError_t matrix(const LinearArgs& a, void* work, hipStream_t st) {
-    const MatrixPlan plan = matrix_plan(TYPE, a.n, a.k, a.t);
+    const MatrixPlan plan = matrix_plan(TYPE, false, a.n, a.k, a.t);
     uint8_t *xl = static_cast<uint8_t*>(work), *wl = xl + plan.x_bytes;
     const int64_t per = (plan.groups + 7) / 8;
     for (int64_t first = 0; first < a.n; first += plan.slice) {
         const int64_t count = a.n - first < plan.slice ? a.n - first : plan.slice;
-        LayoutArgs lay{a.w + first * a.row_bytes, wl, a.q, a.s, xl, a.row_bytes, count, a.t, a.k,
-                       (count + 31) / 32 * per, plan.groups};
+        const LayoutArgs lay{a.w + first * a.row_bytes, wl, a.q, a.s, xl, a.row_bytes, count, a.t, a.k,
+                             (count + 31) / 32 * per, plan.groups};
         const int64_t blocks = lay.w_blocks + (first ? 0 : (a.t + 31) / 32 * per);      // the rows once
         hipError_t e = launch_kernel(k_lay_out<TYPE>, dim3((unsigned)blocks), dim3(256), 0, st, lay);
         if (e != hipSuccess) return e;
         using M = MatrixFormat<TYPE>;
         e = launch_matrix(M::PLANES, M::MINS, MatrixArgs{a, xl, wl, first, count, plan.groups}, st);
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
+}
+
+template <int TYPE>
+hipError_t matrix16(const LinearArgs& a, void* work, hipStream_t st) {
+    const MatrixPlan plan = matrix_plan(TYPE, true, a.n, a.k, a.t);
+    float *xs = static_cast<float*>(work), *ws = xs + a.t;
+    uint8_t *xl = static_cast<uint8_t*>(work) + plan.scale_bytes, *wl = xl + plan.x_bytes;
+    const int64_t per = (plan.groups + 7) / 8;
+    for (int64_t first = 0; first < a.n; first += plan.slice) {
+        const int64_t count = a.n - first < plan.slice ? a.n - first : plan.slice, rows = first ? 0 : a.t;   // the rows once
+        const uint8_t* w = a.w + first * a.row_bytes;
+        const ScaleArgs sc{w, a.s, ws, xs, a.row_bytes, count, a.t, a.k, (count + 31) / 32};
+        hipError_t e = launch_kernel(k_row_scales<TYPE>, dim3((unsigned)(sc.w_blocks + (rows + 31) / 32)), dim3(256), 0, st, sc);
+        if (e != hipSuccess) return e;
+        const Layout16Args lay{w, a.q, a.s, ws, xs, wl, xl, a.row_bytes, count, a.t, a.k, (count + 31) / 32 * per, plan.groups};
+        e = launch_kernel(k_lay_out16<TYPE>, dim3((unsigned)(lay.w_blocks + (rows + 31) / 32 * per)), dim3(256), 0, st, lay);
+        if (e != hipSuccess) return e;
+        e = launch_matrix16(Matrix16Args{a, xl, wl, ws, xs, first, count, plan.groups}, st);
         if (e != hipSuccess) return e;
     }
     return hipSuccess;
@@ -77,13 +98,13 @@ template <int TYPE>
 hipError_t launch_linear(const LinearArgs& a, void* work, hipStream_t st) {
     // Up to 8 rows: dot products. 16 lanes to a weight row, or a wave where
     // that leaves too few workgroups or rows too long for LDS.
-    if (a.t <= 8) {
+    if (a.t <= FEW_ROWS) {
         const int t = a.t <= 6 ? (int)a.t : 8;
         const FewPlan p16 = few_plan<TYPE, 16>(a), p64 = few_plan<TYPE, 64>(a);
         if (p16.blocks >= 512 && few_lds<TYPE>(p16, t, a.k) <= 80 * 1024) return few_rows<TYPE, 16>(t, a, p16, st);
         if (few_lds<TYPE>(p64, t, a.k) <= 160 * 1024) return few_rows<TYPE, 64>(t, a, p64, st);
     }
-    if (takes_matrix(a.t)) return matrix<TYPE>(a, work, st);
+    if (takes_matrix(a.t)) return takes_f16(a.dst_type, a.t, a.n, a.k) ? matrix16<TYPE>(a, work, st) : matrix<TYPE>(a, work, st);
     // the rows in one tile, so that the weight is read and decoded once; four
     // waves share its groups
     if (a.t <= 32) return tile<TYPE, 32, 32, 1, 1, 4, 8, 3>(a, st);

@@ -13,53 +13,6 @@ namespace {
 using qs_host::fail;
 using qsl::LinearArgs;
 
-struct ShrinkArgs {
-    const int8_t* q;
-    const float* s;
-    const uint16_t* a;          // adapter i: rows off[i] .. off[i + 1] of k
-    const int32_t *ids, *off;
-    const float* scales;
-    float* v;
-    int64_t k, ldv;
-    int32_t adapters;
-    int type;
-};
-
-// v[t, r] = scale * sum over k of A[r, k] x[t, k] for the adapter of row t:
-// a workgroup per row and 16 ranks, four to a wave.
-__global__ __launch_bounds__(256) void k_adapter_rows(ShrinkArgs a) {
-    const int64_t t = blockIdx.x;
-    const int id = a.ids[t];
-    if (id < 0 || id >= a.adapters) return;
-    const int o = a.off[id], rank = a.off[id + 1] - o;
-    const int r0 = blockIdx.y * 16 + threadIdx.x / 64 * 4, lane = threadIdx.x % 64;
-    if (r0 >= rank) return;         // the ranks are multiples of 8: four rows or none
-    const uint16_t* rows = a.a + (int64_t)(o + r0) * a.k;
-    float sum[4] = {};
-    for (int64_t c = lane * 8; c < a.k; c += 512) {
-        const uint2 x = *reinterpret_cast<const uint2*>(a.q + t * a.k + c);
-        const float s = a.s[t * (a.k / 32) + c / 32];
-        float xv[8];
-#pragma unroll
-        for (int i = 0; i < 8; i++) xv[i] = (float)(int8_t)((i < 4 ? x.x : x.y) >> (8 * (i & 3)));
-#pragma unroll
-        for (int r = 0; r < 4; r++) {
-            const uint4 w = *reinterpret_cast<const uint4*>(rows + r * a.k + c);
-            const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
-            float p = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 8; i++)
-                p = __builtin_fmaf(xv[i], qsl::value16((ww[i >> 1] >> (16 * (i & 1))) & 0xffffu, a.type), p);
-            sum[r] = __builtin_fmaf(s, p, sum[r]);
-        }
-    }
-#pragma unroll
-    for (int r = 0; r < 4; r++)
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) sum[r] += __shfl_xor(sum[r], d);
-    if (lane < 4) a.v[t * a.ldv + r0 + lane] = a.scales[id] * (lane < 2 ? (lane ? sum[1] : sum[0]) : lane == 2 ? sum[2] : sum[3]);
-}
-
 template <int TYPE>
 constexpr int64_t row_bytes_of(int64_t k) {
     return k % qsl::Format<TYPE>::BLK ? -1 : k / qsl::Format<TYPE>::BLK * qsl::Format<TYPE>::BYTES;
@@ -84,6 +37,8 @@ bool off16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 != 0; }
 bool off4(const void* p) { return reinterpret_cast<uintptr_t>(p) % 4 != 0; }
 constexpr int64_t kMaxValues = INT64_C(1) << 34, kMaxRows = INT64_C(1) << 24, kMaxRank = 4096;
 
+int dst_size(int type) { return type == QS_SRC_F32 ? 4 : (type == QS_SRC_F16 || type == QS_SRC_BF16) ? 2 : 0; }
+
 const Entry* find(int type) {
     for (const Entry& c : kEntries)
         if (c.type == type) return &c;
@@ -99,23 +54,33 @@ int bad_sizes(const Entry& e, int64_t n, int64_t k, int64_t t) {
     return 0;
 }
 
-// the rows' products with the adapters' A, then the factors as laid out
-int64_t adapter_bytes(int64_t t, int max_rank) { return (t * max_rank * 4 + 255) / 256 * 256; }
-int64_t workspace_of(int type, int64_t n, int64_t k, int64_t t, int max_rank) {
-    if (n == 0 || t == 0) return 0;
-    int64_t bytes = adapter_bytes(t, max_rank);
-    if (qsl::takes_matrix(t)) {
-        const qsl::MatrixPlan p = qsl::matrix_plan(type, n, k, t);
-        bytes += p.x_bytes + p.w_bytes;
+// The workspace: what the adapters' products leave for the weight's, then the
+// factors as laid out.
+struct Work {
+    int64_t v, delta, lo, unit, layouts, bytes;     // offsets; v is hi where there is a lo
+};
+Work work_of(int type, int dst_type, int64_t n, int64_t k, int64_t t, int max_rank) {
+    using qsl::round_up;
+    Work w{};
+    if (n == 0 || t == 0) return w;
+    const bool matrix = qsl::takes_matrix(t);
+    if (max_rank > 0 && matrix) {
+        w.lo = round_up(t * max_rank * 2, 256);
+        w.unit = 2 * w.lo;
+        w.layouts = w.unit + round_up(t * ((max_rank + 31) / 32) * 4, 256);
+    } else if (max_rank > 0) {
+        w.delta = round_up(t * max_rank * 4, 256);
+        w.layouts = w.delta + (t > qsl::FEW_ROWS ? round_up(t * n * 4, 256) : 0);
     }
-    return bytes;
+    w.bytes = w.layouts + (matrix ? qsl::matrix_plan(type, qsl::takes_f16(dst_type, t, n, k), n, k, t).bytes() : 0);
+    return w;
 }
 
 }  // namespace
 
 extern "C" {
 
-int64_t qs_packed_linear_workspace(int ggml_type, int64_t n, int64_t k, int64_t t, int max_rank) {
+int64_t qs_packed_linear_workspace(int ggml_type, int64_t n, int64_t k, int64_t t, int dst_type, int max_rank) {
     qs_host::clear_error();
     const Entry* e = find(ggml_type);
     if (!e) return fail(QS_ENOTSUP, "unknown ggml type %d", ggml_type);
@@ -123,7 +88,9 @@ int64_t qs_packed_linear_workspace(int ggml_type, int64_t n, int64_t k, int64_t 
     if (bad) return bad;
     if (max_rank < 0 || max_rank > kMaxRank || max_rank % 8)
         return fail(QS_EINVAL, "max_rank %d must be a multiple of 8 in 0..%lld", max_rank, (long long)kMaxRank);
-    return workspace_of(ggml_type, n, k, t, max_rank);
+    if (!dst_size(dst_type))
+        return fail(QS_EINVAL, "unsupported destination type %d (F32=0, F16=1, BF16=30)", dst_type);
+    return work_of(ggml_type, dst_type, n, k, t, max_rank).bytes;
 }
 
 int qs_packed_linear(int ggml_type, const void* weight, int64_t n, int64_t k, const int8_t* q, const float* scales,
@@ -132,7 +99,7 @@ int qs_packed_linear(int ggml_type, const void* weight, int64_t n, int64_t k, co
     qs_host::clear_error();
     const Entry* e = find(ggml_type);
     if (!e) return fail(QS_ENOTSUP, "unknown ggml type %d", ggml_type);
-    const int esz = dst_type == QS_SRC_F32 ? 4 : (dst_type == QS_SRC_F16 || dst_type == QS_SRC_BF16) ? 2 : 0;
+    const int esz = dst_size(dst_type);
     if (!esz) return fail(QS_EINVAL, "unsupported destination type %d (F32=0, F16=1, BF16=30)", dst_type);
     const int bad = bad_sizes(*e, n, k, t);
     if (bad) return bad;
@@ -169,26 +136,43 @@ int qs_packed_linear(int ggml_type, const void* weight, int64_t n, int64_t k, co
         if (off16(adapters->a) || off16(adapters->b) || off4(ids))
             return fail(QS_EINVAL, "adapter a and b must be 16-byte aligned, ids 4-byte");
     }
-    const int64_t need = workspace_of(ggml_type, n, k, t, rank);
-    if (need && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256 || workspace_bytes < need))
+    const Work work = work_of(ggml_type, dst_type, n, k, t, rank);
+    if (work.bytes && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256 || workspace_bytes < work.bytes))
         return fail(QS_EINVAL, "workspace holds %lld bytes at %p, %lld needed, 256-byte aligned",
-                    (long long)workspace_bytes, workspace, (long long)need);
+                    (long long)workspace_bytes, workspace, (long long)work.bytes);
+    uint8_t* base = static_cast<uint8_t*>(workspace);
     if (adapted) {
-        a.ids = ids;
-        a.off = adapters->offsets;
-        a.b = static_cast<const uint16_t*>(adapters->b);
-        a.b_type = adapters->type;
-        a.v = static_cast<const float*>(workspace);
-        a.ldv = adapters->max_rank;
-        a.adapters = adapters->count;
-        const ShrinkArgs s{q, scales, static_cast<const uint16_t*>(adapters->a), ids, adapters->offsets,
-                           adapters->scales, static_cast<float*>(workspace), k, a.ldv, a.adapters, a.b_type};
-        const hipError_t r = qs_host::launch_kernel(k_adapter_rows, dim3((unsigned)t, (unsigned)((a.ldv + 15) / 16)),
-                                                    dim3(256), 0, st, s);
+        qsl::AdapterArgs s{};
+        s.q = q;
+        s.s = scales;
+        s.a = static_cast<const uint16_t*>(adapters->a);
+        s.b = static_cast<const uint16_t*>(adapters->b);
+        s.ids = ids;
+        s.off = adapters->offsets;
+        s.scales = adapters->scales;
+        s.k = k;
+        s.n = n;
+        s.t = t;
+        s.ldv = rank;
+        s.adapters = adapters->count;
+        s.v = reinterpret_cast<float*>(base + work.v);
+        s.delta = reinterpret_cast<float*>(base + work.delta);
+        s.hi = reinterpret_cast<uint16_t*>(base + work.v);
+        s.lo = reinterpret_cast<uint16_t*>(base + work.lo);
+        s.unit = reinterpret_cast<float*>(base + work.unit);
+        const hipError_t r = qsl::launch_adapters(adapters->type, s, st);
         if (r != hipSuccess) return fail(QS_EIO, "packed_linear: launch failed: %s", hipGetErrorString(r));
+        a.ids = ids;
+        a.off = s.off;
+        a.b = s.b;
+        a.b_type = adapters->type;
+        a.ldv = rank;
+        a.adapters = s.adapters;
+        if (qsl::takes_matrix(t)) a.v_hi = s.hi, a.v_lo = s.lo, a.v_unit = s.unit;
+        else if (t > qsl::FEW_ROWS) a.delta = s.delta;
+        else a.v = s.v;
     }
-    void* layouts = static_cast<uint8_t*>(workspace) + adapter_bytes(t, rank);
-    const hipError_t r = e->launch(a, layouts, st);
+    const hipError_t r = e->launch(a, base + work.layouts, st);
     if (r != hipSuccess) return fail(QS_EIO, "packed_linear: launch failed: %s", hipGetErrorString(r));
     return 0;
 }

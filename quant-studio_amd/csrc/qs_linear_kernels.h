@@ -207,7 +207,7 @@ __global__ __launch_bounds__(256) void k_linear_few(LinearArgs a, FewPlan plan) 
             }
         }
         const int64_t n = block * ROWS + r0;
-        if (a.ids && r0 < rows)
+        if (a.v && r0 < rows)
 #pragma unroll
             for (int t = 0; t < T; t++) {
                 const int id = t <= t1 ? adapter_of(a, t) : -1;
@@ -503,13 +503,12 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_linear_tile(LinearArgs
         for (int i = 0; i < 16; i++) {
             const int64_t t = t0 + (wmr * UM + um) * 32 + 8 * (i / 4) + 4 * half + i % 4;
             if (t >= a.t) continue;
-            const int id = a.ids ? adapter_of(a, t) : -1;
 #pragma unroll
             for (int un = 0; un < UN; un++) {
                 const int64_t n = n0 + (wn * UN + un) * 32 + col;
                 if (n >= a.n) continue;
                 float y = acc[um][un][i];
-                if (id >= 0) y += adapter_sum(a, id, t, n, 0, 1);
+                if (a.delta) y += a.delta[t * a.n + n];
                 store_value(a, t * a.n + n, y);
             }
         }

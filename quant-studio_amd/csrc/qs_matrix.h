@@ -4,6 +4,9 @@
 // again for each tile of rows.
 #pragma once
 
+#include <type_traits>
+
+#include "qs_adapters.h"
 #include "qs_linear_kernels.h"
 
 namespace qsl {
@@ -147,6 +150,33 @@ __global__ __launch_bounds__(256) void k_lay_out(LayoutArgs a) {
 
 // ---- the product ----
 
+QS_DEV AdapterTile adapter_tile(const LinearArgs& l) {
+    return {l.ids, l.off, l.b, l.v_hi, l.v_lo, l.v_unit, l.ldv, l.adapters};
+}
+
+// A wave's units to memory: rows from t0, columns from n0 to `end`. Element i
+// of a unit: row 8 (i / 4) + 4 half + i % 4, column lane % 32.
+template <int UM, int UN>
+QS_DEV void store_tile(const LinearArgs& l, const f32x16 (&y)[UM][UN], int64_t t0, int64_t n0, int64_t end) {
+    const int lane = threadIdx.x % 64, col = lane % 32, half = lane / 32;
+    const auto store = [&](auto* dst) {
+        using T = std::remove_pointer_t<decltype(dst)>;
+#pragma unroll
+        for (int um = 0; um < UM; um++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const int64_t t = t0 + um * 32 + 8 * (i / 4) + 4 * half + i % 4;
+                T* row = dst + t * l.n + n0 + col;
+#pragma unroll
+                for (int un = 0; un < UN; un++)
+                    if (t < l.t && n0 + un * 32 + col < end) row[un * 32] = (T)y[um][un][i];
+            }
+    };
+    if (l.dst_type == QS_SRC_F32) store(static_cast<float*>(l.dst));
+    else if (l.dst_type == QS_SRC_F16) store(static_cast<_Float16*>(l.dst));
+    else store(static_cast<__bf16*>(l.dst));
+}
+
 // 16 bytes a lane from memory to LDS, a wave's 1,024 in a row from `to`
 QS_DEV void copy_to_lds(const uint8_t* from, uint8_t* to) {
     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
@@ -155,7 +185,7 @@ QS_DEV void copy_to_lds(const uint8_t* from, uint8_t* to) {
 
 // A tile of BM rows by BN weight rows, WM x WN waves, G groups a stage, two
 // stages in LDS: while one is multiplied the next one's copies are in flight.
-template <int PLANES, int MINS, int BM, int BN, int WM, int WN, int G, int OCC>
+template <int PLANES, int MINS, int BM, int BN, int WM, int WN, int G, int OCC, int ADAPT>
 __global__ __launch_bounds__(64 * WM * WN, OCC) void k_matrix(MatrixArgs a) {
     constexpr int WAVES = WM * WN, UM = BM / WM / 32, UN = BN / WN / 32;
     constexpr int XB = panel_group_bytes(1, MINS), WB = panel_group_bytes(PLANES, MINS);
@@ -257,7 +287,7 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void k_matrix(MatrixArgs a) {
         const uint8_t* stage = lds + turn * STAGE;
         // this wave's copies of the stage have landed; after the barrier all have,
         // and no wave reads the other stage any more
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(0x0f70);     // vmcnt(0)
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
         // The matrix instructions of a step are issued before the vector ones
@@ -290,23 +320,9 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void k_matrix(MatrixArgs a) {
             }
         }
     }
-    // place of element i of a unit: row 8 (i / 4) + 4 half + i % 4, column `col`
-#pragma unroll
-    for (int um = 0; um < UM; um++)
-#pragma unroll
-        for (int i = 0; i < 16; i++) {
-            const int64_t t = t0 + (wm * UM + um) * 32 + 8 * (i / 4) + 4 * half + i % 4;
-            if (t >= l.t) continue;
-            const int id = l.ids ? adapter_of(l, t) : -1;
-#pragma unroll
-            for (int un = 0; un < UN; un++) {
-                const int64_t n = n0 + (wn * UN + un) * 32 + col;
-                if (n >= a.count) continue;
-                float y = acc[um][un][i];
-                if (id >= 0) y += adapter_sum(l, id, t, a.first + n, 0, 1);
-                store_value(l, t * l.n + a.first + n, y);
-            }
-        }
+    __builtin_amdgcn_s_waitcnt(0x0f70);     // no copy to LDS outlives the workgroup
+    if constexpr (ADAPT) add_adapters<ADAPT>(adapter_tile(l), acc, t0 + wm * UM * 32, l.t, a.first + n0 + wn * UN * 32, l.n);
+    store_tile(l, acc, t0 + wm * UM * 32, a.first + n0 + wn * UN * 32, a.first + a.count);
 }
 
 }  // namespace qsl

@@ -286,7 +286,8 @@ def packed_linear(rows, weight: PackedWeight, dtype=None, adapters: AdapterBank 
         _same_device(q, "packed_linear", adapters=adapters.a, ids=ids)
         ids = ids.contiguous()
         bank = ctypes.byref(adapters._c)
-    need = library().qs_packed_linear_workspace(weight.ggml_type, weight.n, k, t, 0 if bank is None else adapters._c.max_rank)
+    need = library().qs_packed_linear_workspace(weight.ggml_type, weight.n, k, t, dst,
+                                                0 if bank is None else adapters._c.max_rank)
     if need < 0:
         _fail()
     work = torch.empty((need,), dtype=torch.uint8, device=q.device) if need else None

@@ -74,10 +74,10 @@ def test_linear_refuses_adapters(qs):
                       (dict(max_rank=8192), b"multiple of 8"), (dict(a=None), b"null adapter"), (dict(b=72), b"aligned"),
                       (dict(offsets=None), b"null adapter"), (dict(work=None), b"workspace"), (dict(wsize=100), b"workspace")):
         assert call(**bad) == -22 and word in L.qs_last_error(), (bad, L.qs_last_error())
-    assert L.qs_packed_linear_workspace(12, 4, 256, 10, 16) >= 640
-    assert L.qs_packed_linear_workspace(12, 4, 256, -1, 16) == -22 and L.qs_packed_linear_workspace(12, 4, 256, 1, 3) == -22
-    assert L.qs_packed_linear_workspace(99, 4, 256, 1, 0) == -95 and L.qs_packed_linear_workspace(12, 4, 100, 1, 0) == -22
-    assert L.qs_packed_linear_workspace(12, 4, 256, 1, 0) == 0
+    size = L.qs_packed_linear_workspace
+    assert size(12, 4, 256, 10, 30, 16) >= 640 and size(12, 4, 256, 1, 30, 0) == 0 and size(12, 0, 256, 10, 30, 16) == 0
+    assert size(12, 4, 256, -1, 30, 16) == -22 and size(12, 4, 256, 1, 30, 3) == -22 and size(12, 4, 256, 1, 5, 0) == -22
+    assert size(99, 4, 256, 1, 30, 0) == -95 and size(12, 4, 100, 1, 30, 0) == -22
 
 
 def test_python_refuses_what_it_can_see(qs):
