@@ -29,6 +29,8 @@ struct LinearArgs {
     int b_type;             // QS_SRC_F16 / QS_SRC_BF16
     const float* v;         // to FEW_ROWS rows: scale * A x, t rows of ldv
     const float* delta;     // to TILE_ROWS rows: B v, t rows of n
+    float* parts;           // of a product split over its groups: splits x t rows of n
+    int splits;
     const uint16_t *v_hi, *v_lo;    // above: scale * A x as hi + lo, t rows of ldv
     const float* v_unit;            // and what that is to be multiplied by (F16), t rows of ldv / 32
 };
@@ -37,7 +39,7 @@ struct LinearArgs {
 // A weight is taken in slices of at most SLICE values, whose layout the 256 MB
 // cache behind the L2s holds.
 constexpr int64_t SLICE = INT64_C(1) << 26;
-constexpr int STAGE_GROUPS = 2, STAGE_GROUPS16 = 8, TILE = 256;
+constexpr int STAGE_GROUPS = 8, STAGE_GROUPS16 = 8, TILE = 256;     // a row's groups are laid out in whole eights
 
 constexpr bool two_planes(int type) { return type == QS_TYPE_Q6_K || type == QS_TYPE_IQ2_XS || type == QS_TYPE_IQ2_S; }
 constexpr int minima(int type) {
@@ -76,6 +78,21 @@ inline bool takes_matrix(int64_t t) { return t > TILE_ROWS; }
 inline bool takes_f16(int dst_type, int64_t t, int64_t n, int64_t k) {
     return dst_type == QS_SRC_BF16 && takes_matrix(t) && k >= 1024 && t * n >= (INT64_C(1) << 31) / k;
 }
+
+// Parts that a product of 9 .. TILE_ROWS rows is split into over its groups, so
+// that there are two workgroups for every CU; a part is whole stages of 8
+// groups. 61 rows with q8_0 1,024 x 2,560: 18.7 us whole, 12.5 in four parts; 16
+// with q6_k 2,560 x 9,728 50 and 27. More parts than workgroups for two a CU
+// were no faster.
+inline int tile_splits(int64_t t, int64_t n, int64_t k) {
+    const int64_t tiles = (t + 63) / 64 * ((n + 31) / 32), stages = (k / 32 + 7) / 8;
+    int64_t s = 512 / tiles < 4 ? 512 / tiles : 4;
+    s = s < stages ? s : stages;
+    if (s < 2) return 1;
+    const int64_t per = (stages + s - 1) / s;
+    return (int)((stages + per - 1) / per);
+}
+hipError_t launch_join(const LinearArgs& a, hipStream_t st);
 
 template <int TYPE>
 hipError_t launch_linear(const LinearArgs& a, void* work, hipStream_t st);

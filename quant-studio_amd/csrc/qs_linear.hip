@@ -46,7 +46,7 @@ hipError_t few_rows(int t, const LinearArgs& a, const FewPlan& p, hipStream_t st
 
 template <int TYPE, int BM, int BN, int WM, int WN, int WK, int G, int D>
 hipError_t tile(const LinearArgs& a, hipStream_t st) {
-    const int64_t tiles = ((a.t + BM - 1) / BM) * ((a.n + BN - 1) / BN);
+    const int64_t tiles = ((a.t + BM - 1) / BM) * ((a.n + BN - 1) / BN) * a.splits;
     // a multiple of the 8 XCDs: each takes a run of tiles
     return launch_kernel(k_linear_tile<TYPE, BM, BN, WM, WN, WK, G, D>, dim3((unsigned)((tiles + 7) / 8 * 8)),
                          dim3(64 * WM * WN * WK), 0, st, a);
@@ -105,10 +105,10 @@ hipError_t launch_linear(const LinearArgs& a, void* work, hipStream_t st) {
         if (few_lds<TYPE>(p64, t, a.k) <= 160 * 1024) return few_rows<TYPE, 64>(t, a, p64, st);
     }
     if (takes_matrix(a.t)) return takes_f16(a.dst_type, a.t, a.n, a.k) ? matrix16<TYPE>(a, work, st) : matrix<TYPE>(a, work, st);
-    // the rows in one tile, so that the weight is read and decoded once; four
-    // waves share its groups
-    if (a.t <= 32) return tile<TYPE, 32, 32, 1, 1, 4, 8, 3>(a, st);
-    return tile<TYPE, 64, 32, 1, 1, 4, 8, 2>(a, st);
+    // up to 64 rows in one tile, so that the weight is decoded once; four waves
+    // share its groups (eight took 37 us where four take 28: q4_k, 64 rows, 9,728 x 2,560)
+    const hipError_t e = a.t <= 32 ? tile<TYPE, 32, 32, 1, 1, 4, 8, 3>(a, st) : tile<TYPE, 64, 32, 1, 1, 4, 8, 2>(a, st);
+    return e != hipSuccess || a.splits == 1 ? e : launch_join(a, st);
 }
 
 #define QS_LINEAR(T) template hipError_t launch_linear<T>(const LinearArgs&, void*, hipStream_t);

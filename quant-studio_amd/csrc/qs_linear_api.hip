@@ -57,7 +57,8 @@ int bad_sizes(const Entry& e, int64_t n, int64_t k, int64_t t) {
 // The workspace: what the adapters' products leave for the weight's, then the
 // factors as laid out.
 struct Work {
-    int64_t v, delta, lo, unit, layouts, bytes;     // offsets; v is hi where there is a lo
+    int64_t v, delta, lo, unit, layouts, bytes;     // offsets; v is hi where there is a lo, layouts the parts of a split
+    int splits;
 };
 Work work_of(int type, int dst_type, int64_t n, int64_t k, int64_t t, int max_rank) {
     using qsl::round_up;
@@ -72,7 +73,10 @@ Work work_of(int type, int dst_type, int64_t n, int64_t k, int64_t t, int max_ra
         w.delta = round_up(t * max_rank * 4, 256);
         w.layouts = w.delta + (t > qsl::FEW_ROWS ? round_up(t * n * 4, 256) : 0);
     }
-    w.bytes = w.layouts + (matrix ? qsl::matrix_plan(type, qsl::takes_f16(dst_type, t, n, k), n, k, t).bytes() : 0);
+    w.splits = matrix || t <= qsl::FEW_ROWS ? 1 : qsl::tile_splits(t, n, k);
+    w.bytes = w.layouts + (matrix         ? qsl::matrix_plan(type, qsl::takes_f16(dst_type, t, n, k), n, k, t).bytes()
+                           : w.splits > 1 ? w.splits * t * n * 4
+                                          : 0);
     return w;
 }
 
@@ -172,6 +176,8 @@ int qs_packed_linear(int ggml_type, const void* weight, int64_t n, int64_t k, co
         else if (t > qsl::FEW_ROWS) a.delta = s.delta;
         else a.v = s.v;
     }
+    a.parts = reinterpret_cast<float*>(base + work.layouts);
+    a.splits = work.splits;
     const hipError_t r = e->launch(a, base + work.layouts, st);
     if (r != hipSuccess) return fail(QS_EIO, "packed_linear: launch failed: %s", hipGetErrorString(r));
     return 0;

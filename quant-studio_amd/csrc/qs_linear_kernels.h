@@ -275,7 +275,8 @@ struct Tile {
     static constexpr int WTASKS = (BN * G + THREADS - 1) / THREADS, XTASKS = (BM * G + THREADS - 1) / THREADS;
     // matrix steps of a wave between two stages
     static constexpr int UNITS = UM * UN, STEPS = G / WK * UNITS * SUB;
-    static_assert(G % WK == 0 && (SUB == 2 || !MIN || G / WK % 2 == 0), "groups of a wave");
+    static constexpr bool PAIR = SUB == 1 && G / WK % 2 == 0;      // minima of two groups in a matrix instruction
+    static_assert(G % WK == 0, "groups of a wave");
 };
 
 // A tile of BM rows by BN weight rows. The workgroup's WM x WN x WK waves
@@ -298,12 +299,13 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_linear_tile(LinearArgs
     // strips of 8 columns of tiles, so that what it works on at a time shares
     // rows and weights in its L2.
     const int64_t tiles_m = (a.t + BM - 1) / BM, tiles_n = (a.n + BN - 1) / BN, tiles = tiles_m * tiles_n;
-    const int64_t at = (int64_t)(blockIdx.x % 8) * (gridDim.x / 8) + blockIdx.x / 8;
-    if (at >= tiles) return;
+    const int64_t place = (int64_t)(blockIdx.x % 8) * (gridDim.x / 8) + blockIdx.x / 8, at = place % tiles;
+    if (place >= tiles * a.splits) return;
     const int64_t strip = at / (8 * tiles_m), left = tiles_n - 8 * strip, wide = left < 8 ? left : 8;
     const int64_t in = at - strip * 8 * tiles_m;
     const int64_t t0 = in / wide * BM, n0 = (8 * strip + in % wide) * BN;
-    const int groups = (int)(a.k / 32);
+    const int groups = (int)(a.k / 32), stages = (groups + G - 1) / G, per = (stages + a.splits - 1) / a.splits;
+    const int split = (int)(place / tiles), begin = split * per * G, end = (split + 1) * per * G < groups ? (split + 1) * per * G : groups;
 
     qsd::stage_grid<TYPE>(grid, tid, THREADS);
     if (tid < 4) reinterpret_cast<uint32_t*>(lds + S::ZERO)[tid] = 0;
@@ -344,7 +346,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_linear_tile(LinearArgs
         }
     };
     auto put = [&](int at, uint4 v) { *reinterpret_cast<uint4*>(lds + at) = v; };
-    auto place = [&](int d, int g0) {
+    auto put_stage = [&](int d, int g0) {
 #pragma unroll
         for (int j = 0; j < S::WTASKS; j++) {
             const int i = tid + j * THREADS, g = i % G, r = i / G;
@@ -410,14 +412,15 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_linear_tile(LinearArgs
                 wp[h][u] = __builtin_bit_cast(bf16x8, at128(half ? S::ZERO : S::WP + (g * SUB + h) * S::WPS + c0 + 512 * u));
         }
     };
-    // - m * (s * sum of codes) is an outer product too: two groups (or the two
-    // halves of one) in a matrix instruction, straight into the sums
+    // - m * (s * sum of codes) is an outer product too: of two groups, or of the
+    // two halves of one, in a matrix instruction, straight into the sums
     auto min_operands = [&](int g) {
-        const int mine = SUB == 2 ? g * 2 + half : g - (1 - half) * WK;
+        const int mine = SUB == 2 ? g * 2 + half : S::PAIR ? g - (1 - half) * WK : g;
+        const bool none = SUB == 1 && !S::PAIR && half;
 #pragma unroll
-        for (int u = 0; u < UM; u++) xm[u] = __builtin_bit_cast(bf16x8, at128(S::XM + mine * S::XPS + m0 + 512 * u));
+        for (int u = 0; u < UM; u++) xm[u] = __builtin_bit_cast(bf16x8, at128(none ? S::ZERO : S::XM + mine * S::XPS + m0 + 512 * u));
 #pragma unroll
-        for (int u = 0; u < UN; u++) wm[u] = __builtin_bit_cast(bf16x8, at128(S::WMN + mine * S::WPS + c0 + 512 * u));
+        for (int u = 0; u < UN; u++) wm[u] = __builtin_bit_cast(bf16x8, at128(none ? S::ZERO : S::WMN + mine * S::WPS + c0 + 512 * u));
     };
     f32x16 ds[2];
     i32x16 p[2];
@@ -440,14 +443,14 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_linear_tile(LinearArgs
     };
 
 #pragma unroll
-    for (int d = 0; d < D; d++) load(d, d * G);
-    for (int from = 0; from < groups; from += D * G)
+    for (int d = 0; d < D; d++) load(d, begin + d * G);
+    for (int from = begin; from < end; from += D * G)
 #pragma unroll
     for (int d = 0; d < D; d++) {
         const int g0 = from + d * G;
-        if (g0 >= groups) break;
+        if (g0 >= end) break;
         lds_barrier();
-        place(d, g0);
+        put_stage(d, g0);
         load(d, g0 + D * G);
         lds_barrier();
         // The matrix instructions of a step are issued before the vector ones
@@ -471,7 +474,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_linear_tile(LinearArgs
             __builtin_amdgcn_sched_barrier(0);
             add(s, 8);
             if constexpr (MIN) {
-                if (SUB == 2 || s / PER % 2 == 1) {
+                if (!S::PAIR || s / PER % 2 == 1) {
                     if (s % PER == 0) min_operands(g);
                     if (s % SUB == SUB - 1) {
                         const int u = s / SUB % S::UNITS;
@@ -508,10 +511,24 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_linear_tile(LinearArgs
                 const int64_t n = n0 + (wn * UN + un) * 32 + col;
                 if (n >= a.n) continue;
                 float y = acc[um][un][i];
+                if (a.splits > 1) {
+                    a.parts[(split * a.t + t) * a.n + n] = y;
+                    continue;
+                }
                 if (a.delta) y += a.delta[t * a.n + n];
                 store_value(a, t * a.n + n, y);
             }
         }
+}
+
+// The sum of a split product's parts, one after another.
+static __global__ __launch_bounds__(256) void k_join(LinearArgs a) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, all = a.t * a.n;
+    if (i >= all) return;
+    float y = a.parts[i];
+    for (int s = 1; s < a.splits; s++) y += a.parts[s * all + i];
+    if (a.delta) y += a.delta[i];
+    store_value(a, i, y);
 }
 
 }  // namespace qsl

@@ -177,24 +177,52 @@ QS_DEV void store_tile(const LinearArgs& l, const f32x16 (&y)[UM][UN], int64_t t
     else store(static_cast<__bf16*>(l.dst));
 }
 
+// The sums of WK waves that hold the same units, in the first one, one wave's
+// after another's; a column of units of all PARTS waves at a time in LDS.
+template <int WK, int PARTS, int UM, int UN>
+QS_DEV void join_waves(f32x16 (&acc)[UM][UN], float* lds, int wk, int part) {
+    const int lane = threadIdx.x % 64;
+#pragma unroll
+    for (int w = 1; w < WK; w++)
+#pragma unroll
+        for (int un = 0; un < UN; un++) {
+            __syncthreads();
+            if (wk == w)
+#pragma unroll
+                for (int um = 0; um < UM; um++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) lds[((part * UM + um) * 16 + i) * 64 + lane] = acc[um][un][i];
+            __syncthreads();
+            if (wk == 0)
+#pragma unroll
+                for (int um = 0; um < UM; um++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) acc[um][un][i] += lds[((part * UM + um) * 16 + i) * 64 + lane];
+        }
+}
+
 // 16 bytes a lane from memory to LDS, a wave's 1,024 in a row from `to`
 QS_DEV void copy_to_lds(const uint8_t* from, uint8_t* to) {
     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
                                      (__attribute__((address_space(3))) void*)to, 16, 0, 0);
 }
 
-// A tile of BM rows by BN weight rows, WM x WN waves, G groups a stage, two
-// stages in LDS: while one is multiplied the next one's copies are in flight.
-template <int PLANES, int MINS, int BM, int BN, int WM, int WN, int G, int OCC, int ADAPT>
-__global__ __launch_bounds__(64 * WM * WN, OCC) void k_matrix(MatrixArgs a) {
-    constexpr int WAVES = WM * WN, UM = BM / WM / 32, UN = BN / WN / 32;
+// A tile of BM rows by BN weight rows. Two stages of G groups lie in LDS; while
+// one is multiplied the next one's copies are in flight. WM x WN waves split the
+// tile, WK the groups of a stage (their sums are joined in LDS at the end, in
+// order). The stages are two arrays, and places in them one sum, so that the
+// compiler sees that a read of one does not wait for copies to the other.
+template <int PLANES, int MINS, int BM, int BN, int WM, int WN, int WK, int G, int ADAPT>
+__global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_matrix(MatrixArgs a) {
+    constexpr int WAVES = WM * WN * WK, UM = BM / WM / 32, UN = BN / WN / 32, GW = G / WK;
     constexpr int XB = panel_group_bytes(1, MINS), WB = panel_group_bytes(PLANES, MINS);
     // a panel's G groups lie together in memory and in LDS
     constexpr int XP = G * XB, WP = G * WB, XS = BM / 32 * XP, WS = BN / 32 * WP, STAGE = XS + WS;
-    static_assert(XP % 256 == 0 && WP % 256 == 0 && STAGE % 1024 == 0, "copies of 1,024 bytes");
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * STAGE];
-    const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
-    const int wn = wave % WN, wm = wave / WN, col = lane % 32, half = lane / 32;
+    constexpr int COPIES = (STAGE / 1024 + WAVES - 1) / WAVES;
+    static_assert(XP % 256 == 0 && WP % 256 == 0 && XS % 1024 == 0 && WS % 1024 == 0 && G % WK == 0, "copies of 1,024 bytes");
+    __shared__ __attribute__((aligned(1024))) uint8_t even[STAGE], odd[STAGE];
+    const int tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64);
+    const int wn = wave % WN, wm = wave / WN % WM, wk = wave / WN / WM, col = lane % 32, half = lane / 32;
     const LinearArgs& l = a.l;
     // Workgroups go round the 8 XCDs in turn; each XCD takes a run of tiles, in
     // strips of 8 columns of tiles, so that what it works on at a time shares
@@ -205,22 +233,27 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void k_matrix(MatrixArgs a) {
     const int64_t strip = at / (8 * tiles_m), left = tiles_n - 8 * strip, wide = left < 8 ? left : 8;
     const int64_t in = at - strip * 8 * tiles_m;
     const int64_t t0 = in / wide * BM, n0 = (8 * strip + in % wide) * BN;
+    const int stages = a.groups / G;
 
-    // copies: 1,024 bytes an instruction, over both factors' panels of a stage
-    const uint8_t* xbase = a.xl + t0 / 32 * a.groups * XB;
-    const uint8_t* wbase = a.wl + n0 / 32 * a.groups * WB;
+    // This wave's copies of a stage: 1,024 bytes each, over both factors' panels;
+    // panels past the last (a tile may reach past the layout) are the last again.
     const int64_t x_step = (int64_t)a.groups * XB, w_step = (int64_t)a.groups * WB;
-    auto copy = [&](int g0, uint8_t* to) {
-        constexpr int XN = XS / 1024, N = STAGE / 1024;
+    const int last_x = (int)((l.t - 1) / 32 - t0 / 32), last_w = (int)((a.count - 1) / 32 - n0 / 32);
+    const uint8_t* from[COPIES];
 #pragma unroll
-        for (int i = 0; i < (N + WAVES - 1) / WAVES; i++) {
+    for (int i = 0; i < COPIES; i++) {
+        const int c = i * WAVES + wave, byte = c * 1024 + lane * 16;
+        const bool x = byte < XS;
+        const int in_s = x ? byte : byte - XS, p = in_s / (x ? XP : WP), o = in_s - p * (x ? XP : WP);
+        from[i] = x ? a.xl + (t0 / 32 + (p < last_x ? p : last_x)) * x_step + o
+                    : a.wl + (n0 / 32 + (p < last_w ? p : last_w)) * w_step + o;
+    }
+    auto copy = [&](int stage, uint8_t* to) {
+#pragma unroll
+        for (int i = 0; i < COPIES; i++) {
             const int c = i * WAVES + wave;
-            if (N % WAVES && c >= N) break;
-            const int byte = c * 1024 + lane * 16;
-            const bool x = c < XN;
-            const int in_s = x ? byte : byte - XS, p = in_s / (x ? XP : WP), o = in_s - p * (x ? XP : WP);
-            copy_to_lds(x ? xbase + p * x_step + (int64_t)g0 * XB + o : wbase + p * w_step + (int64_t)g0 * WB + o,
-                        to + c * 1024);
+            if (STAGE / 1024 % WAVES && c >= STAGE / 1024) break;
+            copy_to_lds(from[i] + (int64_t)stage * (c * 1024 < XS ? XP : WP), to + c * 1024);
         }
     };
 
@@ -236,24 +269,25 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void k_matrix(MatrixArgs a) {
         const uint2 w = *reinterpret_cast<const uint2*>(p);
         return __builtin_bit_cast(s16x4, uint2{__builtin_amdgcn_perm(w.y, w.x, s0), __builtin_amdgcn_perm(w.y, w.x, s1)});
     };
+    const int x0 = wm * UM * XP + wk * GW * XB, w0 = XS + wn * UN * WP + wk * GW * WB;
+    const int xl0 = x0 + lane * 16, xs0 = x0 + 1024 + col * 8, wl0 = w0 + lane * 16, ws0 = w0 + 1024 * PLANES + col * 8;
     auto operands = [&](const uint8_t* stage, int g) {
 #pragma unroll
         for (int u = 0; u < UM; u++) {
-            const uint8_t* p = stage + (wm * UM + u) * XP + g * XB;
-            xa[u] = *reinterpret_cast<const i32x4*>(p + lane * 16);
+            xa[u] = *reinterpret_cast<const i32x4*>(stage + (xl0 + (u * XP + g * XB)));
 #pragma unroll
-            for (int h = 0; h <= MINS; h++) xp[h][u] = slots(p + 1024 + 256 * h + col * 8, xsel0, xsel1);
+            for (int h = 0; h <= MINS; h++) xp[h][u] = slots(stage + (xs0 + (u * XP + g * XB + 256 * h)), xsel0, xsel1);
         }
 #pragma unroll
         for (int u = 0; u < UN; u++) {
-            const uint8_t* p = stage + XS + (wn * UN + u) * WP + g * WB;
 #pragma unroll
-            for (int j = 0; j < PLANES; j++) wb[j][u] = *reinterpret_cast<const i32x4*>(p + 1024 * j + lane * 16);
+            for (int j = 0; j < PLANES; j++)
+                wb[j][u] = *reinterpret_cast<const i32x4*>(stage + (wl0 + (u * WP + g * WB + 1024 * j)));
 #pragma unroll
-            for (int h = 0; h <= MINS; h++) wp[h][u] = slots(p + 1024 * PLANES + 256 * h + col * 8, wsel0, wsel1);
+            for (int h = 0; h <= MINS; h++) wp[h][u] = slots(stage + (ws0 + (u * WP + g * WB + 256 * h)), wsel0, wsel1);
         }
     };
-    constexpr int UNITS = UM * UN, STEPS = G * UNITS;
+    constexpr int UNITS = UM * UN, STEPS = GW * UNITS;
     static_assert(UNITS > 1, "the operands of a group are read two steps ahead");
     f32x16 ds[2];
     i32x16 p[2], ph[2];
@@ -281,15 +315,14 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void k_matrix(MatrixArgs a) {
             acc[u / UN][u % UN][i] = __builtin_fmaf(c, ds[s % 2][i], acc[u / UN][u % UN][i]);
         }
     };
-
-    copy(0, lds);
-    for (int g0 = 0, turn = 0; g0 < a.groups; g0 += G, turn ^= 1) {
-        const uint8_t* stage = lds + turn * STAGE;
+    auto turn = [&](const uint8_t* stage, uint8_t* next, int after) {
         // this wave's copies of the stage have landed; after the barrier all have,
         // and no wave reads the other stage any more
         __builtin_amdgcn_s_waitcnt(0x0f70);     // vmcnt(0)
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
+        copy(after < stages ? after : stages - 1, next);    // no branch: the last stage again
+        __builtin_amdgcn_sched_barrier(0);                  // they go out first
         // The matrix instructions of a step are issued before the vector ones
         // of the step before it, so a wave's vector work covers their latency.
         operands(stage, 0);
@@ -310,17 +343,19 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void k_matrix(MatrixArgs a) {
             __builtin_amdgcn_sched_barrier(0);
             if (more) min_step(s + 1);
             if ((s + 2) % UNITS == 0 && s + 2 < STEPS) operands(stage, (s + 2) / UNITS);
-            // The next stage's copies go out once all of this one's operands are
-            // read: the compiler holds an LDS read that follows a copy to LDS
-            // until the copy has landed.
-            if (s == STEPS - UNITS - 2 + (STEPS == UNITS)) {
-                __builtin_amdgcn_sched_barrier(0);
-                copy(g0 + G < a.groups ? g0 + G : g0, lds + (turn ^ 1) * STAGE);     // no branch: the last stage's again
-                __builtin_amdgcn_sched_barrier(0);
-            }
         }
+    };
+    copy(0, even);
+    for (int s = 0; s < stages; s += 2) {       // an even number of stages
+        turn(even, odd, s + 1);
+        turn(odd, even, s + 2);
     }
     __builtin_amdgcn_s_waitcnt(0x0f70);     // no copy to LDS outlives the workgroup
+    if constexpr (WK > 1) {
+        join_waves<WK, WM * WN>(acc, reinterpret_cast<float*>(even), wk, wm * WN + wn);
+        static_assert(STAGE >= BM * BN * 4 / UN, "a column of units");
+        if (wk > 0) return;
+    }
     if constexpr (ADAPT) add_adapters<ADAPT>(adapter_tile(l), acc, t0 + wm * UM * 32, l.t, a.first + n0 + wn * UN * 32, l.n);
     store_tile(l, acc, t0 + wm * UM * 32, a.first + n0 + wn * UN * 32, a.first + a.count);
 }

@@ -231,28 +231,9 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_matrix16(Matrix16Args 
         turn(odd, even, s + 3, STEPS % 2);
     }
     __builtin_amdgcn_s_waitcnt(0x0f70);     // no copy to LDS outlives the workgroup
-    // the sums of the waves that share steps, one wave's after another's
     if constexpr (WK > 1) {
         static_assert(STAGE >= BM * BN * 4 / UN, "a column of units");
-        float* join = reinterpret_cast<float*>(even);
-        // one column of units at a time: it fits wherever a stage does
-#pragma unroll
-        for (int w = 1; w < WK; w++)
-#pragma unroll
-            for (int un = 0; un < UN; un++) {
-                __syncthreads();
-                if (wk == w)
-#pragma unroll
-                    for (int um = 0; um < UM; um++)
-#pragma unroll
-                        for (int i = 0; i < 16; i++) join[(((wm * WN + wn) * UM + um) * 16 + i) * 64 + lane] = acc[um][un][i];
-                __syncthreads();
-                if (wk == 0)
-#pragma unroll
-                    for (int um = 0; um < UM; um++)
-#pragma unroll
-                        for (int i = 0; i < 16; i++) acc[um][un][i] += join[(((wm * WN + wn) * UM + um) * 16 + i) * 64 + lane];
-            }
+        join_waves<WK, WM * WN>(acc, reinterpret_cast<float*>(even), wk, wm * WN + wn);
         if (wk > 0) return;
     }
     float unw[UN];
