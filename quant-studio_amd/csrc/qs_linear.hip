@@ -105,9 +105,15 @@ hipError_t launch_linear(const LinearArgs& a, void* work, hipStream_t st) {
         if (few_lds<TYPE>(p64, t, a.k) <= 160 * 1024) return few_rows<TYPE, 64>(t, a, p64, st);
     }
     if (takes_matrix(a.t)) return takes_f16(a.dst_type, a.t, a.n, a.k) ? matrix16<TYPE>(a, work, st) : matrix<TYPE>(a, work, st);
-    // up to 64 rows in one tile, so that the weight is decoded once; four waves
-    // share its groups (eight took 37 us where four take 28: q4_k, 64 rows, 9,728 x 2,560)
-    const hipError_t e = a.t <= 32 ? tile<TYPE, 32, 32, 1, 1, 4, 8, 3>(a, st) : tile<TYPE, 64, 32, 1, 1, 4, 8, 2>(a, st);
+    // Up to 64 rows in one tile, so that the weight is decoded once; four waves
+    // share its groups. Eight waves, 64 columns, halve what each does to stage the
+    // rows: 64 rows with q4_k 9,728 x 2,560 24 us where 32 columns take 28, with
+    // q6_k 2,560 x 9,728 36 and 46; a narrow weight makes too few such tiles (61
+    // rows with q8_0 1,024 x 2,560: 14.0 and 12.4), and to 32 rows they are no
+    // faster (q6_k 151,936 x 2,560, 16 rows: 261 and 211).
+    const hipError_t e = a.t <= 32      ? tile<TYPE, 32, 32, 1, 1, 4, 8, 3>(a, st)
+                         : a.n >= 2048 ? tile<TYPE, 64, 64, 1, 2, 4, 8, 2>(a, st)
+                                       : tile<TYPE, 64, 32, 1, 1, 4, 8, 2>(a, st);
     return e != hipSuccess || a.splits == 1 ? e : launch_join(a, st);
 }
 
