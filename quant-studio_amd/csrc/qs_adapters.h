@@ -1,6 +1,7 @@
 // Low-rank adapters beside a product with a packed weight (gfx950):
 //     y[t] += B[id] (scale * A[id] x[t]),   id = ids[t]
-// First v = scale * A x for every row (k_adapter_few, k_adapter_many), then
+// First v = scale * A x for every row (k_adapter_few; k_adapter_many
+// and k_adapter_join), then
 // B v: for up to 8 rows in the product's own lanes (adapter_sum), to 128 rows by
 // a kernel that writes the sums for the product to add (k_adapter_delta), above
 // by matrix instructions on the product's tile (add_adapters).
@@ -136,16 +137,19 @@ QS_DEV void split16(float v, uint16_t& hi, uint16_t& lo) {
 // memory is 32 runs of 16 bytes), those of the next two turns in flight; a wave
 // takes one of the groups. The codes are exact in the adapters' type: only the
 // products' sums are scaled, in f32. The rows' adapters are taken one after
-// another (packed sequences have one or two to 32 rows).
+// another (packed sequences have one or two to 32 rows). A row's values are
+// split over `parts` workgroups, whose sums k_adapter_join adds.
 template <int TYPE>
 __global__ __launch_bounds__(512) void k_adapter_many(AdapterArgs a) {
     constexpr int XS = 256 + 16, AS = 512 + 16;     // strides that spread rows over the banks
     __shared__ __attribute__((aligned(16))) uint8_t xl[2][32 * XS], al[2][32 * AS];
     __shared__ float sl[2][8][32];
-    __shared__ float join[8][32][33];
+    static_assert(sizeof(al) >= 8 * 32 * 33 * 4, "the waves' sums, over A's place");
+    float(*join)[32][33] = reinterpret_cast<float(*)[32][33]>(al);
     const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, col = lane % 32, half = lane / 32;
     const int64_t t0 = (int64_t)blockIdx.x * 32, t = t0 + col < a.t ? t0 + col : a.t - 1;
     const int r0 = blockIdx.y * 32, groups = (int)(a.k / 32), turns = (groups + 7) / 8;
+    const int per = (turns + a.parts - 1) / a.parts, begin = blockIdx.z * per, end = begin + per < turns ? begin + per : turns;
     const int raw = a.ids[t], id = t0 + col < a.t && raw >= 0 && raw < a.adapters ? raw : -1;
     uint32_t left = (uint32_t)__ballot(id >= 0);
     // this thread's copies of a turn: 16 bytes of codes, 32 of A, a scale
@@ -185,17 +189,18 @@ __global__ __launch_bounds__(512) void k_adapter_many(AdapterArgs a) {
                 p = mfma16<TYPE>(*reinterpret_cast<const uint4*>(al[b] + col * AS + 64 * wave + 32 * h + 16 * half),
                                  codes16<TYPE>(*reinterpret_cast<const uint2*>(xl[b] + col * XS + 32 * wave + 16 * h + 8 * half)), p);
             const float s = sl[b][wave][col];
-            const bool live = turn * 8 + wave < groups;     // past the end lie the last values again
+            const bool live = turn < end && turn * 8 + wave < groups;   // past the end lie other values
 #pragma unroll
             for (int i = 0; i < 16; i++) acc[i] = live ? __builtin_fmaf(p[i], s, acc[i]) : acc[i];
         };
-        load(ahead0, 0);
-        load(ahead1, 1);
+        load(ahead0, begin);
+        load(ahead1, begin + 1);
         lds_barrier();      // the places are free
-        for (int turn = 0; turn < turns; turn += 2) {       // turns past the end count nothing
+        for (int turn = begin; turn < end; turn += 2) {     // turns past the end count nothing
             turn_of(0, ahead0, turn);
             turn_of(1, ahead1, turn + 1);
         }
+        __syncthreads();
 #pragma unroll
         for (int i = 0; i < 16; i++) join[wave][col][8 * (i / 4) + 4 * half + i % 4] = acc[i];
         __syncthreads();
@@ -204,29 +209,46 @@ __global__ __launch_bounds__(512) void k_adapter_many(AdapterArgs a) {
         float v[2] = {};
 #pragma unroll
         for (int w = 0; w < 8; w++) v[0] += join[w][row32][r], v[1] += join[w][row32][r + 1];
-        const float scale = a.scales[now];
-        v[0] *= scale, v[1] *= scale;
-        float unit = 1.0f;
-        if constexpr (TYPE == QS_SRC_F16) {
-            // a power of two that takes the largest of the 32 to f16's upper range
-            float top = fmaxf(fabsf(v[0]), fabsf(v[1]));
-            top = fmaxf(top, __shfl_xor(top, 1)), top = fmaxf(top, __shfl_xor(top, 2));
-            top = fmaxf(top, __shfl_xor(top, 4)), top = fmaxf(top, __shfl_xor(top, 8));
-            int e = 0;
-            if (top > 0.0f && top < __builtin_inff()) (void)__builtin_frexpf(top, &e);
-            e = e < -80 ? -80 : e;
-            unit = __builtin_ldexpf(1.0f, e - 15);
-            v[0] = __builtin_ldexpf(v[0], 15 - e), v[1] = __builtin_ldexpf(v[1], 15 - e);
-        }
         if ((mine >> row32) & 1) {
-            const int64_t at = (t0 + row32) * a.ldv + r0 + r;
-#pragma unroll
-            for (int i = 0; i < 2; i++)
-                if (r0 + r + i < rank) split16<TYPE>(v[i], a.hi[at + i], a.lo[at + i]);
-            if (TYPE == QS_SRC_F16 && r == 0) a.unit[(t0 + row32) * ((a.ldv + 31) / 32) + r0 / 32] = unit;
+            float* sum = a.sums + (blockIdx.z * a.t + t0 + row32) * a.ldv + r0 + r;
+            if (r0 + r < rank) sum[0] = v[0];
+            if (r0 + r + 1 < rank) sum[1] = v[1];
         }
         __syncthreads();
     }
+}
+
+// The parts' sums, scaled, as hi + lo: 16 lanes to a row's 32 ranks, two each.
+template <int TYPE>
+__global__ __launch_bounds__(256) void k_adapter_join(AdapterArgs a) {
+    const int64_t t = (int64_t)blockIdx.x * 16 + threadIdx.x / 16;
+    const int r0 = blockIdx.y * 32, r = r0 + threadIdx.x % 16 * 2;
+    const int id = t < a.t ? a.ids[t] : -1;
+    const bool has = id >= 0 && id < a.adapters;
+    const int rank = has ? a.off[id + 1] - a.off[id] : 0;
+    const bool live = r < rank;     // ranks are multiples of 8
+    float v[2] = {};
+    for (int z = 0; z < a.parts; z++)
+#pragma unroll
+        for (int i = 0; i < 2; i++) v[i] += live ? a.sums[(z * a.t + t) * a.ldv + r + i] : 0.0f;
+    const float scale = has ? a.scales[id] : 0.0f;
+    v[0] = live ? v[0] * scale : 0.0f, v[1] = live ? v[1] * scale : 0.0f;
+    float unit = 1.0f;
+    if constexpr (TYPE == QS_SRC_F16) {
+        // a power of two that takes the largest of the 32 to f16's upper range
+        float top = fmaxf(fabsf(v[0]), fabsf(v[1]));
+        top = fmaxf(top, __shfl_xor(top, 1)), top = fmaxf(top, __shfl_xor(top, 2));
+        top = fmaxf(top, __shfl_xor(top, 4)), top = fmaxf(top, __shfl_xor(top, 8));
+        int e = 0;
+        if (top > 0.0f && top < __builtin_inff()) (void)__builtin_frexpf(top, &e);
+        e = e < -80 ? -80 : e;
+        unit = __builtin_ldexpf(1.0f, e - 15);
+        v[0] = __builtin_ldexpf(v[0], 15 - e), v[1] = __builtin_ldexpf(v[1], 15 - e);
+    }
+    if (!live) return;
+#pragma unroll
+    for (int i = 0; i < 2; i++) split16<TYPE>(v[i], a.hi[t * a.ldv + r + i], a.lo[t * a.ldv + r + i]);
+    if (TYPE == QS_SRC_F16 && r == r0) a.unit[t * ((a.ldv + 31) / 32) + r0 / 32] = unit;
 }
 
 // What add_adapters reads.
@@ -239,13 +261,17 @@ struct AdapterTile {
 };
 
 // y += B v on UM x UN units of 32 x 32 (rows t0 .., columns n0 ..) that a wave
-// holds. The rows' adapters are taken one after another; a unit's products are
-// kept apart and added to the rows that have the adapter, so that a NaN in
-// another's B does not reach them.
-template <int TYPE, int UM, int UN>
-QS_DEV void add_adapters(const AdapterTile& a, f32x16 (&y)[UM][UN], int64_t t0, int64_t rows, int64_t n0, int64_t n) {
+// holds. The rows' adapters are taken one after another, 32 ranks a step; a
+// unit's products are kept apart and added to the rows that have the adapter,
+// so that a NaN in another's B does not reach them. Of WK waves that share the
+// sums of these units each takes every WK-th step: a step is bound by the
+// latency of what it reads (512 rows with q4_k 2,560 x 2,560, 4 adapters: the
+// product took 44 us with the steps in one wave of eight).
+template <int TYPE, int WK, int UM, int UN>
+QS_DEV void add_adapters(const AdapterTile& a, f32x16 (&y)[UM][UN], int64_t t0, int64_t rows, int64_t n0, int64_t n, int wk) {
     const int lane = threadIdx.x % 64, col = lane % 32, half = lane / 32;
     const int64_t units = (a.ldv + 31) / 32;
+    int step = 0;
 #pragma unroll
     for (int um = 0; um < UM; um++) {
         const int64_t tb = t0 + 32 * um, t = tb + col < rows ? tb + col : rows - 1;
@@ -259,6 +285,7 @@ QS_DEV void add_adapters(const AdapterTile& a, f32x16 (&y)[UM][UN], int64_t t0, 
             const uint16_t* vh = a.hi + t * a.ldv;
             const uint16_t* vl = a.lo + t * a.ldv;
             for (int r0 = 0; r0 < rank; r0 += 32) {
+                if (step++ % WK != wk) continue;
                 uint4 h[2], l[2];
 #pragma unroll
                 for (int s = 0; s < 2; s++) {

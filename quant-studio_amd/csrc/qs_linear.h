@@ -124,9 +124,19 @@ struct AdapterArgs {
     uint16_t *hi, *lo;          // v as hi + lo in the adapters' type: [t][ldv]
     float* unit;                // what that is to be multiplied by (F16): [t][ldv / 32]
     float* delta;               // [t][n]
+    float* sums;                // [parts][t][ldv]
     int64_t k, n, t, ldv;
     int32_t adapters;
+    int parts;
 };
+// Parts that the rows' values are split into: up to 1,024 workgroups, where a
+// row has 512 values or more for each. The CUs hold 512 at a time; parts half as
+// long leave less to the 32 rows that have two adapters (2,047 rows of 9,728
+// values, ranks to 128: 41 us for 512 workgroups, 32 for 1,024, 47 unsplit).
+inline int adapter_parts(int64_t t, int64_t k, int64_t ldv) {
+    const int64_t blocks = (t + 31) / 32 * ((ldv + 31) / 32), p = 1024 / blocks < k / 512 ? 1024 / blocks : k / 512;
+    return p < 1 ? 1 : (int)p;
+}
 hipError_t launch_adapters(int type, const AdapterArgs& a, hipStream_t st);
 
 }  // namespace qsl

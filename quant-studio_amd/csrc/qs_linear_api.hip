@@ -58,7 +58,7 @@ int bad_sizes(const Entry& e, int64_t n, int64_t k, int64_t t) {
 // factors as laid out.
 struct Work {
     int64_t v, delta, lo, unit, layouts, bytes;     // offsets; v is hi where there is a lo, layouts the parts of a split
-    int splits;
+    int splits, parts;
 };
 Work work_of(int type, int dst_type, int64_t n, int64_t k, int64_t t, int max_rank) {
     using qsl::round_up;
@@ -69,14 +69,17 @@ Work work_of(int type, int dst_type, int64_t n, int64_t k, int64_t t, int max_ra
         w.lo = round_up(t * max_rank * 2, 256);
         w.unit = 2 * w.lo;
         w.layouts = w.unit + round_up(t * ((max_rank + 31) / 32) * 4, 256);
+        w.parts = qsl::adapter_parts(t, k, max_rank);
     } else if (max_rank > 0) {
         w.delta = round_up(t * max_rank * 4, 256);
         w.layouts = w.delta + (t > qsl::FEW_ROWS ? round_up(t * n * 4, 256) : 0);
     }
     w.splits = matrix || t <= qsl::FEW_ROWS ? 1 : qsl::tile_splits(t, n, k);
-    w.bytes = w.layouts + (matrix         ? qsl::matrix_plan(type, qsl::takes_f16(dst_type, t, n, k), n, k, t).bytes()
-                           : w.splits > 1 ? w.splits * t * n * 4
-                                          : 0);
+    const int64_t layouts = matrix         ? qsl::matrix_plan(type, qsl::takes_f16(dst_type, t, n, k), n, k, t).bytes()
+                            : w.splits > 1 ? w.splits * t * n * 4
+                                           : 0;
+    const int64_t sums = w.parts * t * max_rank * 4;        // read before the layouts are written, in their place
+    w.bytes = w.layouts + (layouts > sums ? layouts : sums);
     return w;
 }
 
@@ -164,6 +167,8 @@ int qs_packed_linear(int ggml_type, const void* weight, int64_t n, int64_t k, co
         s.hi = reinterpret_cast<uint16_t*>(base + work.v);
         s.lo = reinterpret_cast<uint16_t*>(base + work.lo);
         s.unit = reinterpret_cast<float*>(base + work.unit);
+        s.sums = reinterpret_cast<float*>(base + work.layouts);
+        s.parts = work.parts;
         const hipError_t r = qsl::launch_adapters(adapters->type, s, st);
         if (r != hipSuccess) return fail(QS_EIO, "packed_linear: launch failed: %s", hipGetErrorString(r));
         a.ids = ids;

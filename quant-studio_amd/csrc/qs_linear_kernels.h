@@ -485,6 +485,13 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_linear_tile(LinearArgs
         }
     }
     // place of element i of a unit: row 8 (i / 4) + 4 half + i % 4, column `col`
+    if (a.delta && a.splits == 1 && wk == 0)        // all at once, before the first store
+#pragma unroll
+        for (int u = 0; u < UM * UN * 16; u++) {
+            const int64_t t = t0 + (wmr * UM + u / 16 / UN) * 32 + 8 * (u % 16 / 4) + 4 * half + u % 4;
+            const int64_t n = n0 + (wn * UN + u / 16 % UN) * 32 + col;
+            acc[u / 16 / UN][u / 16 % UN][u % 16] += a.delta[(t < a.t ? t : a.t - 1) * a.n + (n < a.n ? n : a.n - 1)];
+        }
     if constexpr (WK > 1) {
         float* join = reinterpret_cast<float*>(lds);
         const int mine = (wmr * WN + wn) * UM * UN * 16;
@@ -515,7 +522,6 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_linear_tile(LinearArgs
                     a.parts[(split * a.t + t) * a.n + n] = y;
                     continue;
                 }
-                if (a.delta) y += a.delta[t * a.n + n];
                 store_value(a, t * a.n + n, y);
             }
         }

@@ -351,12 +351,13 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_matrix(MatrixArgs a) {
         turn(odd, even, s + 2);
     }
     __builtin_amdgcn_s_waitcnt(0x0f70);     // no copy to LDS outlives the workgroup
+    if constexpr (ADAPT)
+        add_adapters<ADAPT, WK>(adapter_tile(l), acc, t0 + wm * UM * 32, l.t, a.first + n0 + wn * UN * 32, l.n, wk);
     if constexpr (WK > 1) {
         join_waves<WK, WM * WN>(acc, reinterpret_cast<float*>(even), wk, wm * WN + wn);
         static_assert(STAGE >= BM * BN * 4 / UN, "a column of units");
         if (wk > 0) return;
     }
-    if constexpr (ADAPT) add_adapters<ADAPT>(adapter_tile(l), acc, t0 + wm * UM * 32, l.t, a.first + n0 + wn * UN * 32, l.n);
     store_tile(l, acc, t0 + wm * UM * 32, a.first + n0 + wn * UN * 32, a.first + a.count);
 }
 

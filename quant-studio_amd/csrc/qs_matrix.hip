@@ -62,9 +62,12 @@ hipError_t product16(const Matrix16Args& a, hipStream_t st) {
 
 template <int TYPE>
 hipError_t adapters(const AdapterArgs& a, hipStream_t st) {
-    if (takes_matrix(a.t))
-        return launch_kernel(k_adapter_many<TYPE>, dim3((unsigned)((a.t + 31) / 32), (unsigned)((a.ldv + 31) / 32)), dim3(512),
-                             0, st, a);
+    if (takes_matrix(a.t)) {
+        const unsigned ranks = (unsigned)((a.ldv + 31) / 32);
+        const hipError_t e = launch_kernel(k_adapter_many<TYPE>, dim3((unsigned)((a.t + 31) / 32), ranks, (unsigned)a.parts),
+                                           dim3(512), 0, st, a);
+        return e != hipSuccess ? e : launch_kernel(k_adapter_join<TYPE>, dim3((unsigned)((a.t + 15) / 16), ranks), dim3(256), 0, st, a);
+    }
     const hipError_t e = launch_kernel(k_adapter_few<TYPE>, dim3((unsigned)a.t, (unsigned)(a.ldv / 8)), dim3(256), 0, st, a);
     if (e != hipSuccess || a.t <= FEW_ROWS) return e;
     return launch_kernel(k_adapter_delta<TYPE>, dim3((unsigned)((a.n + 255) / 256), (unsigned)a.t), dim3(256), 0, st, a);
@@ -79,10 +82,10 @@ hipError_t launch_matrix(int planes, int mins, const MatrixArgs& a, hipStream_t 
 
 // Larger tiles do more per LDS byte (256 x 320: 1.02 PFLOP/s where they fill the
 // chip, 64 x 64: 0.56). Adapters need registers that 160 columns a wave do not
-// leave.
+// leave, and with them a CU has registers for one workgroup of 64 x 64.
 hipError_t launch_matrix16(const Matrix16Args& a, hipStream_t st) {
-    constexpr Choice choices[] = {{256, 320, 256, 1000}, {256, 256, 256, 770}, {128, 160, 256, 385}, {128, 96, 256, 258},
-                                  {64, 64, 512, 227}};
+    const Choice choices[] = {{256, 320, 256, 1000}, {256, 256, 256, 770}, {128, 160, 256, 385}, {128, 96, 256, 258},
+                              {64, 64, a.l.ids ? 256 : 512, 227}};
     switch (choose(choices, a.l.ids ? 1 : 0, a.l.t, a.count)) {
     case 0: return product16<256, 320, 4, 2, 1, 4>(a, st);
     case 1: return product16<256, 256, 2, 4, 1, 4>(a, st);

@@ -231,11 +231,6 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_matrix16(Matrix16Args 
         turn(odd, even, s + 3, STEPS % 2);
     }
     __builtin_amdgcn_s_waitcnt(0x0f70);     // no copy to LDS outlives the workgroup
-    if constexpr (WK > 1) {
-        static_assert(STAGE >= BM * BN * 4 / UN, "a column of units");
-        join_waves<WK, WM * WN>(acc, reinterpret_cast<float*>(even), wk, wm * WN + wn);
-        if (wk > 0) return;
-    }
     float unw[UN];
 #pragma unroll
     for (int un = 0; un < UN; un++) {
@@ -251,7 +246,13 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_matrix16(Matrix16Args 
 #pragma unroll
             for (int un = 0; un < UN; un++) acc[um][un][i] = acc[um][un][i] * unw[un] * unx;
         }
-    if constexpr (ADAPT) add_adapters<ADAPT>(adapter_tile(l), acc, t0 + wm * UM * 32, l.t, a.first + n0 + wn * UN * 32, l.n);
+    if constexpr (ADAPT)
+        add_adapters<ADAPT, WK>(adapter_tile(l), acc, t0 + wm * UM * 32, l.t, a.first + n0 + wn * UN * 32, l.n, wk);
+    if constexpr (WK > 1) {
+        static_assert(STAGE >= BM * BN * 4 / UN, "a column of units");
+        join_waves<WK, WM * WN>(acc, reinterpret_cast<float*>(even), wk, wm * WN + wn);
+        if (wk > 0) return;
+    }
     store_tile(l, acc, t0 + wm * UM * 32, a.first + n0 + wn * UN * 32, a.first + a.count);
 }
 
