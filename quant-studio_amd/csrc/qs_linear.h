@@ -71,12 +71,53 @@ inline MatrixPlan matrix_plan(int type, bool f16, int64_t n, int64_t k, int64_t 
 }
 inline bool takes_matrix(int64_t t) { return t > TILE_ROWS; }
 // Large products whose result is bf16 (8 bits) take factors of f16 (11 bits);
-// everything else exact codes. Rows of 256 values and products of 2^30 take as
-// long either way (q4_k, 2,000 rows, 3,000 x 256: 19 us f16, 20 us exact; 513
-// rows, 1,025 x 768: 17 and 16); 512 rows with 2,560 x 2,560 37 and 48, 4,096
-// with 9,728 x 2,560 248 and 418.
+// everything else exact codes. F16 factors are laid out in two launches and twice
+// the bytes, and multiplied at up to 1.0 PFLOP/s where exact codes reach 0.62.
+// q4_k, us f16 and exact: 512 rows, 2,560 x 2,560 38 and 34; 2,048, 1,024 x 2,560
+// 42 and 38; 1,024, 2,560 x 2,560 42 and 50; 300, 9,728 x 2,560 55 and 56; 4,096,
+// 9,728 x 2,560 234 and 389. Rows under 1,024 values give neither time to start:
+// 2,000 rows, 3,000 x 256 19 and 19.
 inline bool takes_f16(int dst_type, int64_t t, int64_t n, int64_t k) {
-    return dst_type == QS_SRC_BF16 && takes_matrix(t) && k >= 1024 && t * n >= (INT64_C(1) << 31) / k;
+    return dst_type == QS_SRC_BF16 && takes_matrix(t) && k >= 1024 && t * n >= INT64_C(3) * (INT64_C(1) << 31) / k;
+}
+
+// Tiles of a product of laid-out factors, and the time measured for a round of
+// as many as the 256 CUs hold, in tenths of a microsecond at rows of 2,560
+// values (it grows with the rows).
+struct Tiles {
+    int bm, bn, held, cost;
+};
+inline int64_t tile_count(int64_t t, int64_t n, int bm, int bn) { return ((t + bm - 1) / bm) * ((n + bn - 1) / bn); }
+
+// F16 factors. Larger tiles do more per LDS byte (256 x 320: 1.02 PFLOP/s where
+// they fill the chip, 64 x 64: 0.56). Adapters need registers that 160 columns a
+// wave do not leave, and with them a CU has registers for one workgroup of 64 x 64.
+constexpr Tiles TILES16[] = {{256, 320, 256, 1000}, {256, 256, 256, 770}, {128, 160, 256, 385}, {128, 96, 256, 258},
+                             {64, 64, 512, 227}};
+constexpr int MOST_PARTS = 4;
+struct Choice16 {
+    int tile, splits;
+};
+// The tile, and the parts of the groups, that cost least: few tiles leave CUs
+// idle, each of the rest waiting for its copies; parts cost what writing and
+// joining their f32 sums takes, 12 bytes of each at 4 TB/s, and two launches'
+// ends. 509 rows with q5_k 2,560 x 9,728: product and join 45 us in four parts of
+// 128 x 160, 62 whole in 64 x 64; 2,047 rows with q6_k: three parts of 256 x 256
+// 121, 115 whole in 128 x 160, which the rule takes.
+inline Choice16 choose16(bool adapted, int64_t t, int64_t n, int64_t k, int most) {
+    Choice16 best{};
+    double least = 1e300;
+    for (int i = adapted ? 1 : 0; i < 5; i++)
+        for (int s = 1; s <= most; s++) {
+            const int64_t pairs = (k / 32 + 7) / 8, per = (pairs + s - 1) / s;
+            if ((s - 1) * per >= pairs) continue;       // of stages: no part is empty
+            const Tiles& c = TILES16[i];
+            const int64_t held = adapted && c.held > 256 ? 256 : c.held, rounds = (tile_count(t, n, c.bm, c.bn) * s + held - 1) / held;
+            const double cost = (double)rounds * c.cost * (double)k / (2560.0 * s) +
+                                (s > 1 ? (adapted ? 100 : 40) + (double)(t * n) * 12 * s / 4e5 : 0);
+            if (cost < least) least = cost, best = {i, s};
+        }
+    return best;
 }
 
 // Parts that a product of 9 .. TILE_ROWS rows is split into over its groups, so

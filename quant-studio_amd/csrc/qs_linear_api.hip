@@ -57,7 +57,7 @@ int bad_sizes(const Entry& e, int64_t n, int64_t k, int64_t t) {
 // The workspace: what the adapters' products leave for the weight's, then the
 // factors as laid out.
 struct Work {
-    int64_t v, delta, lo, unit, layouts, bytes;     // offsets; v is hi where there is a lo, layouts the parts of a split
+    int64_t v, delta, lo, unit, layouts, sums, bytes;   // offsets; v is hi where there is a lo, sums a split product's
     int splits, parts;
 };
 Work work_of(int type, int dst_type, int64_t n, int64_t k, int64_t t, int max_rank) {
@@ -74,12 +74,16 @@ Work work_of(int type, int dst_type, int64_t n, int64_t k, int64_t t, int max_ra
         w.delta = round_up(t * max_rank * 4, 256);
         w.layouts = w.delta + (t > qsl::FEW_ROWS ? round_up(t * n * 4, 256) : 0);
     }
-    w.splits = matrix || t <= qsl::FEW_ROWS ? 1 : qsl::tile_splits(t, n, k);
-    const int64_t layouts = matrix         ? qsl::matrix_plan(type, qsl::takes_f16(dst_type, t, n, k), n, k, t).bytes()
-                            : w.splits > 1 ? w.splits * t * n * 4
-                                           : 0;
-    const int64_t sums = w.parts * t * max_rank * 4;        // read before the layouts are written, in their place
-    w.bytes = w.layouts + (layouts > sums ? layouts : sums);
+    const bool f16 = qsl::takes_f16(dst_type, t, n, k);
+    const qsl::MatrixPlan plan = qsl::matrix_plan(type, f16, n, k, t);
+    w.splits = f16                                ? qsl::choose16(max_rank > 0, t, n, k, plan.slice < n ? 1 : qsl::MOST_PARTS).splits
+               : matrix || t <= qsl::FEW_ROWS ? 1
+                                                  : qsl::tile_splits(t, n, k);
+    w.sums = w.layouts + (matrix ? qsl::round_up(plan.bytes(), 256) : 0);
+    w.bytes = w.sums + (w.splits > 1 ? w.splits * t * n * 4 : 0);
+    // the adapters' sums are read before the layouts are written, in their place
+    const int64_t adapted = w.layouts + w.parts * t * max_rank * 4;
+    w.bytes = w.bytes > adapted ? w.bytes : adapted;
     return w;
 }
 
@@ -181,7 +185,7 @@ int qs_packed_linear(int ggml_type, const void* weight, int64_t n, int64_t k, co
         else if (t > qsl::FEW_ROWS) a.delta = s.delta;
         else a.v = s.v;
     }
-    a.parts = reinterpret_cast<float*>(base + work.layouts);
+    a.parts = reinterpret_cast<float*>(base + work.sums);
     a.splits = work.splits;
     const hipError_t r = e->launch(a, base + work.layouts, st);
     if (r != hipSuccess) return fail(QS_EIO, "packed_linear: launch failed: %s", hipGetErrorString(r));

@@ -154,10 +154,10 @@ QS_DEV AdapterTile adapter_tile(const LinearArgs& l) {
     return {l.ids, l.off, l.b, l.v_hi, l.v_lo, l.v_unit, l.ldv, l.adapters};
 }
 
-// A wave's units to memory: rows from t0, columns from n0 to `end`. Element i
+// A wave's units to memory of a type: rows from t0, columns from n0 to `end`. Element i
 // of a unit: row 8 (i / 4) + 4 half + i % 4, column lane % 32.
 template <int UM, int UN>
-QS_DEV void store_tile(const LinearArgs& l, const f32x16 (&y)[UM][UN], int64_t t0, int64_t n0, int64_t end) {
+QS_DEV void store_tile(void* to, int type, const LinearArgs& l, const f32x16 (&y)[UM][UN], int64_t t0, int64_t n0, int64_t end) {
     const int lane = threadIdx.x % 64, col = lane % 32, half = lane / 32;
     const auto store = [&](auto* dst) {
         using T = std::remove_pointer_t<decltype(dst)>;
@@ -172,9 +172,9 @@ QS_DEV void store_tile(const LinearArgs& l, const f32x16 (&y)[UM][UN], int64_t t
                     if (t < l.t && n0 + un * 32 + col < end) row[un * 32] = (T)y[um][un][i];
             }
     };
-    if (l.dst_type == QS_SRC_F32) store(static_cast<float*>(l.dst));
-    else if (l.dst_type == QS_SRC_F16) store(static_cast<_Float16*>(l.dst));
-    else store(static_cast<__bf16*>(l.dst));
+    if (type == QS_SRC_F32) store(static_cast<float*>(to));
+    else if (type == QS_SRC_F16) store(static_cast<_Float16*>(to));
+    else store(static_cast<__bf16*>(to));
 }
 
 // The sums of WK waves that hold the same units, in the first one, one wave's
@@ -358,7 +358,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_matrix(MatrixArgs a) {
         static_assert(STAGE >= BM * BN * 4 / UN, "a column of units");
         if (wk > 0) return;
     }
-    store_tile(l, acc, t0 + wm * UM * 32, a.first + n0 + wn * UN * 32, a.first + a.count);
+    store_tile(l.dst, l.dst_type, l, acc, t0 + wm * UM * 32, a.first + n0 + wn * UN * 32, a.first + a.count);
 }
 
 }  // namespace qsl

@@ -11,23 +11,17 @@ using qs_host::launch_kernel;
 
 namespace {
 
-int64_t tiles(int64_t t, int64_t n, int bm, int bn) { return ((t + bm - 1) / bm) * ((n + bn - 1) / bn); }
 // a multiple of the 8 XCDs: each takes a run of tiles
 dim3 grid_of(int64_t tiles) { return dim3((unsigned)((tiles + 7) / 8 * 8)); }
 
-// The tile whose rounds over the 256 CUs cost least. A round's cost is the time
-// measured for it, in tenths of a microsecond at rows of 2,560 values (they
-// grow with the rows alike).
-struct Choice {
-    int bm, bn, held, cost;     // held: tiles that the CUs take at a time
-};
+// The tile whose rounds over the 256 CUs cost least.
 template <int N>
-int choose(const Choice (&choices)[N], int from, int64_t t, int64_t n) {
-    int best = from;
+int choose(const Tiles (&choices)[N], int64_t t, int64_t n) {
+    int best = 0;
     int64_t least = INT64_MAX;
-    for (int i = from; i < N; i++) {
-        const Choice& c = choices[i];
-        const int64_t cost = (tiles(t, n, c.bm, c.bn) + c.held - 1) / c.held * c.cost;
+    for (int i = 0; i < N; i++) {
+        const Tiles& c = choices[i];
+        const int64_t cost = (tile_count(t, n, c.bm, c.bn) + c.held - 1) / c.held * c.cost;
         if (cost < least) least = cost, best = i;
     }
     return best;
@@ -35,7 +29,7 @@ int choose(const Choice (&choices)[N], int from, int64_t t, int64_t n) {
 
 template <int PLANES, int MINS, int BM, int BN, int WM, int WN, int WK, int G>
 hipError_t product(const MatrixArgs& a, hipStream_t st) {
-    const dim3 grid = grid_of(tiles(a.l.t, a.count, BM, BN)), block(64 * WM * WN * WK);
+    const dim3 grid = grid_of(tile_count(a.l.t, a.count, BM, BN)), block(64 * WM * WN * WK);
     if (!a.l.ids) return launch_kernel(k_matrix<PLANES, MINS, BM, BN, WM, WN, WK, G, 0>, grid, block, 0, st, a);
     if (a.l.b_type == QS_SRC_BF16) return launch_kernel(k_matrix<PLANES, MINS, BM, BN, WM, WN, WK, G, QS_SRC_BF16>, grid, block, 0, st, a);
     return launch_kernel(k_matrix<PLANES, MINS, BM, BN, WM, WN, WK, G, QS_SRC_F16>, grid, block, 0, st, a);
@@ -43,8 +37,8 @@ hipError_t product(const MatrixArgs& a, hipStream_t st) {
 
 template <int PLANES, int MINS>
 hipError_t any(const MatrixArgs& a, hipStream_t st) {
-    constexpr Choice choices[] = {{128, 128, 512, 690}, {128, 128, 256, 430}, {64, 64, 512, 230}};
-    switch (choose(choices, 0, a.l.t, a.count)) {
+    constexpr Tiles choices[] = {{128, 128, 512, 690}, {128, 128, 256, 430}, {64, 64, 512, 230}};
+    switch (choose(choices, a.l.t, a.count)) {
     case 0: return product<PLANES, MINS, 128, 128, 2, 2, 1, 2>(a, st);
     case 1: return product<PLANES, MINS, 128, 128, 2, 2, 2, 4>(a, st);
     default: return product<PLANES, MINS, 64, 64, 1, 2, 2, 4>(a, st);
@@ -53,7 +47,7 @@ hipError_t any(const MatrixArgs& a, hipStream_t st) {
 
 template <int BM, int BN, int WM, int WN, int WK, int S>
 hipError_t product16(const Matrix16Args& a, hipStream_t st) {
-    const dim3 grid = grid_of(tiles(a.l.t, a.count, BM, BN)), block(64 * WM * WN * WK);
+    const dim3 grid = grid_of(tile_count(a.l.t, a.count, BM, BN) * a.l.splits), block(64 * WM * WN * WK);
     if (!a.l.ids) return launch_kernel(k_matrix16<BM, BN, WM, WN, WK, S, 0>, grid, block, 0, st, a);
     if constexpr (BN / WN / 32 * (BM / WM / 32) > 8) return hipErrorInvalidValue;       // not chosen with adapters
     else if (a.l.b_type == QS_SRC_BF16) return launch_kernel(k_matrix16<BM, BN, WM, WN, WK, S, QS_SRC_BF16>, grid, block, 0, st, a);
@@ -80,19 +74,21 @@ hipError_t launch_matrix(int planes, int mins, const MatrixArgs& a, hipStream_t 
     return mins == 0 ? any<1, 0>(a, st) : mins == 1 ? any<1, 1>(a, st) : any<1, 2>(a, st);
 }
 
-// Larger tiles do more per LDS byte (256 x 320: 1.02 PFLOP/s where they fill the
-// chip, 64 x 64: 0.56). Adapters need registers that 160 columns a wave do not
-// leave, and with them a CU has registers for one workgroup of 64 x 64.
-hipError_t launch_matrix16(const Matrix16Args& a, hipStream_t st) {
-    const Choice choices[] = {{256, 320, 256, 1000}, {256, 256, 256, 770}, {128, 160, 256, 385}, {128, 96, 256, 258},
-                              {64, 64, a.l.ids ? 256 : 512, 227}};
-    switch (choose(choices, a.l.ids ? 1 : 0, a.l.t, a.count)) {
+static hipError_t tile16(int tile, const Matrix16Args& a, hipStream_t st) {
+    switch (tile) {
     case 0: return product16<256, 320, 4, 2, 1, 4>(a, st);
     case 1: return product16<256, 256, 2, 4, 1, 4>(a, st);
     case 2: return product16<128, 160, 4, 1, 2, 8>(a, st);
     case 3: return product16<128, 96, 2, 1, 4, 8>(a, st);
     default: return product16<64, 64, 1, 1, 8, 8>(a, st);
     }
+}
+
+hipError_t launch_matrix16(const Matrix16Args& a, hipStream_t st) {
+    // a product of one slice was split with its workspace in view
+    const int tile = choose16(a.l.ids, a.l.t, a.count, a.l.k, a.count < a.l.n ? 1 : MOST_PARTS).tile;
+    const hipError_t e = tile16(tile, a, st);
+    return e != hipSuccess || a.l.splits == 1 ? e : launch_join(a.l, st);
 }
 
 hipError_t launch_join(const LinearArgs& a, hipStream_t st) {

@@ -142,6 +142,7 @@ __global__ __launch_bounds__(256) void k_lay_out16(Layout16Args a) {
 // while one is multiplied the next one's copies are in flight. WM x WN waves
 // split the tile, WK the steps of a stage (their sums are joined in LDS at the
 // end, in order): a wave's part of the tile stays large where the tile is not.
+// Where tiles are few the stages are split over workgroups too.
 // The stages are two arrays, so that the compiler sees that a read of one does
 // not wait for copies to the other.
 template <int BM, int BN, int WM, int WN, int WK, int S, int ADAPT>
@@ -155,12 +156,14 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_matrix16(Matrix16Args 
     const LinearArgs& l = a.l;
     // XCDs and strips as in k_matrix
     const int64_t tiles_m = (l.t + BM - 1) / BM, tiles_n = (a.count + BN - 1) / BN, tiles = tiles_m * tiles_n;
-    const int64_t at = (int64_t)(blockIdx.x % 8) * (gridDim.x / 8) + blockIdx.x / 8;
-    if (at >= tiles) return;
+    const int64_t place = (int64_t)(blockIdx.x % 8) * (gridDim.x / 8) + blockIdx.x / 8, at = place % tiles;
+    if (place >= tiles * l.splits) return;
     const int64_t strip = at / (8 * tiles_m), left = tiles_n - 8 * strip, wide = left < 8 ? left : 8;
     const int64_t in = at - strip * 8 * tiles_m;
     const int64_t t0 = in / wide * BM, n0 = (8 * strip + in % wide) * BN;
-    const int stages = a.groups * 2 / S;
+    // an even number of stages, and this part's of them (no part is empty)
+    const int all = a.groups * 2 / S, per = (all / 2 + l.splits - 1) / l.splits * 2, split = (int)(place / tiles);
+    const int begin = split * per, end = begin + per < all ? begin + per : all;
 
     // This wave's copies of a stage: 1,024 bytes each, panel after panel; panels
     // past the last (a tile may reach past the layout) are the last one again.
@@ -213,20 +216,20 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_matrix16(Matrix16Args 
         __builtin_amdgcn_s_waitcnt(0x0070);         // vmcnt(0), lgkmcnt(0)
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        copy(after < stages ? after : stages - 1, stage);   // no branch: the last stage again
+        copy(after < end ? after : end - 1, stage);     // no branch: the last stage again
         __builtin_amdgcn_sched_barrier(0);                  // they go out first
         read(next, 0, (b + STEPS) % 2);
         __builtin_amdgcn_sched_barrier(0);
         multiply((b + STEPS - 1) % 2);
         __builtin_amdgcn_sched_barrier(0);
     };
-    copy(0, even);
-    copy(1, odd);
+    copy(begin, even);
+    copy(begin + 1, odd);
     __builtin_amdgcn_s_waitcnt(0x0f70);             // vmcnt(0)
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     read(even, 0, 0);
-    for (int s = 0; s < stages; s += 2) {       // an even number of stages
+    for (int s = begin; s < end; s += 2) {
         turn(even, odd, s + 2, 0);
         turn(odd, even, s + 3, STEPS % 2);
     }
@@ -247,13 +250,14 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_matrix16(Matrix16Args 
             for (int un = 0; un < UN; un++) acc[um][un][i] = acc[um][un][i] * unw[un] * unx;
         }
     if constexpr (ADAPT)
-        add_adapters<ADAPT, WK>(adapter_tile(l), acc, t0 + wm * UM * 32, l.t, a.first + n0 + wn * UN * 32, l.n, wk);
+        if (split == 0) add_adapters<ADAPT, WK>(adapter_tile(l), acc, t0 + wm * UM * 32, l.t, a.first + n0 + wn * UN * 32, l.n, wk);
     if constexpr (WK > 1) {
         static_assert(STAGE >= BM * BN * 4 / UN, "a column of units");
         join_waves<WK, WM * WN>(acc, reinterpret_cast<float*>(even), wk, wm * WN + wn);
         if (wk > 0) return;
     }
-    store_tile(l, acc, t0 + wm * UM * 32, a.first + n0 + wn * UN * 32, a.first + a.count);
+    store_tile(l.splits > 1 ? l.parts + split * l.t * l.n : l.dst, l.splits > 1 ? QS_SRC_F32 : l.dst_type, l, acc,
+               t0 + wm * UM * 32, a.first + n0 + wn * UN * 32, a.first + a.count);
 }
 
 }  // namespace qsl
