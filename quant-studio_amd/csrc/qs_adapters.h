@@ -2,9 +2,9 @@
 //     y[t] += B[id] (scale * A[id] x[t]),   id = ids[t]
 // First v = scale * A x for every row (k_adapter_few; k_adapter_many
 // and k_adapter_join), then
-// B v: for up to 8 rows in the product's own lanes (adapter_sum), to 128 rows by
-// a kernel that writes the sums for the product to add (k_adapter_delta), above
-// by matrix instructions on the product's tile (add_adapters).
+// B v: for up to 8 rows in the product's own lanes (adapter_sum), for tiles by a
+// kernel that writes the sums for the product to add (k_adapter_delta), for
+// laid-out factors by matrix instructions on the product's tile (add_adapters).
 #pragma once
 
 #include "qs_linear_kernels.h"
@@ -19,8 +19,9 @@ QS_DEV float from16(uint32_t bits) {
 }
 
 // A workgroup takes a row and 8 ranks, a wave two of them; a lane 8 values at a
-// time. Up to 128 rows, where a row or two use an adapter: bound by the latency
-// of ids, offsets and A, one after another.
+// time. Up to 192 rows, where a row or two use an adapter: bound by the latency
+// of ids, offsets and A, one after another (3.5 us for a row of 2,560 values and
+// rank 16, 6 us for 64 rows and ranks to 64).
 template <int TYPE>
 __global__ __launch_bounds__(256) void k_adapter_few(AdapterArgs a) {
     const int64_t t = blockIdx.x;
@@ -67,7 +68,8 @@ __global__ __launch_bounds__(256) void k_adapter_few(AdapterArgs a) {
 }
 
 // delta[t, n] = sum over r of v[t, r] * B[n, r]; 0 for a row without an adapter.
-// A lane takes a column: the wave's rows of B are one run of bytes.
+// A lane takes a column: the wave's rows of B are one run of bytes. Bound by
+// reading B for each row: 64 rows, 9,728 columns, ranks 64, 32 and 16, 46 MB: 13 us.
 template <int TYPE>
 __global__ __launch_bounds__(256) void k_adapter_delta(AdapterArgs a) {
     const int64_t t = blockIdx.y, n = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -138,7 +140,10 @@ QS_DEV void split16(float v, uint16_t& hi, uint16_t& lo) {
 // takes one of the groups. The codes are exact in the adapters' type: only the
 // products' sums are scaled, in f32. The rows' adapters are taken one after
 // another (packed sequences have one or two to 32 rows). A row's values are
-// split over `parts` workgroups, whose sums k_adapter_join adds.
+// split over `parts` workgroups, whose sums k_adapter_join adds. 2,047 rows of
+// 9,728 values, ranks 128, 64 and 32: 30 us, bound by the vector instructions that
+// widen the codes and scale the products, 32 of each for two matrix instructions;
+// the join takes 4 us.
 template <int TYPE>
 __global__ __launch_bounds__(512) void k_adapter_many(AdapterArgs a) {
     constexpr int XS = 256 + 16, AS = 512 + 16;     // strides that spread rows over the banks

@@ -9,9 +9,9 @@
 
 namespace qsl {
 
-// rows up to which a product takes dot products, and tiles that decode the
-// weight themselves; above, both factors are laid out for the matrix units
-constexpr int64_t FEW_ROWS = 8, TILE_ROWS = 128;
+// rows up to which a product takes dot products; above, tiles that decode the
+// weight themselves, or both factors laid out for the matrix units (takes_matrix)
+constexpr int64_t FEW_ROWS = 8;
 
 struct LinearArgs {
     const uint8_t* w;       // n rows of row_bytes
@@ -28,10 +28,10 @@ struct LinearArgs {
     int32_t adapters;
     int b_type;             // QS_SRC_F16 / QS_SRC_BF16
     const float* v;         // to FEW_ROWS rows: scale * A x, t rows of ldv
-    const float* delta;     // to TILE_ROWS rows: B v, t rows of n
+    const float* delta;     // tiles: B v, t rows of n
     float* parts;           // of a product split over its groups: splits x t rows of n
     int splits;
-    const uint16_t *v_hi, *v_lo;    // above: scale * A x as hi + lo, t rows of ldv
+    const uint16_t *v_hi, *v_lo;    // laid-out factors: scale * A x as hi + lo, t rows of ldv
     const float* v_unit;            // and what that is to be multiplied by (F16), t rows of ldv / 32
 };
 
@@ -69,7 +69,11 @@ inline MatrixPlan matrix_plan(int type, bool f16, int64_t n, int64_t k, int64_t 
     p.w_bytes = p.slice / 32 * p.groups * (f16 ? 2048 : panel_group_bytes(two_planes(type) ? 2 : 1, minima(type)));
     return p;
 }
-inline bool takes_matrix(int64_t t) { return t > TILE_ROWS; }
+// Tiles that decode the weight for each 64 rows save its layout's way through
+// memory. us of tiles and of laid-out factors: 100 rows with q4_k 9,728 x 2,560
+// 43 and 39 (64, one tile: 24), 128 44 and 40; 192 with q4_0 1,024 x 2,560 15 and 21, 4,096 x 4,096 29
+// and 36, with q6_k 2,560 x 9,728 58 and 89; q4_k 9,728 x 2,560 46 and 41.
+inline bool takes_matrix(int64_t t, int64_t n) { return t > (n > 8192 ? 64 : 192); }
 // Large products whose result is bf16 (8 bits) take factors of f16 (11 bits);
 // everything else exact codes. F16 factors are laid out in two launches and twice
 // the bytes, and multiplied at up to 1.0 PFLOP/s where exact codes reach 0.62.
@@ -78,7 +82,7 @@ inline bool takes_matrix(int64_t t) { return t > TILE_ROWS; }
 // 9,728 x 2,560 234 and 389. Rows under 1,024 values give neither time to start:
 // 2,000 rows, 3,000 x 256 19 and 19.
 inline bool takes_f16(int dst_type, int64_t t, int64_t n, int64_t k) {
-    return dst_type == QS_SRC_BF16 && takes_matrix(t) && k >= 1024 && t * n >= INT64_C(3) * (INT64_C(1) << 31) / k;
+    return dst_type == QS_SRC_BF16 && takes_matrix(t, n) && k >= 1024 && t * n >= INT64_C(3) * (INT64_C(1) << 31) / k;
 }
 
 // Tiles of a product of laid-out factors, and the time measured for a round of
@@ -120,7 +124,7 @@ inline Choice16 choose16(bool adapted, int64_t t, int64_t n, int64_t k, int most
     return best;
 }
 
-// Parts that a product of 9 .. TILE_ROWS rows is split into over its groups, so
+// Parts that a product that is not laid out is split into over its groups, so
 // that there are two workgroups for every CU; a part is whole stages of 8
 // groups. 61 rows with q8_0 1,024 x 2,560: 18.7 us whole, 12.5 in four parts; 16
 // with q6_k 2,560 x 9,728 50 and 27. More parts than workgroups for two a CU

@@ -124,6 +124,11 @@ QS_DEV uint4 read_end(const Run& r, int c, const uint8_t* lo, const uint8_t* hi)
 // codes that an offset of the weight's integers (OFFSET) or a minimum multiplies:
 // 48 bytes, the T of a group together, so that a lane reads them at constant
 // offsets, and an odd number of 16s a group, which spreads lanes over the banks.
+// One row is bound by reading a large weight (151,936 x 2,560: q8_0 75 us, 5.5
+// TB/s; q6_k 68 us, 4.7 TB/s; q4_k 50 us, 4.4 TB/s) and by the latency of what
+// comes one after another in a small one (q4_k 9,728 x 2,560, 14 MB: 6 us). More
+// rows add LDS reads and dot products: five with q6_k 151,936 x 2,560 95 us, 3.4
+// TB/s.
 template <int TYPE, int T, int L>
 __global__ __launch_bounds__(256) void k_linear_few(LinearArgs a, FewPlan plan) {
     constexpr int SUB = Format<TYPE>::SUB, AHEAD = 8, ROWS = 256 / L, OFFSET = qsd::offset<TYPE>();
@@ -284,7 +289,13 @@ struct Tile {
 // a thread a group, the rows' copied; the bytes of the next D stages are in
 // flight while one is multiplied (what a CU has in flight is what bounds a
 // weight read once). WM x WN waves split the tile, WK the
-// groups (their sums are joined in LDS at the end, in order).
+// groups (their sums are joined in LDS at the end, in order). A group's 16
+// products a lane are scaled by an outer product of the scales, d * s, that a
+// matrix instruction makes from three bf16 pieces of each, exact to f32.
+// Bound by staging, which neither overlaps the products: a thread's decode and
+// copies of a stage take about 1,200 clocks, a wave's matrix steps about 900, and
+// two barriers lie between. 64 rows with q4_k 9,728 x 2,560: 24 us, 131 TFLOP/s;
+// 16 rows 16.5 us; 128 with q6_k 151,936 x 2,560 630 us, 158 TFLOP/s.
 template <int TYPE, int BM, int BN, int WM, int WN, int WK, int G, int D>
 __global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_linear_tile(LinearArgs a) {
     using S = Tile<TYPE, BM, BN, WM, WN, WK, G>;

@@ -73,7 +73,9 @@ struct NormArgs {
 // for the sum of squares: one pass over the row gives both, and only the K/32
 // group steps are kept (in LDS, read back by the lane that wrote them) until
 // the sum is known. P lanes share a row, eight values each at a time; four
-// lanes make a group of 32.
+// lanes make a group of 32. Many rows are bound by memory (8,191 x 2,560 bf16 with
+// a residual, 149 MB read and written: 28 us, 5.3 TB/s, a copy's rate), a few by
+// latency (a row of 2,560: 3.2 us).
 // A NaN or an infinity makes its group's scale NaN, so its values are NaN, as
 // the plain computation has them; an infinity's row has 1 / sqrt(inf) = 0 and
 // its other groups 0.
@@ -145,7 +147,8 @@ __global__ __launch_bounds__(P > 256 ? P : 256) void k_rms_norm_q8(NormArgs a) {
         }
 }
 
-// the values q * s of 8-bit rows; 16 to a thread
+// the values q * s of 8-bit rows; 16 to a thread; bound by memory (8,191 x 2,560 to
+// bf16, 65 MB: 12.5 us, 5.2 TB/s)
 template <int DST>
 __global__ __launch_bounds__(256) void k_q8_values(const int8_t* q, const float* s, void* dst, int64_t n16) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -163,9 +166,12 @@ __global__ __launch_bounds__(256) void k_q8_values(const int8_t* q, const float*
 
 template <int SRC>
 hipError_t launch_norm(const NormArgs& a, hipStream_t st) {
-    // A wave per row where there are rows enough to fill the 1,024 SIMDs;
-    // fewer rows take a workgroup each, of 1,024 lanes where the row is long.
-    const int p = a.rows >= 2048 ? 64 : a.k > 2048 ? 1024 : 256;
+    // A wave per row where rows fill the 1,024 SIMDs several times (us with 64, 256
+    // and 1,024 lanes, bf16 with a residual: 8,191 x 2,560 24.5, 27.7, 48; 4,096 x
+    // 1,024 8.2, 10.3, 22), else a workgroup each (2,048 x 9,728 31, 24.5, 26; 1,024
+    // x 2,560 8.2, 6.6, 8.5), a large one where they are few and long (64 x 2,560
+    // 7.0, 4.1, 3.6; 1 x 2,560 6.2, 3.8, 3.2; 333 x 1,024 4.2, 3.6, 4.0).
+    const int p = a.rows >= 4096 ? 64 : a.rows <= 256 && a.k > 2048 ? 1024 : 256;
     const int rows = p > 256 ? 1 : 256 / p;
     const dim3 grid((unsigned)((a.rows + rows - 1) / rows));
     const size_t lds = (size_t)rows * (a.k / 32) * 4;
