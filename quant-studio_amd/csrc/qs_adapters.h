@@ -141,9 +141,9 @@ QS_DEV void split16(float v, uint16_t& hi, uint16_t& lo) {
 // products' sums are scaled, in f32. The rows' adapters are taken one after
 // another (packed sequences have one or two to 32 rows). A row's values are
 // split over `parts` workgroups, whose sums k_adapter_join adds. 2,047 rows of
-// 9,728 values, ranks 128, 64 and 32: 30 us, bound by the vector instructions that
-// widen the codes and scale the products, 32 of each for two matrix instructions;
-// the join takes 4 us.
+// 9,728 values, ranks 128, 64 and 32: 30 us, bound by the latency of a turn's
+// copies, LDS and barrier (vector instructions, which widen the codes and scale the
+// products, take 0.22 of the cycles, matrix ones 0.03); the join takes 4 us.
 template <int TYPE>
 __global__ __launch_bounds__(512) void k_adapter_many(AdapterArgs a) {
     constexpr int XS = 256 + 16, AS = 512 + 16;     // strides that spread rows over the banks

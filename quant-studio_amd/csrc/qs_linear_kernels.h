@@ -292,9 +292,10 @@ struct Tile {
 // groups (their sums are joined in LDS at the end, in order). A group's 16
 // products a lane are scaled by an outer product of the scales, d * s, that a
 // matrix instruction makes from three bf16 pieces of each, exact to f32.
-// Bound by staging, which neither overlaps the products: a thread's decode and
-// copies of a stage take about 1,200 clocks, a wave's matrix steps about 900, and
-// two barriers lie between. 64 rows with q4_k 9,728 x 2,560: 24 us, 131 TFLOP/s;
+// Bound by the turn of a stage: decode and copies to LDS, a barrier, products, a
+// barrier, one after another (64 rows with q4_k 9,728 x 2,560, 152 workgroups:
+// vector instructions take 0.18 of the SIMDs' cycles, matrix ones 0.05). That
+// product 24 us, 131 TFLOP/s;
 // 16 rows 16.5 us; 128 with q6_k 151,936 x 2,560 630 us, 158 TFLOP/s.
 template <int TYPE, int BM, int BN, int WM, int WN, int WK, int G, int D>
 __global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_linear_tile(LinearArgs a) {
