@@ -208,13 +208,13 @@ int64_t qs_packed_linear_workspace(int ggml_type, int64_t n, int64_t k, int64_t 
  *   workspace: qs_packed_linear_workspace() bytes, 256-byte aligned, used by
  *              this call alone until it is done; may be NULL where that is 0
  * Codes are multiplied exactly, scales applied in f32, y rounded once; but a
- * bf16 result with k >= 1024 and t*n*k >= 3 * 2^31, of more than 192 rows (64
- * where n > 8192), takes both factors' values rounded to f16 (11 bits; rows
- * scaled by powers of two first, so that nothing overflows), whose error is some
- * 1% of that of the result's own rounding. The result of a row does not depend
- * on timing; it may differ in the last bits of f32 with t and n, and with
- * adapters (another split of the sum). t is at most 2^24, each of n*k, t*k and
- * n*t at most 2^34. */
+ * bf16 result of more than 128 rows with k >= 1024 and t*n*k >= 3 * 2^31 (where
+ * few tiles do not make the exact form the faster) takes both factors' values
+ * rounded to f16 (11 bits; rows scaled by powers of two first, so that nothing
+ * overflows), whose error is some 1% of that of the result's own rounding. The
+ * result of a row does not depend on timing; it may differ in the last bits of
+ * f32 with t and n, and with adapters (another split of the sum). t is at most
+ * 2^24, each of n*k, t*k and n*t at most 2^34. */
 int qs_packed_linear(int ggml_type, const void *weight, int64_t n, int64_t k, const int8_t *q, const float *scales,
                      int64_t t, int dst_type, void *dst, int64_t dst_bytes, const qs_adapters *adapters,
                      const int32_t *ids, void *workspace, int64_t workspace_bytes, void *hip_stream);

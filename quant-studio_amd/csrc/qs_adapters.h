@@ -19,7 +19,7 @@ QS_DEV float from16(uint32_t bits) {
 }
 
 // A workgroup takes a row and 8 ranks, a wave two of them; a lane 8 values at a
-// time. Up to 192 rows, where a row or two use an adapter: bound by the latency
+// time. Up to 512 rows, where a row or two use an adapter: bound by the latency
 // of ids, offsets and A, one after another (3.5 us for a row of 2,560 values and
 // rank 16, 6 us for 64 rows and ranks to 64).
 template <int TYPE>

@@ -69,11 +69,19 @@ inline MatrixPlan matrix_plan(int type, bool f16, int64_t n, int64_t k, int64_t 
     p.w_bytes = p.slice / 32 * p.groups * (f16 ? 2048 : panel_group_bytes(two_planes(type) ? 2 : 1, minima(type)));
     return p;
 }
+inline int64_t tile_count(int64_t t, int64_t n, int bm, int bn) { return ((t + bm - 1) / bm) * ((n + bn - 1) / bn); }
 // Tiles that decode the weight for each 64 rows save its layout's way through
-// memory. us of tiles and of laid-out factors: 100 rows with q4_k 9,728 x 2,560
-// 43 and 39 (64, one tile: 24), 128 44 and 40; 192 with q4_0 1,024 x 2,560 15 and 21, 4,096 x 4,096 29
-// and 36, with q6_k 2,560 x 9,728 58 and 89; q4_k 9,728 x 2,560 46 and 41.
-inline bool takes_matrix(int64_t t, int64_t n) { return t > (n > 8192 ? 64 : 192); }
+// memory, as long as one round of 64 x 64 takes them all, or a split half a round
+// where rows are long. us of tiles and of laid-out factors: 128 rows with q4_k
+// 9,728 x 2,560 39 and 40; 192 with q6_k 2,560 x 9,728 53 and 89; 256 with q4_0
+// 4,096 x 4,096 27 and 37; 512 with 1,024 x 2,560 15 and 23, with 8 adapters of
+// rank 64 33 and 39; but 320 with 4,096 x 4,096 47 and 42, 512 with q6_k 2,048 x
+// 9,728 92 and 72. Above 512 rows the adapters' products row by row lose.
+inline bool takes_matrix(int64_t t, int64_t n, int64_t k) {
+    const int64_t tiles = tile_count(t, n, 64, 64);
+    return t > 512 || (t > 128 && tiles > (k <= 4096 ? 256 : 128));
+}
+
 // Large products whose result is bf16 (8 bits) take factors of f16 (11 bits);
 // everything else exact codes. F16 factors are laid out in two launches and twice
 // the bytes, and multiplied at up to 1.0 PFLOP/s where exact codes reach 0.62.
@@ -82,7 +90,7 @@ inline bool takes_matrix(int64_t t, int64_t n) { return t > (n > 8192 ? 64 : 192
 // 9,728 x 2,560 234 and 389. Rows under 1,024 values give neither time to start:
 // 2,000 rows, 3,000 x 256 19 and 19.
 inline bool takes_f16(int dst_type, int64_t t, int64_t n, int64_t k) {
-    return dst_type == QS_SRC_BF16 && takes_matrix(t, n) && k >= 1024 && t * n >= INT64_C(3) * (INT64_C(1) << 31) / k;
+    return dst_type == QS_SRC_BF16 && takes_matrix(t, n, k) && k >= 1024 && t * n >= INT64_C(3) * (INT64_C(1) << 31) / k;
 }
 
 // Tiles of a product of laid-out factors, and the time measured for a round of
@@ -91,7 +99,6 @@ inline bool takes_f16(int dst_type, int64_t t, int64_t n, int64_t k) {
 struct Tiles {
     int bm, bn, held, cost;
 };
-inline int64_t tile_count(int64_t t, int64_t n, int bm, int bn) { return ((t + bm - 1) / bm) * ((n + bn - 1) / bn); }
 
 // F16 factors. Larger tiles do more per LDS byte (256 x 320: 1.02 PFLOP/s where
 // they fill the chip, 64 x 64: 0.56). Adapters need registers that 160 columns a
@@ -126,12 +133,12 @@ inline Choice16 choose16(bool adapted, int64_t t, int64_t n, int64_t k, int most
 
 // Parts that a product that is not laid out is split into over its groups, so
 // that there are two workgroups for every CU; a part is whole stages of 8
-// groups. 61 rows with q8_0 1,024 x 2,560: 18.7 us whole, 12.5 in four parts; 16
-// with q6_k 2,560 x 9,728 50 and 27. More parts than workgroups for two a CU
-// were no faster.
+// groups. us whole, in up to 4 parts and in up to 8: 61 rows with q8_0 1,024 x
+// 2,560 18.7, 10.2 and 9.6; 64 with q6_k 2,560 x 9,728 46, 32 and 27. Parts for four
+// workgroups a CU: 37.
 inline int tile_splits(int64_t t, int64_t n, int64_t k) {
     const int64_t tiles = (t + 63) / 64 * ((n + 31) / 32), stages = (k / 32 + 7) / 8;
-    int64_t s = 512 / tiles < 4 ? 512 / tiles : 4;
+    int64_t s = 512 / tiles < 8 ? 512 / tiles : 8;
     s = s < stages ? s : stages;
     if (s < 2) return 1;
     const int64_t per = (stages + s - 1) / s;

@@ -44,11 +44,11 @@ hipError_t few_rows(int t, const LinearArgs& a, const FewPlan& p, hipStream_t st
     }
 }
 
-template <int TYPE, int BM, int BN, int WM, int WN, int WK, int G, int D>
+template <int TYPE, int BM, int BN, int WM, int WN, int WK, int G>
 hipError_t tile(const LinearArgs& a, hipStream_t st) {
     const int64_t tiles = ((a.t + BM - 1) / BM) * ((a.n + BN - 1) / BN) * a.splits;
     // a multiple of the 8 XCDs: each takes a run of tiles
-    return launch_kernel(k_linear_tile<TYPE, BM, BN, WM, WN, WK, G, D>, dim3((unsigned)((tiles + 7) / 8 * 8)),
+    return launch_kernel(k_linear_tile<TYPE, BM, BN, WM, WN, WK, G>, dim3((unsigned)((tiles + 7) / 8 * 8)),
                          dim3(64 * WM * WN * WK), 0, st, a);
 }
 
@@ -107,16 +107,15 @@ hipError_t launch_linear(const LinearArgs& a, void* work, hipStream_t st) {
         if (p16.blocks >= 256 && few_lds<TYPE>(p16, t, a.k) <= 80 * 1024) return few_rows<TYPE, 16>(t, a, p16, st);
         if (few_lds<TYPE>(p64, t, a.k) <= 160 * 1024) return few_rows<TYPE, 64>(t, a, p64, st);
     }
-    if (takes_matrix(a.t, a.n)) return takes_f16(a.dst_type, a.t, a.n, a.k) ? matrix16<TYPE>(a, work, st) : matrix<TYPE>(a, work, st);
-    // Up to 64 rows in one tile, so that the weight is decoded once; four waves
-    // share its groups. Eight waves, 64 columns, halve what each does to stage the
-    // rows: 64 rows with q4_k 9,728 x 2,560 24 us where 32 columns take 28, with
-    // q6_k 2,560 x 9,728 36 and 46; a narrow weight makes too few such tiles (61
-    // rows with q8_0 1,024 x 2,560: 14.0 and 12.4), and to 32 rows they are no
-    // faster (q6_k 151,936 x 2,560, 16 rows: 261 and 211).
-    const hipError_t e = a.t <= 32      ? tile<TYPE, 32, 32, 1, 1, 4, 8, 3>(a, st)
-                         : a.n >= 2048 ? tile<TYPE, 64, 64, 1, 2, 4, 8, 2>(a, st)
-                                       : tile<TYPE, 64, 32, 1, 1, 4, 8, 2>(a, st);
+    if (takes_matrix(a.t, a.n, a.k)) return takes_f16(a.dst_type, a.t, a.n, a.k) ? matrix16<TYPE>(a, work, st) : matrix<TYPE>(a, work, st);
+    // Up to 64 rows in one tile, so that the weight is decoded once. 64 columns
+    // halve what each thread does to stage the rows (64 rows with q4_k 9,728 x 2,560
+    // 21.8 us, 32 columns 24.2; q6_k 2,560 x 9,728 31.7 and 34.5), 32 make enough
+    // tiles of a narrow weight (61 rows with q8_0 1,024 x 2,560 10.2 us, 64 columns
+    // 11.6) and are faster to 32 rows (16 with q6_k 151,936 x 2,560 184 and 237).
+    const hipError_t e = a.t <= 32      ? tile<TYPE, 32, 32, 1, 1, 4, 8>(a, st)
+                         : a.n >= 2048 ? tile<TYPE, 64, 64, 2, 2, 2, 8>(a, st)
+                                       : tile<TYPE, 64, 32, 2, 1, 2, 8>(a, st);
     return e != hipSuccess || a.splits == 1 ? e : launch_join(a, st);
 }
 

@@ -64,7 +64,7 @@ Work work_of(int type, int dst_type, int64_t n, int64_t k, int64_t t, int max_ra
     using qsl::round_up;
     Work w{};
     if (n == 0 || t == 0) return w;
-    const bool matrix = qsl::takes_matrix(t, n);
+    const bool matrix = qsl::takes_matrix(t, n, k);
     if (max_rank > 0 && matrix) {
         w.lo = round_up(t * max_rank * 2, 256);
         w.unit = 2 * w.lo;
@@ -181,7 +181,7 @@ int qs_packed_linear(int ggml_type, const void* weight, int64_t n, int64_t k, co
         a.b_type = adapters->type;
         a.ldv = rank;
         a.adapters = s.adapters;
-        if (qsl::takes_matrix(t, n)) a.v_hi = s.hi, a.v_lo = s.lo, a.v_unit = s.unit;
+        if (qsl::takes_matrix(t, n, k)) a.v_hi = s.hi, a.v_lo = s.lo, a.v_unit = s.unit;
         else if (t > qsl::FEW_ROWS) a.delta = s.delta;
         else a.v = s.v;
     }

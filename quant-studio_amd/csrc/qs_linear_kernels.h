@@ -286,18 +286,18 @@ struct Tile {
 
 // A tile of BM rows by BN weight rows. The workgroup's WM x WN x WK waves
 // stage G groups of 32 values at a time: the weight's are decoded to bytes by
-// a thread a group, the rows' copied; the bytes of the next D stages are in
-// flight while one is multiplied (what a CU has in flight is what bounds a
-// weight read once). WM x WN waves split the tile, WK the
+// a thread a group, the rows' copied; the bytes of the next stage are in
+// flight while one is multiplied (two or three stages ahead, whose registers
+// leave fewer waves, took 5 to 15% longer). WM x WN waves split the tile, WK the
 // groups (their sums are joined in LDS at the end, in order). A group's 16
 // products a lane are scaled by an outer product of the scales, d * s, that a
 // matrix instruction makes from three bf16 pieces of each, exact to f32.
 // Bound by the turn of a stage: decode and copies to LDS, a barrier, products, a
-// barrier, one after another (64 rows with q4_k 9,728 x 2,560, 152 workgroups:
-// vector instructions take 0.18 of the SIMDs' cycles, matrix ones 0.05). That
-// product 24 us, 131 TFLOP/s;
-// 16 rows 16.5 us; 128 with q6_k 151,936 x 2,560 630 us, 158 TFLOP/s.
-template <int TYPE, int BM, int BN, int WM, int WN, int WK, int G, int D>
+// barrier, one after another: with 64 rows of q4_k 9,728 x 2,560 vector
+// instructions take about a fifth of the SIMDs' cycles, matrix ones a twentieth.
+// 64 rows 22 us, 146 TFLOP/s; 16 rows 16.6 us; 128 with q6_k 151,936 x 2,560 553
+// us, 180 TFLOP/s.
+template <int TYPE, int BM, int BN, int WM, int WN, int WK, int G>
 __global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_linear_tile(LinearArgs a) {
     using S = Tile<TYPE, BM, BN, WM, WN, WK, G>;
     constexpr int THREADS = S::THREADS, SUB = S::SUB, UM = S::UM, UN = S::UN;
@@ -325,9 +325,9 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_linear_tile(LinearArgs
     const uint8_t* wrow[S::WTASKS];
     const int8_t* xrow[S::XTASKS];
     const float* srow[S::XTASKS];
-    Raw<TYPE> wraw[D][S::WTASKS];
-    uint4 xraw[D][S::XTASKS][2];
-    float sraw[D][S::XTASKS];
+    Raw<TYPE> wraw[S::WTASKS];
+    uint4 xraw[S::XTASKS][2];
+    float sraw[S::XTASKS];
 #pragma unroll
     for (int j = 0; j < S::WTASKS; j++) {
         const int64_t n = n0 + (tid + j * THREADS) / G;
@@ -340,32 +340,32 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_linear_tile(LinearArgs
         srow[j] = a.s + (t < a.t ? t : a.t - 1) * groups;
     }
     // past the last group: its bytes again, to be placed with scales of 0
-    auto load = [&](int d, int g0) {
+    auto load = [&](int g0) {
 #pragma unroll
         for (int j = 0; j < S::WTASKS; j++) {
             const int i = tid + j * THREADS, g = g0 + i % G < groups ? g0 + i % G : groups - 1;
-            if (BN * G % THREADS == 0 || i < BN * G) qsd::load_row_group<TYPE>(wrow[j], g, wraw[d][j]);
+            if (BN * G % THREADS == 0 || i < BN * G) qsd::load_row_group<TYPE>(wrow[j], g, wraw[j]);
         }
 #pragma unroll
         for (int j = 0; j < S::XTASKS; j++) {
             const int i = tid + j * THREADS, g = g0 + i % G < groups ? g0 + i % G : groups - 1;
             if (BM * G % THREADS == 0 || i < BM * G) {
                 const uint4* p = reinterpret_cast<const uint4*>(xrow[j] + 32 * g);
-                xraw[d][j][0] = p[0];
-                xraw[d][j][1] = p[1];
-                sraw[d][j] = srow[j][g];
+                xraw[j][0] = p[0];
+                xraw[j][1] = p[1];
+                sraw[j] = srow[j][g];
             }
         }
     };
     auto put = [&](int at, uint4 v) { *reinterpret_cast<uint4*>(lds + at) = v; };
-    auto put_stage = [&](int d, int g0) {
+    auto put_stage = [&](int g0) {
 #pragma unroll
         for (int j = 0; j < S::WTASKS; j++) {
             const int i = tid + j * THREADS, g = i % G, r = i / G;
             if (!(BN * G % THREADS == 0 || i < BN * G)) continue;
             const bool live = g0 + g < groups;
             Group<TYPE> w;
-            qsd::decode_group<TYPE>(wraw[d][j], qsd::group_in_block<TYPE>(live ? g0 + g : groups - 1), grid, w);
+            qsd::decode_group<TYPE>(wraw[j], qsd::group_in_block<TYPE>(live ? g0 + g : groups - 1), grid, w);
             put(S::WQ + g * S::WQS + r * 16, uint4{w.c[0], w.c[1], w.c[2], w.c[3]});
             put(S::WQ + g * S::WQS + (BN + r) * 16, uint4{w.c[4], w.c[5], w.c[6], w.c[7]});
 #pragma unroll
@@ -378,8 +378,8 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_linear_tile(LinearArgs
         for (int j = 0; j < S::XTASKS; j++) {
             const int i = tid + j * THREADS, g = i % G, r = i / G;
             if (!(BM * G % THREADS == 0 || i < BM * G)) continue;
-            const uint4 lo = xraw[d][j][0], hi = xraw[d][j][1];
-            const float s = g0 + g < groups ? sraw[d][j] : 0.0f;
+            const uint4 lo = xraw[j][0], hi = xraw[j][1];
+            const float s = g0 + g < groups ? sraw[j] : 0.0f;
             put(S::XQ + g * S::XQS + r * 16, lo);
             put(S::XQ + g * S::XQS + (BM + r) * 16, hi);
             put(S::XP + g * S::XPS + r * 16, row_slots(s));
@@ -454,16 +454,11 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_linear_tile(LinearArgs
                 __builtin_fmaf(__int_as_float(p[s % 2][i]) - INT_BIAS, ds[s % 2][i], acc[u / UN][u % UN][i]);
     };
 
-#pragma unroll
-    for (int d = 0; d < D; d++) load(d, begin + d * G);
-    for (int from = begin; from < end; from += D * G)
-#pragma unroll
-    for (int d = 0; d < D; d++) {
-        const int g0 = from + d * G;
-        if (g0 >= end) break;
+    load(begin);
+    for (int g0 = begin; g0 < end; g0 += G) {
         lds_barrier();
-        put_stage(d, g0);
-        load(d, g0 + D * G);
+        put_stage(g0);
+        load(g0 + G);
         lds_barrier();
         // The matrix instructions of a step are issued before the vector ones
         // of the step before it, so a wave's vector work covers their latency.

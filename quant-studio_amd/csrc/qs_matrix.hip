@@ -56,7 +56,7 @@ hipError_t product16(const Matrix16Args& a, hipStream_t st) {
 
 template <int TYPE>
 hipError_t adapters(const AdapterArgs& a, hipStream_t st) {
-    if (takes_matrix(a.t, a.n)) {
+    if (takes_matrix(a.t, a.n, a.k)) {
         const unsigned ranks = (unsigned)((a.ldv + 31) / 32);
         const hipError_t e = launch_kernel(k_adapter_many<TYPE>, dim3((unsigned)((a.t + 31) / 32), ranks, (unsigned)a.parts),
                                            dim3(512), 0, st, a);

@@ -13,11 +13,12 @@ from test_gpu_packed_linear import DEV, TORCH, check, make_adapters, rows_on
 
 pytestmark = pytest.mark.gpu
 
-# tiles that decode the weight, of 32 and of 64 columns, in 1 to 4 parts with a
-# shorter last one; above 64 or 192 rows, by the columns, laid-out factors in
-# tiles of 64 x 64, of 128 x 128 by eight waves and by four
+# tiles that decode the weight, of 32 and of 64 columns, in 1 to 8 parts with a
+# shorter last one; above 128 rows and a round of such tiles, or 512 rows,
+# laid-out factors in tiles of 64 x 64, of 128 x 128 by eight waves and by four
 SHAPES = [(12, 70, 4352), (33, 2047, 768), (61, 1024, 2560), (64, 2048, 512), (65, 2050, 1312), (100, 4100, 2336),
-          (128, 2304, 1056), (70, 8200, 544), (150, 8192, 512), (192, 1500, 1056), (193, 600, 800),
+          (128, 2304, 1056), (70, 8200, 544), (150, 8192, 512), (192, 1500, 1056), (193, 600, 800), (140, 8300, 256),
+          (300, 1500, 544), (500, 2048, 256), (513, 640, 288), (700, 1030, 544),
           (129, 515, 1312), (1030, 2100, 256), (2000, 3100, 96), (400, 1000, 800)]
 
 
