@@ -35,7 +35,8 @@ def test_every_format(qs, i, qtype):
     check(qs.packed_linear(rows_on(qs, q, s), w), *want, f"{qtype} {t}x{n}x{k}")
 
 
-@pytest.mark.parametrize("t,n,k", [(509, 2560, 9728), (300, 2050, 10752), (1000, 1030, 7680), (250, 10000, 2560), (2049, 1281, 2816)])
+@pytest.mark.parametrize("t,n,k", [(509, 2560, 9728), (300, 2050, 10752), (1000, 1030, 7680), (250, 10000, 2560), (2049, 1281, 2816),
+                                   (2329, 2497, 1280), (1054, 957, 6656)])
 def test_tiles_and_parts(qs, t, n, k):
     """Long rows, whose groups are split over workgroups, in parts with a shorter last one."""
     print(t, n, k, flush=True)
@@ -47,7 +48,7 @@ def test_tiles_and_parts(qs, t, n, k):
 
 
 @pytest.mark.parametrize("dtype,t,n,k", [("bf16", 2000, 3300, 1024), ("f16", 700, 9300, 1024), ("bf16", 509, 2560, 9728),
-                                         ("f16", 300, 2050, 10752), ("f16", 2049, 2560, 1280)])
+                                         ("f16", 300, 2050, 10752), ("f16", 2049, 2560, 1280), ("bf16", 140, 4437, 14592)])
 def test_adapters(qs, dtype, t, n, k):
     """Packed sequences and mixed rows; ranks from 1 to 128; a NaN stays in its adapter's rows."""
     q, s, w, (want, bound) = case(qs, "q4_k", t, n, k)
