@@ -2,7 +2,7 @@
 //     y[t] += B[id] (scale * A[id] x[t]),   id = ids[t]
 // First v = scale * A x for every row (k_adapter_few; k_adapter_many
 // and k_adapter_join), then
-// B v: for up to 8 rows in the product's own lanes (adapter_sum), for tiles by a
+// B v: for dot products in the product's own lanes (adapter_sum), for tiles by a
 // kernel that writes the sums for the product to add (k_adapter_delta), for
 // laid-out factors by matrix instructions on the product's tile (add_adapters).
 #pragma once

@@ -9,9 +9,19 @@
 
 namespace qsl {
 
-// rows up to which a product takes dot products; above, tiles that decode the
-// weight themselves, or both factors laid out for the matrix units (takes_matrix)
-constexpr int64_t FEW_ROWS = 8;
+// A few rows take dot products (takes_few), more tiles that decode the weight
+// themselves, or both factors laid out for the matrix units (takes_matrix).
+
+constexpr int few_record(int t) { return 3 * t + (3 * t + 1) % 2; }     // 16s of a group of x
+constexpr int FEW_LDS = 160 * 1024, FEW_GRID = 4096;    // bytes of a CU, and of the largest code book
+// Up to 8 rows, 4 where they are long, of which four weight rows and the rows
+// themselves fit in LDS. us, and of a tile: 8 rows with q6_k 151,936 x 2,560 150 and
+// 178, q4_k 9,728 x 2,560 16.1 and 15.8, q4_0 1,024 x 2,560 7.7 and 7.9, q6_k 2,560 x
+// 9,728 29 and 20, 5 of those 22 and 20.
+inline bool takes_few(int64_t row_bytes, int64_t t, int64_t k) {
+    if (t > (k > 4096 ? 4 : 8)) return false;
+    return 4 * row_bytes + 48 + k / 32 * few_record(t <= 6 ? (int)t : 8) * 16 + FEW_GRID <= FEW_LDS;
+}
 
 struct LinearArgs {
     const uint8_t* w;       // n rows of row_bytes
@@ -27,7 +37,7 @@ struct LinearArgs {
     int64_t ldv;
     int32_t adapters;
     int b_type;             // QS_SRC_F16 / QS_SRC_BF16
-    const float* v;         // to FEW_ROWS rows: scale * A x, t rows of ldv
+    const float* v;         // dot products: scale * A x, t rows of ldv
     const float* delta;     // tiles: B v, t rows of n
     float* parts;           // of a product split over its groups: splits x t rows of n
     int splits;
@@ -180,6 +190,7 @@ struct AdapterArgs {
     int64_t k, n, t, ldv;
     int32_t adapters;
     int parts;
+    bool few;                   // the product takes v itself
 };
 // Parts that the rows' values are split into: up to 1,024 workgroups, where a
 // row has 512 values or more for each. The CUs hold 512 at a time; parts half as

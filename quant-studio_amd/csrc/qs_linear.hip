@@ -96,16 +96,15 @@ hipError_t matrix16(const LinearArgs& a, void* work, hipStream_t st) {
 
 template <int TYPE>
 hipError_t launch_linear(const LinearArgs& a, void* work, hipStream_t st) {
-    // Up to 8 rows: dot products (8 rows, us, and as a tile: q6_k 151,936 x 2,560
-    // 150 and 206, q4_k 9,728 x 2,560 16.3 and 16.3, q6_k 2,560 x 9,728 29 and 27).
     // 16 lanes to a weight row, or a wave where that leaves too few workgroups or
     // rows too long for LDS (a row with q4_k, us for 16 lanes and 64: 9,728 x 2,560
     // 7.2 and 10.1; 4,096 x 2,560 4.8 and 5.2; 1,024 x 2,560 4.3 and 3.9).
-    if (a.t <= FEW_ROWS) {
+    if (takes_few(a.row_bytes, a.t, a.k)) {
+        static_assert(Format<TYPE>::GRID * 2 <= FEW_GRID, "the code book's place");
         const int t = a.t <= 6 ? (int)a.t : 8;
         const FewPlan p16 = few_plan<TYPE, 16>(a), p64 = few_plan<TYPE, 64>(a);
         if (p16.blocks >= 256 && few_lds<TYPE>(p16, t, a.k) <= 80 * 1024) return few_rows<TYPE, 16>(t, a, p16, st);
-        if (few_lds<TYPE>(p64, t, a.k) <= 160 * 1024) return few_rows<TYPE, 64>(t, a, p64, st);
+        return few_rows<TYPE, 64>(t, a, p64, st);
     }
     if (takes_matrix(a.t, a.n, a.k)) return takes_f16(a.dst_type, a.t, a.n, a.k) ? matrix16<TYPE>(a, work, st) : matrix<TYPE>(a, work, st);
     // Up to 64 rows in one tile, so that the weight is decoded once. 64 columns

@@ -59,12 +59,14 @@ int bad_sizes(const Entry& e, int64_t n, int64_t k, int64_t t) {
 struct Work {
     int64_t v, delta, lo, unit, layouts, sums, bytes;   // offsets; v is hi where there is a lo, sums a split product's
     int splits, parts;
+    bool few;
 };
-Work work_of(int type, int dst_type, int64_t n, int64_t k, int64_t t, int max_rank) {
+Work work_of(int type, int64_t row_bytes, int dst_type, int64_t n, int64_t k, int64_t t, int max_rank) {
     using qsl::round_up;
     Work w{};
     if (n == 0 || t == 0) return w;
-    const bool matrix = qsl::takes_matrix(t, n, k);
+    const bool matrix = qsl::takes_matrix(t, n, k), few = qsl::takes_few(row_bytes, t, k);
+    w.few = few;
     if (max_rank > 0 && matrix) {
         w.lo = round_up(t * max_rank * 2, 256);
         w.unit = 2 * w.lo;
@@ -72,12 +74,12 @@ Work work_of(int type, int dst_type, int64_t n, int64_t k, int64_t t, int max_ra
         w.parts = qsl::adapter_parts(t, k, max_rank);
     } else if (max_rank > 0) {
         w.delta = round_up(t * max_rank * 4, 256);
-        w.layouts = w.delta + (t > qsl::FEW_ROWS ? round_up(t * n * 4, 256) : 0);
+        w.layouts = w.delta + (few ? 0 : round_up(t * n * 4, 256));
     }
     const bool f16 = qsl::takes_f16(dst_type, t, n, k);
     const qsl::MatrixPlan plan = qsl::matrix_plan(type, f16, n, k, t);
     w.splits = f16                                ? qsl::choose16(max_rank > 0, t, n, k, plan.slice < n ? 1 : qsl::MOST_PARTS).splits
-               : matrix || t <= qsl::FEW_ROWS ? 1
+               : matrix || few ? 1
                                                   : qsl::tile_splits(t, n, k);
     w.sums = w.layouts + (matrix ? qsl::round_up(plan.bytes(), 256) : 0);
     w.bytes = w.sums + (w.splits > 1 ? w.splits * t * n * 4 : 0);
@@ -101,7 +103,7 @@ int64_t qs_packed_linear_workspace(int ggml_type, int64_t n, int64_t k, int64_t 
         return fail(QS_EINVAL, "max_rank %d must be a multiple of 8 in 0..%lld", max_rank, (long long)kMaxRank);
     if (!dst_size(dst_type))
         return fail(QS_EINVAL, "unsupported destination type %d (F32=0, F16=1, BF16=30)", dst_type);
-    return work_of(ggml_type, dst_type, n, k, t, max_rank).bytes;
+    return work_of(ggml_type, e->row_bytes(k), dst_type, n, k, t, max_rank).bytes;
 }
 
 int qs_packed_linear(int ggml_type, const void* weight, int64_t n, int64_t k, const int8_t* q, const float* scales,
@@ -147,7 +149,7 @@ int qs_packed_linear(int ggml_type, const void* weight, int64_t n, int64_t k, co
         if (off16(adapters->a) || off16(adapters->b) || off4(ids))
             return fail(QS_EINVAL, "adapter a and b must be 16-byte aligned, ids 4-byte");
     }
-    const Work work = work_of(ggml_type, dst_type, n, k, t, rank);
+    const Work work = work_of(ggml_type, e->row_bytes(k), dst_type, n, k, t, rank);
     if (work.bytes && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256 || workspace_bytes < work.bytes))
         return fail(QS_EINVAL, "workspace holds %lld bytes at %p, %lld needed, 256-byte aligned",
                     (long long)workspace_bytes, workspace, (long long)work.bytes);
@@ -173,6 +175,7 @@ int qs_packed_linear(int ggml_type, const void* weight, int64_t n, int64_t k, co
         s.unit = reinterpret_cast<float*>(base + work.unit);
         s.sums = reinterpret_cast<float*>(base + work.layouts);
         s.parts = work.parts;
+        s.few = work.few;
         const hipError_t r = qsl::launch_adapters(adapters->type, s, st);
         if (r != hipSuccess) return fail(QS_EIO, "packed_linear: launch failed: %s", hipGetErrorString(r));
         a.ids = ids;
@@ -182,8 +185,8 @@ int qs_packed_linear(int ggml_type, const void* weight, int64_t n, int64_t k, co
         a.ldv = rank;
         a.adapters = s.adapters;
         if (qsl::takes_matrix(t, n, k)) a.v_hi = s.hi, a.v_lo = s.lo, a.v_unit = s.unit;
-        else if (t > qsl::FEW_ROWS) a.delta = s.delta;
-        else a.v = s.v;
+        else if (work.few) a.v = s.v;
+        else a.delta = s.delta;
     }
     a.parts = reinterpret_cast<float*>(base + work.sums);
     a.splits = work.splits;

@@ -84,7 +84,6 @@ QS_DEV float sum16(float v) {
 
 // The LDS of a workgroup of k_linear_few: the bytes of its weight rows, up to
 // whole 16s at both ends, then x, then the grid.
-constexpr int few_record(int t) { return 3 * t + (3 * t + 1) % 2; }     // 16s of a group of x
 struct FewPlan {
     int w_bytes;
     int64_t blocks;         // of a workgroup's weight rows

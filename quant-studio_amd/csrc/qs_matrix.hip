@@ -63,7 +63,7 @@ hipError_t adapters(const AdapterArgs& a, hipStream_t st) {
         return e != hipSuccess ? e : launch_kernel(k_adapter_join<TYPE>, dim3((unsigned)((a.t + 15) / 16), ranks), dim3(256), 0, st, a);
     }
     const hipError_t e = launch_kernel(k_adapter_few<TYPE>, dim3((unsigned)a.t, (unsigned)(a.ldv / 8)), dim3(256), 0, st, a);
-    if (e != hipSuccess || a.t <= FEW_ROWS) return e;
+    if (e != hipSuccess || a.few) return e;
     return launch_kernel(k_adapter_delta<TYPE>, dim3((unsigned)((a.n + 255) / 256), (unsigned)a.t), dim3(256), 0, st, a);
 }
 
