@@ -164,21 +164,36 @@ __global__ __launch_bounds__(256) void k_q8_values(const int8_t* q, const float*
     }
 }
 
+// Rows of a launch: a wave to a row, the threads of a launch are under 2^32.
+constexpr int64_t MOST_ROWS = INT64_C(1) << 24;
+
 template <int SRC>
-hipError_t launch_norm(const NormArgs& a, hipStream_t st) {
+hipError_t launch_norm(const NormArgs& all, hipStream_t st) {
     // A wave per row where rows fill the 1,024 SIMDs several times (us with 64, 256
     // and 1,024 lanes, bf16 with a residual: 8,191 x 2,560 24.5, 27.7, 48; 4,096 x
     // 1,024 8.2, 10.3, 22), else a workgroup each (2,048 x 9,728 31, 24.5, 26; 1,024
     // x 2,560 8.2, 6.6, 8.5), a large one where they are few and long (64 x 2,560
     // 7.0, 4.1, 3.6; 1 x 2,560 6.2, 3.8, 3.2; 333 x 1,024 4.2, 3.6, 4.0).
-    const int p = a.rows >= 4096 ? 64 : a.rows <= 256 && a.k > 2048 ? 1024 : 256;
+    const int p = all.rows >= 4096 ? 64 : all.rows <= 256 && all.k > 2048 ? 1024 : 256;
     const int rows = p > 256 ? 1 : 256 / p;
-    const dim3 grid((unsigned)((a.rows + rows - 1) / rows));
-    const size_t lds = (size_t)rows * (a.k / 32) * 4;
+    const size_t lds = (size_t)rows * (all.k / 32) * 4;
+    constexpr int64_t esz = SRC == qs::SRC_F32 ? 4 : 2;
     using qs_host::launch_kernel;
-    if (p == 64) return launch_kernel(k_rms_norm_q8<SRC, 64>, grid, dim3(256), lds, st, a);
-    if (p == 256) return launch_kernel(k_rms_norm_q8<SRC, 256>, grid, dim3(256), lds, st, a);
-    return launch_kernel(k_rms_norm_q8<SRC, 1024>, grid, dim3(1024), lds, st, a);
+    for (int64_t first = 0; first < all.rows; first += MOST_ROWS) {
+        NormArgs a = all;
+        a.rows = all.rows - first < MOST_ROWS ? all.rows - first : MOST_ROWS;
+        a.x = static_cast<const char*>(all.x) + first * all.stride * esz;
+        if (all.residual) a.residual = static_cast<const char*>(all.residual) + first * all.rstride * esz;
+        if (all.sum) a.sum = static_cast<char*>(all.sum) + first * all.k * esz;
+        a.q = all.q + first * all.k;
+        a.s = all.s + first * (all.k / 32);
+        const dim3 grid((unsigned)((a.rows + rows - 1) / rows));
+        const hipError_t e = p == 64    ? launch_kernel(k_rms_norm_q8<SRC, 64>, grid, dim3(256), lds, st, a)
+                             : p == 256 ? launch_kernel(k_rms_norm_q8<SRC, 256>, grid, dim3(256), lds, st, a)
+                                        : launch_kernel(k_rms_norm_q8<SRC, 1024>, grid, dim3(1024), lds, st, a);
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 }  // namespace
