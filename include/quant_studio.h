@@ -198,19 +198,22 @@ typedef struct qs_adapters {
  * (max_rank 0: without adapters); 0 where it needs none. */
 int64_t qs_packed_linear_workspace(int ggml_type, int64_t n, int64_t k, int64_t t, int dst_type, int max_rank);
 
+/* Or'ed to a result's dst_type: codes are multiplied exactly at every size. */
+#define QS_EXACT 0x100
+
 /* y = x W^T for t 8-bit rows x and a packed weight W of n rows of k values (as
  * qs_quantize() writes them: n contiguous rows of qs_row_bytes(k)), and for
  * rows with an adapter  y += scale * B (A x).
  *   weight:    4-byte aligned, 2-byte where the type's blocks are not whole words
- *   dst:       t contiguous rows of n values of dst_type (QS_SRC_*)
+ *   dst:       t contiguous rows of n values of dst_type (QS_SRC_*, QS_EXACT)
  *   adapters, ids: both or neither; ids[r] (device) is the adapter of row r,
  *              any value outside 0..count-1 means none
  *   workspace: qs_packed_linear_workspace() bytes, 256-byte aligned, used by
  *              this call alone until it is done; may be NULL where that is 0
- * Codes are multiplied exactly, scales applied in f32, y rounded once; but a
- * bf16 result of more than 128 rows with k >= 1024 and t*n*k >= 3 * 2^31 (where
- * few tiles do not make the exact form the faster) takes both factors' values
- * rounded to f16 (11 bits; rows scaled by powers of two first, so that nothing
+ * Codes are multiplied exactly, scales applied in f32, y rounded once; but
+ * without QS_EXACT a bf16 result of more than 128 rows with k >= 1024 and
+ * t*n*k >= 3 * 2^31 (where few tiles do not make the exact form the faster)
+ * takes both factors' values rounded to f16 (11 bits; rows scaled by powers of two first, so that nothing
  * overflows), whose error is some 1% of that of the result's own rounding. The
  * result of a row does not depend on timing; it may differ in the last bits of
  * f32 with t and n, and with adapters (another split of the sum). t is at most

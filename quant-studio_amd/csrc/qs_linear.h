@@ -30,6 +30,7 @@ struct LinearArgs {
     void* dst;              // t rows of n values of dst_type
     int64_t row_bytes, n, k, t;
     int dst_type;           // QS_SRC_*
+    bool f16;               // laid-out factors are rounded to f16 (takes_f16)
     // low-rank adapters: ids is null without them
     const int32_t* ids;     // adapter of each row; outside 0..adapters-1: none
     const int32_t* off;     // adapters + 1 rank offsets, multiples of 8
@@ -92,15 +93,15 @@ inline bool takes_matrix(int64_t t, int64_t n, int64_t k) {
     return t > 512 || (t > 128 && tiles > (k <= 4096 ? 256 : 128));
 }
 
-// Large products whose result is bf16 (8 bits) take factors of f16 (11 bits);
-// everything else exact codes. F16 factors are laid out in two launches and twice
+// Large products whose result is bf16 (8 bits) take factors of f16 (11 bits) where
+// the caller leaves that open (`dst` without QS_EXACT); everything else exact codes. F16 factors are laid out in two launches and twice
 // the bytes, and multiplied at up to 1.0 PFLOP/s where exact codes reach 0.62.
 // q4_k, us f16 and exact: 512 rows, 2,560 x 2,560 38 and 34; 2,048, 1,024 x 2,560
 // 42 and 38; 1,024, 2,560 x 2,560 42 and 50; 300, 9,728 x 2,560 55 and 56; 4,096,
 // 9,728 x 2,560 234 and 389. Rows under 1,024 values give neither time to start:
 // 2,000 rows, 3,000 x 256 19 and 19.
-inline bool takes_f16(int dst_type, int64_t t, int64_t n, int64_t k) {
-    return dst_type == QS_SRC_BF16 && takes_matrix(t, n, k) && k >= 1024 && t * n >= INT64_C(3) * (INT64_C(1) << 31) / k;
+inline bool takes_f16(int dst, int64_t t, int64_t n, int64_t k) {
+    return dst == QS_SRC_BF16 && takes_matrix(t, n, k) && k >= 1024 && t * n >= INT64_C(3) * (INT64_C(1) << 31) / k;
 }
 
 // Tiles of a product of laid-out factors, and the time measured for a round of

@@ -106,7 +106,7 @@ hipError_t launch_linear(const LinearArgs& a, void* work, hipStream_t st) {
         if (p16.blocks >= 256 && few_lds<TYPE>(p16, t, a.k) <= 80 * 1024) return few_rows<TYPE, 16>(t, a, p16, st);
         return few_rows<TYPE, 64>(t, a, p64, st);
     }
-    if (takes_matrix(a.t, a.n, a.k)) return takes_f16(a.dst_type, a.t, a.n, a.k) ? matrix16<TYPE>(a, work, st) : matrix<TYPE>(a, work, st);
+    if (takes_matrix(a.t, a.n, a.k)) return a.f16 ? matrix16<TYPE>(a, work, st) : matrix<TYPE>(a, work, st);
     // Up to 64 rows in one tile, so that the weight is decoded once. 64 columns
     // halve what each thread does to stage the rows (64 rows with q4_k 9,728 x 2,560
     // 21.8 us, 32 columns 24.2; q6_k 2,560 x 9,728 31.7 and 34.5), 32 make enough

@@ -37,7 +37,11 @@ bool off16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 != 0; }
 bool off4(const void* p) { return reinterpret_cast<uintptr_t>(p) % 4 != 0; }
 constexpr int64_t kMaxValues = INT64_C(1) << 34, kMaxRows = INT64_C(1) << 24, kMaxRank = 4096;
 
-int dst_size(int type) { return type == QS_SRC_F32 ? 4 : (type == QS_SRC_F16 || type == QS_SRC_BF16) ? 2 : 0; }
+// bytes of a result's value; `dst`: QS_SRC_*, alone or with QS_EXACT
+int dst_size(int dst) {
+    const int type = dst & ~QS_EXACT;
+    return type == QS_SRC_F32 ? 4 : (type == QS_SRC_F16 || type == QS_SRC_BF16) ? 2 : 0;
+}
 
 const Entry* find(int type) {
     for (const Entry& c : kEntries)
@@ -59,9 +63,9 @@ int bad_sizes(const Entry& e, int64_t n, int64_t k, int64_t t) {
 struct Work {
     int64_t v, delta, lo, unit, layouts, sums, bytes;   // offsets; v is hi where there is a lo, sums a split product's
     int splits, parts;
-    bool few;
+    bool few, f16;
 };
-Work work_of(int type, int64_t row_bytes, int dst_type, int64_t n, int64_t k, int64_t t, int max_rank) {
+Work work_of(int type, int64_t row_bytes, int dst, int64_t n, int64_t k, int64_t t, int max_rank) {
     using qsl::round_up;
     Work w{};
     if (n == 0 || t == 0) return w;
@@ -76,7 +80,7 @@ Work work_of(int type, int64_t row_bytes, int dst_type, int64_t n, int64_t k, in
         w.delta = round_up(t * max_rank * 4, 256);
         w.layouts = w.delta + (few ? 0 : round_up(t * n * 4, 256));
     }
-    const bool f16 = qsl::takes_f16(dst_type, t, n, k);
+    const bool f16 = w.f16 = qsl::takes_f16(dst, t, n, k);
     const qsl::MatrixPlan plan = qsl::matrix_plan(type, f16, n, k, t);
     w.splits = f16                                ? qsl::choose16(max_rank > 0, t, n, k, plan.slice < n ? 1 : qsl::MOST_PARTS).splits
                : matrix || few ? 1
@@ -133,7 +137,7 @@ int qs_packed_linear(int ggml_type, const void* weight, int64_t n, int64_t k, co
     a.n = n;
     a.k = k;
     a.t = t;
-    a.dst_type = dst_type;
+    a.dst_type = dst_type & ~QS_EXACT;
     hipStream_t st = static_cast<hipStream_t>(hip_stream);
     if ((adapters != nullptr) != (ids != nullptr)) return fail(QS_EINVAL, "adapters and ids go together");
     const bool adapted = adapters && adapters->count > 0 && adapters->max_rank > 0;
@@ -190,6 +194,7 @@ int qs_packed_linear(int ggml_type, const void* weight, int64_t n, int64_t k, co
     }
     a.parts = reinterpret_cast<float*>(base + work.sums);
     a.splits = work.splits;
+    a.f16 = work.f16;
     const hipError_t r = e->launch(a, base + work.layouts, st);
     if (r != hipSuccess) return fail(QS_EIO, "packed_linear: launch failed: %s", hipGetErrorString(r));
     return 0;

@@ -23,6 +23,7 @@ import ctypes
 torch = None            # imported with the library when a function is first called
 _L = None
 _TYPE_ID: dict = {}     # dtype -> source type id of the C ABI
+_EXACT = 0x100          # QS_EXACT of include/quant_studio.h
 
 
 def _lib():
@@ -281,20 +282,24 @@ class AdapterBank:
         return len(self.ranks)
 
 
-def packed_linear(rows, weight: PackedWeight, dtype=None, adapters: AdapterBank | None = None, ids=None, out=None):
+def packed_linear(rows, weight: PackedWeight, dtype=None, adapters: AdapterBank | None = None, ids=None, out=None,
+                  exact: bool = False):
     """y = x W^T, (t, n) of dtype (bfloat16 by default), for 8-bit rows x (or a
     float tensor (t, k), which goes through q8_rows first) and a packed weight.
 
     adapters, ids: each row's low-rank adapter beside the product,
     y[r] += scale * B (A x[r]) for adapter ids[r] (int32 (t,), on the rows'
     device; a value outside 0 .. len(adapters) - 1, such as -1, means none).
-    out: a contiguous (t, n) tensor to write instead of a new one."""
+    out: a contiguous (t, n) tensor to write instead of a new one.
+    exact: large products with a bfloat16 result round both factors to float16
+    (include/quant_studio.h has the sizes), which takes a half to two thirds of
+    the time; with exact=True they multiply exact codes, as all others do."""
     lib = _lib()
     if not isinstance(rows, Q8Rows):
         rows = q8_rows(rows)
     t, k, dev = rows.t, rows.k, rows._dev
     dtype = torch.bfloat16 if dtype is None else dtype
-    dst = _type_id(dtype, "packed_linear")
+    dst = _type_id(dtype, "packed_linear") | (_EXACT if exact else 0)
     n = weight.n
     if weight.k != k:
         raise ValueError(f"packed_linear: rows of {k} values, the weight's have {weight.k}")
