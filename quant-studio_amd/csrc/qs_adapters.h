@@ -7,6 +7,8 @@
 // laid-out factors by matrix instructions on the product's tile (add_adapters).
 #pragma once
 
+#include <type_traits>
+
 #include "qs_linear_kernels.h"
 
 namespace qsl {
@@ -120,18 +122,14 @@ QS_DEV uint4 codes16(uint2 c) {
     }
     return uint4{o[0], o[1], o[2], o[3]};
 }
-// v = hi + lo to 16 bits (BF16) or 22 (F16) of it
+// v to 16 bits, and what that leaves of it (exactly). Two pieces hold 16 (BF16) or
+// 22 (F16) bits of v, three of BF16 all 24.
 template <int TYPE>
-QS_DEV void split16(float v, uint16_t& hi, uint16_t& lo) {
-    if constexpr (TYPE == QS_SRC_BF16) {
-        const __bf16 h = (__bf16)v;
-        hi = __builtin_bit_cast(uint16_t, h);
-        lo = __builtin_bit_cast(uint16_t, (__bf16)(v - (float)h));
-    } else {
-        const _Float16 h = (_Float16)v;
-        hi = __builtin_bit_cast(uint16_t, h);
-        lo = __builtin_bit_cast(uint16_t, (_Float16)(v - (float)h));
-    }
+QS_DEV float piece16(float v, uint16_t& piece) {
+    using T = std::conditional_t<TYPE == QS_SRC_BF16, __bf16, _Float16>;
+    const T h = (T)v;
+    piece = __builtin_bit_cast(uint16_t, h);
+    return v - (float)h;
 }
 
 // A workgroup takes 32 rows and 32 ranks. Eight groups of 32 values at a time
@@ -223,7 +221,7 @@ __global__ __launch_bounds__(512) void k_adapter_many(AdapterArgs a) {
     }
 }
 
-// The parts' sums, scaled, as hi + lo: 16 lanes to a row's 32 ranks, two each.
+// The parts' sums, scaled, as hi + lo (+ rest, BF16): 16 lanes to a row's 32 ranks, two each.
 template <int TYPE>
 __global__ __launch_bounds__(256) void k_adapter_join(AdapterArgs a) {
     const int64_t t = (int64_t)blockIdx.x * 16 + threadIdx.x / 16;
@@ -252,14 +250,18 @@ __global__ __launch_bounds__(256) void k_adapter_join(AdapterArgs a) {
     }
     if (!live) return;
 #pragma unroll
-    for (int i = 0; i < 2; i++) split16<TYPE>(v[i], a.hi[t * a.ldv + r + i], a.lo[t * a.ldv + r + i]);
+    for (int i = 0; i < 2; i++) {
+        const int64_t at = t * a.ldv + r + i;
+        const float left = piece16<TYPE>(piece16<TYPE>(v[i], a.hi[at]), a.lo[at]);
+        if (TYPE == QS_SRC_BF16 && a.rest) piece16<TYPE>(left, a.rest[at]);
+    }
     if (TYPE == QS_SRC_F16 && r == r0) a.unit[t * ((a.ldv + 31) / 32) + r0 / 32] = unit;
 }
 
 // What add_adapters reads.
 struct AdapterTile {
     const int32_t *ids, *off;
-    const uint16_t *b, *hi, *lo;
+    const uint16_t *b, *hi, *lo, *rest;
     const float* unit;
     int64_t ldv;
     int32_t adapters;
@@ -271,8 +273,10 @@ struct AdapterTile {
 // so that a NaN in another's B does not reach them. Of WK waves that share the
 // sums of these units each takes every WK-th step: a step is bound by the
 // latency of what it reads (512 rows with q4_k 2,560 x 2,560, 4 adapters: the
-// product took 44 us with the steps in one wave of eight).
-template <int TYPE, int WK, int UM, int UN>
+// product took 44 us with the steps in one wave of eight). PIECES of v: with exact
+// codes as many as hold it to f32 (22 bits where B is f16), two with factors of f16,
+// whose result is bf16.
+template <int TYPE, int PIECES, int WK, int UM, int UN>
 QS_DEV void add_adapters(const AdapterTile& a, f32x16 (&y)[UM][UN], int64_t t0, int64_t rows, int64_t n0, int64_t n, int wk) {
     const int lane = threadIdx.x % 64, col = lane % 32, half = lane / 32;
     const int64_t units = (a.ldv + 31) / 32;
@@ -287,17 +291,17 @@ QS_DEV void add_adapters(const AdapterTile& a, f32x16 (&y)[UM][UN], int64_t t0, 
             const uint32_t mine = (uint32_t)__ballot(id == now), elements = mine >> (4 * half);
             left &= ~mine;
             const int o = a.off[now], rank = a.off[now + 1] - o;
-            const uint16_t* vh = a.hi + t * a.ldv;
-            const uint16_t* vl = a.lo + t * a.ldv;
+            const uint16_t* const from[3] = {a.hi + t * a.ldv, a.lo + t * a.ldv, PIECES > 2 ? a.rest + t * a.ldv : nullptr};
             for (int r0 = 0; r0 < rank; r0 += 32) {
                 if (step++ % WK != wk) continue;
-                uint4 h[2], l[2];
+                uint4 v[PIECES][2];
 #pragma unroll
                 for (int s = 0; s < 2; s++) {
                     const int r = r0 + 16 * s + 8 * half;
                     const bool live = id == now && r < rank;
-                    h[s] = live ? *reinterpret_cast<const uint4*>(vh + r) : uint4{0, 0, 0, 0};
-                    l[s] = live ? *reinterpret_cast<const uint4*>(vl + r) : uint4{0, 0, 0, 0};
+#pragma unroll
+                    for (int j = 0; j < PIECES; j++)
+                        v[j][s] = live ? *reinterpret_cast<const uint4*>(from[j] + r) : uint4{0, 0, 0, 0};
                 }
                 float unit[16];
                 if constexpr (TYPE == QS_SRC_F16)
@@ -316,8 +320,8 @@ QS_DEV void add_adapters(const AdapterTile& a, f32x16 (&y)[UM][UN], int64_t t0, 
                     for (int s = 0; s < 2; s++) {
                         const int r = r0 + 16 * s + 8 * half;
                         const uint4 w = r < rank ? *reinterpret_cast<const uint4*>(b + r) : uint4{0, 0, 0, 0};
-                        p = mfma16<TYPE>(l[s], w, p);
-                        p = mfma16<TYPE>(h[s], w, p);
+#pragma unroll
+                        for (int j = PIECES - 1; j >= 0; j--) p = mfma16<TYPE>(v[j][s], w, p);
                     }
 #pragma unroll
                     for (int i = 0; i < 16; i++) {

@@ -42,7 +42,8 @@ struct LinearArgs {
     const float* delta;     // tiles: B v, t rows of n
     float* parts;           // of a product split over its groups: splits x t rows of n
     int splits;
-    const uint16_t *v_hi, *v_lo;    // laid-out factors: scale * A x as hi + lo, t rows of ldv
+    // laid-out factors: scale * A x as hi + lo (+ rest: exact codes, BF16), t rows of ldv
+    const uint16_t *v_hi, *v_lo, *v_rest;
     const float* v_unit;            // and what that is to be multiplied by (F16), t rows of ldv / 32
 };
 
@@ -184,7 +185,7 @@ struct AdapterArgs {
     const int32_t *ids, *off;
     const float* scales;
     float* v;                   // [t][ldv]
-    uint16_t *hi, *lo;          // v as hi + lo in the adapters' type: [t][ldv]
+    uint16_t *hi, *lo, *rest;   // v as a sum of values of the adapters' type: [t][ldv]; rest is null for factors of f16
     float* unit;                // what that is to be multiplied by (F16): [t][ldv / 32]
     float* delta;               // [t][n]
     float* sums;                // [parts][t][ldv]

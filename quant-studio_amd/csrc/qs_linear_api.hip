@@ -61,7 +61,7 @@ int bad_sizes(const Entry& e, int64_t n, int64_t k, int64_t t) {
 // The workspace: what the adapters' products leave for the weight's, then the
 // factors as laid out.
 struct Work {
-    int64_t v, delta, lo, unit, layouts, sums, bytes;   // offsets; v is hi where there is a lo, sums a split product's
+    int64_t v, delta, lo, rest, unit, layouts, sums, bytes; // offsets; v is hi where there is a lo, sums a split product's
     int splits, parts;
     bool few, f16;
 };
@@ -71,16 +71,17 @@ Work work_of(int type, int64_t row_bytes, int dst, int64_t n, int64_t k, int64_t
     if (n == 0 || t == 0) return w;
     const bool matrix = qsl::takes_matrix(t, n, k), few = qsl::takes_few(row_bytes, t, k);
     w.few = few;
+    const bool f16 = w.f16 = qsl::takes_f16(dst, t, n, k);
     if (max_rank > 0 && matrix) {
         w.lo = round_up(t * max_rank * 2, 256);
-        w.unit = 2 * w.lo;
+        w.rest = 2 * w.lo;
+        w.unit = w.rest + (f16 ? 0 : w.lo);
         w.layouts = w.unit + round_up(t * ((max_rank + 31) / 32) * 4, 256);
         w.parts = qsl::adapter_parts(t, k, max_rank);
     } else if (max_rank > 0) {
         w.delta = round_up(t * max_rank * 4, 256);
         w.layouts = w.delta + (few ? 0 : round_up(t * n * 4, 256));
     }
-    const bool f16 = w.f16 = qsl::takes_f16(dst, t, n, k);
     const qsl::MatrixPlan plan = qsl::matrix_plan(type, f16, n, k, t);
     w.splits = f16                                ? qsl::choose16(max_rank > 0, t, n, k, plan.slice < n ? 1 : qsl::MOST_PARTS).splits
                : matrix || few ? 1
@@ -176,6 +177,7 @@ int qs_packed_linear(int ggml_type, const void* weight, int64_t n, int64_t k, co
         s.delta = reinterpret_cast<float*>(base + work.delta);
         s.hi = reinterpret_cast<uint16_t*>(base + work.v);
         s.lo = reinterpret_cast<uint16_t*>(base + work.lo);
+        s.rest = work.f16 ? nullptr : reinterpret_cast<uint16_t*>(base + work.rest);
         s.unit = reinterpret_cast<float*>(base + work.unit);
         s.sums = reinterpret_cast<float*>(base + work.layouts);
         s.parts = work.parts;
@@ -188,7 +190,7 @@ int qs_packed_linear(int ggml_type, const void* weight, int64_t n, int64_t k, co
         a.b_type = adapters->type;
         a.ldv = rank;
         a.adapters = s.adapters;
-        if (qsl::takes_matrix(t, n, k)) a.v_hi = s.hi, a.v_lo = s.lo, a.v_unit = s.unit;
+        if (qsl::takes_matrix(t, n, k)) a.v_hi = s.hi, a.v_lo = s.lo, a.v_rest = s.rest, a.v_unit = s.unit;
         else if (work.few) a.v = s.v;
         else a.delta = s.delta;
     }

@@ -256,7 +256,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_matrix16(Matrix16Args 
             for (int un = 0; un < UN; un++) acc[um][un][i] = acc[um][un][i] * unw[un] * unx;
         }
     if constexpr (ADAPT)
-        if (split == 0) add_adapters<ADAPT, WK>(adapter_tile(l), acc, t0 + wm * UM * 32, l.t, a.first + n0 + wn * UN * 32, l.n, wk);
+        if (split == 0) add_adapters<ADAPT, 2, WK>(adapter_tile(l), acc, t0 + wm * UM * 32, l.t, a.first + n0 + wn * UN * 32, l.n, wk);
     if constexpr (WK > 1) {
         static_assert(STAGE >= BM * BN * 4 / UN, "a column of units");
         join_waves<WK, WM * WN>(acc, reinterpret_cast<float*>(even), wk, wm * WN + wn);

@@ -1,0 +1,64 @@
+"""What a low-rank adapter adds, alone: on a weight of zeros, with one value in
+each row of A and one in each row of B, a result is a product of four numbers,
+so that what each path keeps of scale * A x shows in full."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+import packed_ref as ref
+from test_gpu_packed_linear import DEV, TORCH, rows_on
+
+pytestmark = pytest.mark.gpu
+
+# dot products; tiles whole, in parts and of 64 columns; laid-out factors in 64 x
+# 64, in 128 x 128 by eight waves and by four, two planes, minima
+PATHS = [("q8_0", 1, 33), ("q4_k", 8, 130), ("q8_0", 20, 70), ("q4_k", 64, 2100), ("q6_k", 300, 300), ("q8_0", 513, 300),
+         ("q4_k", 1030, 2100), ("q6_k", 4000, 2060), ("q2_k", 150, 9000)]
+K = 512
+
+
+def zero_weight(qs, qtype, n):
+    size = ref.BYTES[qtype] * (K // (32 if qtype == "q8_0" else 256))
+    return qs.PackedWeight(qtype, torch.zeros((n, size), dtype=torch.uint8, device=DEV))
+
+
+def picks(rng, n, ranks, dtype):
+    """Adapters of one value a row: (A, B, scale), and where and what they are."""
+    made, places = [], []
+    for i, r in enumerate(ranks):
+        a, b = torch.zeros((r, K)), torch.zeros((n, r))
+        col, av = rng.permutation(K)[:r], rng.uniform(0.5, 2, r)
+        rank, bv = rng.integers(0, r, n), rng.uniform(-2, 2, n)
+        a[np.arange(r), col] = torch.from_numpy(av).float()
+        b[np.arange(n), rank] = torch.from_numpy(bv).float()
+        made.append((a.to(dtype), b.to(dtype), 0.3 * (i + 1)))
+        places.append((col, rank))
+    return made, places
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("qtype,t,n", PATHS)
+def test_a_x_keeps_its_bits(qs, qtype, t, n, dtype):
+    """An f32 result. Roundings of a term, relative: the row's scale and the
+    adapter's (1 U each), B's product and the sums of its at most three pieces,
+    U each, twice that where a matrix instruction cuts: 8. With f16 adapters A x
+    is held to 22 bits: 4 U more."""
+    rng = np.random.default_rng(t)
+    made, places = picks(rng, n, [16, 5, 40], TORCH[dtype])
+    q, s = ref.random_rows(t, K, 2)
+    ids = (np.arange(t) % 4 - 1).astype(np.int32) if t > 1 else np.array([2], np.int32)
+    bank = qs.AdapterBank([(a.to(DEV), b.to(DEV), c) for a, b, c in made])
+    print(qtype, t, n, dtype, flush=True)
+    y = qs.packed_linear(rows_on(qs, q, s), zero_weight(qs, qtype, n), dtype=torch.float32, adapters=bank,
+                         ids=torch.from_numpy(ids).to(DEV)).double().cpu().numpy()
+    x, want = ref.rows64(q, s), np.zeros((t, n))
+    for i, ((a, b, c), (col, rank)) in enumerate(zip(made, places)):
+        a, b = a.double().numpy(), b.double().numpy()
+        v = np.float64(np.float32(c)) * x[:, col] * a[np.arange(len(col)), col]
+        want[ids == i] = (v[:, rank] * b[np.arange(n), rank])[ids == i]
+    off = np.abs(y - want) / np.maximum(np.abs(want), 1e-30)
+    print("off by", off.max() / ref.U, "of 2^-24")
+    assert (off <= (10 if dtype == "bf16" else 14) * ref.U).all()
