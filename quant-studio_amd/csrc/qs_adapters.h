@@ -123,13 +123,17 @@ QS_DEV uint4 codes16(uint2 c) {
     return uint4{o[0], o[1], o[2], o[3]};
 }
 // v to 16 bits, and what that leaves of it (exactly). Two pieces hold 16 (BF16) or
-// 22 (F16) bits of v, three of BF16 all 24.
+// 22 (F16) bits of v, three of BF16 all 24. An infinity leaves nothing, and a finite
+// v that bf16 would round to one is cut, so that the pieces' sum stays v.
 template <int TYPE>
 QS_DEV float piece16(float v, uint16_t& piece) {
     using T = std::conditional_t<TYPE == QS_SRC_BF16, __bf16, _Float16>;
-    const T h = (T)v;
+    T h = (T)v;
+    if constexpr (TYPE == QS_SRC_BF16)
+        if (fabsf(v) < __builtin_inff() && !(fabsf((float)h) < __builtin_inff()))
+            h = __builtin_bit_cast(__bf16, (uint16_t)(__float_as_uint(v) >> 16));
     piece = __builtin_bit_cast(uint16_t, h);
-    return v - (float)h;
+    return fabsf((float)h) < __builtin_inff() ? v - (float)h : 0.0f;
 }
 
 // A workgroup takes 32 rows and 32 ranks. Eight groups of 32 values at a time
@@ -238,12 +242,13 @@ __global__ __launch_bounds__(256) void k_adapter_join(AdapterArgs a) {
     v[0] = live ? v[0] * scale : 0.0f, v[1] = live ? v[1] * scale : 0.0f;
     float unit = 1.0f;
     if constexpr (TYPE == QS_SRC_F16) {
-        // a power of two that takes the largest of the 32 to f16's upper range
-        float top = fmaxf(fabsf(v[0]), fabsf(v[1]));
+        // a power of two that takes the largest finite one of the 32 to f16's upper range
+        const auto finite = [](float f) { return fabsf(f) < __builtin_inff() ? fabsf(f) : 0.0f; };
+        float top = fmaxf(finite(v[0]), finite(v[1]));
         top = fmaxf(top, __shfl_xor(top, 1)), top = fmaxf(top, __shfl_xor(top, 2));
         top = fmaxf(top, __shfl_xor(top, 4)), top = fmaxf(top, __shfl_xor(top, 8));
         int e = 0;
-        if (top > 0.0f && top < __builtin_inff()) (void)__builtin_frexpf(top, &e);
+        if (top > 0.0f) (void)__builtin_frexpf(top, &e);
         e = e < -80 ? -80 : e;
         unit = __builtin_ldexpf(1.0f, e - 15);
         v[0] = __builtin_ldexpf(v[0], 15 - e), v[1] = __builtin_ldexpf(v[1], 15 - e);

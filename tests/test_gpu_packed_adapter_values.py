@@ -62,3 +62,29 @@ def test_a_x_keeps_its_bits(qs, qtype, t, n, dtype):
     off = np.abs(y - want) / np.maximum(np.abs(want), 1e-30)
     print("off by", off.max() / ref.U, "of 2^-24")
     assert (off <= (10 if dtype == "bf16" else 14) * ref.U).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("qtype,t,n", PATHS)
+def test_the_largest_and_infinite_a_x(qs, qtype, t, n, dtype):
+    """A x that rounds to infinity in bf16 but is finite (its product with B is
+    too), and one that overflows: an infinity of B's sign, on every path."""
+    r = 8
+    a, b = torch.zeros((r, K)), torch.full((n, r), 2.0 ** -4)
+    a[0, 5], a[1, 70], a[2, 40] = 1.0, 100.0, 1.0
+    b[n // 2:] *= -1
+    bank = qs.AdapterBank([(a.to(DEV, TORCH[dtype]), b.to(DEV, TORCH[dtype]), 1.0)])
+    q, s = np.zeros((t, K), np.int8), np.ones((t, K // 32), np.float32)
+    q[:, 5] = 1
+    s[0, 0] = 3.4e38                    # finite; over bf16's largest number
+    if t > 2:
+        s[1, 2], q[1, 70], q[1, 40] = 3e38, 1, 3        # times 100 over f32's, with finite ones beside it
+        q[2, 5], q[2, 40] = 7, 1
+    print(qtype, t, n, dtype, flush=True)
+    y = qs.packed_linear(rows_on(qs, q, s), zero_weight(qs, qtype, n), dtype=torch.float32, adapters=bank,
+                         ids=torch.zeros((t,), dtype=torch.int32, device=DEV)).cpu().numpy()
+    sign = np.where(np.arange(n) < n // 2, 1.0, -1.0)
+    assert (np.abs(y[0] / (sign * (np.float32(3.4e38) / 16)) - 1) <= 14 * ref.U).all()
+    if t > 2:
+        assert (y[1] == sign * np.inf).all()
+        assert (y[2] == sign * 0.5).all() and (y[3:] == sign / 16).all()
