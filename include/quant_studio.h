@@ -217,7 +217,8 @@ int64_t qs_packed_linear_workspace(int ggml_type, int64_t n, int64_t k, int64_t 
  * overflows), whose error is some 1% of that of the result's own rounding. The
  * result of a row does not depend on timing; it may differ in the last bits of
  * f32 with t and n, and with adapters (another split of the sum). t is at most
- * 2^24, each of n*k, t*k and n*t at most 2^34. */
+ * 2^24, each of n*k, t*k and n*t at most 2^34. An infinite scale, of a row or of
+ * a weight's block, stands for no values: what it reaches is NaN. */
 int qs_packed_linear(int ggml_type, const void *weight, int64_t n, int64_t k, const int8_t *q, const float *scales,
                      int64_t t, int dst_type, void *dst, int64_t dst_bytes, const qs_adapters *adapters,
                      const int32_t *ids, void *workspace, int64_t workspace_bytes, void *hip_stream);

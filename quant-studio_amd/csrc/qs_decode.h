@@ -128,6 +128,12 @@ QS_DEV uint32_t load_u32(P p) {
 }
 QS_DEV float half_bits(uint32_t b) { return __half2float(__ushort_as_half((unsigned short)b)); }
 
+// A scale as it is, NaN where it is infinite: such a scale stands for no values.
+// Codes summed before it is applied would else give an infinity where the values
+// singly, infinities of both signs and inf * 0, add up to a NaN.
+QS_DEV float scale_of(float s) { return __builtin_fmaf(s, 0.0f, s); }
+QS_DEV float scale_bits(uint32_t b) { return scale_of(half_bits(b)); }
+
 // ---- four bytes at a time ----
 
 constexpr uint32_t ONES = 0x01010101u;
@@ -291,8 +297,8 @@ QS_DEV void decode_group(const Raw<TYPE>& r, int g, const uint16_t* grid, Group<
     const uint32_t(&w)[Format<TYPE>::RAW] = r.w;
     o.m[0] = o.m[Format<TYPE>::SUB - 1] = 0.0f;
     if constexpr (TYPE == QS_TYPE_Q4_0 || TYPE == QS_TYPE_Q4_1 || TYPE == QS_TYPE_IQ4_NL) {
-        o.d[0] = half_bits(w[4] & 0xffffu);
-        if constexpr (TYPE == QS_TYPE_Q4_1) o.m[0] = -half_bits(w[4] >> 16);
+        o.d[0] = scale_bits(w[4] & 0xffffu);
+        if constexpr (TYPE == QS_TYPE_Q4_1) o.m[0] = -scale_bits(w[4] >> 16);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const uint32_t lo = w[i] & 0x0f0f0f0fu, hi = (w[i] >> 4) & 0x0f0f0f0fu;
@@ -300,8 +306,8 @@ QS_DEV void decode_group(const Raw<TYPE>& r, int g, const uint16_t* grid, Group<
             else o.c[i] = codes<TYPE, STORED>(lo), o.c[4 + i] = codes<TYPE, STORED>(hi);
         }
     } else if constexpr (TYPE == QS_TYPE_Q5_0 || TYPE == QS_TYPE_Q5_1) {
-        o.d[0] = half_bits(w[5] & 0xffffu);
-        if constexpr (TYPE == QS_TYPE_Q5_1) o.m[0] = -half_bits(w[5] >> 16);
+        o.d[0] = scale_bits(w[5] & 0xffffu);
+        if constexpr (TYPE == QS_TYPE_Q5_1) o.m[0] = -scale_bits(w[5] >> 16);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const uint32_t lo = (w[1 + i] & 0x0f0f0f0fu) | (spread4(w[0] >> (4 * i)) << 4);
@@ -311,17 +317,17 @@ QS_DEV void decode_group(const Raw<TYPE>& r, int g, const uint16_t* grid, Group<
     } else if constexpr (TYPE == QS_TYPE_Q8_0) {
 #pragma unroll
         for (int i = 0; i < 8; i++) o.c[i] = w[i];
-        o.d[0] = half_bits(w[8]);
+        o.d[0] = scale_bits(w[8]);
     } else if constexpr (TYPE == QS_TYPE_Q2_K) {
         const uint32_t sc = w[9];
-        const float d = half_bits(w[8] & 0xffffu), dmin = half_bits(w[8] >> 16);
+        const float d = scale_bits(w[8] & 0xffffu), dmin = scale_bits(w[8] >> 16);
         o.d[0] = d * (float)(sc & 15u), o.m[0] = dmin * (float)((sc >> 4) & 15u);
         o.d[1] = d * (float)((sc >> 8) & 15u), o.m[1] = dmin * (float)(sc >> 12);
         const int sh = 2 * (g & 3);
 #pragma unroll
         for (int i = 0; i < 8; i++) o.c[i] = (w[i] >> sh) & 0x03030303u;
     } else if constexpr (TYPE == QS_TYPE_Q3_K) {
-        const float d = half_bits(w[19]);
+        const float d = scale_bits(w[19]);
         const int sh = 2 * (g & 3);
 #pragma unroll
         for (int i = 0; i < 8; i++)
@@ -332,8 +338,8 @@ QS_DEV void decode_group(const Raw<TYPE>& r, int g, const uint16_t* grid, Group<
         uint32_t sc, mn;
         const uint32_t s[3] = {w[9], w[10], w[11]};
         scale_min(s, g, sc, mn);
-        o.d[0] = half_bits(w[8] & 0xffffu) * (float)sc;
-        o.m[0] = half_bits(w[8] >> 16) * (float)mn;
+        o.d[0] = scale_bits(w[8] & 0xffffu) * (float)sc;
+        o.m[0] = scale_bits(w[8] >> 16) * (float)mn;
         const int sh = 4 * (g & 1);
 #pragma unroll
         for (int i = 0; i < 8; i++) {
@@ -341,7 +347,7 @@ QS_DEV void decode_group(const Raw<TYPE>& r, int g, const uint16_t* grid, Group<
             if constexpr (TYPE == QS_TYPE_Q5_K) o.c[i] |= ((w[12 + i] >> g) & ONES) << 4;
         }
     } else if constexpr (TYPE == QS_TYPE_Q6_K) {
-        const float d = half_bits(w[17]);
+        const float d = scale_bits(w[17]);
         o.d[0] = d * (float)(int8_t)(w[16] & 0xffu), o.d[1] = d * (float)(int8_t)(w[16] >> 8);
         const int sl = 4 * ((g >> 1) & 1), sh = 2 * (g & 3);
 #pragma unroll
@@ -349,19 +355,19 @@ QS_DEV void decode_group(const Raw<TYPE>& r, int g, const uint16_t* grid, Group<
             o.c[i] = codes<TYPE, STORED>(((w[i] >> sl) & 0x0f0f0f0fu) | (((w[8 + i] >> sh) & 0x03030303u) << 4));
     } else if constexpr (TYPE == QS_TYPE_IQ4_XS) {
         const uint32_t ls = ((w[5] >> (4 * g)) & 15u) | (((w[4] >> (16 + 2 * g)) & 3u) << 4);
-        o.d[0] = half_bits(w[4] & 0xffffu) * (float)((int)ls - 32);
+        o.d[0] = scale_bits(w[4] & 0xffffu) * (float)((int)ls - 32);
 #pragma unroll
         for (int i = 0; i < 4; i++)
             o.c[i] = iq4_levels(w[i] & 0x0f0f0f0fu), o.c[4 + i] = iq4_levels((w[i] >> 4) & 0x0f0f0f0fu);
     } else if constexpr (TYPE == QS_TYPE_IQ2_XXS) {
-        o.d[0] = half_bits(w[2]) * (0.5f + (float)(w[1] >> 28)) * 0.25f;
+        o.d[0] = scale_bits(w[2]) * (0.5f + (float)(w[1] >> 28)) * 0.25f;
 #pragma unroll
         for (int l = 0; l < 4; l++) {
             const uint32_t e = grid[(w[0] >> (8 * l)) & 255u], s = signs8((w[1] >> (7 * l)) & 127u);
             o.c[2 * l] = sign4(iq2_levels(e), s), o.c[2 * l + 1] = sign4(iq2_levels(e >> 8), s >> 4);
         }
     } else if constexpr (TYPE == QS_TYPE_IQ2_XS) {
-        const float d = half_bits(w[2]);
+        const float d = scale_bits(w[2]);
         o.d[0] = d * (0.5f + (float)(w[3] & 15u)) * 0.25f, o.d[1] = d * (0.5f + (float)(w[3] >> 4)) * 0.25f;
 #pragma unroll
         for (int l = 0; l < 4; l++) {
@@ -370,7 +376,7 @@ QS_DEV void decode_group(const Raw<TYPE>& r, int g, const uint16_t* grid, Group<
             o.c[2 * l] = sign4(iq2_levels(e), s), o.c[2 * l + 1] = sign4(iq2_levels(e >> 8), s >> 4);
         }
     } else if constexpr (TYPE == QS_TYPE_IQ2_S) {
-        const float d = half_bits(w[2]);
+        const float d = scale_bits(w[2]);
         o.d[0] = d * (0.5f + (float)(w[4] & 15u)) * 0.25f, o.d[1] = d * (0.5f + (float)(w[4] >> 4)) * 0.25f;
 #pragma unroll
         for (int l = 0; l < 4; l++) {
@@ -378,7 +384,7 @@ QS_DEV void decode_group(const Raw<TYPE>& r, int g, const uint16_t* grid, Group<
             o.c[2 * l] = sign4(iq2_levels(e), s), o.c[2 * l + 1] = sign4(iq2_levels(e >> 8), s >> 4);
         }
     } else if constexpr (TYPE == QS_TYPE_IQ3_XXS) {
-        o.d[0] = half_bits(w[3]) * (0.5f + (float)(w[2] >> 28)) * 0.5f;
+        o.d[0] = scale_bits(w[3]) * (0.5f + (float)(w[2] >> 28)) * 0.5f;
 #pragma unroll
         for (int l = 0; l < 4; l++) {
             const uint32_t s = signs8((w[2] >> (7 * l)) & 127u), i2 = w[l >> 1] >> (16 * (l & 1));
@@ -388,7 +394,7 @@ QS_DEV void decode_group(const Raw<TYPE>& r, int g, const uint16_t* grid, Group<
         }
     } else {
         static_assert(TYPE == QS_TYPE_IQ3_S, "format");
-        o.d[0] = half_bits(w[3]) * (float)(1 + 2 * ((w[5] >> (4 * (g & 1))) & 15u));
+        o.d[0] = scale_bits(w[3]) * (float)(1 + 2 * ((w[5] >> (4 * (g & 1))) & 15u));
 #pragma unroll
         for (int l = 0; l < 4; l++) {
             const uint32_t s = w[2] >> (8 * l), i2 = w[l >> 1] >> (16 * (l & 1)), h = w[4] >> (2 * l);

@@ -162,7 +162,7 @@ __global__ __launch_bounds__(256) void k_linear_few(LinearArgs a, FewPlan plan) 
             uint4* x = x0 + REC * g + 3 * t;
             x[0] = lo;
             x[1] = hi;
-            x[2] = uint4{__float_as_uint(a.s[row * groups + g]), (uint32_t)(F * (SUB == 2 ? o0 : o0 + o1)), (uint32_t)(F * o1), 0};
+            x[2] = uint4{__float_as_uint(qsd::scale_of(a.s[row * groups + g])), (uint32_t)(F * (SUB == 2 ? o0 : o0 + o1)), (uint32_t)(F * o1), 0};
         }
     }
     const int lane = tid % L, r0 = tid / L;

@@ -126,7 +126,7 @@ __global__ __launch_bounds__(256) void k_lay_out16(Layout16Args a) {
         const uint4* x = reinterpret_cast<const uint4*>(a.q + at * a.k + 32 * (live ? g : live_groups - 1));
         const uint4 lo = x[0], hi = x[1];
         c[0] = lo.x, c[1] = lo.y, c[2] = lo.z, c[3] = lo.w, c[4] = hi.x, c[5] = hi.y, c[6] = hi.z, c[7] = hi.w;
-        d[0] = d[1] = live ? a.s[at * live_groups + g] * a.xs[at] : 0.0f;
+        d[0] = d[1] = live ? qsd::scale_of(a.s[at * live_groups + g]) * a.xs[at] : 0.0f;
         m[0] = m[1] = 0.0f;
     }
     uint4* p = reinterpret_cast<uint4*>((weight ? a.wl : a.xl) + (panel * a.groups + g) * 2048) + row;
