@@ -9,7 +9,8 @@ quantizers write.
 The reference ends at the GGUF file and has none of this. Every function is
 calls into the gfx950 library (C ABI in include/quant_studio.h) on torch's
 current stream; nothing is synchronised, and every failure raises. These are
-serving forms: 8-bit rows and packed weights carry no gradient.
+serving forms: 8-bit rows and packed weights carry no gradient, and a tensor that
+requires one is refused while gradients are recorded.
 
 A decode step makes hundreds of these calls, each a few microseconds of GPU
 work, so what Python does per call counts as much: devices are compared as
@@ -60,6 +61,12 @@ def _same_device(dev: int, what: str, name: str, x) -> None:
         raise ValueError(f"{what}: {name} is on {x.device}, the rows on cuda:{dev}")
 
 
+def _no_gradient(what: str, name: str, x) -> None:
+    if x.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{what}: {name} requires a gradient and there is no gradient through 8-bit rows: "
+                         "detach it, or call under torch.no_grad()")
+
+
 def _call(dev: int, fn, *args) -> None:
     """fn(*args, the current stream of device dev) with dev the current device."""
     stream = torch._C._cuda_getCurrentRawStream(dev)
@@ -105,6 +112,7 @@ class Q8Rows:
         if scale.dtype != torch.float32 or tuple(scale.shape) != (q.shape[0], q.shape[1] // 32):
             raise ValueError(f"Q8Rows: scale must be float32 {(q.shape[0], q.shape[1] // 32)}, "
                              f"got {scale.dtype} {tuple(scale.shape)}")
+        _no_gradient("Q8Rows", "scale", scale)
         self._dev = _device_of(q, "Q8Rows")
         _same_device(self._dev, "Q8Rows", "scale", scale)
         self.t, self.k = q.shape
@@ -153,6 +161,11 @@ def _rows_q8(what: str, x, weight, eps: float, residual):
     if x.dim() != 2:
         raise ValueError(f"{what}: x must be 2-D (t, k), got shape {tuple(x.shape)}")
     src = _type_id(x.dtype, what)
+    _no_gradient(what, "x", x)
+    if weight is not None:
+        _no_gradient(what, "weight", weight)
+    if residual is not None:
+        _no_gradient(what, "residual", residual)
     dev = _device_of(x, what)
     t, k = x.shape
     weight_ptr = residual_ptr = total_ptr = total = None
@@ -239,7 +252,8 @@ class _Adapters(ctypes.Structure):
 class AdapterBank:
     """Low-rank adapters of one weight: a list of (A (r, k), B (n, r), scale),
     float16 or bfloat16 (all alike), on a ROCm device; ranks may differ. They
-    are laid side by side once, ranks padded with zeros to multiples of 8."""
+    are laid side by side once, ranks padded with zeros to multiples of 8: copies,
+    without gradients, which later changes of A and B do not reach."""
 
     __slots__ = ("n", "k", "dtype", "ranks", "a", "b", "offsets", "scales", "_c", "_dev")
 
@@ -255,6 +269,7 @@ class AdapterBank:
         self._dev = _device_of(a0, "AdapterBank")
         self.ranks, parts_a, parts_b, scales, offsets = [], [], [], [], [0]
         for i, (a, b, scale) in enumerate(adapters):
+            a, b = a.detach(), b.detach()
             r = a.shape[0]
             if a.dim() != 2 or b.dim() != 2 or a.shape[1] != self.k or tuple(b.shape) != (self.n, r) or r == 0:
                 raise ValueError(f"AdapterBank: adapter {i}: A {tuple(a.shape)} and B {tuple(b.shape)} are not "
@@ -332,6 +347,8 @@ def packed_linear(rows, weight: PackedWeight, dtype=None, adapters: AdapterBank 
         out = weight.data.new_empty((t, n), dtype=dtype)
     elif out.dtype != dtype or tuple(out.shape) != (t, n) or not out.is_contiguous() or not out.is_cuda or out.get_device() != dev:
         raise ValueError(f"packed_linear: out must be contiguous {dtype} {(t, n)} on cuda:{dev}")
+    else:
+        _no_gradient("packed_linear", "out", out)
     _call(dev, lib.qs_packed_linear, weight.ggml_type, weight.data.data_ptr(), n, k, rows._q_ptr, rows._scale_ptr, t,
           dst, out.data_ptr(), out.numel() * out.element_size(), bank, ids_ptr, work_ptr, need)
     return out
