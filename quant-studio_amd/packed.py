@@ -297,6 +297,21 @@ class AdapterBank:
         return len(self.ranks)
 
 
+_SIZES = 256        # of workspaces that a weight remembers
+
+
+def _workspace(weight: PackedWeight, t: int, dst: int, rank: int) -> int:
+    """The workspace of a call in bytes, remembered until _SIZES others are:
+    decoding asks for a few row counts again and again, prompts for any."""
+    need = _lib().qs_packed_linear_workspace(weight.ggml_type, weight.n, weight.k, t, dst, rank)
+    if need < 0:
+        _fail()
+    if len(weight._work) >= _SIZES:
+        weight._work.clear()
+    weight._work[(t, dst, rank)] = need
+    return need
+
+
 def packed_linear(rows, weight: PackedWeight, dtype=None, adapters: AdapterBank | None = None, ids=None, out=None,
                   exact: bool = False):
     """y = x W^T, (t, n) of dtype (bfloat16 by default), for 8-bit rows x (or a
@@ -336,10 +351,7 @@ def packed_linear(rows, weight: PackedWeight, dtype=None, adapters: AdapterBank 
         ids_ptr, bank, rank = ids.data_ptr(), ctypes.byref(adapters._c), adapters._c.max_rank
     need = weight._work.get((t, dst, rank))
     if need is None:
-        need = lib.qs_packed_linear_workspace(weight.ggml_type, n, k, t, dst, rank)
-        if need < 0:
-            _fail()
-        weight._work[(t, dst, rank)] = need
+        need = _workspace(weight, t, dst, rank)
     if need:
         work = weight.data.new_empty((need,))
         work_ptr = work.data_ptr()
