@@ -47,8 +47,10 @@ hipError_t few_rows(int t, const LinearArgs& a, const FewPlan& p, hipStream_t st
 template <int TYPE, int BM, int BN, int WM, int WN, int WK, int G>
 hipError_t tile(const LinearArgs& a, hipStream_t st) {
     const int64_t tiles = ((a.t + BM - 1) / BM) * ((a.n + BN - 1) / BN) * a.splits;
-    // a multiple of the 8 XCDs: each takes a run of tiles
-    return launch_kernel(k_linear_tile<TYPE, BM, BN, WM, WN, WK, G>, dim3((unsigned)((tiles + 7) / 8 * 8)),
+    // a multiple of the 8 XCDs: each takes a run of tiles; 2^23 workgroups at most
+    // in a row of the grid, whose threads are under 2^32
+    const int64_t rows = (tiles + (1 << 23) - 1) >> 23, row = ((tiles + rows - 1) / rows + 7) / 8 * 8;
+    return launch_kernel(k_linear_tile<TYPE, BM, BN, WM, WN, WK, G>, dim3((unsigned)row, (unsigned)rows),
                          dim3(64 * WM * WN * WK), 0, st, a);
 }
 

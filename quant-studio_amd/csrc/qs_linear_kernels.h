@@ -310,7 +310,8 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_linear_tile(LinearArgs
     // strips of 8 columns of tiles, so that what it works on at a time shares
     // rows and weights in its L2.
     const int64_t tiles_m = (a.t + BM - 1) / BM, tiles_n = (a.n + BN - 1) / BN, tiles = tiles_m * tiles_n;
-    const int64_t place = (int64_t)(blockIdx.x % 8) * (gridDim.x / 8) + blockIdx.x / 8, at = place % tiles;
+    const int64_t number = (int64_t)blockIdx.y * gridDim.x + blockIdx.x, workgroups = (int64_t)gridDim.y * gridDim.x;
+    const int64_t place = number % 8 * (workgroups / 8) + number / 8, at = place % tiles;
     if (place >= tiles * a.splits) return;
     const int64_t strip = at / (8 * tiles_m), left = tiles_n - 8 * strip, wide = left < 8 ? left : 8;
     const int64_t in = at - strip * 8 * tiles_m;

@@ -5,7 +5,8 @@ from __future__ import annotations
 import pytest
 import torch
 
-from test_gpu_packed_linear import DEV
+import packed_ref as ref
+from test_gpu_packed_linear import DEV, check, rows_on
 
 pytestmark = pytest.mark.gpu
 
@@ -26,3 +27,16 @@ def test_norm_of_2_26_short_rows(qs):
     assert torch.equal(rows.q[times * base:], want.q[:5]) and torch.equal(h[times * base:], total[:5])
     assert torch.equal(rows.scale[times * base:], want.scale[:5])
 
+@pytest.mark.parametrize("t", [9, 32])
+def test_product_with_2_29_short_weight_rows(qs, t):
+    """256 threads to 32 of them: 2^32 threads. Runs of 2^15 weight rows repeat."""
+    base, k, times = 1 << 15, 32, 1 << 14
+    part = ref.random_packed("q4_0", base, k, 3)
+    q, s = ref.random_rows(t, k, t)
+    rows, small = rows_on(qs, q, s), torch.from_numpy(part).to(DEV)
+    want = qs.packed_linear(rows, qs.PackedWeight("q4_0", small))
+    check(want, *ref.linear64("q4_0", part, q, s, "bf16"), "one run")
+    print(t, base * times, flush=True)
+    y = qs.packed_linear(rows, qs.PackedWeight("q4_0", small.repeat(times, 1))).view(t, times, base)
+    for i in range(0, times, 1024):
+        assert torch.equal(y[:, i:i + 1024], want[:, None].expand(t, 1024, base)), i
