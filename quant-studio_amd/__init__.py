@@ -87,6 +87,62 @@ def library() -> ctypes.CDLL:
         return _load_library()
 
 
+def _bind(L: ctypes.CDLL) -> None:
+    """The signatures of the functions in include/quant_studio.h."""
+    L.qs_type_supported.restype = ctypes.c_int
+    L.qs_type_supported.argtypes = [ctypes.c_int]
+    L.qs_type_needs_imatrix.restype = ctypes.c_int
+    L.qs_type_needs_imatrix.argtypes = [ctypes.c_int]
+    L.qs_type_uses_imatrix.restype = ctypes.c_int
+    L.qs_type_uses_imatrix.argtypes = [ctypes.c_int]
+    L.qs_row_bytes.restype = ctypes.c_int64
+    L.qs_row_bytes.argtypes = [ctypes.c_int, ctypes.c_int64]
+    L.qs_quantize.restype = ctypes.c_int
+    L.qs_quantize.argtypes = [ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.c_int64,
+                              ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p,
+                              ctypes.c_int64, ctypes.c_void_p]
+    L.qs_init.restype = ctypes.c_int
+    L.qs_init.argtypes = [ctypes.c_int]
+    L.qs_set_sqrt_rounding.restype = ctypes.c_int
+    L.qs_set_sqrt_rounding.argtypes = [ctypes.c_int]
+    L.qs_get_sqrt_rounding.restype = ctypes.c_int
+    L.qs_last_error.restype = ctypes.c_char_p
+    L.qs_device_count.restype = ctypes.c_int
+    L.qs_pipeline_create.restype = ctypes.c_int
+    L.qs_pipeline_create.argtypes = [ctypes.c_int, ctypes.c_int, ctypes.c_int,
+                                     ctypes.POINTER(ctypes.c_void_p)]
+    L.qs_pipeline_quantize.restype = ctypes.c_int
+    L.qs_pipeline_quantize.argtypes = [ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_void_p,
+                                       ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p,
+                                       ctypes.c_int64, ctypes.c_int, ctypes.c_int64]
+    L.qs_pipeline_quantize_fd.restype = ctypes.c_int
+    L.qs_pipeline_quantize_fd.argtypes = [ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_int,
+                                          ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p,
+                                          ctypes.c_int64, ctypes.c_int, ctypes.c_int64]
+    L.qs_pipeline_write.restype = ctypes.c_int
+    L.qs_pipeline_write.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int,
+                                    ctypes.c_int64]
+    L.qs_pipeline_finish.restype = ctypes.c_int
+    L.qs_pipeline_finish.argtypes = [ctypes.c_void_p]
+    L.qs_pipeline_destroy.restype = None
+    L.qs_pipeline_destroy.argtypes = [ctypes.c_void_p]
+    L.qs_rms_norm_q8.restype = ctypes.c_int
+    L.qs_rms_norm_q8.argtypes = [ctypes.c_int, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
+                                 ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_float,
+                                 ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]
+    L.qs_q8_values.restype = ctypes.c_int
+    L.qs_q8_values.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_int,
+                               ctypes.c_void_p, ctypes.c_void_p]
+    L.qs_packed_linear_workspace.restype = ctypes.c_int64
+    L.qs_packed_linear_workspace.argtypes = [ctypes.c_int, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
+                                             ctypes.c_int, ctypes.c_int]
+    L.qs_packed_linear.restype = ctypes.c_int
+    L.qs_packed_linear.argtypes = [ctypes.c_int, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64,
+                                   ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int,
+                                   ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p,
+                                   ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p]
+
+
 def _load_library() -> ctypes.CDLL:
     global _lib
     if _lib is None:
@@ -95,61 +151,15 @@ def _load_library() -> ctypes.CDLL:
                               "quant-studio_amd/build.py (or __graft_entry__.build())")
         _bind_torch_hip_runtime()
         L = ctypes.CDLL(str(LIB_PATH))
+        if not hasattr(L, "qs_abi_version"):
+            raise ImportError(f"{LIB_PATH} lacks qs_abi_version: it is another library")
         L.qs_abi_version.restype = ctypes.c_int
-        L.qs_type_supported.restype = ctypes.c_int
-        L.qs_type_supported.argtypes = [ctypes.c_int]
-        L.qs_type_needs_imatrix.restype = ctypes.c_int
-        L.qs_type_needs_imatrix.argtypes = [ctypes.c_int]
-        L.qs_type_uses_imatrix.restype = ctypes.c_int
-        L.qs_type_uses_imatrix.argtypes = [ctypes.c_int]
-        L.qs_row_bytes.restype = ctypes.c_int64
-        L.qs_row_bytes.argtypes = [ctypes.c_int, ctypes.c_int64]
-        L.qs_quantize.restype = ctypes.c_int
-        L.qs_quantize.argtypes = [ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.c_int64,
-                                  ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p,
-                                  ctypes.c_int64, ctypes.c_void_p]
-        L.qs_init.restype = ctypes.c_int
-        L.qs_init.argtypes = [ctypes.c_int]
-        L.qs_set_sqrt_rounding.restype = ctypes.c_int
-        L.qs_set_sqrt_rounding.argtypes = [ctypes.c_int]
-        L.qs_get_sqrt_rounding.restype = ctypes.c_int
-        L.qs_last_error.restype = ctypes.c_char_p
-        L.qs_device_count.restype = ctypes.c_int
-        L.qs_pipeline_create.restype = ctypes.c_int
-        L.qs_pipeline_create.argtypes = [ctypes.c_int, ctypes.c_int, ctypes.c_int,
-                                         ctypes.POINTER(ctypes.c_void_p)]
-        L.qs_pipeline_quantize.restype = ctypes.c_int
-        L.qs_pipeline_quantize.argtypes = [ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_void_p,
-                                           ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p,
-                                           ctypes.c_int64, ctypes.c_int, ctypes.c_int64]
-        L.qs_pipeline_quantize_fd.restype = ctypes.c_int
-        L.qs_pipeline_quantize_fd.argtypes = [ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_int,
-                                              ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p,
-                                              ctypes.c_int64, ctypes.c_int, ctypes.c_int64]
-        L.qs_pipeline_write.restype = ctypes.c_int
-        L.qs_pipeline_write.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int,
-                                        ctypes.c_int64]
-        L.qs_pipeline_finish.restype = ctypes.c_int
-        L.qs_pipeline_finish.argtypes = [ctypes.c_void_p]
-        L.qs_pipeline_destroy.restype = None
-        L.qs_pipeline_destroy.argtypes = [ctypes.c_void_p]
-        L.qs_rms_norm_q8.restype = ctypes.c_int
-        L.qs_rms_norm_q8.argtypes = [ctypes.c_int, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
-                                     ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_float,
-                                     ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]
-        L.qs_q8_values.restype = ctypes.c_int
-        L.qs_q8_values.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_int,
-                                   ctypes.c_void_p, ctypes.c_void_p]
-        L.qs_packed_linear_workspace.restype = ctypes.c_int64
-        L.qs_packed_linear_workspace.argtypes = [ctypes.c_int, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
-                                                 ctypes.c_int, ctypes.c_int]
-        L.qs_packed_linear.restype = ctypes.c_int
-        L.qs_packed_linear.argtypes = [ctypes.c_int, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64,
-                                       ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int,
-                                       ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p,
-                                       ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p]
         if L.qs_abi_version() != ABI_VERSION:
             raise ImportError(f"{LIB_PATH}: ABI version {L.qs_abi_version()} != {ABI_VERSION}")
+        try:
+            _bind(L)
+        except AttributeError as e:         # functions were added without a change of version
+            raise ImportError(f"{LIB_PATH} is an older build, build it again: {e}") from e
         _lib = L
     return _lib
 
