@@ -185,7 +185,7 @@ int qs_q8_values(const int8_t *q, const float *scales, int64_t rows, int64_t k, 
  * offsets[i+1] - offsets[i], a multiple of 8 up to max_rank (pad with zero
  * rows of a and zero columns of b). All pointers are device pointers. */
 typedef struct qs_adapters {
-    int32_t count;          /* adapters */
+    int32_t count;          /* adapters; 0: none */
     int32_t type;           /* QS_SRC_F16 or QS_SRC_BF16 */
     int32_t max_rank;       /* of any adapter; a multiple of 8, at most 4096 */
     const void *a;          /* offsets[count] rows of k */

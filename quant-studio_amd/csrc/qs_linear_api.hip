@@ -141,6 +141,8 @@ int qs_packed_linear(int ggml_type, const void* weight, int64_t n, int64_t k, co
     a.dst_type = dst_type & ~QS_EXACT;
     hipStream_t st = static_cast<hipStream_t>(hip_stream);
     if ((adapters != nullptr) != (ids != nullptr)) return fail(QS_EINVAL, "adapters and ids go together");
+    if (adapters && (adapters->count < 0 || adapters->max_rank < 0))
+        return fail(QS_EINVAL, "adapter count %d or max_rank %d is negative", adapters->count, adapters->max_rank);
     const bool adapted = adapters && adapters->count > 0 && adapters->max_rank > 0;
     const int rank = adapted ? adapters->max_rank : 0;
     if (adapted) {
