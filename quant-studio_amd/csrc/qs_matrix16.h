@@ -6,10 +6,11 @@
 // their times, 37 and 80 clocks), so products that are scaled group by group
 // cost three times those that are not. Here d * c - m and s * q are rounded to
 // f16, 2^-11 of each value, an eighth of what rounding the result to bf16 does
-// to it: the error of a sum of them is about 1% more than that of its rounding.
-// Each row is first multiplied by a power of two that takes its largest
-// possible value near 2^15, so nothing overflows and what is lost below f16's
-// range is under 2^-39 of that value.
+// to it: together with that rounding the error of a sum of them is 1.5% larger
+// than the rounding's alone, and far larger where its terms cancel. Each row is
+// first multiplied by a power of two that takes its largest possible value near
+// 2^15, so nothing overflows and what is lost below f16's range is under 2^-39 of
+// that value.
 #pragma once
 
 #include "qs_matrix.h"

@@ -323,7 +323,8 @@ def packed_linear(rows, weight: PackedWeight, dtype=None, adapters: AdapterBank 
     out: a contiguous (t, n) tensor to write instead of a new one.
     exact: large products with a bfloat16 result round both factors to float16
     (include/quant_studio.h has the sizes), which takes a half to two thirds of
-    the time; with exact=True they multiply exact codes, as all others do."""
+    the time and, where the terms of a sum cancel, costs more than its rounding
+    does; with exact=True they multiply exact codes, as all others do."""
     lib = _lib()
     if not isinstance(rows, Q8Rows):
         rows = q8_rows(rows)
