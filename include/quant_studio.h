@@ -217,11 +217,10 @@ int64_t qs_packed_linear_workspace(int ggml_type, int64_t n, int64_t k, int64_t 
  * two first, so that nothing overflows). That moves y by at most
  * (2^-10 + 2^-22) * sum |x w| beside its rounding to bf16: some 18% of that
  * rounding where the terms do not cancel (1.5% more error in all), and many times
- * it where they do. A x is then held to 16 bits (bf16 adapters) or 22 (f16);
- * else in f32, but to 22 bits with f16 adapters in calls of more than 512 rows, or
- * of more than 128 where n is large. The result of a row does not depend on
- * timing. With t and n, and with adapters, it may differ in the last bits of f32
- * (another split of the sum) and by the roundings named here. t is at most
+ * it where they do. A x is then held to 16 bits (bf16 adapters) or 22 (f16), else
+ * in f32. The result of a row does not depend on timing. With t and n, and with
+ * adapters, it may differ in the last bits of f32 (another split of the sum) and by
+ * the roundings named here. t is at most
  * 2^24, each of n*k, t*k and n*t at most 2^34. An infinite scale, of a row or of
  * a weight's block, stands for no values: what it reaches is NaN. */
 int qs_packed_linear(int ggml_type, const void *weight, int64_t n, int64_t k, const int8_t *q, const float *scales,

@@ -123,7 +123,7 @@ QS_DEV uint4 codes16(uint2 c) {
     return uint4{o[0], o[1], o[2], o[3]};
 }
 // v to 16 bits, and what that leaves of it (exactly). Two pieces hold 16 (BF16) or
-// 22 (F16) bits of v, three of BF16 all 24. An infinity leaves nothing, and a finite
+// 22 (F16) bits of v, three all 24. An infinity leaves nothing, and a finite
 // v that bf16 would round to one is cut, so that the pieces' sum stays v.
 template <int TYPE>
 QS_DEV float piece16(float v, uint16_t& piece) {
@@ -225,7 +225,7 @@ __global__ __launch_bounds__(512) void k_adapter_many(AdapterArgs a) {
     }
 }
 
-// The parts' sums, scaled, as hi + lo (+ rest, BF16): 16 lanes to a row's 32 ranks, two each.
+// The parts' sums, scaled, as hi + lo (+ rest): 16 lanes to a row's 32 ranks, two each.
 template <int TYPE>
 __global__ __launch_bounds__(256) void k_adapter_join(AdapterArgs a) {
     const int64_t t = (int64_t)blockIdx.x * 16 + threadIdx.x / 16;
@@ -258,7 +258,7 @@ __global__ __launch_bounds__(256) void k_adapter_join(AdapterArgs a) {
     for (int i = 0; i < 2; i++) {
         const int64_t at = t * a.ldv + r + i;
         const float left = piece16<TYPE>(piece16<TYPE>(v[i], a.hi[at]), a.lo[at]);
-        if (TYPE == QS_SRC_BF16 && a.rest) piece16<TYPE>(left, a.rest[at]);
+        if (a.rest) piece16<TYPE>(left, a.rest[at]);
     }
     if (TYPE == QS_SRC_F16 && r == r0) a.unit[t * ((a.ldv + 31) / 32) + r0 / 32] = unit;
 }
@@ -279,8 +279,7 @@ struct AdapterTile {
 // sums of these units each takes every WK-th step: a step is bound by the
 // latency of what it reads (512 rows with q4_k 2,560 x 2,560, 4 adapters: the
 // product took 44 us with the steps in one wave of eight). PIECES of v: with exact
-// codes as many as hold it to f32 (22 bits where B is f16), two with factors of f16,
-// whose result is bf16.
+// codes three, which hold it whole, two with factors of f16, whose result is bf16.
 template <int TYPE, int PIECES, int WK, int UM, int UN>
 QS_DEV void add_adapters(const AdapterTile& a, f32x16 (&y)[UM][UN], int64_t t0, int64_t rows, int64_t n0, int64_t n, int wk) {
     const int lane = threadIdx.x % 64, col = lane % 32, half = lane / 32;

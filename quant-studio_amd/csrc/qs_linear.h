@@ -42,7 +42,7 @@ struct LinearArgs {
     const float* delta;     // tiles: B v, t rows of n
     float* parts;           // of a product split over its groups: splits x t rows of n
     int splits;
-    // laid-out factors: scale * A x as hi + lo (+ rest: exact codes, BF16), t rows of ldv
+    // laid-out factors: scale * A x as hi + lo (+ rest: exact codes), t rows of ldv
     const uint16_t *v_hi, *v_lo, *v_rest;
     const float* v_unit;            // and what that is to be multiplied by (F16), t rows of ldv / 32
 };

@@ -357,7 +357,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_matrix(MatrixArgs a) {
     }
     __builtin_amdgcn_s_waitcnt(0x0f70);     // no copy to LDS outlives the workgroup
     if constexpr (ADAPT)
-        add_adapters<ADAPT, ADAPT == QS_SRC_BF16 ? 3 : 2, WK>(adapter_tile(l), acc, t0 + wm * UM * 32, l.t, a.first + n0 + wn * UN * 32, l.n, wk);
+        add_adapters<ADAPT, 3, WK>(adapter_tile(l), acc, t0 + wm * UM * 32, l.t, a.first + n0 + wn * UN * 32, l.n, wk);
     if constexpr (WK > 1) {
         join_waves<WK, WM * WN>(acc, reinterpret_cast<float*>(even), wk, wm * WN + wn);
         static_assert(STAGE >= BM * BN * 4 / UN, "a column of units");

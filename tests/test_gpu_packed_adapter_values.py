@@ -44,8 +44,8 @@ def picks(rng, n, ranks, dtype):
 def test_a_x_keeps_its_bits(qs, qtype, t, n, dtype):
     """An f32 result. Roundings of a term, relative: the row's scale and the
     adapter's (1 U each), B's product and the sums of its at most three pieces,
-    U each, twice that where a matrix instruction cuts: 8. With f16 adapters A x
-    is held to 22 bits: 4 U more."""
+    U each, twice that where a matrix instruction cuts: 8; two more are allowed,
+    and with f16 adapters the roundings of the pieces' common scale and the result's: 4."""
     rng = np.random.default_rng(t)
     made, places = picks(rng, n, [16, 5, 40], TORCH[dtype])
     q, s = ref.random_rows(t, K, 2)
@@ -88,3 +88,23 @@ def test_the_largest_and_infinite_a_x(qs, qtype, t, n, dtype):
     if t > 2:
         assert (y[1] == sign * np.inf).all()
         assert (y[2] == sign * 0.5).all() and (y[3:] == sign / 16).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("qtype,t,n", PATHS)
+def test_all_bits_of_a_x(qs, qtype, t, n, dtype):
+    """Scales of 24 bits times powers of two: every step is exact, and so is the result."""
+    r, rng = 40, np.random.default_rng(t)
+    a, b = torch.zeros((r, K)), torch.zeros((n, r))
+    col, rank = rng.permutation(K)[:r], rng.integers(0, r, n)
+    a[np.arange(r), col] = torch.from_numpy(2.0 ** rng.integers(-2, 3, r)).float()
+    b[np.arange(n), rank] = torch.from_numpy(2.0 ** rng.integers(-2, 3, n) * rng.choice([-1, 1], n)).float()
+    bank = qs.AdapterBank([(a.to(DEV, TORCH[dtype]), b.to(DEV, TORCH[dtype]), 0.5)])
+    q = (2 ** rng.integers(0, 7, (t, K))).astype(np.int8)
+    s = rng.uniform(0.5, 2, (t, K // 32)).astype(np.float32)
+    print(qtype, t, n, dtype, flush=True)
+    y = qs.packed_linear(rows_on(qs, q, s), zero_weight(qs, qtype, n), dtype=torch.float32, adapters=bank,
+                         ids=torch.zeros((t,), dtype=torch.int32, device=DEV)).double().cpu().numpy()
+    a, b = a.double().numpy(), b.double().numpy()
+    want = 0.5 * (ref.rows64(q, s)[:, col] * a[np.arange(r), col])[:, rank] * b[np.arange(n), rank]
+    assert np.array_equal(y, want)
