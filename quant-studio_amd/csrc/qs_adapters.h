@@ -22,7 +22,7 @@ QS_DEV float from16(uint32_t bits) {
 
 // A workgroup takes a row and 8 ranks, a wave two of them; a lane 8 values at a
 // time. Up to 512 rows, where a row or two use an adapter: bound by the latency
-// of ids, offsets and A, one after another (3.5 us for a row of 2,560 values and
+// of ids, offsets and A, one after another (4 us for a row of 2,560 values and
 // rank 16, 6 us for 64 rows and ranks to 64).
 template <int TYPE>
 __global__ __launch_bounds__(256) void k_adapter_few(AdapterArgs a) {
@@ -71,7 +71,7 @@ __global__ __launch_bounds__(256) void k_adapter_few(AdapterArgs a) {
 
 // delta[t, n] = sum over r of v[t, r] * B[n, r]; 0 for a row without an adapter.
 // A lane takes a column: the wave's rows of B are one run of bytes. Bound by
-// reading B for each row: 64 rows, 9,728 columns, ranks 64, 32 and 16, 46 MB: 13 us.
+// reading B for each row: 64 rows, 9,728 columns, ranks 64, 32 and 16, 46 MB: 14 us.
 template <int TYPE>
 __global__ __launch_bounds__(256) void k_adapter_delta(AdapterArgs a) {
     const int64_t t = blockIdx.y, n = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -143,9 +143,9 @@ QS_DEV float piece16(float v, uint16_t& piece) {
 // products' sums are scaled, in f32. The rows' adapters are taken one after
 // another (packed sequences have one or two to 32 rows). A row's values are
 // split over `parts` workgroups, whose sums k_adapter_join adds. 2,047 rows of
-// 9,728 values, ranks 128, 64 and 32: 30 us, bound by the latency of a turn's
+// 9,728 values, ranks 128, 64 and 32: 30 to 36 us, bound by the latency of a turn's
 // copies, LDS and barrier (vector instructions, which widen the codes and scale the
-// products, take 0.22 of the cycles, matrix ones 0.03); the join takes 4 us.
+// products, take 0.22 of the cycles, matrix ones 0.03); the join takes 4 to 5 us.
 template <int TYPE>
 __global__ __launch_bounds__(512) void k_adapter_many(AdapterArgs a) {
     constexpr int XS = 256 + 16, AS = 512 + 16;     // strides that spread rows over the banks

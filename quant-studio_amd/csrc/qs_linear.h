@@ -15,9 +15,9 @@ namespace qsl {
 constexpr int few_record(int t) { return 3 * t + (3 * t + 1) % 2; }     // 16s of a group of x
 constexpr int FEW_LDS = 160 * 1024, FEW_GRID = 4096;    // bytes of a CU, and of the largest code book
 // Up to 8 rows, 4 where they are long, of which four weight rows and the rows
-// themselves fit in LDS. us, and of a tile: 8 rows with q6_k 151,936 x 2,560 150 and
-// 178, q4_k 9,728 x 2,560 16.1 and 15.8, q4_0 1,024 x 2,560 7.7 and 7.9, q6_k 2,560 x
-// 9,728 29 and 20, 5 of those 22 and 20.
+// themselves fit in LDS. us, and of a tile: 8 rows with q6_k 151,936 x 2,560 133 and
+// 161, q4_k 9,728 x 2,560 15.9 and 15.6, q4_0 1,024 x 2,560 7.7 and 8.2, q6_k 2,560 x
+// 9,728 28 and 20, 5 of those 22 and 19.
 inline bool takes_few(int64_t row_bytes, int64_t t, int64_t k) {
     if (t > (k > 4096 ? 4 : 8)) return false;
     return 4 * row_bytes + 48 + k / 32 * few_record(t <= 6 ? (int)t : 8) * 16 + FEW_GRID <= FEW_LDS;
@@ -85,22 +85,23 @@ inline int64_t tile_count(int64_t t, int64_t n, int bm, int bn) { return ((t + b
 // Tiles that decode the weight for each 64 rows save its layout's way through
 // memory, as long as one round of 64 x 64 takes them all, or a split half a round
 // where rows are long. us of tiles and of laid-out factors: 128 rows with q4_k
-// 9,728 x 2,560 39 and 40; 192 with q6_k 2,560 x 9,728 53 and 89; 256 with q4_0
-// 4,096 x 4,096 27 and 37; 512 with 1,024 x 2,560 15 and 23, with 8 adapters of
-// rank 64 33 and 39; but 320 with 4,096 x 4,096 47 and 42, 512 with q6_k 2,048 x
-// 9,728 92 and 72. Above 512 rows the adapters' products row by row lose.
+// 9,728 x 2,560 38 and 38; 192 with q6_k 2,560 x 9,728 51 and 90; 256 with q4_0
+// 4,096 x 4,096 26 and 36; 512 with 1,024 x 2,560 14 and 23, with 8 adapters of
+// rank 64 32 and 40; but 320 with 4,096 x 4,096 46 and 41, 512 with q6_k 2,048 x
+// 9,728 90 and 87, 71 with factors of f16. Above 512 rows the adapters' products row by row lose.
 inline bool takes_matrix(int64_t t, int64_t n, int64_t k) {
     const int64_t tiles = tile_count(t, n, 64, 64);
     return t > 512 || (t > 128 && tiles > (k <= 4096 ? 256 : 128));
 }
 
 // Large products whose result is bf16 (8 bits) take factors of f16 (11 bits) where
-// the caller leaves that open (`dst` without QS_EXACT); everything else exact codes. F16 factors are laid out in two launches and twice
-// the bytes, and multiplied at up to 1.0 PFLOP/s where exact codes reach 0.62.
-// q4_k, us f16 and exact: 512 rows, 2,560 x 2,560 38 and 34; 2,048, 1,024 x 2,560
-// 42 and 38; 1,024, 2,560 x 2,560 42 and 50; 300, 9,728 x 2,560 55 and 56; 4,096,
-// 9,728 x 2,560 234 and 389. Rows under 1,024 values give neither time to start:
-// 2,000 rows, 3,000 x 256 19 and 19.
+// the caller leaves that open (`dst` without QS_EXACT); everything else exact codes.
+// F16 factors are laid out in two launches and twice the bytes, and multiplied at up
+// to 1.0 PFLOP/s where exact codes reach 0.8, 0.64 with minima. q4_k, us f16 and
+// exact: 512 rows, 2,560 x 2,560 40 and 34; 2,048, 1,024 x 2,560 41 and 35; 1,024,
+// 2,560 x 2,560 41 and 49; 300, 9,728 x 2,560 52 and 54; 4,096, 9,728 x 2,560 215
+// and 336. Rows under 1,024 values do not repay a launch more: 2,000 rows, 3,000 x
+// 256 33 and 18.
 inline bool takes_f16(int dst, int64_t t, int64_t n, int64_t k) {
     return dst == QS_SRC_BF16 && takes_matrix(t, n, k) && k >= 1024 && t * n >= INT64_C(3) * (INT64_C(1) << 31) / k;
 }
@@ -113,7 +114,7 @@ struct Tiles {
 };
 
 // F16 factors. Larger tiles do more per LDS byte (256 x 320: 1.02 PFLOP/s where
-// they fill the chip, 64 x 64: 0.56). Adapters need registers that 160 columns a
+// they fill the chip, 64 x 64: 0.46). Adapters need registers that 160 columns a
 // wave do not leave, and with them a CU has registers for one workgroup of 64 x 64.
 constexpr Tiles TILES16[] = {{256, 320, 256, 1000}, {256, 256, 256, 770}, {128, 160, 256, 385}, {128, 96, 256, 258},
                              {64, 64, 512, 227}};
@@ -124,9 +125,9 @@ struct Choice16 {
 // The tile, and the parts of the groups, that cost least: few tiles leave CUs
 // idle, each of the rest waiting for its copies; parts cost what writing and
 // joining their f32 sums takes, 12 bytes of each at 4 TB/s, and two launches'
-// ends. 509 rows with q5_k 2,560 x 9,728: product and join 45 us in four parts of
-// 128 x 160, 62 whole in 64 x 64; 2,047 rows with q6_k: three parts of 256 x 256
-// 121, 115 whole in 128 x 160, which the rule takes.
+// ends. us of a call: 509 rows with q5_k 2,560 x 9,728 71 in four parts of 128 x
+// 160, 88 whole in 64 x 64; 2,047 rows with q6_k 160 in three parts of 256 x 256,
+// 152 whole in 128 x 160, which the rule takes.
 inline Choice16 choose16(bool adapted, int64_t t, int64_t n, int64_t k, int most) {
     Choice16 best{};
     double least = 1e300;
@@ -144,10 +145,10 @@ inline Choice16 choose16(bool adapted, int64_t t, int64_t n, int64_t k, int most
 }
 
 // Parts that a product that is not laid out is split into over its groups, so
-// that there are two workgroups for every CU; a part is whole stages of 8
-// groups. us whole, in up to 4 parts and in up to 8: 61 rows with q8_0 1,024 x
-// 2,560 18.7, 10.2 and 9.6; 64 with q6_k 2,560 x 9,728 46, 32 and 27. Parts for four
-// workgroups a CU: 37.
+// that there are two workgroups of 64 x 32 for every CU (where they are 64 x 64,
+// one); a part is whole stages of 8 groups. us whole, in up to 4 parts and in up to
+// 8: 61 rows with q8_0 1,024 x 2,560 14.3, 10.3 and 9.6; 64 with q6_k 2,560 x 9,728
+// 90, 31 and 27. Parts for twice the workgroups: 9.5 and 37.
 inline int tile_splits(int64_t t, int64_t n, int64_t k) {
     const int64_t tiles = (t + 63) / 64 * ((n + 31) / 32), stages = (k / 32 + 7) / 8;
     int64_t s = 512 / tiles < 8 ? 512 / tiles : 8;
@@ -196,8 +197,9 @@ struct AdapterArgs {
 };
 // Parts that the rows' values are split into: up to 1,024 workgroups, where a
 // row has 512 values or more for each. The CUs hold 512 at a time; parts half as
-// long leave less to the 32 rows that have two adapters (2,047 rows of 9,728
-// values, ranks to 128: 41 us for 512 workgroups, 32 for 1,024, 47 unsplit).
+// long leave less to the 32 rows that have two adapters (us of a call, 2,047 rows
+// with q6_k 2,560 x 9,728, ranks to 128: 211 for 512 workgroups, 196 for 1,024, 212
+// unsplit).
 inline int adapter_parts(int64_t t, int64_t k, int64_t ldv) {
     const int64_t blocks = (t + 31) / 32 * ((ldv + 31) / 32), p = 1024 / blocks < k / 512 ? 1024 / blocks : k / 512;
     return p < 1 ? 1 : (int)p;

@@ -111,9 +111,9 @@ hipError_t launch_linear(const LinearArgs& a, void* work, hipStream_t st) {
     if (takes_matrix(a.t, a.n, a.k)) return a.f16 ? matrix16<TYPE>(a, work, st) : matrix<TYPE>(a, work, st);
     // Up to 64 rows in one tile, so that the weight is decoded once. 64 columns
     // halve what each thread does to stage the rows (64 rows with q4_k 9,728 x 2,560
-    // 21.8 us, 32 columns 24.2; q6_k 2,560 x 9,728 31.7 and 34.5), 32 make enough
-    // tiles of a narrow weight (61 rows with q8_0 1,024 x 2,560 10.2 us, 64 columns
-    // 11.6) and are faster to 32 rows (16 with q6_k 151,936 x 2,560 184 and 237).
+    // 21.5 us, 32 columns 24.5; q6_k 2,560 x 9,728 27 and 29), 32 make enough tiles of
+    // a narrow weight (61 rows with q8_0 1,024 x 2,560 9.7 us, 64 columns 10.7). 32 x
+    // 32 to 32 rows: 16 with q6_k 151,936 x 2,560 164 us, in 64 x 32 242, 64 x 64 250.
     const hipError_t e = a.t <= 32      ? tile<TYPE, 32, 32, 1, 1, 4, 8>(a, st)
                          : a.n >= 2048 ? tile<TYPE, 64, 64, 2, 2, 2, 8>(a, st)
                                        : tile<TYPE, 64, 32, 2, 1, 2, 8>(a, st);

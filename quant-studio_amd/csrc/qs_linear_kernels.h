@@ -123,11 +123,11 @@ QS_DEV uint4 read_end(const Run& r, int c, const uint8_t* lo, const uint8_t* hi)
 // codes that an offset of the weight's integers (OFFSET) or a minimum multiplies:
 // 48 bytes, the T of a group together, so that a lane reads them at constant
 // offsets, and an odd number of 16s a group, which spreads lanes over the banks.
-// One row is bound by reading a large weight (151,936 x 2,560: q8_0 75 us, 5.5
-// TB/s; q6_k 68 us, 4.7 TB/s; q4_k 50 us, 4.4 TB/s) and by the latency of what
-// comes one after another in a small one (q4_k 9,728 x 2,560, 14 MB: 6 us). More
-// rows add LDS reads and dot products: five with q6_k 151,936 x 2,560 95 us, 3.4
-// TB/s.
+// One row is bound by reading a large weight (151,936 x 2,560: q8_0 72 us, 5.7
+// TB/s; q6_k 65 us, 4.9 TB/s; q4_k 47 us, 4.6 TB/s), of the types under 4 bits by
+// decoding it (iq2_xxs 60 us, q3_k 62), and by the latency of what comes one after
+// another in a small one (q4_k 9,728 x 2,560, 14 MB: 7.2 us). More rows add LDS
+// reads and dot products: five with q6_k 151,936 x 2,560 90 us, 3.6 TB/s.
 template <int TYPE, int T, int L>
 __global__ __launch_bounds__(256) void k_linear_few(LinearArgs a, FewPlan plan) {
     constexpr int SUB = Format<TYPE>::SUB, AHEAD = 8, ROWS = 256 / L, OFFSET = qsd::offset<TYPE>();
@@ -293,9 +293,9 @@ struct Tile {
 // matrix instruction makes from three bf16 pieces of each, exact to f32.
 // Bound by the turn of a stage: decode and copies to LDS, a barrier, products, a
 // barrier, one after another: with 64 rows of q4_k 9,728 x 2,560 vector
-// instructions take about a fifth of the SIMDs' cycles, matrix ones a twentieth.
-// 64 rows 22 us, 146 TFLOP/s; 16 rows 16.6 us; 128 with q6_k 151,936 x 2,560 553
-// us, 180 TFLOP/s.
+// instructions take about a fifth of the SIMDs' cycles, matrix ones a twentieth,
+// with 128 of q6_k 151,936 x 2,560 half and a sixth. 64 rows 21 us, 152 TFLOP/s; 16
+// rows 16 us; 128 with q6_k 151,936 x 2,560 493 us, 202 TFLOP/s.
 template <int TYPE, int BM, int BN, int WM, int WN, int WK, int G>
 __global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_linear_tile(LinearArgs a) {
     using S = Tile<TYPE, BM, BN, WM, WN, WK, G>;

@@ -107,7 +107,7 @@ struct LayoutArgs {
 };
 
 // A workgroup lays out 32 rows by 8 groups, a group to a thread: the lanes of
-// a half wave write 512 bytes in a row. 333 rows and q4_0 4,099 x 4,096: 12 us.
+// a half wave write 512 bytes in a row. 333 rows and q4_0 4,099 x 4,096: 13 us.
 template <int TYPE>
 __global__ __launch_bounds__(256) void k_lay_out(LayoutArgs a) {
     using M = MatrixFormat<TYPE>;
@@ -215,8 +215,8 @@ QS_DEV void copy_to_lds(const uint8_t* from, uint8_t* to) {
 // Each 32 x 32 x 32 of codes takes three units of matrix time or more: the codes'
 // instruction (37 clocks), the scales' outer product (32), a minimum's (32) and 32
 // vector instructions that apply it (80), which do not overlap with them. 4,000
-// rows with q4_0 4,096 x 2,560, layout included: 136 us, 0.62 PFLOP/s; 333 with
-// 4,099 x 4,096: 33 us of product, where one round of 64 x 64 fills the chip once.
+// rows with q4_0 4,096 x 2,560, layout included: 121 us, 0.69 PFLOP/s; 333 with
+// 4,099 x 4,096: 31 us of product, where one round of 64 x 64 fills the chip once.
 template <int PLANES, int MINS, int BM, int BN, int WM, int WN, int WK, int G, int ADAPT>
 __global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_matrix(MatrixArgs a) {
     constexpr int WAVES = WM * WN * WK, UM = BM / WM / 32, UN = BN / WN / 32, GW = G / WK;

@@ -95,7 +95,7 @@ struct Layout16Args {
 // Layout: panels of 32 rows; in a panel, for each 16 values, [2][32 rows][8]:
 // an operand of the 32x32x16 instructions is 1,024 bytes in a row. A workgroup
 // lays out 32 rows by 8 groups, a group to a thread. Bound by memory: 4,096 rows
-// and q4_k 9,728 x 2,560, 96 MB read and written, 18.5 us, as fast as a copy.
+// and q4_k 9,728 x 2,560, 96 MB read and written, 19 to 22 us, a copy's rate.
 template <int TYPE>
 __global__ __launch_bounds__(256) void k_lay_out16(Layout16Args a) {
     __shared__ uint16_t grid[Format<TYPE>::GRID ? Format<TYPE>::GRID : 1];
@@ -146,7 +146,7 @@ __global__ __launch_bounds__(256) void k_lay_out16(Layout16Args a) {
 // split the tile, WK the steps of a stage (their sums are joined in LDS at the
 // end, in order): a wave's part of the tile stays large where the tile is not.
 // Where tiles are few the stages are split over workgroups too. 4,096 rows with
-// q4_k 9,728 x 2,560 in tiles of 256 x 320: 203 us, 1.0 PFLOP/s, what a library's
+// q4_k 9,728 x 2,560 in tiles of 256 x 320: 197 us, 1.0 PFLOP/s, what a library's
 // product of the same size in bf16 takes; bound there by the power that matrix
 // instructions draw (the clock falls from 2.4 GHz to 1.9 to 2.0), in smaller
 // products by the latency of a stage's copies, of which one is in flight.

@@ -170,10 +170,10 @@ constexpr int64_t MOST_ROWS = INT64_C(1) << 24;
 template <int SRC>
 hipError_t launch_norm(const NormArgs& all, hipStream_t st) {
     // A wave per row where rows fill the 1,024 SIMDs several times (us with 64, 256
-    // and 1,024 lanes, bf16 with a residual: 8,191 x 2,560 24.5, 27.7, 48; 4,096 x
-    // 1,024 8.2, 10.3, 22), else a workgroup each (2,048 x 9,728 31, 24.5, 26; 1,024
-    // x 2,560 8.2, 6.6, 8.5), a large one where they are few and long (64 x 2,560
-    // 7.0, 4.1, 3.6; 1 x 2,560 6.2, 3.8, 3.2; 333 x 1,024 4.2, 3.6, 4.0).
+    // and 1,024 lanes, bf16 with a residual: 8,191 x 2,560 28, 31, 53; 4,096 x 1,024
+    // 9.9, 11.7, 24.5), else a workgroup each (2,048 x 9,728 37, 28.5, 31; 1,024 x
+    // 2,560 10.7, 8.0, 9.6), a large one where they are few and long (64 x 2,560 7.5,
+    // 4.3, 3.8; 1 x 2,560 6.2, 3.8, 3.3; 333 x 1,024 5.0, 4.1, 4.3).
     const int p = all.rows >= 4096 ? 64 : all.rows <= 256 && all.k > 2048 ? 1024 : 256;
     const int rows = p > 256 ? 1 : 256 / p;
     const size_t lds = (size_t)rows * (all.k / 32) * 4;
