@@ -235,6 +235,10 @@ __global__ __launch_bounds__(256) void k_linear_few(LinearArgs a, FewPlan plan) 
 // a subtraction at full rate in place of a conversion at half rate.
 constexpr float INT_BIAS = 12582912.0f;
 
+// A minimum is multiplied by s * (sum of codes), which can pass f32's largest number
+// where no value does: 2^-12 of it, against 2^12 times the minimum.
+constexpr float CODE_SUM_UNIT = 0x1p-12f, MIN_UNIT = 0x1p12f;
+
 // Each sum is scaled by d[n] * s[t]: a product per element and group, as much
 // vector work as the sums themselves are matrix work. It is an outer product,
 // so the matrix units form it: a factor is cut into three bf16 pieces that add
@@ -371,7 +375,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_linear_tile(LinearArgs
 #pragma unroll
             for (int h = 0; h < SUB; h++) {
                 put(S::WP + (g * SUB + h) * S::WPS + r * 16, weight_slots(live ? w.d[h] : 0.0f));
-                if constexpr (MIN) put(S::WMN + (g * SUB + h) * S::WPS + r * 16, weight_slots(live ? -w.m[h] : 0.0f));
+                if constexpr (MIN) put(S::WMN + (g * SUB + h) * S::WPS + r * 16, weight_slots(live ? -w.m[h] * MIN_UNIT : 0.0f));
             }
         }
 #pragma unroll
@@ -386,8 +390,8 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void k_linear_tile(LinearArgs
             if constexpr (MIN) {
                 const int o0 = dot4(lo.x, qsd::ONES, dot4(lo.y, qsd::ONES, dot4(lo.z, qsd::ONES, dot4(lo.w, qsd::ONES, 0))));
                 const int o1 = dot4(hi.x, qsd::ONES, dot4(hi.y, qsd::ONES, dot4(hi.z, qsd::ONES, dot4(hi.w, qsd::ONES, 0))));
-                put(S::XM + g * SUB * S::XPS + r * 16, row_slots(s * (float)(SUB == 2 ? o0 : o0 + o1)));
-                if constexpr (SUB == 2) put(S::XM + (g * SUB + 1) * S::XPS + r * 16, row_slots(s * (float)o1));
+                put(S::XM + g * SUB * S::XPS + r * 16, row_slots(s * ((float)(SUB == 2 ? o0 : o0 + o1) * CODE_SUM_UNIT)));
+                if constexpr (SUB == 2) put(S::XM + (g * SUB + 1) * S::XPS + r * 16, row_slots(s * ((float)o1 * CODE_SUM_UNIT)));
             }
         }
     };

@@ -92,7 +92,7 @@ QS_DEV void lay_out_weight(const Raw<TYPE>& raw, int g, const uint16_t* grid, bo
     uint2* s = reinterpret_cast<uint2*>(p + 1024 * M::PLANES) + row;
     s[0] = piece_words(live ? d : 0.0f);
 #pragma unroll
-    for (int h = 0; h < M::MINS; h++) s[32 * (1 + h)] = piece_words(live ? -w.m[h] : 0.0f);
+    for (int h = 0; h < M::MINS; h++) s[32 * (1 + h)] = piece_words(live ? -w.m[h] * MIN_UNIT : 0.0f);
 }
 
 struct LayoutArgs {
@@ -143,8 +143,8 @@ __global__ __launch_bounds__(256) void k_lay_out(LayoutArgs a) {
     if constexpr (M::MINS > 0) {
         const int o0 = dot4(lo.x, qsd::ONES, dot4(lo.y, qsd::ONES, dot4(lo.z, qsd::ONES, dot4(lo.w, qsd::ONES, 0))));
         const int o1 = dot4(hi.x, qsd::ONES, dot4(hi.y, qsd::ONES, dot4(hi.z, qsd::ONES, dot4(hi.w, qsd::ONES, 0))));
-        o[32] = piece_words(s * (float)(M::MINS == 2 ? o0 : o0 + o1));
-        if constexpr (M::MINS == 2) o[64] = piece_words(s * (float)o1);
+        o[32] = piece_words(s * ((float)(M::MINS == 2 ? o0 : o0 + o1) * CODE_SUM_UNIT));
+        if constexpr (M::MINS == 2) o[64] = piece_words(s * ((float)o1 * CODE_SUM_UNIT));
     }
 }
 

@@ -38,11 +38,13 @@ QS_DEV float block_bound(P b) {
     else return 167 * h(0);                                             // IQ2: 0.25 * 15.5 * 43
 }
 
-// 2^-e for the largest possible |value| of a row, which that takes to 2^14 .. 2^15
-QS_DEV float row_scale(float bound) {
+// 2^-e for the largest possible |value| of a row, bound * 2^bits (which may pass f32's
+// largest number), that takes it to 2^14 .. 2^15
+QS_DEV float row_scale(float bound, int bits) {
     if (!(bound > 0.0f && bound < __builtin_inff())) return 1.0f;
     int e;
     (void)__builtin_frexpf(bound, &e);          // 2^(e-1) <= bound < 2^e
+    e += bits;
     e = e < -110 ? -110 : e;
     return __builtin_ldexpf(1.0f, 15 - e);
 }
@@ -75,11 +77,11 @@ __global__ __launch_bounds__(256) void k_row_scales(ScaleArgs a) {
         const int groups = (int)(a.k / 32);
         if (row < a.t)
 #pragma unroll 4
-            for (int g = lane; g < groups; g += 8) take(128 * fabsf(a.s[row * groups + g]));
+            for (int g = lane; g < groups; g += 8) take(fabsf(a.s[row * groups + g]));
     }
 #pragma unroll
     for (int o = 1; o < 8; o *= 2) take(__shfl_xor(top, o));
-    if (lane == 0 && row < (weight ? a.n : a.t)) (weight ? a.ws : a.xs)[row] = row_scale(top);
+    if (lane == 0 && row < (weight ? a.n : a.t)) (weight ? a.ws : a.xs)[row] = row_scale(top, weight ? 0 : 7);
 }
 
 struct Layout16Args {
