@@ -227,6 +227,86 @@ int qs_packed_linear(int ggml_type, const void *weight, int64_t n, int64_t k, co
                      int64_t t, int dst_type, void *dst, int64_t dst_bytes, const qs_adapters *adapters,
                      const int32_t *ids, void *workspace, int64_t workspace_bytes, void *hip_stream);
 
+/* ---- a quantised key-value cache ----
+ *
+ * The other half of a layer on packed weights: keys and values quantised to Q8_0
+ * or Q4_0 as they are written to the pages of a cache, read back, and the
+ * attention of new tokens over it. The reference has none of this. Serving forms,
+ * as above: asynchronous and stream-ordered on hip_stream, no allocation, no
+ * synchronisation, no gradient; safe to call from several threads.
+ *
+ * A page holds page_size slots; slot s of the cache is slot s % page_size of page
+ * s / page_size. A slot holds a key and a value of each of `heads` heads, head_dim
+ * values each, in blocks of 32 with an f16 step: the codes and steps that
+ * qs_quantize() gives the same values, in an order of the library's own. Pages are
+ * contiguous and do not refer to each other: bytes of a page may be copied to
+ * another page, of another cache of the same sizes too. A page of zeros holds
+ * slots of zeros. */
+typedef struct qs_kv_cache {
+    int32_t k_type, v_type;     /* QS_TYPE_Q8_0 or QS_TYPE_Q4_0 */
+    int32_t heads;              /* key/value heads, 1..1024 */
+    int32_t head_dim;           /* 64, 128, 192 or 256 */
+    int32_t page_size;          /* slots of a page: a power of two in 16..1024 */
+    int32_t pages;              /* at least 1; pages * page_size < 2^31 */
+    void *data;                 /* pages * qs_kv_page_bytes() bytes, 16-byte aligned */
+} qs_kv_cache;
+
+/* Bytes of a page; negative for sizes that a cache cannot have. */
+int64_t qs_kv_page_bytes(int k_type, int v_type, int heads, int head_dim, int page_size);
+
+/* Rows of keys and values into slots.
+ *   k, v:      rows of heads * head_dim values of src_type (QS_SRC_*), 16-byte
+ *              aligned, row strides multiples of 16 bytes
+ *   slots:     (device) the slot of each row; a row whose slot is not in the cache,
+ *              such as -1, is left out. Of rows with the same slot the last one is
+ *              written.
+ * A NaN, an infinity or a step over f16's largest number makes the values of its
+ * block NaN. rows is at most 2^24. Calls that write the same slot, or read it
+ * meanwhile, must be ordered by the caller. */
+int qs_kv_write(const qs_kv_cache *cache, int src_type, const void *k, int64_t k_row_stride_bytes, const void *v,
+                int64_t v_row_stride_bytes, const int32_t *slots, int64_t rows, void *hip_stream);
+
+/* The values that slots hold, code * step rounded to dst_type: rows of
+ * heads * head_dim values, contiguous, k and v 16-byte aligned. A slot that is not
+ * in the cache gives zeros. rows is at most 2^24. */
+int qs_kv_read(const qs_kv_cache *cache, const int32_t *slots, int64_t rows, int dst_type, void *k, void *v,
+               void *hip_stream);
+
+/* Bytes of workspace that a qs_kv_attention call of these sizes needs; 0 where it
+ * needs none, negative for sizes that it refuses. */
+int64_t qs_kv_attention_workspace(const qs_kv_cache *cache, int64_t batch, int64_t new_tokens, int64_t query_heads,
+                                  int64_t pages_each);
+
+/* Attention of the last new_tokens tokens of each sequence over its slots, which
+ * hold those tokens' keys and values already:
+ *   out[b][i][h] = sum_p softmax_p(scale * q[b][i][h] . K_p) V_p
+ * over positions p <= P = lengths[b] - new_tokens + i, with a window also
+ * p > P - window. Query head h reads key/value head h / (query_heads / heads).
+ *   type:      of q and out (QS_SRC_*)
+ *   q:         batch * new_tokens rows of query_heads * head_dim values, 16-byte
+ *              aligned, the stride between rows a multiple of 16 bytes
+ *   tables:    (device) batch rows of pages_each page numbers, table_stride numbers
+ *              apart: position p of sequence b is slot p % page_size of page
+ *              tables[b][p / page_size]. Positions of a page that is not in the
+ *              cache, such as -1, are seen by no query.
+ *   lengths:   (device) batch lengths, the new tokens counted; they are cut to
+ *              0 .. pages_each * page_size
+ *   window:    0: none
+ *   out:       contiguous, 16-byte aligned
+ *   workspace: qs_kv_attention_workspace() bytes, 256-byte aligned, used by this
+ *              call alone until it is done; may be NULL where that is 0
+ * A query that sees no position gives zeros; what lies at positions that it does
+ * not see does not matter, whatever it is. Sums and statistics are f32; q is held to
+ * 22 bits or more beside its row's largest value, p times a step of V to 21
+ * beside the largest. The result does not depend on timing; in the last bits of f32 it
+ * may depend on the call's other sequences (another split of the sum). batch is at
+ * most 2^14, new_tokens 16, query_heads / heads a whole number up to 128,
+ * pages_each * page_size 2^30. */
+int qs_kv_attention(const qs_kv_cache *cache, int type, const void *q, int64_t q_token_stride_bytes, int64_t batch,
+                    int64_t new_tokens, int64_t query_heads, const int32_t *tables, int64_t pages_each,
+                    int64_t table_stride, const int32_t *lengths, float scale, int64_t window, void *out,
+                    int64_t out_bytes, void *workspace, int64_t workspace_bytes, void *hip_stream);
+
 /* ---- host pipeline of the command line ----
  *
  * Replaces the reference's CudaPipeline (quant-studio.py:148-213), its

@@ -141,6 +141,21 @@ def _bind(L: ctypes.CDLL) -> None:
                                    ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int,
                                    ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p,
                                    ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p]
+    L.qs_kv_page_bytes.restype = ctypes.c_int64
+    L.qs_kv_page_bytes.argtypes = [ctypes.c_int] * 5
+    L.qs_kv_write.restype = ctypes.c_int
+    L.qs_kv_write.argtypes = [ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p,
+                              ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p]
+    L.qs_kv_read.restype = ctypes.c_int
+    L.qs_kv_read.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_void_p,
+                             ctypes.c_void_p, ctypes.c_void_p]
+    L.qs_kv_attention_workspace.restype = ctypes.c_int64
+    L.qs_kv_attention_workspace.argtypes = [ctypes.c_void_p] + [ctypes.c_int64] * 4
+    L.qs_kv_attention.restype = ctypes.c_int
+    L.qs_kv_attention.argtypes = [ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64,
+                                  ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64,
+                                  ctypes.c_void_p, ctypes.c_float, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64,
+                                  ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p]
 
 
 def _load_library() -> ctypes.CDLL:
@@ -365,8 +380,10 @@ QUANT_TYPES: dict[str, QuantSpec] = _registry()
 # a layer on packed weights (torch is imported when one of them is called)
 from .packed import (AdapterBank, PackedWeight, Q8Rows, packed_linear, q8_rows,  # noqa: E402
                      rms_norm_q8)
+# a quantised key-value cache and the attention over it
+from .kv_cache import KVCache, kv_attention, kv_read, kv_write  # noqa: E402
 
-__all__ = ["AdapterBank", "PackedWeight", "Q8Rows", "packed_linear", "q8_rows", "rms_norm_q8",
+__all__ = ["KVCache", "kv_attention", "kv_read", "kv_write", "AdapterBank", "PackedWeight", "Q8Rows", "packed_linear", "q8_rows", "rms_norm_q8",
            "QUANT_TYPES", "ALL_SPECS", "QuantSpec", "QuantSpecError", "TORCH_DTYPES",
            "GGMLQuantizationType", "LlamaFileType", "library", "quantize", "row_bytes", "init",
            "set_sqrt_rounding", "sqrt_rounding"]

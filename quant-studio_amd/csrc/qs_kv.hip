@@ -1,0 +1,402 @@
+// Rows of keys and values quantised into a cache's pages and read back
+// (declarations: include/quant_studio.h; the layout: qs_kv.h).
+#include <hip/hip_runtime.h>
+
+#include "qs_host.h"
+#include "qs_kernels.h"
+#include "qs_kv.h"
+#include "qs_kv_attention.h"
+#include "qs_launch_kernel.h"
+#include "qs_rows.h"
+
+namespace {
+
+using namespace qsr;
+using qs_host::fail;
+using qskv::Cache;
+
+struct RowsArgs {
+    Cache c;
+    void *k, *v;                    // rows of heads x 32 blocks values
+    int64_t k_stride, v_stride;     // between rows, in values
+    const int32_t* slots;
+    int32_t rows, units;            // units: of eight values in a row's keys and values
+    int32_t group;                  // rows of a workgroup
+};
+
+// the eight values of a thread: a quarter of a block, keys or values
+struct Unit {
+    int head, block, quarter;
+    bool value;
+};
+QS_DEV Unit unit_of(const Cache& c, int u) {
+    const int per_head = 4 * c.blocks;
+    Unit o;
+    o.value = u >= per_head * c.heads;
+    u -= o.value ? per_head * c.heads : 0;
+    o.head = u / per_head;
+    u -= o.head * per_head;
+    o.block = u >> 2;
+    o.quarter = u & 3;
+    return o;
+}
+// the codes of the unit's head and kind in the slot's row, and its step
+struct Place {
+    uint8_t* row;
+    uint16_t* step;
+};
+QS_DEV Place place_of(const Cache& c, const Unit& u, int slot) {
+    const int at = slot & (c.page - 1);
+    uint8_t* p = qskv::head_of(c, slot >> c.shift, u.head);
+    const int bits = u.value ? c.v_bits : c.k_bits, row = qskv::row_bytes(bits, c.blocks);
+    if (u.value) p += c.page * (qskv::row_bytes(c.k_bits, c.blocks) + 2 * c.blocks);
+    return {p + at * row, reinterpret_cast<uint16_t*>(p + c.page * row) + at * c.blocks + u.block};
+}
+
+constexpr int MOST_GROUP = 32;
+
+// A thread takes eight values, four threads a block of 32: its step from their
+// largest magnitude, then eight codes each, in the order of the cache's rows.
+// Of rows with the same slot the last is written: every workgroup looks its rows'
+// slots up among all later ones, which a launch's few rows make cheap.
+template <int SRC>
+__global__ __launch_bounds__(256) void k_kv_write(RowsArgs a) {
+    __shared__ int mine[MOST_GROUP];
+    const int first = (int)blockIdx.x * a.group;
+    const int count = a.rows - first < a.group ? a.rows - first : a.group;
+    const int slots = a.c.pages << a.c.shift;
+    if ((int)threadIdx.x < count) {
+        const int s = a.slots[first + threadIdx.x];
+        mine[threadIdx.x] = (unsigned)s < (unsigned)slots ? s : -1;
+    }
+    __syncthreads();
+    if (a.rows - first > 1) {
+        uint32_t later = 0;     // rows of this group that a later one replaces
+        for (int r = first + 1 + (int)threadIdx.x; r < a.rows; r += 256) {
+            const int s = a.slots[r];
+            for (int i = 0; i < count; i++) later |= s == mine[i] && first + i < r ? 1u << i : 0u;
+        }
+        __syncthreads();
+        for (int i = 0; i < count; i++)
+            if (later >> i & 1) mine[i] = -1;
+        __syncthreads();
+    }
+    const int wide = a.units < 256 ? a.units : 256, step_rows = 256 / wide;
+    const int sub = (int)threadIdx.x / wide;
+    const int at = (int)blockIdx.y * 256 + ((int)threadIdx.x - sub * wide);
+    if (sub >= step_rows || at >= a.units) return;
+    const Unit u = unit_of(a.c, at);
+    const void* src = u.value ? a.v : a.k;
+    const int64_t stride = u.value ? a.v_stride : a.k_stride;
+    const int bits = u.value ? a.c.v_bits : a.c.k_bits;
+    for (int i = sub; i < count; i += step_rows) {
+        const int slot = mine[i];
+        if (slot < 0) continue;     // the same for the four threads of a block
+        Eight<SRC> in;
+        load8<SRC>(src, (first + i) * stride + (int64_t)u.head * 32 * a.c.blocks + 32 * u.block + 8 * u.quarter, in);
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) x[j] = value8<SRC>(in, j);
+        float d;
+        uint32_t code[8];           // as the cache holds them
+        if (bits == 8) {
+            float top = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const float m = fabsf(x[j]);
+                top = m > top || m != m ? m : top;      // keeps a NaN
+            }
+            const float m1 = qs::quad_xor<1>(top);
+            top = m1 > top || m1 != m1 ? m1 : top;
+            const float m2 = qs::quad_xor<2>(top);
+            top = m2 > top || m2 != m2 ? m2 : top;
+            d = top / 127.0f;
+            const float id = d != 0.0f ? 1.0f / d : 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                // -128 comes of steps below f16's smallest only, where the value is 0
+                const int q = max(qs::code_of(x[j], id), -127);
+                code[j] = q < 0 ? 128u - (uint32_t)q : (uint32_t)q;
+            }
+        } else {
+            d = qs::quad_absmax_first(x, u.quarter) * -0.125f;
+            const float id = d != 0.0f ? 1.0f / d : 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; j++) code[j] = qs::level_of(x[j], id, 8.5f, 15.5f);
+        }
+        const Place p = place_of(a.c, u, slot);
+        // a step that f16 cannot hold, like a NaN or an infinity in the block, stands for no values
+        const uint32_t h = qs::f16_bits(d);
+        if (u.quarter == 0) *p.step = (uint16_t)((h & 0x7fffu) < 0x7c00u ? h : 0x7e00u);
+        if (!u.value) {
+            uint8_t* o = p.row + qskv::k_unit(bits, a.c.blocks, u.quarter, u.block);
+            if (bits == 8) {
+                uint32_t w[2];
+                qs::bytes_of(code, w);
+                *reinterpret_cast<uint2*>(o) = uint2{w[0], w[1]};
+            } else {
+                uint32_t w = 0;
+#pragma unroll
+                for (int j = 0; j < 8; j++) w |= code[j] << (4 * (j >> 1) + 16 * (j & 1));
+                *reinterpret_cast<uint32_t*>(o) = w;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                uint8_t* o = p.row + qskv::v_unit(bits, a.c.blocks, 4 * u.quarter + j, u.block);
+                if (bits == 8) *reinterpret_cast<uint16_t*>(o) = (uint16_t)(code[2 * j] | code[2 * j + 1] << 8);
+                else *o = (uint8_t)(code[2 * j] | code[2 * j + 1] << 4);
+            }
+        }
+    }
+}
+
+// The values of some slots' rows; a slot outside the cache gives zeros.
+template <int DST>
+__global__ __launch_bounds__(256) void k_kv_read(RowsArgs a) {
+    const int first = (int)blockIdx.x * a.group;
+    const int count = a.rows - first < a.group ? a.rows - first : a.group;
+    const int slots = a.c.pages << a.c.shift;
+    const int wide = a.units < 256 ? a.units : 256, step_rows = 256 / wide;
+    const int sub = (int)threadIdx.x / wide;
+    const int at = (int)blockIdx.y * 256 + ((int)threadIdx.x - sub * wide);
+    if (sub >= step_rows || at >= a.units) return;
+    const Unit u = unit_of(a.c, at);
+    void* dst = u.value ? a.v : a.k;
+    const int64_t stride = u.value ? a.v_stride : a.k_stride;
+    const int bits = u.value ? a.c.v_bits : a.c.k_bits;
+    for (int i = sub; i < count; i += step_rows) {
+        const int slot = a.slots[first + i];
+        float x[8] = {};
+        if ((unsigned)slot < (unsigned)slots) {
+            const Place p = place_of(a.c, u, slot);
+            const float d = qskv::half_of(*p.step);
+            if (!u.value) {
+                const uint8_t* o = p.row + qskv::k_unit(bits, a.c.blocks, u.quarter, u.block);
+                if (bits == 8) {
+                    const uint2 w = *reinterpret_cast<const uint2*>(o);
+#pragma unroll
+                    for (int j = 0; j < 8; j++) x[j] = qskv::code8((j < 4 ? w.x : w.y) >> (8 * (j & 3))) * d;
+                } else {
+                    const uint32_t w = *reinterpret_cast<const uint32_t*>(o);
+#pragma unroll
+                    for (int j = 0; j < 8; j++) x[j] = qskv::code4(w >> (4 * (j >> 1) + 16 * (j & 1))) * d;
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const uint8_t* o = p.row + qskv::v_unit(bits, a.c.blocks, 4 * u.quarter + j, u.block);
+                    if (bits == 8) {
+                        const uint32_t w = *reinterpret_cast<const uint16_t*>(o);
+                        x[2 * j] = qskv::code8(w) * d, x[2 * j + 1] = qskv::code8(w >> 8) * d;
+                    } else {
+                        x[2 * j] = qskv::code4(*o) * d, x[2 * j + 1] = qskv::code4(*o >> 4) * d;
+                    }
+                }
+            }
+        }
+        store8<DST>(dst, (first + i) * stride + (int64_t)u.head * 32 * a.c.blocks + 32 * u.block + 8 * u.quarter, x);
+    }
+}
+
+// rows of a launch: what a workgroup looks its slots up among
+constexpr int64_t MOST_ROWS = 8192;
+
+template <typename F>
+hipError_t launch_rows(const RowsArgs& all, int esz, F&& kernel, hipStream_t st) {
+    const int wide = all.units < 256 ? all.units : 256, step_rows = 256 / wide;
+    for (int64_t first = 0; first < all.rows; first += MOST_ROWS) {
+        RowsArgs a = all;
+        a.rows = (int32_t)(all.rows - first < MOST_ROWS ? all.rows - first : MOST_ROWS);
+        a.k = static_cast<char*>(all.k) + first * all.k_stride * esz;
+        a.v = static_cast<char*>(all.v) + first * all.v_stride * esz;
+        a.slots = all.slots + first;
+        a.group = step_rows * (a.rows > 1024 ? (step_rows > 4 ? 2 : 8) : 1);
+        const dim3 grid((unsigned)((a.rows + a.group - 1) / a.group), (unsigned)((a.units + 255) / 256));
+        const hipError_t e = qs_host::launch_kernel(kernel, grid, dim3(256), 0, st, a);
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
+}
+
+constexpr int64_t kMaxRows = INT64_C(1) << 24, kMaxBatch = INT64_C(1) << 14, kMaxSpan = INT64_C(1) << 62;
+bool off16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 != 0; }
+bool off4(const void* p) { return reinterpret_cast<uintptr_t>(p) % 4 != 0; }
+int bits_of(int type) { return type == QS_TYPE_Q8_0 ? 8 : type == QS_TYPE_Q4_0 ? 4 : 0; }
+int size_of(int src) { return src == QS_SRC_F32 ? 4 : (src == QS_SRC_F16 || src == QS_SRC_BF16) ? 2 : 0; }
+
+int bad_layout(int k_type, int v_type, int heads, int head_dim, int page_size) {
+    if (!bits_of(k_type) || !bits_of(v_type))
+        return fail(QS_ENOTSUP, "cache types %d and %d: Q8_0 (8) or Q4_0 (2)", k_type, v_type);
+    if (heads < 1 || heads > 1024) return fail(QS_EINVAL, "%d heads, not 1..1024", heads);
+    if (head_dim < 64 || head_dim > 256 || head_dim % 64)
+        return fail(QS_EINVAL, "head size %d is not 64, 128, 192 or 256", head_dim);
+    if (page_size < 16 || page_size > 1024 || (page_size & (page_size - 1)))
+        return fail(QS_EINVAL, "page of %d slots: not a power of two in 16..1024", page_size);
+    return 0;
+}
+
+int attention_sizes(const qs_kv_cache* cache, int64_t batch, int64_t fresh, int64_t query_heads, int64_t pages_each,
+                    qskv::AttentionArgs& a) {
+    const int bad = qskv::cache_of(cache, a.c);
+    if (bad) return bad;
+    if (batch < 0 || batch > kMaxBatch) return fail(QS_EINVAL, "%lld sequences: negative, or over 2^14", (long long)batch);
+    if (fresh < 0 || fresh > 16) return fail(QS_EINVAL, "%lld new tokens of a sequence: not 0..16", (long long)fresh);
+    if (query_heads < 1 || query_heads % a.c.heads || query_heads / a.c.heads > 128)
+        return fail(QS_EINVAL, "%lld query heads: not 1 to 128 for each of %d key/value heads", (long long)query_heads, a.c.heads);
+    if (pages_each < 0 || pages_each > (INT32_C(1) << 30) / a.c.page)
+        return fail(QS_EINVAL, "tables of %lld pages of %d slots: negative, or over 2^30 slots", (long long)pages_each, a.c.page);
+    a.batch = (int32_t)batch;
+    a.fresh = (int32_t)fresh;
+    a.group = (int32_t)(query_heads / a.c.heads);
+    a.pages_each = (int32_t)pages_each;
+    return 0;
+}
+
+}  // namespace
+
+namespace qskv {
+
+extern template hipError_t launch_attention<8, 8>(const AttentionArgs&, hipStream_t);
+extern template hipError_t launch_attention<8, 4>(const AttentionArgs&, hipStream_t);
+extern template hipError_t launch_attention<4, 8>(const AttentionArgs&, hipStream_t);
+extern template hipError_t launch_attention<4, 4>(const AttentionArgs&, hipStream_t);
+
+int cache_of(const qs_kv_cache* cache, Cache& c) {
+    if (!cache) return fail(QS_EINVAL, "null cache");
+    const int bad = bad_layout(cache->k_type, cache->v_type, cache->heads, cache->head_dim, cache->page_size);
+    if (bad) return bad;
+    if (cache->pages < 1 || cache->pages > INT32_MAX / cache->page_size)
+        return fail(QS_EINVAL, "%d pages of %d slots: none, or over 2^31 - 1 slots", cache->pages, cache->page_size);
+    if (!cache->data || off16(cache->data)) return fail(QS_EINVAL, "cache data %p is null or not 16-byte aligned", cache->data);
+    c.data = static_cast<uint8_t*>(cache->data);
+    c.pages = cache->pages;
+    c.page = cache->page_size;
+    c.shift = __builtin_ctz(cache->page_size);
+    c.heads = cache->heads;
+    c.blocks = cache->head_dim / 32;
+    c.k_bits = bits_of(cache->k_type);
+    c.v_bits = bits_of(cache->v_type);
+    c.page_bytes = (int64_t)c.page * c.heads * slot_bytes(c.k_bits, c.v_bits, c.blocks);
+    return 0;
+}
+
+}  // namespace qskv
+
+extern "C" {
+
+int64_t qs_kv_page_bytes(int k_type, int v_type, int heads, int head_dim, int page_size) {
+    qs_host::clear_error();
+    const int bad = bad_layout(k_type, v_type, heads, head_dim, page_size);
+    if (bad) return bad;
+    return (int64_t)page_size * heads * qskv::slot_bytes(bits_of(k_type), bits_of(v_type), head_dim / 32);
+}
+
+int qs_kv_write(const qs_kv_cache* cache, int src_type, const void* k, int64_t k_row_stride_bytes, const void* v,
+                int64_t v_row_stride_bytes, const int32_t* slots, int64_t rows, void* hip_stream) {
+    qs_host::clear_error();
+    RowsArgs a{};
+    const int bad = qskv::cache_of(cache, a.c);
+    if (bad) return bad;
+    const int esz = size_of(src_type);
+    if (!esz) return fail(QS_EINVAL, "unsupported source type %d (F32=0, F16=1, BF16=30)", src_type);
+    if (rows < 0 || rows > kMaxRows) return fail(QS_EINVAL, "%lld rows: negative, or over 2^24", (long long)rows);
+    if (rows == 0) return 0;
+    if (!k || !v || !slots) return fail(QS_EINVAL, "null k, v or slots");
+    if (off16(k) || off16(v) || off4(slots)) return fail(QS_EINVAL, "k and v must be 16-byte aligned, slots 4-byte");
+    const int64_t width = (int64_t)a.c.heads * 32 * a.c.blocks * esz;
+    for (int64_t s : {k_row_stride_bytes, v_row_stride_bytes})
+        if ((s < width && rows > 1) || s < 0 || s % 16 || s > kMaxSpan / rows)
+            return fail(QS_EINVAL, "row stride %lld must be >= %lld, a multiple of 16 and in a 2^62-byte span", (long long)s,
+                        (long long)width);
+    a.k = const_cast<void*>(k);
+    a.v = const_cast<void*>(v);
+    a.k_stride = k_row_stride_bytes / esz;
+    a.v_stride = v_row_stride_bytes / esz;
+    a.slots = slots;
+    a.rows = (int32_t)rows;
+    a.units = 8 * a.c.heads * a.c.blocks;
+    const auto kernel = src_type == QS_SRC_F32   ? k_kv_write<qs::SRC_F32>
+                        : src_type == QS_SRC_F16 ? k_kv_write<qs::SRC_F16>
+                                                 : k_kv_write<qs::SRC_BF16>;
+    const hipError_t e = launch_rows(a, esz, kernel, static_cast<hipStream_t>(hip_stream));
+    if (e != hipSuccess) return fail(QS_EIO, "kv_write: launch failed: %s", hipGetErrorString(e));
+    return 0;
+}
+
+int qs_kv_read(const qs_kv_cache* cache, const int32_t* slots, int64_t rows, int dst_type, void* k, void* v,
+               void* hip_stream) {
+    qs_host::clear_error();
+    RowsArgs a{};
+    const int bad = qskv::cache_of(cache, a.c);
+    if (bad) return bad;
+    const int esz = size_of(dst_type);
+    if (!esz) return fail(QS_EINVAL, "unsupported destination type %d (F32=0, F16=1, BF16=30)", dst_type);
+    if (rows < 0 || rows > kMaxRows) return fail(QS_EINVAL, "%lld rows: negative, or over 2^24", (long long)rows);
+    if (rows == 0) return 0;
+    if (!k || !v || !slots) return fail(QS_EINVAL, "null k, v or slots");
+    if (off16(k) || off16(v) || off4(slots)) return fail(QS_EINVAL, "k and v must be 16-byte aligned, slots 4-byte");
+    a.k = k;
+    a.v = v;
+    a.k_stride = a.v_stride = (int64_t)a.c.heads * 32 * a.c.blocks;
+    a.slots = slots;
+    a.rows = (int32_t)rows;
+    a.units = 8 * a.c.heads * a.c.blocks;
+    const auto kernel = dst_type == QS_SRC_F32   ? k_kv_read<qs::SRC_F32>
+                        : dst_type == QS_SRC_F16 ? k_kv_read<qs::SRC_F16>
+                                                 : k_kv_read<qs::SRC_BF16>;
+    const hipError_t e = launch_rows(a, esz, kernel, static_cast<hipStream_t>(hip_stream));
+    if (e != hipSuccess) return fail(QS_EIO, "kv_read: launch failed: %s", hipGetErrorString(e));
+    return 0;
+}
+
+int64_t qs_kv_attention_workspace(const qs_kv_cache* cache, int64_t batch, int64_t new_tokens, int64_t query_heads,
+                                  int64_t pages_each) {
+    qs_host::clear_error();
+    qskv::AttentionArgs a{};
+    const int bad = attention_sizes(cache, batch, new_tokens, query_heads, pages_each, a);
+    return bad ? bad : 0;
+}
+
+int qs_kv_attention(const qs_kv_cache* cache, int type, const void* q, int64_t q_token_stride_bytes, int64_t batch,
+                    int64_t new_tokens, int64_t query_heads, const int32_t* tables, int64_t pages_each,
+                    int64_t table_stride, const int32_t* lengths, float scale, int64_t window, void* out,
+                    int64_t out_bytes, void* workspace, int64_t workspace_bytes, void* hip_stream) {
+    qs_host::clear_error();
+    qskv::AttentionArgs a{};
+    const int bad = attention_sizes(cache, batch, new_tokens, query_heads, pages_each, a);
+    if (bad) return bad;
+    const int esz = size_of(type);
+    if (!esz) return fail(QS_EINVAL, "unsupported query type %d (F32=0, F16=1, BF16=30)", type);
+    if (window < 0) return fail(QS_EINVAL, "window %lld < 0", (long long)window);
+    const int64_t tokens = batch * new_tokens, width = query_heads * cache->head_dim * esz;
+    if (tokens == 0) return 0;
+    if (!q || !lengths || !out || (pages_each > 0 && !tables)) return fail(QS_EINVAL, "null q, tables, lengths or out");
+    if (off16(q) || off16(out) || off4(tables) || off4(lengths))
+        return fail(QS_EINVAL, "q and out must be 16-byte aligned, tables and lengths 4-byte");
+    if ((q_token_stride_bytes < width && tokens > 1) || q_token_stride_bytes < 0 || q_token_stride_bytes % 16 ||
+        q_token_stride_bytes > kMaxSpan / tokens)
+        return fail(QS_EINVAL, "token stride %lld must be >= %lld, a multiple of 16 and in a 2^62-byte span",
+                    (long long)q_token_stride_bytes, (long long)width);
+    if (table_stride < pages_each || table_stride > kMaxSpan / batch / 4)
+        return fail(QS_EINVAL, "table stride %lld must be >= %lld and in a 2^62-byte span", (long long)table_stride,
+                    (long long)pages_each);
+    if (out_bytes < tokens * width)
+        return fail(QS_EINVAL, "out holds %lld bytes, %lld needed", (long long)out_bytes, (long long)(tokens * width));
+    a.q = q;
+    a.out = out;
+    a.tables = tables;
+    a.lengths = lengths;
+    a.q_stride = q_token_stride_bytes / esz;
+    a.table_stride = table_stride;
+    a.window = (int32_t)(window < INT32_MAX ? window : 0);      // as long as any sequence: none
+    a.type = type;
+    a.scale = scale;
+    hipStream_t st = static_cast<hipStream_t>(hip_stream);
+    const hipError_t e = a.c.k_bits == 8 ? (a.c.v_bits == 8 ? qskv::launch_attention<8, 8>(a, st) : qskv::launch_attention<8, 4>(a, st))
+                                         : (a.c.v_bits == 8 ? qskv::launch_attention<4, 8>(a, st) : qskv::launch_attention<4, 4>(a, st));
+    if (e != hipSuccess) return fail(QS_EIO, "kv_attention: launch failed: %s", hipGetErrorString(e));
+    return 0;
+}
+
+}  // extern "C"

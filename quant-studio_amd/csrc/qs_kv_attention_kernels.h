@@ -1,0 +1,453 @@
+// The attention kernel (gfx950).
+//
+// A wave takes 32 slots of one key/value head at a time and up to eight of its
+// queries (the head's group of query heads, times the new tokens). Two matrix
+// products of 16 x 16 x 32 f16 per 16 slots and block of 32 dimensions:
+//
+//   scores   D[slot][query] = codes[slot][dim] q[dim][query], one product for a
+//            block, so that the slot's step multiplies its sum: S += step D
+//   values   acc[dim][query] += codes[dim][slot] P[slot][query], one for 16 of a
+//            block's dimensions, with P = p step (the step runs along the sum)
+//
+// The scores' D has its slots where the values' P wants them (a lane: one query,
+// slots 4 g .. 4 g + 3 of both sixteens), so nothing moves between lanes; codes go
+// to f16 without a conversion, as subnormal numbers (c 2^-24), which the matrix
+// units multiply exactly. p and P are held to 22 bits: a query has two of the 16
+// columns, one takes f16(P), the other f16(P - f16(P)). So that the second does
+// not fall below f16's range, p is relative to R = m - s, with m the running
+// maximum and 2^s the power of two that takes the largest step so far to 2^14 ..
+// 2^15: what is lost is under 2^-39 of the largest P. q is rounded to f16 after its
+// row is scaled to 2^14 .. 2^15 in the same way: all of a bf16 or f16 q down to
+// 2^-39 of the row's largest; an f32 q takes two products, 22 bits.
+// Four-bit codes have an offset: q's sums over each block start the scores'
+// products, and P's sums over the slots are taken off at the end.
+#pragma once
+
+#include "qs_kv_attention.h"
+#include "qs_launch_kernel.h"
+#include "qs_rows.h"
+
+namespace qskv {
+
+typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
+typedef __fp16 fp16x2_t __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int TILE = 32;                // slots of a wave's step
+constexpr float LOG2E = 1.44269504088896341f;
+
+QS_DEV f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c, 0, 0, 0);
+}
+
+// f over the four lanes that hold a query's slots (lane ^ 16, ^ 32), for an f
+// whose value does not depend on its operands' order
+template <typename F>
+QS_DEV uint32_t over_slots(uint32_t v, F&& f) {
+    const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = f(a[0], a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return f(b[0], b[1]);
+}
+QS_DEV float max_over_slots(float v) {
+    return __uint_as_float(over_slots(__float_as_uint(v), [](uint32_t a, uint32_t b) {
+        return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+    }));
+}
+QS_DEV float sum_over_slots(float v) {
+    return __uint_as_float(over_slots(__float_as_uint(v), [](uint32_t a, uint32_t b) {
+        return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+    }));
+}
+// the other column of the lane's query (lane ^ 8)
+QS_DEV float other_column(float v) {
+    return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), 0x128, 0xF, 0xF, true));
+}
+
+// N bytes of consecutive codes as words
+template <int N>
+struct Codes {
+    uint32_t w[(N + 3) / 4];
+};
+template <int N>
+QS_DEV void load(Codes<N>& o, const uint8_t* p) {
+    if constexpr (N % 16 == 0) {
+#pragma unroll
+        for (int i = 0; i < N / 16; i++) {
+            const u32x4 v = reinterpret_cast<const u32x4*>(p)[i];
+#pragma unroll
+            for (int j = 0; j < 4; j++) o.w[4 * i + j] = v[j];
+        }
+    } else if constexpr (N % 8 == 0) {
+#pragma unroll
+        for (int i = 0; i < N / 8; i++) {
+            const u32x2 v = reinterpret_cast<const u32x2*>(p)[i];
+            o.w[2 * i] = v[0], o.w[2 * i + 1] = v[1];
+        }
+    } else if constexpr (N % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < N / 4; i++) o.w[i] = reinterpret_cast<const uint32_t*>(p)[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < (N + 3) / 4; i++) {
+            const uint16_t* h = reinterpret_cast<const uint16_t*>(p) + 2 * i;
+            o.w[i] = 4 * i + 2 < N ? (uint32_t)h[0] | (uint32_t)h[1] << 16 : (uint32_t)h[0];
+        }
+    }
+}
+
+QS_DEV uint32_t sign_and_magnitude(uint32_t w, uint32_t pick) {
+    return __builtin_amdgcn_perm(0u, w, pick) & 0x807f807fu;
+}
+
+// eight codes of a key's block as f16
+template <int BITS, int BLOCKS>
+QS_DEV u32x4 key_block(const Codes<BITS * BLOCKS>& c, int b) {
+    u32x4 o;
+    if constexpr (BITS == 8) {
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            o[2 * i] = sign_and_magnitude(c.w[2 * b + i], 0x01010000u);
+            o[2 * i + 1] = sign_and_magnitude(c.w[2 * b + i], 0x03030202u);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) o[i] = (c.w[b] >> (4 * i)) & 0x000f000fu;
+    }
+    return o;
+}
+// code n of two slots as f16
+template <int BITS, int N>
+QS_DEV uint32_t value_pair(const Codes<N>& x, const Codes<N>& y, int n) {
+    if constexpr (BITS == 8) {
+        const uint32_t at = n & 3;
+        return __builtin_amdgcn_perm(y.w[n >> 2], x.w[n >> 2], at * 0x01010101u + 0x04040000u) & 0x807f807fu;
+    } else {
+        const uint32_t both = __builtin_amdgcn_perm(y.w[n >> 3], x.w[n >> 3], n & 4 ? 0x07060302u : 0x05040100u);
+        return (both >> (4 * (n & 3))) & 0x000f000fu;
+    }
+}
+
+// the queries of a wave, as the scores' products take them
+template <int BLOCKS, bool WIDE, bool OFFSET>
+struct Queries {
+    u32x4 q[BLOCKS], lo[WIDE ? BLOCKS : 1];
+    float start[OFFSET ? BLOCKS : 1];       // what a block's offset comes to
+    float scale;                            // of the scores, beside 2^up
+    int up;
+    int first, last;                        // slots that the lane's query sees: first .. last - 1
+    bool live;
+};
+
+template <int K_BITS, int BLOCKS, bool WIDE>
+QS_DEV void load_queries(const AttentionArgs& a, int seq, int head, int tile, int length,
+                         Queries<BLOCKS, WIDE, K_BITS == 4>& o) {
+    const int lane = threadIdx.x & 63, g = lane >> 4, column = tile * COLUMNS + (lane & 7);
+    o.live = column < a.group * a.fresh;
+    const int token = o.live ? column / a.group : 0, mine = o.live ? column - token * a.group : 0;
+    const int64_t at = ((int64_t)seq * a.fresh + token) * a.q_stride + (int64_t)(head * a.group + mine) * 32 * BLOCKS;
+    float x[BLOCKS][8];
+    float top = 0.0f;
+#pragma unroll
+    for (int b = 0; b < BLOCKS; b++) {
+        if constexpr (WIDE) {
+            qsr::Eight<qs::SRC_F32> e;
+            qsr::load8<qs::SRC_F32>(a.q, at + 32 * b + 8 * g, e);
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[b][i] = qsr::value8<qs::SRC_F32>(e, i);
+        } else {
+            qsr::Eight<qs::SRC_BF16> e;
+            qsr::load8<qs::SRC_BF16>(a.q, at + 32 * b + 8 * g, e);
+            const bool bf16 = a.type == QS_SRC_BF16;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const uint32_t h = e.w[0][i >> 1] >> (16 * (i & 1));
+                x[b][i] = bf16 ? __uint_as_float(h << 16) : half_of(h);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            x[b][i] = o.live ? x[b][i] : 0.0f;
+            top = fmaxf(top, fabsf(x[b][i]));
+        }
+    }
+    top = max_over_slots(top);
+    const bool scaled = top > 0.0f && top < __builtin_inff();
+    const int e = scaled ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;     // top 2^e in 2^14 .. 2^15
+#pragma unroll
+    for (int b = 0; b < BLOCKS; b++) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            half2_t h, l;
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const float v = __builtin_ldexpf(x[b][2 * i + j], e);
+                h[j] = (_Float16)v;
+                sum += (float)h[j];
+                if constexpr (WIDE) {
+                    l[j] = (_Float16)(v - (float)h[j]);
+                    sum += (float)l[j];
+                }
+            }
+            o.q[b][i] = __builtin_bit_cast(uint32_t, h);
+            if constexpr (WIDE) o.lo[b][i] = __builtin_bit_cast(uint32_t, l);
+        }
+        if constexpr (K_BITS == 4) o.start[b] = sum_over_slots(sum) * (-8.0f * 0x1p-24f);
+    }
+    o.scale = a.scale * LOG2E;
+    o.up = 24 - e;
+    o.last = length - a.fresh + 1 + token;
+    o.first = a.window > 0 && o.last > a.window ? o.last - a.window : 0;
+}
+
+// what a wave has summed up of its slots
+template <int BLOCKS, bool OFFSET>
+struct Sums {
+    f32x4 acc[BLOCKS][2];               // dims 32 block + 8 g + 2 r + e at [block][e][r]
+    float offset[OFFSET ? BLOCKS : 1];
+    float top, ref, total;              // running maximum, R, sum of p
+    int step;                           // bits of the largest step so far
+};
+template <int BLOCKS, bool OFFSET>
+QS_DEV void clear(Sums<BLOCKS, OFFSET>& o) {
+#pragma unroll
+    for (int b = 0; b < BLOCKS; b++) {
+        o.acc[b][0] = o.acc[b][1] = f32x4{0, 0, 0, 0};
+        if constexpr (OFFSET) o.offset[b] = 0.0f;
+    }
+    o.top = o.ref = -__builtin_inff();
+    o.total = 0.0f;
+    o.step = 0;
+}
+
+// What the queries of a wave see: any of them slots first .. last - 1, all of them
+// slots all_first .. all_last - 1.
+struct Span {
+    int first, last, all_first, all_last;
+};
+QS_DEV Span span_of(const AttentionArgs& a, int tile, int length) {
+    const int high = min(a.group * a.fresh, (tile + 1) * COLUMNS) - 1;
+    Span s;
+    s.last = length - a.fresh + 1 + high / a.group;
+    s.all_last = length - a.fresh + 1 + tile * COLUMNS / a.group;
+    s.first = a.window > 0 && s.all_last > a.window ? s.all_last - a.window : 0;
+    s.all_first = a.window > 0 && s.last > a.window ? s.last - a.window : 0;
+    return s;
+}
+
+// One step: the slots start .. start + 31 of a sequence whose pages are `table`
+// (`pages_each` of them).
+template <int K_BITS, int V_BITS, int BLOCKS, bool WIDE>
+QS_DEV void attend(const AttentionArgs& a, const int32_t* table, int head, int start, const Span& span,
+                   const Queries<BLOCKS, WIDE, K_BITS == 4>& q, Sums<BLOCKS, V_BITS == 4>& sums) {
+    constexpr int KROW = row_bytes(K_BITS, BLOCKS), VROW = row_bytes(V_BITS, BLOCKS), STEPS = 2 * BLOCKS;
+    const int lane = threadIdx.x & 63, g = lane >> 4, m = lane & 15;
+    Codes<KROW / 4> kc[2];
+    Codes<4 * STEPS> ks[2], vs[2];
+    Codes<VROW / 16> vc[2][4];
+    bool held[2];
+#pragma unroll
+    for (int s = 0; s < 2; s++) {
+        const int at = start + 16 * s, entry = at >> a.c.shift, slot = at & (a.c.page - 1);
+        int page = entry < a.pages_each ? table[entry] : -1;
+        held[s] = (unsigned)page < (unsigned)a.c.pages;
+        page = held[s] ? page : 0;              // there is one; what it holds is not used
+        const uint8_t* p = head_of(a.c, page, head);
+        load(kc[s], p + (slot + m) * KROW + g * (KROW / 4));
+        p += a.c.page * KROW;
+        load(ks[s], p + (slot + 4 * g) * STEPS);
+        p += a.c.page * STEPS;
+#pragma unroll
+        for (int r = 0; r < 4; r++) load(vc[s][r], p + (slot + 4 * g + r) * VROW + m * (VROW / 16));
+        p += a.c.page * VROW;
+        load(vs[s], p + (slot + 4 * g) * STEPS);
+    }
+    const auto step_of = [](const Codes<4 * STEPS>& c, int r, int b) {
+        const int n = r * BLOCKS + b;
+        return half_of(c.w[n >> 1] >> (16 * (n & 1)));
+    };
+    // scores, in powers of two
+    float x[2][4];
+#pragma unroll
+    for (int s = 0; s < 2; s++) {
+#pragma unroll
+        for (int r = 0; r < 4; r++) x[s][r] = 0.0f;
+#pragma unroll
+        for (int b = 0; b < BLOCKS; b++) {
+            const u32x4 k = key_block<K_BITS, BLOCKS>(kc[s], b);
+            const float c0 = K_BITS == 4 ? q.start[K_BITS == 4 ? b : 0] : 0.0f;
+            f32x4 d = mfma(k, q.q[b], f32x4{c0, c0, c0, c0});
+            if constexpr (WIDE) d = mfma(k, q.lo[b], d);
+#pragma unroll
+            for (int r = 0; r < 4; r++) x[s][r] = __builtin_fmaf(d[r], step_of(ks[s], r, b), x[s][r]);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; r++) x[s][r] = __builtin_ldexpf(x[s][r] * q.scale, q.up);
+    }
+    // a step at an edge: what a query does not see counts for nothing, whatever is there
+    uint32_t seen = 0xff;
+    const bool edge = start < span.all_first || start + TILE > span.all_last || !held[0] || !held[1];
+    if (edge) {
+        seen = 0;
+        bool any[2][4];
+#pragma unroll
+        for (int s = 0; s < 2; s++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const int at = start + 16 * s + 4 * g + r;
+                seen |= (held[s] && at >= q.first && at < q.last ? 1u : 0u) << (4 * s + r);
+                any[s][r] = held[s] && at >= span.first && at < span.last;
+                x[s][r] = seen >> (4 * s + r) & 1 ? x[s][r] : -__builtin_inff();
+            }
+        // and steps of slots that none sees are 0
+#pragma unroll
+        for (int s = 0; s < 2; s++)
+#pragma unroll
+            for (int i = 0; i < STEPS; i++) {
+                const uint32_t low = any[s][2 * i / BLOCKS] ? 0xffffu : 0u, high = any[s][(2 * i + 1) / BLOCKS] ? 0xffff0000u : 0u;
+                vs[s].w[i] &= low | high;
+            }
+    }
+    // the running maximum and R
+    float top = sums.top;
+    uint32_t big = 0;
+#pragma unroll
+    for (int s = 0; s < 2; s++) {
+#pragma unroll
+        for (int r = 0; r < 4; r++) top = fmaxf(top, x[s][r]);
+#pragma unroll
+        for (int i = 0; i < STEPS; i++) {
+            big = max(big, vs[s].w[i] & 0x7fffu);
+            big = max(big, (vs[s].w[i] >> 16) & 0x7fffu);
+        }
+    }
+    top = max_over_slots(top);
+    big = over_slots(big, [](uint32_t u, uint32_t v) { return max(u, v); });
+    sums.step = max(sums.step, (int)big);
+    // 2^s takes the largest step to 2^14 .. 2^15; a subnormal one, or none, counts as 2^-14
+    const int s = 29 - max(sums.step >> 10, 1);
+    const float ref = top > -__builtin_inff() ? top - (float)s : -__builtin_inff();
+    const float base = top > -__builtin_inff() ? ref : 0.0f;
+    const float shrink = __builtin_amdgcn_exp2f(sums.ref - base);   // 0 where nothing was seen yet
+    sums.top = top;
+    sums.ref = ref;
+    float p[8];
+    float total = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        p[i] = __builtin_amdgcn_exp2f(x[i >> 2][i & 3] - base);
+        total += p[i];
+    }
+    sums.total = __builtin_fmaf(sums.total, shrink, total);
+    const float second = lane & 8 ? -1.0f : 0.0f;
+#pragma unroll
+    for (int b = 0; b < BLOCKS; b++) {
+        u32x4 w;
+        float off = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            float v[2];
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const int n = 2 * i + j;
+                v[j] = p[n] * step_of(vs[n >> 2], n & 3, b);
+                if (edge) v[j] = seen >> n & 1 ? v[j] : 0.0f;
+            }
+            const fp16x2_t h = __builtin_amdgcn_cvt_pkrtz(v[0], v[1]);
+            const fp16x2_t l = __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf((float)h[0], second, v[0]),
+                                                          __builtin_fmaf((float)h[1], second, v[1]));
+            w[i] = __builtin_bit_cast(uint32_t, l);
+            if constexpr (V_BITS == 4) off += (float)l[0] + (float)l[1];
+        }
+        if constexpr (V_BITS == 4) sums.offset[b] = __builtin_fmaf(sums.offset[b], shrink, off);
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            u32x4 c;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int n = 2 * i;
+                c[i] = value_pair<V_BITS>(vc[n >> 2][n & 3], vc[n >> 2][(n & 3) + 1], 2 * b + e);
+            }
+#pragma unroll
+            for (int r = 0; r < 4; r++) sums.acc[b][e][r] *= shrink;
+            sums.acc[b][e] = mfma(c, w, sums.acc[b][e]);
+        }
+    }
+}
+
+// The wave's sums as one: both columns of a query, the four lanes of its slots,
+// and the offset of four-bit codes.
+template <int BLOCKS, bool OFFSET>
+QS_DEV void finish(Sums<BLOCKS, OFFSET>& o) {
+    o.total = sum_over_slots(o.total);
+#pragma unroll
+    for (int b = 0; b < BLOCKS; b++) {
+        float off = 0.0f;
+        if constexpr (OFFSET) off = sum_over_slots(o.offset[b]) * (-8.0f * 0x1p-24f);
+#pragma unroll
+        for (int e = 0; e < 2; e++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const float v = o.acc[b][e][r] + off;
+                o.acc[b][e][r] = v + other_column(v);
+            }
+    }
+}
+
+template <int TYPE>
+QS_DEV void store_row(void* out, int64_t at, const float (&v)[8]) { qsr::store8<TYPE>(out, at, v); }
+
+template <int K_BITS, int V_BITS, int BLOCKS, bool WIDE>
+__global__ __launch_bounds__(64) void k_kv_attention(AttentionArgs a) {
+    const int tiles = column_tiles(a);
+    const int tile = (int)blockIdx.x % tiles, head = (int)blockIdx.x / tiles % a.c.heads, seq = (int)blockIdx.x / tiles / a.c.heads;
+    const int64_t most = (int64_t)a.pages_each << a.c.shift;
+    int length = a.lengths[seq];
+    length = length < 0 ? 0 : length > most ? (int)most : length;
+    Queries<BLOCKS, WIDE, K_BITS == 4> q;
+    load_queries<K_BITS, BLOCKS, WIDE>(a, seq, head, tile, length, q);
+    const Span span = span_of(a, tile, length);
+    Sums<BLOCKS, V_BITS == 4> sums;
+    clear(sums);
+    const int32_t* table = a.tables + seq * a.table_stride;
+    for (int start = span.first & ~(TILE - 1); start < span.last; start += TILE)
+        attend<K_BITS, V_BITS, BLOCKS, WIDE>(a, table, head, start, span, q, sums);
+    finish(sums);
+    const int lane = threadIdx.x & 63, g = lane >> 4, column = tile * COLUMNS + (lane & 7);
+    if (lane & 8 || !q.live) return;
+    const float inverse = sums.total != 0.0f ? 0x1p24f / sums.total : 0.0f;     // 0: it sees nothing
+    const int token = column / a.group;
+    const int64_t row = (((int64_t)seq * a.fresh + token) * a.c.heads + head) * a.group + column - token * a.group;
+#pragma unroll
+    for (int b = 0; b < BLOCKS; b++) {
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = sums.acc[b][i & 1][i >> 1] * inverse;
+        const int64_t at = (row * BLOCKS + b) * 32 + 8 * g;
+        if constexpr (WIDE) store_row<qs::SRC_F32>(a.out, at, v);
+        else if (a.type == QS_SRC_BF16) store_row<qs::SRC_BF16>(a.out, at, v);
+        else store_row<qs::SRC_F16>(a.out, at, v);
+    }
+}
+
+template <int K_BITS, int V_BITS, int BLOCKS>
+hipError_t launch_blocks(const AttentionArgs& a, hipStream_t st) {
+    const dim3 grid((unsigned)((int64_t)a.batch * a.c.heads * column_tiles(a)));
+    const auto kernel = a.type == QS_SRC_F32 ? k_kv_attention<K_BITS, V_BITS, BLOCKS, true>
+                                             : k_kv_attention<K_BITS, V_BITS, BLOCKS, false>;
+    return qs_host::launch_kernel(kernel, grid, dim3(64), 0, st, a);
+}
+
+template <int K_BITS, int V_BITS>
+hipError_t launch_attention(const AttentionArgs& a, hipStream_t st) {
+    switch (a.c.blocks) {
+        case 2: return launch_blocks<K_BITS, V_BITS, 2>(a, st);
+        case 4: return launch_blocks<K_BITS, V_BITS, 4>(a, st);
+        case 6: return launch_blocks<K_BITS, V_BITS, 6>(a, st);
+        default: return launch_blocks<K_BITS, V_BITS, 8>(a, st);
+    }
+}
+
+}  // namespace qskv

@@ -1,0 +1,54 @@
+// Rows of f32, f16 or bf16 values, eight at a time: their values in f32 and back.
+#pragma once
+
+#include "qs_device.h"
+
+namespace qsr {
+
+using qs::u32x4;
+
+// eight values of the source type in f32
+template <int SRC>
+struct Eight {
+    u32x4 w[SRC == qs::SRC_F32 ? 2 : 1];
+};
+template <int SRC>
+QS_DEV void load8(const void* p, int64_t at, Eight<SRC>& o) {
+    const u32x4* s = reinterpret_cast<const u32x4*>(static_cast<const char*>(p) + at * (SRC == qs::SRC_F32 ? 4 : 2));
+    o.w[0] = s[0];
+    if constexpr (SRC == qs::SRC_F32) o.w[1] = s[1];
+}
+template <int SRC>
+QS_DEV float value8(const Eight<SRC>& o, int i) {
+    if constexpr (SRC == qs::SRC_F32) return __uint_as_float(o.w[i >> 2][i & 3]);
+    const uint32_t h = (o.w[0][i >> 1] >> (16 * (i & 1))) & 0xffffu;
+    if constexpr (SRC == qs::SRC_BF16) return __uint_as_float(h << 16);
+    return (float)__builtin_bit_cast(_Float16, (uint16_t)h);
+}
+// f32 to bf16, to nearest even; a NaN stays one
+QS_DEV uint32_t bf16_bits(float f) {
+    return (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)f);
+}
+template <int DST>
+QS_DEV uint32_t bits16(float f) {
+    if constexpr (DST == qs::SRC_BF16) return bf16_bits(f);
+    // the f32 result is rounded again, as torch's is: the compiler would
+    // otherwise form it and the f16 in one mixed-precision instruction
+    qs::keep_in_register(f);
+    return (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)f);
+}
+template <int DST>
+QS_DEV void store8(void* p, int64_t at, const float (&v)[8]) {
+    u32x4* d = reinterpret_cast<u32x4*>(static_cast<char*>(p) + at * (DST == qs::SRC_F32 ? 4 : 2));
+    if constexpr (DST == qs::SRC_F32) {
+        d[0] = u32x4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
+        d[1] = u32x4{__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7])};
+    } else {
+        u32x4 o;
+#pragma unroll
+        for (int i = 0; i < 4; i++) o[i] = bits16<DST>(v[2 * i]) | (bits16<DST>(v[2 * i + 1]) << 16);
+        d[0] = o;
+    }
+}
+
+}  // namespace qsr
