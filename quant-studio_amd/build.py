@@ -45,6 +45,7 @@ UNITS = [
     *[("qs_linear.hip", [f"-DQS_LINEAR_SET={i}"]) for i in range(6)],
     # a quantised key-value cache; qs_kv_attention.hip holds a pair of types each
     ("qs_kv.hip", []),
+    ("qs_kv_join.hip", []),
     *[("qs_kv_attention.hip", [f"-DQS_KV_BITS={b}"]) for b in (88, 84, 48, 44)],
 ]
 

@@ -246,6 +246,8 @@ int attention_sizes(const qs_kv_cache* cache, int64_t batch, int64_t fresh, int6
         return fail(QS_EINVAL, "%lld query heads: not 1 to 128 for each of %d key/value heads", (long long)query_heads, a.c.heads);
     if (pages_each < 0 || pages_each > (INT32_C(1) << 30) / a.c.page)
         return fail(QS_EINVAL, "tables of %lld pages of %d slots: negative, or over 2^30 slots", (long long)pages_each, a.c.page);
+    if (batch * pages_each * a.c.page > INT64_C(1) << 34)
+        return fail(QS_EINVAL, "%lld tables of %lld pages of %d slots: over 2^34 slots", (long long)batch, (long long)pages_each, a.c.page);
     a.batch = (int32_t)batch;
     a.fresh = (int32_t)fresh;
     a.group = (int32_t)(query_heads / a.c.heads);
@@ -257,10 +259,12 @@ int attention_sizes(const qs_kv_cache* cache, int64_t batch, int64_t fresh, int6
 
 namespace qskv {
 
-extern template hipError_t launch_attention<8, 8>(const AttentionArgs&, hipStream_t);
-extern template hipError_t launch_attention<8, 4>(const AttentionArgs&, hipStream_t);
-extern template hipError_t launch_attention<4, 8>(const AttentionArgs&, hipStream_t);
-extern template hipError_t launch_attention<4, 4>(const AttentionArgs&, hipStream_t);
+static int64_t round_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
+
+extern template hipError_t launch_attention<8, 8>(const AttentionArgs&, const Split&, hipStream_t);
+extern template hipError_t launch_attention<8, 4>(const AttentionArgs&, const Split&, hipStream_t);
+extern template hipError_t launch_attention<4, 8>(const AttentionArgs&, const Split&, hipStream_t);
+extern template hipError_t launch_attention<4, 4>(const AttentionArgs&, const Split&, hipStream_t);
 
 int cache_of(const qs_kv_cache* cache, Cache& c) {
     if (!cache) return fail(QS_EINVAL, "null cache");
@@ -279,6 +283,28 @@ int cache_of(const qs_kv_cache* cache, Cache& c) {
     c.v_bits = bits_of(cache->v_type);
     c.page_bytes = (int64_t)c.page * c.heads * slot_bytes(c.k_bits, c.v_bits, c.blocks);
     return 0;
+}
+
+Split split_of(const AttentionArgs& a, void* workspace) {
+    // Workgroups of a full GPU; fewer where even the longest sequences would not
+    // give each a step for every wave. Sequences of a few steps at most are not split.
+    constexpr int64_t FULL = 3 * 256, FEW = 8;
+    const int64_t heads = (int64_t)a.c.heads * column_tiles(a);
+    const int64_t steps = ((int64_t)a.pages_each * a.c.page + TILE - 1) / TILE;
+    Split s{};
+    if (a.batch == 0 || a.fresh == 0) return s;
+    s.whole = steps <= FEW;
+    const int64_t most = (a.batch * heads * steps + WAVES - 1) / WAVES;
+    s.groups = (int32_t)(s.whole ? a.batch * heads : most < FULL ? most : FULL);
+    if (s.whole) return s;
+    const int64_t parts = round_up((int64_t)s.groups * 2 * COLUMNS * 32 * a.c.blocks * 4, 256);
+    const int64_t stats = round_up((int64_t)s.groups * 2 * COLUMNS * 8, 256);
+    uint8_t* base = static_cast<uint8_t*>(workspace);
+    s.parts = reinterpret_cast<float*>(base);
+    s.stats = reinterpret_cast<float2*>(base + parts);
+    s.segments = reinterpret_cast<int4*>(base + parts + stats);
+    s.bytes = parts + stats + (int64_t)s.groups * 16;
+    return s;
 }
 
 }  // namespace qskv
@@ -355,7 +381,7 @@ int64_t qs_kv_attention_workspace(const qs_kv_cache* cache, int64_t batch, int64
     qs_host::clear_error();
     qskv::AttentionArgs a{};
     const int bad = attention_sizes(cache, batch, new_tokens, query_heads, pages_each, a);
-    return bad ? bad : 0;
+    return bad ? bad : qskv::split_of(a, nullptr).bytes;
 }
 
 int qs_kv_attention(const qs_kv_cache* cache, int type, const void* q, int64_t q_token_stride_bytes, int64_t batch,
@@ -392,9 +418,13 @@ int qs_kv_attention(const qs_kv_cache* cache, int type, const void* q, int64_t q
     a.window = (int32_t)(window < INT32_MAX ? window : 0);      // as long as any sequence: none
     a.type = type;
     a.scale = scale;
+    const qskv::Split split = qskv::split_of(a, workspace);
+    if (split.bytes && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256 || workspace_bytes < split.bytes))
+        return fail(QS_EINVAL, "workspace holds %lld bytes at %p, %lld needed, 256-byte aligned", (long long)workspace_bytes,
+                    workspace, (long long)split.bytes);
     hipStream_t st = static_cast<hipStream_t>(hip_stream);
-    const hipError_t e = a.c.k_bits == 8 ? (a.c.v_bits == 8 ? qskv::launch_attention<8, 8>(a, st) : qskv::launch_attention<8, 4>(a, st))
-                                         : (a.c.v_bits == 8 ? qskv::launch_attention<4, 8>(a, st) : qskv::launch_attention<4, 4>(a, st));
+    const hipError_t e = a.c.k_bits == 8 ? (a.c.v_bits == 8 ? qskv::launch_attention<8, 8>(a, split, st) : qskv::launch_attention<8, 4>(a, split, st))
+                                         : (a.c.v_bits == 8 ? qskv::launch_attention<4, 8>(a, split, st) : qskv::launch_attention<4, 4>(a, split, st));
     if (e != hipSuccess) return fail(QS_EIO, "kv_attention: launch failed: %s", hipGetErrorString(e));
     return 0;
 }

@@ -5,6 +5,7 @@
 #include <hip/hip_runtime.h>
 
 #include "qs_kv.h"
+#include "qs_rows.h"
 
 namespace qskv {
 
@@ -31,7 +32,39 @@ inline __host__ __device__ int column_tiles(const AttentionArgs& a) {
     return (a.group * a.fresh + COLUMNS - 1) / COLUMNS;
 }
 
+// How a call's work is split, and where its workgroups leave what is joined.
+constexpr int TILE = 32;            // slots of a wave's step
+constexpr int WAVES = 4;            // of a workgroup, a step each in turn
+struct Split {
+    int32_t groups;                 // workgroups
+    bool whole;                     // each takes one segment as a whole, and nothing is joined
+    // of each workgroup, first for a segment that begins before it, then for one that goes on after it
+    float* parts;                   // [groups][2][COLUMNS][head size], relative to R
+    float2* stats;                  // [groups][2][COLUMNS]: R, sum of p
+    int4* segments;                 // [groups]: sequence, head and column tile, last workgroup of the segment
+                                    // that begins here and goes on, or -1 for none
+    int64_t bytes;                  // of the workspace
+};
+Split split_of(const AttentionArgs& a, void* workspace);
+
+// two values of a result's row
+QS_DEV void store_two(const AttentionArgs& a, int64_t at, float x, float y) {
+    if (a.type == QS_SRC_F32) *reinterpret_cast<float2*>(static_cast<float*>(a.out) + at) = float2{x, y};
+    else *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + at) =
+        a.type == QS_SRC_BF16 ? qsr::bits16<qs::SRC_BF16>(x) | qsr::bits16<qs::SRC_BF16>(y) << 16
+                              : qsr::bits16<qs::SRC_F16>(x) | qsr::bits16<qs::SRC_F16>(y) << 16;
+}
+// first value of a query's row of the result; -1: the column has no query
+QS_DEV int64_t row_of(const AttentionArgs& a, int seq, int head, int column) {
+    if (column >= a.group * a.fresh) return -1;
+    const int token = column / a.group;
+    return ((((int64_t)seq * a.fresh + token) * a.c.heads + head) * a.group + column - token * a.group) * (32 * a.c.blocks);
+}
+
+// unit: what a result of 1 is in the parts
+hipError_t launch_join(const AttentionArgs& a, const Split& split, float unit, hipStream_t st);
+
 template <int K_BITS, int V_BITS>
-hipError_t launch_attention(const AttentionArgs& a, hipStream_t st);
+hipError_t launch_attention(const AttentionArgs& a, const Split& split, hipStream_t st);
 
 }  // namespace qskv

@@ -5,6 +5,6 @@
 
 namespace qskv {
 
-template hipError_t launch_attention<QS_KV_BITS / 10, QS_KV_BITS % 10>(const AttentionArgs&, hipStream_t);
+template hipError_t launch_attention<QS_KV_BITS / 10, QS_KV_BITS % 10>(const AttentionArgs&, const Split&, hipStream_t);
 
 }  // namespace qskv

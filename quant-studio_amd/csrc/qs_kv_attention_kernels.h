@@ -10,17 +10,17 @@
 //            block's dimensions, with P = p step (the step runs along the sum)
 //
 // The scores' D has its slots where the values' P wants them (a lane: one query,
-// slots 4 g .. 4 g + 3 of both sixteens), so nothing moves between lanes; codes go
-// to f16 without a conversion, as subnormal numbers (c 2^-24), which the matrix
-// units multiply exactly. p and P are held to 22 bits: a query has two of the 16
+// slots 4 g .. 4 g + 3 of both sixteens), so nothing moves between lanes. Eight-bit
+// codes go to f16 without a conversion, as subnormal numbers (c 2^-24), which the
+// matrix units multiply exactly; four-bit ones by a multiply-add that takes their
+// offset off (left on, it would have to come off the sums, and these would cancel).
+// P is held to 22 bits: a query has two of the 16
 // columns, one takes f16(P), the other f16(P - f16(P)). So that the second does
 // not fall below f16's range, p is relative to R = m - s, with m the running
 // maximum and 2^s the power of two that takes the largest step so far to 2^14 ..
 // 2^15: what is lost is under 2^-39 of the largest P. q is rounded to f16 after its
 // row is scaled to 2^14 .. 2^15 in the same way: all of a bf16 or f16 q down to
 // 2^-39 of the row's largest; an f32 q takes two products, 22 bits.
-// Four-bit codes have an offset: q's sums over each block start the scores'
-// products, and P's sums over the slots are taken off at the end.
 #pragma once
 
 #include "qs_kv_attention.h"
@@ -31,10 +31,8 @@ namespace qskv {
 
 typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
-typedef __fp16 fp16x2_t __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int TILE = 32;                // slots of a wave's step
 constexpr float LOG2E = 1.44269504088896341f;
 
 QS_DEV f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
@@ -101,6 +99,17 @@ QS_DEV uint32_t sign_and_magnitude(uint32_t w, uint32_t pick) {
     return __builtin_amdgcn_perm(0u, w, pick) & 0x807f807fu;
 }
 
+// the four-bit codes `i` and i + 4 of a word, less 8, as f16: 1024 + u or 1024 + 16 u
+// by its bits, which an exact multiply-add takes to u - 8
+QS_DEV uint32_t four_bits(uint32_t w, int i) {
+    w = i & 2 ? w >> 8 : w;
+    const uint32_t bits = (w & (i & 1 ? 0x00f000f0u : 0x000f000fu)) | 0x64006400u;
+    const half2_t h = __builtin_bit_cast(half2_t, bits);
+    const half2_t v = i & 1 ? __builtin_elementwise_fma(h, half2_t{(_Float16)0.0625f, (_Float16)0.0625f}, half2_t{(_Float16)-72.0f, (_Float16)-72.0f})
+                            : h + half2_t{(_Float16)-1032.0f, (_Float16)-1032.0f};
+    return __builtin_bit_cast(uint32_t, v);
+}
+
 // eight codes of a key's block as f16
 template <int BITS, int BLOCKS>
 QS_DEV u32x4 key_block(const Codes<BITS * BLOCKS>& c, int b) {
@@ -113,7 +122,7 @@ QS_DEV u32x4 key_block(const Codes<BITS * BLOCKS>& c, int b) {
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < 4; i++) o[i] = (c.w[b] >> (4 * i)) & 0x000f000fu;
+        for (int i = 0; i < 4; i++) o[i] = four_bits(c.w[b], i);
     }
     return o;
 }
@@ -125,15 +134,22 @@ QS_DEV uint32_t value_pair(const Codes<N>& x, const Codes<N>& y, int n) {
         return __builtin_amdgcn_perm(y.w[n >> 2], x.w[n >> 2], at * 0x01010101u + 0x04040000u) & 0x807f807fu;
     } else {
         const uint32_t both = __builtin_amdgcn_perm(y.w[n >> 3], x.w[n >> 3], n & 4 ? 0x07060302u : 0x05040100u);
-        return (both >> (4 * (n & 3))) & 0x000f000fu;
+        return four_bits(both, n & 3);
     }
 }
 
+// Two values as f16: to nearest for f32 results, else by the one instruction that
+// cuts off (a bit less of P)
+template <bool NEAREST>
+QS_DEV half2_t two_halves(float x, float y) {
+    if constexpr (NEAREST) return half2_t{(_Float16)x, (_Float16)y};
+    else return __builtin_bit_cast(half2_t, __builtin_amdgcn_cvt_pkrtz(x, y));
+}
+
 // the queries of a wave, as the scores' products take them
-template <int BLOCKS, bool WIDE, bool OFFSET>
+template <int BLOCKS, bool WIDE>
 struct Queries {
     u32x4 q[BLOCKS], lo[WIDE ? BLOCKS : 1];
-    float start[OFFSET ? BLOCKS : 1];       // what a block's offset comes to
     float scale;                            // of the scores, beside 2^up
     int up;
     int first, last;                        // slots that the lane's query sees: first .. last - 1
@@ -142,7 +158,7 @@ struct Queries {
 
 template <int K_BITS, int BLOCKS, bool WIDE>
 QS_DEV void load_queries(const AttentionArgs& a, int seq, int head, int tile, int length,
-                         Queries<BLOCKS, WIDE, K_BITS == 4>& o) {
+                         Queries<BLOCKS, WIDE>& o) {
     const int lane = threadIdx.x & 63, g = lane >> 4, column = tile * COLUMNS + (lane & 7);
     o.live = column < a.group * a.fresh;
     const int token = o.live ? column / a.group : 0, mine = o.live ? column - token * a.group : 0;
@@ -177,7 +193,6 @@ QS_DEV void load_queries(const AttentionArgs& a, int seq, int head, int tile, in
     const int e = scaled ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;     // top 2^e in 2^14 .. 2^15
 #pragma unroll
     for (int b = 0; b < BLOCKS; b++) {
-        float sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             half2_t h, l;
@@ -185,38 +200,29 @@ QS_DEV void load_queries(const AttentionArgs& a, int seq, int head, int tile, in
             for (int j = 0; j < 2; j++) {
                 const float v = __builtin_ldexpf(x[b][2 * i + j], e);
                 h[j] = (_Float16)v;
-                sum += (float)h[j];
-                if constexpr (WIDE) {
-                    l[j] = (_Float16)(v - (float)h[j]);
-                    sum += (float)l[j];
-                }
+                if constexpr (WIDE) l[j] = (_Float16)(v - (float)h[j]);
             }
             o.q[b][i] = __builtin_bit_cast(uint32_t, h);
             if constexpr (WIDE) o.lo[b][i] = __builtin_bit_cast(uint32_t, l);
         }
-        if constexpr (K_BITS == 4) o.start[b] = sum_over_slots(sum) * (-8.0f * 0x1p-24f);
     }
     o.scale = a.scale * LOG2E;
-    o.up = 24 - e;
+    o.up = (K_BITS == 8 ? 24 : 0) - e;
     o.last = length - a.fresh + 1 + token;
     o.first = a.window > 0 && o.last > a.window ? o.last - a.window : 0;
 }
 
 // what a wave has summed up of its slots
-template <int BLOCKS, bool OFFSET>
+template <int BLOCKS>
 struct Sums {
     f32x4 acc[BLOCKS][2];               // dims 32 block + 8 g + 2 r + e at [block][e][r]
-    float offset[OFFSET ? BLOCKS : 1];
     float top, ref, total;              // running maximum, R, sum of p
     int step;                           // bits of the largest step so far
 };
-template <int BLOCKS, bool OFFSET>
-QS_DEV void clear(Sums<BLOCKS, OFFSET>& o) {
+template <int BLOCKS>
+QS_DEV void clear(Sums<BLOCKS>& o) {
 #pragma unroll
-    for (int b = 0; b < BLOCKS; b++) {
-        o.acc[b][0] = o.acc[b][1] = f32x4{0, 0, 0, 0};
-        if constexpr (OFFSET) o.offset[b] = 0.0f;
-    }
+    for (int b = 0; b < BLOCKS; b++) o.acc[b][0] = o.acc[b][1] = f32x4{0, 0, 0, 0};
     o.top = o.ref = -__builtin_inff();
     o.total = 0.0f;
     o.step = 0;
@@ -241,7 +247,7 @@ QS_DEV Span span_of(const AttentionArgs& a, int tile, int length) {
 // (`pages_each` of them).
 template <int K_BITS, int V_BITS, int BLOCKS, bool WIDE>
 QS_DEV void attend(const AttentionArgs& a, const int32_t* table, int head, int start, const Span& span,
-                   const Queries<BLOCKS, WIDE, K_BITS == 4>& q, Sums<BLOCKS, V_BITS == 4>& sums) {
+                   const Queries<BLOCKS, WIDE>& q, Sums<BLOCKS>& sums) {
     constexpr int KROW = row_bytes(K_BITS, BLOCKS), VROW = row_bytes(V_BITS, BLOCKS), STEPS = 2 * BLOCKS;
     const int lane = threadIdx.x & 63, g = lane >> 4, m = lane & 15;
     Codes<KROW / 4> kc[2];
@@ -277,8 +283,7 @@ QS_DEV void attend(const AttentionArgs& a, const int32_t* table, int head, int s
 #pragma unroll
         for (int b = 0; b < BLOCKS; b++) {
             const u32x4 k = key_block<K_BITS, BLOCKS>(kc[s], b);
-            const float c0 = K_BITS == 4 ? q.start[K_BITS == 4 ? b : 0] : 0.0f;
-            f32x4 d = mfma(k, q.q[b], f32x4{c0, c0, c0, c0});
+            f32x4 d = mfma(k, q.q[b], f32x4{0, 0, 0, 0});
             if constexpr (WIDE) d = mfma(k, q.lo[b], d);
 #pragma unroll
             for (int r = 0; r < 4; r++) x[s][r] = __builtin_fmaf(d[r], step_of(ks[s], r, b), x[s][r]);
@@ -345,7 +350,6 @@ QS_DEV void attend(const AttentionArgs& a, const int32_t* table, int head, int s
 #pragma unroll
     for (int b = 0; b < BLOCKS; b++) {
         u32x4 w;
-        float off = 0.0f;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             float v[2];
@@ -355,13 +359,11 @@ QS_DEV void attend(const AttentionArgs& a, const int32_t* table, int head, int s
                 v[j] = p[n] * step_of(vs[n >> 2], n & 3, b);
                 if (edge) v[j] = seen >> n & 1 ? v[j] : 0.0f;
             }
-            const fp16x2_t h = __builtin_amdgcn_cvt_pkrtz(v[0], v[1]);
-            const fp16x2_t l = __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf((float)h[0], second, v[0]),
-                                                          __builtin_fmaf((float)h[1], second, v[1]));
-            w[i] = __builtin_bit_cast(uint32_t, l);
-            if constexpr (V_BITS == 4) off += (float)l[0] + (float)l[1];
+            // both columns round alike: the first to f16(P), the second what that leaves
+            const half2_t h = two_halves<WIDE>(v[0], v[1]);
+            w[i] = __builtin_bit_cast(uint32_t, two_halves<WIDE>(__builtin_fmaf((float)h[0], second, v[0]),
+                                                                 __builtin_fmaf((float)h[1], second, v[1])));
         }
-        if constexpr (V_BITS == 4) sums.offset[b] = __builtin_fmaf(sums.offset[b], shrink, off);
 #pragma unroll
         for (int e = 0; e < 2; e++) {
             u32x4 c;
@@ -377,76 +379,228 @@ QS_DEV void attend(const AttentionArgs& a, const int32_t* table, int head, int s
     }
 }
 
-// The wave's sums as one: both columns of a query, the four lanes of its slots,
-// and the offset of four-bit codes.
-template <int BLOCKS, bool OFFSET>
-QS_DEV void finish(Sums<BLOCKS, OFFSET>& o) {
+// The wave's sums as one: the four lanes of a query's slots, and its two columns.
+template <int BLOCKS>
+QS_DEV void finish(Sums<BLOCKS>& o) {
     o.total = sum_over_slots(o.total);
 #pragma unroll
-    for (int b = 0; b < BLOCKS; b++) {
-        float off = 0.0f;
-        if constexpr (OFFSET) off = sum_over_slots(o.offset[b]) * (-8.0f * 0x1p-24f);
+    for (int b = 0; b < BLOCKS; b++)
 #pragma unroll
         for (int e = 0; e < 2; e++)
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const float v = o.acc[b][e][r] + off;
-                o.acc[b][e][r] = v + other_column(v);
-            }
-    }
+            for (int r = 0; r < 4; r++) o.acc[b][e][r] += other_column(o.acc[b][e][r]);
 }
 
-template <int TYPE>
-QS_DEV void store_row(void* out, int64_t at, const float (&v)[8]) { qsr::store8<TYPE>(out, at, v); }
+QS_DEV int length_of(const AttentionArgs& a, int seq) {
+    const int most = a.pages_each << a.c.shift, n = a.lengths[seq];
+    return n < 0 ? 0 : n > most ? most : n;
+}
+// Steps of a sequence for any of its queries, from step `begin` on: at least one,
+// so that queries that see nothing get their zeros.
+struct Steps {
+    int begin, count;
+};
+QS_DEV Steps steps_of(const AttentionArgs& a, int length) {
+    const int lowest = length - a.fresh + 1;
+    Steps s;
+    s.begin = (a.window > 0 && lowest > a.window ? lowest - a.window : 0) / TILE;
+    s.count = (length + TILE - 1) / TILE - s.begin;
+    s.count = s.count < 1 ? 1 : s.count;
+    return s;
+}
 
-template <int K_BITS, int V_BITS, int BLOCKS, bool WIDE>
-__global__ __launch_bounds__(64) void k_kv_attention(AttentionArgs a) {
-    const int tiles = column_tiles(a);
-    const int tile = (int)blockIdx.x % tiles, head = (int)blockIdx.x / tiles % a.c.heads, seq = (int)blockIdx.x / tiles / a.c.heads;
-    const int64_t most = (int64_t)a.pages_each << a.c.shift;
-    int length = a.lengths[seq];
-    length = length < 0 ? 0 : length > most ? (int)most : length;
-    Queries<BLOCKS, WIDE, K_BITS == 4> q;
-    load_queries<K_BITS, BLOCKS, WIDE>(a, seq, head, tile, length, q);
-    const Span span = span_of(a, tile, length);
-    Sums<BLOCKS, V_BITS == 4> sums;
-    clear(sums);
-    const int32_t* table = a.tables + seq * a.table_stride;
-    for (int start = span.first & ~(TILE - 1); start < span.last; start += TILE)
-        attend<K_BITS, V_BITS, BLOCKS, WIDE>(a, table, head, start, span, q, sums);
-    finish(sums);
-    const int lane = threadIdx.x & 63, g = lane >> 4, column = tile * COLUMNS + (lane & 7);
-    if (lane & 8 || !q.live) return;
-    const float inverse = sums.total != 0.0f ? 0x1p24f / sums.total : 0.0f;     // 0: it sees nothing
-    const int token = column / a.group;
-    const int64_t row = (((int64_t)seq * a.fresh + token) * a.c.heads + head) * a.group + column - token * a.group;
+// The call's steps in a row (by sequence, head, tile of columns, then along the
+// sequence), dealt to the workgroups in equal runs: `total` of them, `each` to a
+// workgroup, this one's first one in sequence `seq`, whose own begin at `base` of one
+// head's. The lengths are on the device, so every workgroup adds them up.
+struct Deal {
+    int64_t total, each;
+    int seq, base;
+};
+constexpr int64_t LEAST = WAVES;        // steps of a workgroup
+QS_DEV int wave_sum(int v) {
 #pragma unroll
-    for (int b = 0; b < BLOCKS; b++) {
-        float v[8];
+    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
+    return v;
+}
+QS_DEV int wave_scan(int v) {
+    const int lane = threadIdx.x & 63;
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = sums.acc[b][i & 1][i >> 1] * inverse;
-        const int64_t at = (row * BLOCKS + b) * 32 + 8 * g;
-        if constexpr (WIDE) store_row<qs::SRC_F32>(a.out, at, v);
-        else if (a.type == QS_SRC_BF16) store_row<qs::SRC_BF16>(a.out, at, v);
-        else store_row<qs::SRC_F16>(a.out, at, v);
+    for (int o = 1; o < 64; o <<= 1) {
+        const int w = __shfl_up(v, o);
+        v += lane >= o ? w : 0;
     }
+    return v;
+}
+QS_DEV Deal deal(const AttentionArgs& a, int groups, int heads) {
+    __shared__ int sums[WAVES], found[2];
+    const int wave = threadIdx.x >> 6;
+    constexpr int THREADS = 64 * WAVES;
+    Deal d;
+    const int first = (int)threadIdx.x < a.batch ? steps_of(a, length_of(a, threadIdx.x)).count : 0;
+    if (a.batch == 1) {
+        d.total = (int64_t)steps_of(a, length_of(a, 0)).count * heads;
+        d.seq = d.base = 0;
+    } else {
+        int n = first;
+        for (int i = threadIdx.x + THREADS; i < a.batch; i += THREADS) n += steps_of(a, length_of(a, i)).count;
+        n = wave_sum(n);
+        if ((threadIdx.x & 63) == 0) sums[wave] = n;
+        __syncthreads();
+        int all = 0;
+#pragma unroll
+        for (int i = 0; i < WAVES; i++) all += sums[i];
+        d.total = (int64_t)all * heads;
+    }
+    d.each = (d.total + groups - 1) / groups;
+    d.each = d.each < LEAST ? LEAST : d.each;
+    if (a.batch == 1) return d;
+    const int64_t begin = blockIdx.x * d.each;
+    if (begin >= d.total) return d;
+    const int at = (int)(begin / heads);
+    int before = 0;
+    for (int i = 0;; i += THREADS) {        // one of them holds `at`, which is below their sum
+        const int mine = i + (int)threadIdx.x;
+        const int n = i == 0 ? first : mine < a.batch ? steps_of(a, length_of(a, mine)).count : 0;
+        const int scan = wave_scan(n);
+        __syncthreads();
+        if ((threadIdx.x & 63) == 63) sums[wave] = scan;
+        if (threadIdx.x == 0) found[0] = -1;
+        __syncthreads();
+        int end = before + scan;
+#pragma unroll
+        for (int w = 0; w < WAVES; w++) {
+            end += w < wave ? sums[w] : 0;
+            before += sums[w];
+        }
+        if (at >= end - n && at < end) found[0] = mine, found[1] = end - n;
+        __syncthreads();
+        if (found[0] >= 0) break;
+    }
+    d.seq = found[0];
+    d.base = found[1];
+    return d;
+}
+
+// A workgroup of four waves, which take a segment's steps in turn (a segment: what
+// the workgroup has of one head's and column tile's steps of a sequence) and join
+// their sums through LDS. A segment that is a whole one is written as the result,
+// else as a part that k_kv_join takes.
+template <int K_BITS, int V_BITS, int BLOCKS, bool WIDE>
+__global__ __launch_bounds__(64 * WAVES) void k_kv_attention(AttentionArgs a, Split split) {
+    constexpr int D = 32 * BLOCKS, ROW = D + 4;     // 4: the eight columns' words in other banks
+    __shared__ __attribute__((aligned(16))) float acc[WAVES][COLUMNS][ROW];
+    __shared__ float2 stats[WAVES][COLUMNS];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4;
+    const int tiles = column_tiles(a), heads = a.c.heads * tiles;
+    int64_t at, end;
+    int seq, base = 0;
+    int64_t each = 0;
+    int4 going{0, 0, -1, 0};
+    if (split.whole) {
+        seq = (int)blockIdx.x / heads;
+        at = (int)blockIdx.x - seq * heads;         // the head; its steps are not counted
+        end = at + 1;
+    } else {
+        const Deal d = deal(a, split.groups, heads);
+        each = d.each;
+        at = blockIdx.x * d.each;
+        end = at + d.each < d.total ? at + d.each : d.total;
+        seq = d.seq;
+        base = d.base;
+    }
+    while (at < end) {
+        const int length = length_of(a, seq);
+        const Steps steps = steps_of(a, length);
+        int which, from, to;                        // head and column tile, steps of them
+        if (split.whole) {
+            which = (int)at;
+            from = 0;
+            to = steps.count;
+        } else {
+            const int64_t rel = at - (int64_t)base * heads;
+            which = (int)(rel / steps.count);
+            from = (int)(rel - (int64_t)which * steps.count);
+            to = steps.count - from < end - at ? steps.count : from + (int)(end - at);
+        }
+        const int head = which / tiles, tile = which - head * tiles;
+        Queries<BLOCKS, WIDE> q;
+        load_queries<K_BITS, BLOCKS, WIDE>(a, seq, head, tile, length, q);
+        const Span span = span_of(a, tile, length);
+        Sums<BLOCKS> sums;
+        clear(sums);
+        const int32_t* table = a.tables + seq * a.table_stride;
+        for (int i = from + wave; i < to; i += WAVES) {
+            const int start = (steps.begin + i) * TILE;
+            if (start < span.last && start + TILE > span.first)
+                attend<K_BITS, V_BITS, BLOCKS, WIDE>(a, table, head, start, span, q, sums);
+        }
+        finish(sums);
+        if (!(lane & 8)) {
+#pragma unroll
+            for (int b = 0; b < BLOCKS; b++)
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+                    *reinterpret_cast<f32x4*>(&acc[wave][lane & 7][32 * b + 8 * g + 4 * h]) =
+                        f32x4{sums.acc[b][0][2 * h], sums.acc[b][1][2 * h], sums.acc[b][0][2 * h + 1], sums.acc[b][1][2 * h + 1]};
+            if (g == 0) stats[wave][lane & 7] = float2{sums.ref, sums.total};
+        }
+        __syncthreads();
+        // thread: a column, two dims of every 64
+        const int column = threadIdx.x >> 5, sub = threadIdx.x & 31;
+        float ref = -__builtin_inff(), total = 0.0f, part[WAVES];
+#pragma unroll
+        for (int w = 0; w < WAVES; w++) ref = fmaxf(ref, stats[w][column].x);
+#pragma unroll
+        for (int w = 0; w < WAVES; w++) {
+            const float2 s = stats[w][column];
+            part[w] = s.x > -__builtin_inff() ? __builtin_amdgcn_exp2f(s.x - ref) : s.y;    // s.y: 0, or NaN
+            total = __builtin_fmaf(s.y, part[w], total);
+        }
+        const bool whole = from == 0 && to == steps.count;
+        const int64_t row = row_of(a, seq, head, tile * COLUMNS + column);
+        const int64_t slot = ((int64_t)blockIdx.x * 2 + (from == 0)) * COLUMNS + column;
+        const float inverse = total != 0.0f ? (V_BITS == 8 ? 0x1p24f : 1.0f) / total : 0.0f;    // 0: it sees nothing
+#pragma unroll
+        for (int i = 0; i < BLOCKS / 2; i++) {
+            float2 v{0, 0};
+#pragma unroll
+            for (int w = 0; w < WAVES; w++) {
+                const float2 u = *reinterpret_cast<const float2*>(&acc[w][column][64 * i + 2 * sub]);
+                v.x = __builtin_fmaf(u.x, part[w], v.x);
+                v.y = __builtin_fmaf(u.y, part[w], v.y);
+            }
+            if (!whole) *reinterpret_cast<float2*>(split.parts + slot * D + 64 * i + 2 * sub) = v;
+            else if (row >= 0) store_two(a, row + 64 * i + 2 * sub, v.x * inverse, v.y * inverse);
+        }
+        if (!whole && sub == 0) split.stats[slot] = float2{ref, total};
+        __syncthreads();
+        if (split.whole) break;
+        if (from == 0 && !whole) going = int4{seq, which, (int)((at + steps.count - 1) / each), 0};
+        at += to - from;
+        if (to == steps.count && which == heads - 1) {
+            seq++;
+            base += steps.count;
+        }
+    }
+    if (!split.whole && threadIdx.x == 0) split.segments[blockIdx.x] = going;
 }
 
 template <int K_BITS, int V_BITS, int BLOCKS>
-hipError_t launch_blocks(const AttentionArgs& a, hipStream_t st) {
-    const dim3 grid((unsigned)((int64_t)a.batch * a.c.heads * column_tiles(a)));
+hipError_t launch_blocks(const AttentionArgs& a, const Split& split, hipStream_t st) {
     const auto kernel = a.type == QS_SRC_F32 ? k_kv_attention<K_BITS, V_BITS, BLOCKS, true>
                                              : k_kv_attention<K_BITS, V_BITS, BLOCKS, false>;
-    return qs_host::launch_kernel(kernel, grid, dim3(64), 0, st, a);
+    const hipError_t e = qs_host::launch_kernel(kernel, dim3((unsigned)split.groups), dim3(64 * WAVES), 0, st, a, split);
+    return e != hipSuccess || split.whole ? e : launch_join(a, split, V_BITS == 8 ? 0x1p24f : 1.0f, st);
 }
 
 template <int K_BITS, int V_BITS>
-hipError_t launch_attention(const AttentionArgs& a, hipStream_t st) {
+hipError_t launch_attention(const AttentionArgs& a, const Split& split, hipStream_t st) {
     switch (a.c.blocks) {
-        case 2: return launch_blocks<K_BITS, V_BITS, 2>(a, st);
-        case 4: return launch_blocks<K_BITS, V_BITS, 4>(a, st);
-        case 6: return launch_blocks<K_BITS, V_BITS, 6>(a, st);
-        default: return launch_blocks<K_BITS, V_BITS, 8>(a, st);
+        case 2: return launch_blocks<K_BITS, V_BITS, 2>(a, split, st);
+        case 4: return launch_blocks<K_BITS, V_BITS, 4>(a, split, st);
+        case 6: return launch_blocks<K_BITS, V_BITS, 6>(a, split, st);
+        default: return launch_blocks<K_BITS, V_BITS, 8>(a, split, st);
     }
 }
 

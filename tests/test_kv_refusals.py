@@ -74,13 +74,25 @@ def test_read_refuses(qs, bad, word):
 @pytest.mark.parametrize("bad,word", [
     (dict(t=5), b"query type"), (dict(b=-1), b"sequences"), (dict(b=(1 << 14) + 1), b"sequences"), (dict(n=17), b"new tokens"),
     (dict(n=-1), b"new tokens"), (dict(hq=3), b"query heads"), (dict(hq=0), b"query heads"), (dict(hq=258), b"query heads"),
-    (dict(m=-1), b"tables"), (dict(m=1 << 27, ts=1 << 27), b"2^30"), (dict(window=-1), b"window"), (dict(q=None), b"null"),
+    (dict(m=-1), b"tables"), (dict(m=1 << 27, ts=1 << 27), b"2^30"), (dict(b=1 << 12, m=1 << 20, ts=1 << 20), b"2^34"), (dict(window=-1), b"window"), (dict(q=None), b"null"),
     (dict(tables=None), b"null"), (dict(lengths=None), b"null"), (dict(out=None), b"null"), (dict(q=72), b"aligned"),
     (dict(out=72), b"aligned"), (dict(tables=66), b"aligned"), (dict(qs=496), b"token stride"), (dict(qs=520), b"token stride"),
     (dict(qs=1 << 62), b"2^62-byte span"), (dict(ts=2), b"table stride"), (dict(ts=1 << 60), b"2^62-byte span"), (dict(size=1023), b"out holds")])
 def test_attention_refuses(qs, bad, word):
     L = qs.library()
     assert attention(L, cache(), **bad) == -22 and word in L.qs_last_error(), L.qs_last_error()
+
+
+def test_attention_refuses_workspaces(qs):
+    L = qs.library()
+    need = L.qs_kv_attention_workspace
+    assert need(cache(), 2, 1, 4, 3) == 0 and need(cache(), 0, 1, 4, 300) == 0
+    size = need(cache(), 2, 1, 4, 300)
+    assert size > 0
+    for bad in (dict(work=None), dict(work=(1 << 20) + 16), dict(wsize=size - 1)):
+        assert attention(L, cache(), m=300, ts=300, **bad) == -22 and b"workspace" in L.qs_last_error()
+    # a part of every workgroup's two segments and eight queries: not a multiple of the lengths
+    assert need(cache(), 2, 1, 4, 1 << 20) == need(cache(), 2, 1, 4, 1 << 18) <= 768 * 2 * 8 * (64 * 4 + 8) + 768 * 16 + 1024
 
 
 def test_nothing_is_no_work(qs):
