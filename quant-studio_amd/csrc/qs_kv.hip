@@ -286,24 +286,27 @@ int cache_of(const qs_kv_cache* cache, Cache& c) {
 }
 
 Split split_of(const AttentionArgs& a, void* workspace) {
-    // Workgroups of a full GPU; fewer where even the longest sequences would not
-    // give each a step for every wave. Sequences of a few steps at most are not split.
-    constexpr int64_t FULL = 3 * 256, FEW = 8;
+    // As many workgroups as the GPU holds at a time; fewer where even the longest
+    // sequences would not give each a step for every wave. Sequences of a few steps at
+    // most are not split. The workspace is the same for every type.
+    constexpr int64_t CUS = 256, FEW = 8;
+    const int64_t full = CUS * resident(a.c.blocks, a.type == QS_SRC_F32);
     const int64_t heads = (int64_t)a.c.heads * column_tiles(a);
     const int64_t steps = ((int64_t)a.pages_each * a.c.page + TILE - 1) / TILE;
     Split s{};
     if (a.batch == 0 || a.fresh == 0) return s;
     s.whole = steps <= FEW;
     const int64_t most = (a.batch * heads * steps + WAVES - 1) / WAVES;
-    s.groups = (int32_t)(s.whole ? a.batch * heads : most < FULL ? most : FULL);
+    s.groups = (int32_t)(s.whole ? a.batch * heads : most < full ? most : full);
     if (s.whole) return s;
-    const int64_t parts = round_up((int64_t)s.groups * 2 * COLUMNS * 32 * a.c.blocks * 4, 256);
-    const int64_t stats = round_up((int64_t)s.groups * 2 * COLUMNS * 8, 256);
+    const int64_t room = most < CUS * resident(a.c.blocks, false) ? most : CUS * resident(a.c.blocks, false);
+    const int64_t parts = round_up(room * 2 * COLUMNS * 32 * a.c.blocks * 4, 256);
+    const int64_t stats = round_up(room * 2 * COLUMNS * 8, 256);
     uint8_t* base = static_cast<uint8_t*>(workspace);
     s.parts = reinterpret_cast<float*>(base);
     s.stats = reinterpret_cast<float2*>(base + parts);
     s.segments = reinterpret_cast<int4*>(base + parts + stats);
-    s.bytes = parts + stats + (int64_t)s.groups * 16;
+    s.bytes = parts + stats + room * 16;
     return s;
 }
 

@@ -68,29 +68,32 @@ template <int N>
 struct Codes {
     uint32_t w[(N + 3) / 4];
 };
+// through a buffer descriptor: a lane's offset `at` stays the same for every step,
+// and where the step is lies in scalar registers
+typedef __amdgpu_buffer_rsrc_t Buffer;
 template <int N>
-QS_DEV void load(Codes<N>& o, const uint8_t* p) {
+QS_DEV void load(Codes<N>& o, Buffer p, int at, int from) {
     if constexpr (N % 16 == 0) {
 #pragma unroll
         for (int i = 0; i < N / 16; i++) {
-            const u32x4 v = reinterpret_cast<const u32x4*>(p)[i];
+            const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(p, at + 16 * i, from, 0);
 #pragma unroll
             for (int j = 0; j < 4; j++) o.w[4 * i + j] = v[j];
         }
     } else if constexpr (N % 8 == 0) {
 #pragma unroll
         for (int i = 0; i < N / 8; i++) {
-            const u32x2 v = reinterpret_cast<const u32x2*>(p)[i];
+            const u32x2 v = __builtin_amdgcn_raw_buffer_load_b64(p, at + 8 * i, from, 0);
             o.w[2 * i] = v[0], o.w[2 * i + 1] = v[1];
         }
     } else if constexpr (N % 4 == 0) {
 #pragma unroll
-        for (int i = 0; i < N / 4; i++) o.w[i] = reinterpret_cast<const uint32_t*>(p)[i];
+        for (int i = 0; i < N / 4; i++) o.w[i] = __builtin_amdgcn_raw_buffer_load_b32(p, at + 4 * i, from, 0);
     } else {
 #pragma unroll
         for (int i = 0; i < (N + 3) / 4; i++) {
-            const uint16_t* h = reinterpret_cast<const uint16_t*>(p) + 2 * i;
-            o.w[i] = 4 * i + 2 < N ? (uint32_t)h[0] | (uint32_t)h[1] << 16 : (uint32_t)h[0];
+            o.w[i] = __builtin_amdgcn_raw_buffer_load_b16(p, at + 4 * i, from, 0);
+            if (4 * i + 2 < N) o.w[i] |= (uint32_t)__builtin_amdgcn_raw_buffer_load_b16(p, at + 4 * i + 2, from, 0) << 16;
         }
     }
 }
@@ -228,8 +231,8 @@ QS_DEV void clear(Sums<BLOCKS>& o) {
     o.step = 0;
 }
 
-// What the queries of a wave see: any of them slots first .. last - 1, all of them
-// slots all_first .. all_last - 1.
+// What the queries of a wave see: any of them slots first .. last - 1 at most, all of
+// them slots all_first .. all_last - 1.
 struct Span {
     int first, last, all_first, all_last;
 };
@@ -243,33 +246,91 @@ QS_DEV Span span_of(const AttentionArgs& a, int tile, int length) {
     return s;
 }
 
-// One step: the slots start .. start + 31 of a sequence whose pages are `table`
-// (`pages_each` of them).
-template <int K_BITS, int V_BITS, int BLOCKS, bool WIDE>
-QS_DEV void attend(const AttentionArgs& a, const int32_t* table, int head, int start, const Span& span,
-                   const Queries<BLOCKS, WIDE>& q, Sums<BLOCKS>& sums) {
-    constexpr int KROW = row_bytes(K_BITS, BLOCKS), VROW = row_bytes(V_BITS, BLOCKS), STEPS = 2 * BLOCKS;
-    const int lane = threadIdx.x & 63, g = lane >> 4, m = lane & 15;
+// The calls' tables and lengths: nothing writes them meanwhile, so they may come
+// through the scalar cache, and what they give is the same for a wave.
+typedef const __attribute__((address_space(4))) int32_t* Ints;
+QS_DEV Ints constant(const int32_t* p) { return (Ints)(uintptr_t)p; }
+
+// A step's codes and steps (of quantisation) in registers. Both sixteens of slots lie
+// in one page each. A lane has, of each sixteen: a quarter of key m's codes, of the
+// slots 4 g .. 4 g + 3 the values' codes of two dims of every block, and their steps.
+template <int K_BITS, int V_BITS, int BLOCKS>
+struct Tile {
+    static constexpr int KROW = row_bytes(K_BITS, BLOCKS), VROW = row_bytes(V_BITS, BLOCKS), STEPS = 2 * BLOCKS;
     Codes<KROW / 4> kc[2];
     Codes<4 * STEPS> ks[2], vs[2];
     Codes<VROW / 16> vc[2][4];
-    bool held[2];
+};
+// where they are: the same for the whole wave
+struct Place {
+    const uint8_t *head0, *head1;   // of the sixteens' pages
+    int slot0, slot1;               // in them
+    int held;                       // bits 0 and 1: their pages are in the cache
+};
+// the pages of a step, as the table has them
+struct Pages {
+    int first, second;
+};
+QS_DEV Pages pages_of(const AttentionArgs& a, Ints table, int start) {
+    const int first = start >> a.c.shift, second = (start + 16) >> a.c.shift;
+    return {table[first], table[second < a.pages_each ? second : first]};
+}
+QS_DEV Place place_of(const AttentionArgs& a, const Pages& pages, int head, int start) {
+    Place o;
+    const int second = (start + 16) >> a.c.shift;
+    const bool held0 = (unsigned)pages.first < (unsigned)a.c.pages;
+    const bool held1 = (unsigned)pages.second < (unsigned)a.c.pages && second < a.pages_each;
+    // where one is not, page 0, whose slots are not used
+    o.head0 = head_of(a.c, held0 ? pages.first : 0, head);
+    o.head1 = head_of(a.c, held1 ? pages.second : 0, head);
+    o.slot0 = start & (a.c.page - 1);
+    o.slot1 = (start + 16) & (a.c.page - 1);
+    o.held = (held0 ? 1 : 0) | (held1 ? 2 : 0);
+    return o;
+}
+template <int K_BITS, int V_BITS, int BLOCKS>
+QS_DEV Buffer buffer_of(const AttentionArgs& a, const uint8_t* head) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(head), 0, a.c.page * slot_bytes(K_BITS, V_BITS, BLOCKS), 0x00027000);
+}
+template <int K_BITS, int V_BITS, int BLOCKS>
+QS_DEV void load_keys(const AttentionArgs& a, const Place& at, Tile<K_BITS, V_BITS, BLOCKS>& t) {
+    typedef Tile<K_BITS, V_BITS, BLOCKS> T;
+    const int lane = threadIdx.x & 63, g = lane >> 4, m = lane & 15;
 #pragma unroll
     for (int s = 0; s < 2; s++) {
-        const int at = start + 16 * s, entry = at >> a.c.shift, slot = at & (a.c.page - 1);
-        int page = entry < a.pages_each ? table[entry] : -1;
-        held[s] = (unsigned)page < (unsigned)a.c.pages;
-        page = held[s] ? page : 0;              // there is one; what it holds is not used
-        const uint8_t* p = head_of(a.c, page, head);
-        load(kc[s], p + (slot + m) * KROW + g * (KROW / 4));
-        p += a.c.page * KROW;
-        load(ks[s], p + (slot + 4 * g) * STEPS);
-        p += a.c.page * STEPS;
-#pragma unroll
-        for (int r = 0; r < 4; r++) load(vc[s][r], p + (slot + 4 * g + r) * VROW + m * (VROW / 16));
-        p += a.c.page * VROW;
-        load(vs[s], p + (slot + 4 * g) * STEPS);
+        const Buffer p = buffer_of<K_BITS, V_BITS, BLOCKS>(a, s ? at.head1 : at.head0);
+        const int slot = s ? at.slot1 : at.slot0;
+        load(t.kc[s], p, m * T::KROW + g * (T::KROW / 4), slot * T::KROW);
+        load(t.ks[s], p, 4 * T::STEPS * g, a.c.page * T::KROW + slot * T::STEPS);
     }
+}
+template <int K_BITS, int V_BITS, int BLOCKS>
+QS_DEV void load_values(const AttentionArgs& a, const Place& at, Tile<K_BITS, V_BITS, BLOCKS>& t) {
+    typedef Tile<K_BITS, V_BITS, BLOCKS> T;
+    const int lane = threadIdx.x & 63, g = lane >> 4, m = lane & 15;
+#pragma unroll
+    for (int s = 0; s < 2; s++) {
+        const Buffer p = buffer_of<K_BITS, V_BITS, BLOCKS>(a, s ? at.head1 : at.head0);
+        const int slot = s ? at.slot1 : at.slot0, codes = a.c.page * (T::KROW + T::STEPS);
+        load(t.vs[s], p, 4 * T::STEPS * g, codes + a.c.page * T::VROW + slot * T::STEPS);
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+            load(t.vc[s][r], p, 4 * T::VROW * g + m * (T::VROW / 16) + T::VROW * r, codes + slot * T::VROW);
+    }
+}
+
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+
+// One step: the slots start .. start + 31, in `t`. The next step's keys and values
+// (at `next`) are loaded into the registers of this one's as soon as these are done
+// with, and arrive while the other half is computed.
+// edge: some query does not see all of the slots; to it they count for nothing,
+// whatever they hold, since a lane's scores and steps are its query's own copies.
+template <bool WIDE, int K_BITS, int V_BITS, int BLOCKS>
+QS_DEV void attend(const AttentionArgs& a, int start, bool edge, int held, const Place& next,
+                   const Queries<BLOCKS, WIDE>& q, Tile<K_BITS, V_BITS, BLOCKS>& t, Sums<BLOCKS>& sums) {
+    constexpr int STEPS = 2 * BLOCKS;
+    const int lane = threadIdx.x & 63, g = lane >> 4;
     const auto step_of = [](const Codes<4 * STEPS>& c, int r, int b) {
         const int n = r * BLOCKS + b;
         return half_of(c.w[n >> 1] >> (16 * (n & 1)));
@@ -282,54 +343,43 @@ QS_DEV void attend(const AttentionArgs& a, const int32_t* table, int head, int s
         for (int r = 0; r < 4; r++) x[s][r] = 0.0f;
 #pragma unroll
         for (int b = 0; b < BLOCKS; b++) {
-            const u32x4 k = key_block<K_BITS, BLOCKS>(kc[s], b);
+            const u32x4 k = key_block<K_BITS, BLOCKS>(t.kc[s], b);
             f32x4 d = mfma(k, q.q[b], f32x4{0, 0, 0, 0});
             if constexpr (WIDE) d = mfma(k, q.lo[b], d);
 #pragma unroll
-            for (int r = 0; r < 4; r++) x[s][r] = __builtin_fmaf(d[r], step_of(ks[s], r, b), x[s][r]);
+            for (int r = 0; r < 4; r++) x[s][r] = __builtin_fmaf(d[r], step_of(t.ks[s], r, b), x[s][r]);
         }
 #pragma unroll
         for (int r = 0; r < 4; r++) x[s][r] = __builtin_ldexpf(x[s][r] * q.scale, q.up);
     }
-    // a step at an edge: what a query does not see counts for nothing, whatever is there
-    uint32_t seen = 0xff;
-    const bool edge = start < span.all_first || start + TILE > span.all_last || !held[0] || !held[1];
+    __builtin_amdgcn_sched_barrier(0);      // loads that move up would need registers of their own
+    load_keys(a, next, t);
     if (edge) {
-        seen = 0;
-        bool any[2][4];
 #pragma unroll
         for (int s = 0; s < 2; s++)
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                const int at = start + 16 * s + 4 * g + r;
-                seen |= (held[s] && at >= q.first && at < q.last ? 1u : 0u) << (4 * s + r);
-                any[s][r] = held[s] && at >= span.first && at < span.last;
-                x[s][r] = seen >> (4 * s + r) & 1 ? x[s][r] : -__builtin_inff();
-            }
-        // and steps of slots that none sees are 0
+                const int p = start + 16 * s + 4 * g + r;
+                if (!((held >> s & 1) && p >= q.first && p < q.last)) {
+                    x[s][r] = -__builtin_inff();
 #pragma unroll
-        for (int s = 0; s < 2; s++)
-#pragma unroll
-            for (int i = 0; i < STEPS; i++) {
-                const uint32_t low = any[s][2 * i / BLOCKS] ? 0xffffu : 0u, high = any[s][(2 * i + 1) / BLOCKS] ? 0xffff0000u : 0u;
-                vs[s].w[i] &= low | high;
+                    for (int i = 0; i < BLOCKS / 2; i++) t.vs[s].w[r * (BLOCKS / 2) + i] = 0;
+                }
             }
     }
     // the running maximum and R
     float top = sums.top;
-    uint32_t big = 0;
+    u16x2 most{0, 0};
 #pragma unroll
     for (int s = 0; s < 2; s++) {
 #pragma unroll
         for (int r = 0; r < 4; r++) top = fmaxf(top, x[s][r]);
 #pragma unroll
-        for (int i = 0; i < STEPS; i++) {
-            big = max(big, vs[s].w[i] & 0x7fffu);
-            big = max(big, (vs[s].w[i] >> 16) & 0x7fffu);
-        }
+        for (int i = 0; i < STEPS; i++)     // eight-bit steps are not negative
+            most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, V_BITS == 8 ? t.vs[s].w[i] : t.vs[s].w[i] & 0x7fff7fffu));
     }
     top = max_over_slots(top);
-    big = over_slots(big, [](uint32_t u, uint32_t v) { return max(u, v); });
+    const uint32_t big = over_slots(most[0] > most[1] ? most[0] : most[1], [](uint32_t u, uint32_t v) { return max(u, v); });
     sums.step = max(sums.step, (int)big);
     // 2^s takes the largest step to 2^14 .. 2^15; a subnormal one, or none, counts as 2^-14
     const int s = 29 - max(sums.step >> 10, 1);
@@ -346,6 +396,14 @@ QS_DEV void attend(const AttentionArgs& a, const int32_t* table, int head, int s
         total += p[i];
     }
     sums.total = __builtin_fmaf(sums.total, shrink, total);
+    if (__any(shrink != 1.0f)) {
+#pragma unroll
+        for (int b = 0; b < BLOCKS; b++)
+#pragma unroll
+            for (int e = 0; e < 2; e++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) sums.acc[b][e][r] *= shrink;
+    }
     const float second = lane & 8 ? -1.0f : 0.0f;
 #pragma unroll
     for (int b = 0; b < BLOCKS; b++) {
@@ -356,8 +414,8 @@ QS_DEV void attend(const AttentionArgs& a, const int32_t* table, int head, int s
 #pragma unroll
             for (int j = 0; j < 2; j++) {
                 const int n = 2 * i + j;
-                v[j] = p[n] * step_of(vs[n >> 2], n & 3, b);
-                if (edge) v[j] = seen >> n & 1 ? v[j] : 0.0f;
+                // + 0 makes it one instruction that takes the step as f16
+                v[j] = __builtin_fmaf(p[n], step_of(t.vs[n >> 2], n & 3, b), 0.0f);
             }
             // both columns round alike: the first to f16(P), the second what that leaves
             const half2_t h = two_halves<WIDE>(v[0], v[1]);
@@ -370,13 +428,13 @@ QS_DEV void attend(const AttentionArgs& a, const int32_t* table, int head, int s
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 const int n = 2 * i;
-                c[i] = value_pair<V_BITS>(vc[n >> 2][n & 3], vc[n >> 2][(n & 3) + 1], 2 * b + e);
+                c[i] = value_pair<V_BITS>(t.vc[n >> 2][n & 3], t.vc[n >> 2][(n & 3) + 1], 2 * b + e);
             }
-#pragma unroll
-            for (int r = 0; r < 4; r++) sums.acc[b][e][r] *= shrink;
             sums.acc[b][e] = mfma(c, w, sums.acc[b][e]);
         }
     }
+    __builtin_amdgcn_sched_barrier(0);
+    load_values(a, next, t);
 }
 
 // The wave's sums as one: the four lanes of a query's slots, and its two columns.
@@ -392,7 +450,7 @@ QS_DEV void finish(Sums<BLOCKS>& o) {
 }
 
 QS_DEV int length_of(const AttentionArgs& a, int seq) {
-    const int most = a.pages_each << a.c.shift, n = a.lengths[seq];
+    const int most = a.pages_each << a.c.shift, n = constant(a.lengths)[seq];
     return n < 0 ? 0 : n > most ? most : n;
 }
 // Steps of a sequence for any of its queries, from step `begin` on: at least one,
@@ -450,6 +508,7 @@ QS_DEV Deal deal(const AttentionArgs& a, int groups, int heads) {
         int all = 0;
 #pragma unroll
         for (int i = 0; i < WAVES; i++) all += sums[i];
+        all = __builtin_amdgcn_readfirstlane(all);
         d.total = (int64_t)all * heads;
     }
     d.each = (d.total + groups - 1) / groups;
@@ -477,8 +536,8 @@ QS_DEV Deal deal(const AttentionArgs& a, int groups, int heads) {
         __syncthreads();
         if (found[0] >= 0) break;
     }
-    d.seq = found[0];
-    d.base = found[1];
+    d.seq = __builtin_amdgcn_readfirstlane(found[0]);
+    d.base = __builtin_amdgcn_readfirstlane(found[1]);
     return d;
 }
 
@@ -487,20 +546,22 @@ QS_DEV Deal deal(const AttentionArgs& a, int groups, int heads) {
 // their sums through LDS. A segment that is a whole one is written as the result,
 // else as a part that k_kv_join takes.
 template <int K_BITS, int V_BITS, int BLOCKS, bool WIDE>
-__global__ __launch_bounds__(64 * WAVES) void k_kv_attention(AttentionArgs a, Split split) {
+__global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(resident(BLOCKS, WIDE))))
+void k_kv_attention(AttentionArgs a, Split split) {
     constexpr int D = 32 * BLOCKS, ROW = D + 4;     // 4: the eight columns' words in other banks
     __shared__ __attribute__((aligned(16))) float acc[WAVES][COLUMNS][ROW];
     __shared__ float2 stats[WAVES][COLUMNS];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane >> 4;
     const int tiles = column_tiles(a), heads = a.c.heads * tiles;
     int64_t at, end;
-    int seq, base = 0;
+    int seq, base = 0, which = -1, from = 0;        // which: head and column tile
     int64_t each = 0;
     int4 going{0, 0, -1, 0};
     if (split.whole) {
         seq = (int)blockIdx.x / heads;
-        at = (int)blockIdx.x - seq * heads;         // the head; its steps are not counted
-        end = at + 1;
+        which = (int)blockIdx.x - seq * heads;
+        at = 0;
+        end = 1;
     } else {
         const Deal d = deal(a, split.groups, heads);
         each = d.each;
@@ -512,16 +573,14 @@ __global__ __launch_bounds__(64 * WAVES) void k_kv_attention(AttentionArgs a, Sp
     while (at < end) {
         const int length = length_of(a, seq);
         const Steps steps = steps_of(a, length);
-        int which, from, to;                        // head and column tile, steps of them
-        if (split.whole) {
-            which = (int)at;
-            from = 0;
-            to = steps.count;
-        } else {
-            const int64_t rel = at - (int64_t)base * heads;
-            which = (int)(rel / steps.count);
-            from = (int)(rel - (int64_t)which * steps.count);
-            to = steps.count - from < end - at ? steps.count : from + (int)(end - at);
+        int to = steps.count;                       // from .. to - 1 of them
+        if (!split.whole) {
+            if (which < 0) {
+                const int64_t rel = at - (int64_t)base * heads;
+                which = (int)(rel / steps.count);
+                from = (int)(rel - (int64_t)which * steps.count);
+            }
+            to = to - from < end - at ? to : from + (int)(end - at);
         }
         const int head = which / tiles, tile = which - head * tiles;
         Queries<BLOCKS, WIDE> q;
@@ -529,11 +588,27 @@ __global__ __launch_bounds__(64 * WAVES) void k_kv_attention(AttentionArgs a, Sp
         const Span span = span_of(a, tile, length);
         Sums<BLOCKS> sums;
         clear(sums);
-        const int32_t* table = a.tables + seq * a.table_stride;
-        for (int i = from + wave; i < to; i += WAVES) {
-            const int start = (steps.begin + i) * TILE;
-            if (start < span.last && start + TILE > span.first)
-                attend<K_BITS, V_BITS, BLOCKS, WIDE>(a, table, head, start, span, q, sums);
+        const Ints table = constant(a.tables + seq * a.table_stride);
+        // of them, those that this column tile's queries see
+        const int low = span.first / TILE - steps.begin, high = (span.last + TILE - 1) / TILE - steps.begin;
+        const int stop = high < to ? high : to;
+        int i = (low > from ? low : from) + wave;
+        if (i < stop) {
+            // The pages of a step are asked for two steps ahead, its codes one ahead; after
+            // the last step it is that step's again, whose codes are in the caches.
+            const int final = i + (stop - 1 - i) / WAVES * WAVES;
+            const auto start_of = [&](int n) { return (steps.begin + (n < final ? n : final)) * TILE; };
+            Place at = place_of(a, pages_of(a, table, start_of(i)), head, start_of(i));
+            Pages ahead = pages_of(a, table, start_of(i + WAVES));
+            Tile<K_BITS, V_BITS, BLOCKS> t;
+            load_keys(a, at, t);
+            load_values(a, at, t);
+            for (; i < stop; i += WAVES) {
+                const int start = start_of(i), held = at.held;
+                at = place_of(a, ahead, head, start_of(i + WAVES));
+                ahead = pages_of(a, table, start_of(i + 2 * WAVES));
+                attend(a, start, start < span.all_first || start + TILE > span.all_last || held != 3, held, at, q, t, sums);
+            }
         }
         finish(sums);
         if (!(lane & 8)) {
@@ -578,9 +653,10 @@ __global__ __launch_bounds__(64 * WAVES) void k_kv_attention(AttentionArgs a, Sp
         if (split.whole) break;
         if (from == 0 && !whole) going = int4{seq, which, (int)((at + steps.count - 1) / each), 0};
         at += to - from;
-        if (to == steps.count && which == heads - 1) {
+        from = 0;
+        if (++which == heads) {         // only the last segment ends before its steps do
+            which = 0;
             seq++;
-            base += steps.count;
         }
     }
     if (!split.whole && threadIdx.x == 0) split.segments[blockIdx.x] = going;

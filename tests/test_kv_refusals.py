@@ -92,7 +92,7 @@ def test_attention_refuses_workspaces(qs):
     for bad in (dict(work=None), dict(work=(1 << 20) + 16), dict(wsize=size - 1)):
         assert attention(L, cache(), m=300, ts=300, **bad) == -22 and b"workspace" in L.qs_last_error()
     # a part of every workgroup's two segments and eight queries: not a multiple of the lengths
-    assert need(cache(), 2, 1, 4, 1 << 20) == need(cache(), 2, 1, 4, 1 << 18) <= 768 * 2 * 8 * (64 * 4 + 8) + 768 * 16 + 1024
+    assert need(cache(), 2, 1, 4, 1 << 20) == need(cache(), 2, 1, 4, 1 << 18) <= 1024 * 2 * 8 * (64 * 4 + 8) + 1024 * 16 + 1024
 
 
 def test_nothing_is_no_work(qs):
