@@ -296,7 +296,7 @@ Split split_of(const AttentionArgs& a, void* workspace) {
     Split s{};
     if (a.batch == 0 || a.fresh == 0) return s;
     s.whole = steps <= FEW;
-    const int64_t most = (a.batch * heads * steps + WAVES - 1) / WAVES;
+    const int64_t most = (a.batch * heads * (steps + OPENING) + WAVES - 1) / WAVES;
     s.groups = (int32_t)(s.whole ? a.batch * heads : most < full ? most : full);
     if (s.whole) return s;
     const int64_t room = most < CUS * resident(a.c.blocks, false) ? most : CUS * resident(a.c.blocks, false);

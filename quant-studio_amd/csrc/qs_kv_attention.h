@@ -35,6 +35,7 @@ inline __host__ __device__ int column_tiles(const AttentionArgs& a) {
 // How a call's work is split, and where its workgroups leave what is joined.
 constexpr int TILE = 32;            // slots of a wave's step
 constexpr int WAVES = 4;            // of a workgroup, a step each in turn
+constexpr int OPENING = 4;          // steps that beginning with another segment takes as long as
 // workgroups that a CU holds, by the registers of a wave
 __host__ __device__ constexpr int resident(int blocks, bool wide) {
     return blocks == 2 ? 4 : blocks == 4 ? (wide ? 2 : 3) : blocks == 6 ? 2 : wide ? 1 : 2;

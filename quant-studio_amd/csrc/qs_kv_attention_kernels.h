@@ -156,15 +156,14 @@ struct Queries {
     float scale;                            // of the scores, beside 2^up
     int up;
     int first, last;                        // slots that the lane's query sees: first .. last - 1
-    bool live;
 };
 
 template <int K_BITS, int BLOCKS, bool WIDE>
 QS_DEV void load_queries(const AttentionArgs& a, int seq, int head, int tile, int length,
                          Queries<BLOCKS, WIDE>& o) {
     const int lane = threadIdx.x & 63, g = lane >> 4, column = tile * COLUMNS + (lane & 7);
-    o.live = column < a.group * a.fresh;
-    const int token = o.live ? column / a.group : 0, mine = o.live ? column - token * a.group : 0;
+    const bool live = column < a.group * a.fresh;
+    const int token = live ? column / a.group : 0, mine = live ? column - token * a.group : 0;
     const int64_t at = ((int64_t)seq * a.fresh + token) * a.q_stride + (int64_t)(head * a.group + mine) * 32 * BLOCKS;
     float x[BLOCKS][8];
     float top = 0.0f;
@@ -187,7 +186,7 @@ QS_DEV void load_queries(const AttentionArgs& a, int seq, int head, int tile, in
         }
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            x[b][i] = o.live ? x[b][i] : 0.0f;
+            x[b][i] = live ? x[b][i] : 0.0f;
             top = fmaxf(top, fabsf(x[b][i]));
         }
     }
@@ -470,7 +469,9 @@ QS_DEV Steps steps_of(const AttentionArgs& a, int length) {
 // The call's steps in a row (by sequence, head, tile of columns, then along the
 // sequence), dealt to the workgroups in equal runs: `total` of them, `each` to a
 // workgroup, this one's first one in sequence `seq`, whose own begin at `base` of one
-// head's. The lengths are on the device, so every workgroup adds them up.
+// head's. A head's steps count OPENING more than they are, which comes first: what
+// beginning with another one takes. The lengths are on the device, so every workgroup
+// adds them up.
 struct Deal {
     int64_t total, each;
     int seq, base;
@@ -495,13 +496,13 @@ QS_DEV Deal deal(const AttentionArgs& a, int groups, int heads) {
     const int wave = threadIdx.x >> 6;
     constexpr int THREADS = 64 * WAVES;
     Deal d;
-    const int first = (int)threadIdx.x < a.batch ? steps_of(a, length_of(a, threadIdx.x)).count : 0;
+    const int first = (int)threadIdx.x < a.batch ? OPENING + steps_of(a, length_of(a, threadIdx.x)).count : 0;
     if (a.batch == 1) {
-        d.total = (int64_t)steps_of(a, length_of(a, 0)).count * heads;
+        d.total = (int64_t)(OPENING + steps_of(a, length_of(a, 0)).count) * heads;
         d.seq = d.base = 0;
     } else {
         int n = first;
-        for (int i = threadIdx.x + THREADS; i < a.batch; i += THREADS) n += steps_of(a, length_of(a, i)).count;
+        for (int i = threadIdx.x + THREADS; i < a.batch; i += THREADS) n += OPENING + steps_of(a, length_of(a, i)).count;
         n = wave_sum(n);
         if ((threadIdx.x & 63) == 0) sums[wave] = n;
         __syncthreads();
@@ -520,7 +521,7 @@ QS_DEV Deal deal(const AttentionArgs& a, int groups, int heads) {
     int before = 0;
     for (int i = 0;; i += THREADS) {        // one of them holds `at`, which is below their sum
         const int mine = i + (int)threadIdx.x;
-        const int n = i == 0 ? first : mine < a.batch ? steps_of(a, length_of(a, mine)).count : 0;
+        const int n = i == 0 ? first : mine < a.batch ? OPENING + steps_of(a, length_of(a, mine)).count : 0;
         const int scan = wave_scan(n);
         __syncthreads();
         if ((threadIdx.x & 63) == 63) sums[wave] = scan;
@@ -570,6 +571,7 @@ void k_kv_attention(AttentionArgs a, Split split) {
         seq = d.seq;
         base = d.base;
     }
+    const int64_t begin = at;
     while (at < end) {
         const int length = length_of(a, seq);
         const Steps steps = steps_of(a, length);
@@ -577,14 +579,16 @@ void k_kv_attention(AttentionArgs a, Split split) {
         if (!split.whole) {
             if (which < 0) {
                 const int64_t rel = at - (int64_t)base * heads;
-                which = (int)(rel / steps.count);
-                from = (int)(rel - (int64_t)which * steps.count);
+                which = (int)(rel / (OPENING + steps.count));
+                at -= rel - (int64_t)which * (OPENING + steps.count);
+                from = (int)(begin - at) - OPENING;
             }
-            to = to - from < end - at ? to : from + (int)(end - at);
+            // `at`: where the head's begin, `from` below 0 where they do in this workgroup
+            to = to < end - at - OPENING ? to : (int)(end - at) - OPENING;
+            from = from < 0 ? 0 : from;
+            if (to <= from) break;                  // it ends before they do
         }
         const int head = which / tiles, tile = which - head * tiles;
-        Queries<BLOCKS, WIDE> q;
-        load_queries<K_BITS, BLOCKS, WIDE>(a, seq, head, tile, length, q);
         const Span span = span_of(a, tile, length);
         Sums<BLOCKS> sums;
         clear(sums);
@@ -603,6 +607,8 @@ void k_kv_attention(AttentionArgs a, Split split) {
             Tile<K_BITS, V_BITS, BLOCKS> t;
             load_keys(a, at, t);
             load_values(a, at, t);
+            Queries<BLOCKS, WIDE> q;
+            load_queries<K_BITS, BLOCKS, WIDE>(a, seq, head, tile, length, q);
             for (; i < stop; i += WAVES) {
                 const int start = start_of(i), held = at.held;
                 at = place_of(a, ahead, head, start_of(i + WAVES));
@@ -651,8 +657,8 @@ void k_kv_attention(AttentionArgs a, Split split) {
         if (!whole && sub == 0) split.stats[slot] = float2{ref, total};
         __syncthreads();
         if (split.whole) break;
-        if (from == 0 && !whole) going = int4{seq, which, (int)((at + steps.count - 1) / each), 0};
-        at += to - from;
+        if (from == 0 && !whole) going = int4{seq, which, (int)((at + OPENING + steps.count - 1) / each), 0};
+        at += OPENING + steps.count;
         from = 0;
         if (++which == heads) {         // only the last segment ends before its steps do
             which = 0;
