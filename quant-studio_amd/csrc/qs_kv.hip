@@ -53,7 +53,51 @@ QS_DEV Place place_of(const Cache& c, const Unit& u, int slot) {
     return {p + at * row, reinterpret_cast<uint16_t*>(p + c.page * row) + at * c.blocks + u.block};
 }
 
-constexpr int MOST_GROUP = 32;
+// How threads are laid over rows: `wide` of them (whole heads' keys or values, so
+// at most 256 and a multiple of a head's units) on one row, `together` rows at a
+// time, BATCH times over.
+constexpr int BATCH = 4, MOST_GROUP = 4 * 16;
+struct Shape {
+    int wide, together, columns;    // columns: workgroups for a row
+};
+__host__ __device__ inline Shape shape_of(int units, int blocks) {
+    const int most = 256 / (4 * blocks) * (4 * blocks);
+    Shape s;
+    s.wide = units < most ? units : most;
+    s.together = 256 / s.wide;
+    s.columns = (units + s.wide - 1) / s.wide;
+    return s;
+}
+
+// codes of eight values as the cache holds them, their block's step; four threads hold a block
+QS_DEV float codes_of(const float (&x)[8], int bits, int quarter, uint32_t (&code)[8]) {
+    if (bits == 8) {
+        float top = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const float m = fabsf(x[j]);
+            top = m > top || m != m ? m : top;      // keeps a NaN
+        }
+        const float m1 = qs::quad_xor<1>(top);
+        top = m1 > top || m1 != m1 ? m1 : top;
+        const float m2 = qs::quad_xor<2>(top);
+        top = m2 > top || m2 != m2 ? m2 : top;
+        const float d = top / 127.0f;
+        const float id = d != 0.0f ? 1.0f / d : 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            // -128 comes of steps below f16's smallest only, where the value is 0
+            const int q = max(qs::code_of(x[j], id), -127);
+            code[j] = q < 0 ? 128u - (uint32_t)q : (uint32_t)q;
+        }
+        return d;
+    }
+    const float d = qs::quad_absmax_first(x, quarter) * -0.125f;
+    const float id = d != 0.0f ? 1.0f / d : 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; j++) code[j] = qs::level_of(x[j], id, 8.5f, 15.5f);
+    return d;
+}
 
 // A thread takes eight values, four threads a block of 32: its step from their
 // largest magnitude, then eight codes each, in the order of the cache's rows.
@@ -62,68 +106,59 @@ constexpr int MOST_GROUP = 32;
 template <int SRC>
 __global__ __launch_bounds__(256) void k_kv_write(RowsArgs a) {
     __shared__ int mine[MOST_GROUP];
+    const Shape shape = shape_of(a.units, a.c.blocks);
     const int first = (int)blockIdx.x * a.group;
     const int count = a.rows - first < a.group ? a.rows - first : a.group;
     const int slots = a.c.pages << a.c.shift;
+    const int sub = (int)threadIdx.x / shape.wide;
+    const int at = (int)blockIdx.y * shape.wide + ((int)threadIdx.x - sub * shape.wide);
+    const bool live = sub < shape.together && at < a.units;
+    const Unit u = unit_of(a.c, live ? at : 0);
+    const void* src = u.value ? a.v : a.k;
+    const int64_t stride = u.value ? a.v_stride : a.k_stride;
+    const int64_t from = (int64_t)u.head * 32 * a.c.blocks + 32 * u.block + 8 * u.quarter;
+    const int bits = u.value ? a.c.v_bits : a.c.k_bits;
+    // every row's values are on their way before anything waits
+    Eight<SRC> in[BATCH];
+#pragma unroll
+    for (int i = 0; i < BATCH; i++) {
+        const int row = sub + i * shape.together;
+        if (live && row < count) load8<SRC>(src, (first + row) * stride + from, in[i]);
+    }
     if ((int)threadIdx.x < count) {
         const int s = a.slots[first + threadIdx.x];
         mine[threadIdx.x] = (unsigned)s < (unsigned)slots ? s : -1;
     }
     __syncthreads();
     if (a.rows - first > 1) {
-        uint32_t later = 0;     // rows of this group that a later one replaces
-        for (int r = first + 1 + (int)threadIdx.x; r < a.rows; r += 256) {
-            const int s = a.slots[r];
-            for (int i = 0; i < count; i++) later |= s == mine[i] && first + i < r ? 1u << i : 0u;
+        // slots of later rows, eight to a thread at a time
+        for (int r0 = first + 1; r0 < a.rows; r0 += 8 * 256) {
+            int s[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const int r = r0 + 256 * j + (int)threadIdx.x;
+                s[j] = r < a.rows ? a.slots[r] : -1;
+            }
+            for (int i = 0; i < count; i++) {
+                const int m = mine[i];
+                bool same = false;
+#pragma unroll
+                for (int j = 0; j < 8; j++) same |= s[j] == m && first + i < r0 + 256 * j + (int)threadIdx.x;
+                if (same) mine[i] = -1;         // one that reads it meanwhile has nothing to add
+            }
         }
-        __syncthreads();
-        for (int i = 0; i < count; i++)
-            if (later >> i & 1) mine[i] = -1;
         __syncthreads();
     }
-    const int wide = a.units < 256 ? a.units : 256, step_rows = 256 / wide;
-    const int sub = (int)threadIdx.x / wide;
-    const int at = (int)blockIdx.y * 256 + ((int)threadIdx.x - sub * wide);
-    if (sub >= step_rows || at >= a.units) return;
-    const Unit u = unit_of(a.c, at);
-    const void* src = u.value ? a.v : a.k;
-    const int64_t stride = u.value ? a.v_stride : a.k_stride;
-    const int bits = u.value ? a.c.v_bits : a.c.k_bits;
-    for (int i = sub; i < count; i += step_rows) {
-        const int slot = mine[i];
+#pragma unroll
+    for (int i = 0; i < BATCH; i++) {
+        const int row = sub + i * shape.together;
+        const int slot = live && row < count ? mine[row] : -1;
         if (slot < 0) continue;     // the same for the four threads of a block
-        Eight<SRC> in;
-        load8<SRC>(src, (first + i) * stride + (int64_t)u.head * 32 * a.c.blocks + 32 * u.block + 8 * u.quarter, in);
         float x[8];
 #pragma unroll
-        for (int j = 0; j < 8; j++) x[j] = value8<SRC>(in, j);
-        float d;
-        uint32_t code[8];           // as the cache holds them
-        if (bits == 8) {
-            float top = 0.0f;
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const float m = fabsf(x[j]);
-                top = m > top || m != m ? m : top;      // keeps a NaN
-            }
-            const float m1 = qs::quad_xor<1>(top);
-            top = m1 > top || m1 != m1 ? m1 : top;
-            const float m2 = qs::quad_xor<2>(top);
-            top = m2 > top || m2 != m2 ? m2 : top;
-            d = top / 127.0f;
-            const float id = d != 0.0f ? 1.0f / d : 0.0f;
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                // -128 comes of steps below f16's smallest only, where the value is 0
-                const int q = max(qs::code_of(x[j], id), -127);
-                code[j] = q < 0 ? 128u - (uint32_t)q : (uint32_t)q;
-            }
-        } else {
-            d = qs::quad_absmax_first(x, u.quarter) * -0.125f;
-            const float id = d != 0.0f ? 1.0f / d : 0.0f;
-#pragma unroll
-            for (int j = 0; j < 8; j++) code[j] = qs::level_of(x[j], id, 8.5f, 15.5f);
-        }
+        for (int j = 0; j < 8; j++) x[j] = value8<SRC>(in[i], j);
+        uint32_t code[8];
+        const float d = codes_of(x, bits, u.quarter, code);
         const Place p = place_of(a.c, u, slot);
         // a step that f16 cannot hold, like a NaN or an infinity in the block, stands for no values
         const uint32_t h = qs::f16_bits(d);
@@ -151,68 +186,85 @@ __global__ __launch_bounds__(256) void k_kv_write(RowsArgs a) {
     }
 }
 
-// The values of some slots' rows; a slot outside the cache gives zeros.
+// The values of some slots' rows; a slot outside the cache gives zeros. Eight to a
+// thread, of BATCH rows at a time.
 template <int DST>
 __global__ __launch_bounds__(256) void k_kv_read(RowsArgs a) {
-    const int first = (int)blockIdx.x * a.group;
-    const int count = a.rows - first < a.group ? a.rows - first : a.group;
+    const Shape shape = shape_of(a.units, a.c.blocks);
+    const int64_t first = (int64_t)blockIdx.x * a.group;
+    const int count = (int)(a.rows - first < a.group ? a.rows - first : a.group);
     const int slots = a.c.pages << a.c.shift;
-    const int wide = a.units < 256 ? a.units : 256, step_rows = 256 / wide;
-    const int sub = (int)threadIdx.x / wide;
-    const int at = (int)blockIdx.y * 256 + ((int)threadIdx.x - sub * wide);
-    if (sub >= step_rows || at >= a.units) return;
+    const int sub = (int)threadIdx.x / shape.wide;
+    const int at = (int)blockIdx.y * shape.wide + ((int)threadIdx.x - sub * shape.wide);
+    if (sub >= shape.together || at >= a.units) return;
     const Unit u = unit_of(a.c, at);
     void* dst = u.value ? a.v : a.k;
     const int64_t stride = u.value ? a.v_stride : a.k_stride;
     const int bits = u.value ? a.c.v_bits : a.c.k_bits;
-    for (int i = sub; i < count; i += step_rows) {
-        const int slot = a.slots[first + i];
-        float x[8] = {};
-        if ((unsigned)slot < (unsigned)slots) {
-            const Place p = place_of(a.c, u, slot);
-            const float d = qskv::half_of(*p.step);
-            if (!u.value) {
-                const uint8_t* o = p.row + qskv::k_unit(bits, a.c.blocks, u.quarter, u.block);
-                if (bits == 8) {
-                    const uint2 w = *reinterpret_cast<const uint2*>(o);
+    int slot[BATCH];
 #pragma unroll
-                    for (int j = 0; j < 8; j++) x[j] = qskv::code8((j < 4 ? w.x : w.y) >> (8 * (j & 3))) * d;
-                } else {
-                    const uint32_t w = *reinterpret_cast<const uint32_t*>(o);
+    for (int i = 0; i < BATCH; i++) {
+        const int row = sub + i * shape.together;
+        slot[i] = row < count ? a.slots[first + row] : -1;
+    }
+    uint32_t w[BATCH][4];       // keys: their words; values: a unit each
+    uint16_t step[BATCH];
 #pragma unroll
-                    for (int j = 0; j < 8; j++) x[j] = qskv::code4(w >> (4 * (j >> 1) + 16 * (j & 1))) * d;
-                }
+    for (int i = 0; i < BATCH; i++) {
+        w[i][0] = w[i][1] = w[i][2] = w[i][3] = 0;
+        step[i] = 0;
+        if ((unsigned)slot[i] >= (unsigned)slots) continue;
+        const Place p = place_of(a.c, u, slot[i]);
+        step[i] = *p.step;
+        if (!u.value) {
+            const uint8_t* o = p.row + qskv::k_unit(bits, a.c.blocks, u.quarter, u.block);
+            if (bits == 8) {
+                const uint2 c = *reinterpret_cast<const uint2*>(o);
+                w[i][0] = c.x, w[i][1] = c.y;
             } else {
+                w[i][0] = *reinterpret_cast<const uint32_t*>(o);
+            }
+        } else {
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const uint8_t* o = p.row + qskv::v_unit(bits, a.c.blocks, 4 * u.quarter + j, u.block);
-                    if (bits == 8) {
-                        const uint32_t w = *reinterpret_cast<const uint16_t*>(o);
-                        x[2 * j] = qskv::code8(w) * d, x[2 * j + 1] = qskv::code8(w >> 8) * d;
-                    } else {
-                        x[2 * j] = qskv::code4(*o) * d, x[2 * j + 1] = qskv::code4(*o >> 4) * d;
-                    }
-                }
+            for (int j = 0; j < 4; j++) {
+                const uint8_t* o = p.row + qskv::v_unit(bits, a.c.blocks, 4 * u.quarter + j, u.block);
+                w[i][j] = bits == 8 ? *reinterpret_cast<const uint16_t*>(o) : *o;
             }
         }
-        store8<DST>(dst, (first + i) * stride + (int64_t)u.head * 32 * a.c.blocks + 32 * u.block + 8 * u.quarter, x);
+    }
+#pragma unroll
+    for (int i = 0; i < BATCH; i++) {
+        const int row = sub + i * shape.together;
+        if (row >= count) break;
+        float x[8] = {};
+        if ((unsigned)slot[i] < (unsigned)slots) {
+            const float d = qskv::half_of(step[i]);
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const uint32_t c = u.value ? w[i][j >> 1] >> (bits * (j & 1))
+                                   : bits == 8 ? w[i][j >> 2] >> (8 * (j & 3))
+                                               : w[i][0] >> (4 * (j >> 1) + 16 * (j & 1));
+                x[j] = (bits == 8 ? qskv::code8(c) : qskv::code4(c)) * d;
+            }
+        }
+        store8<DST>(dst, (first + row) * stride + (int64_t)u.head * 32 * a.c.blocks + 32 * u.block + 8 * u.quarter, x);
     }
 }
 
-// rows of a launch: what a workgroup looks its slots up among
+// Rows of a launch that writes: what a workgroup looks its slots up among.
 constexpr int64_t MOST_ROWS = 8192;
 
 template <typename F>
-hipError_t launch_rows(const RowsArgs& all, int esz, F&& kernel, hipStream_t st) {
-    const int wide = all.units < 256 ? all.units : 256, step_rows = 256 / wide;
-    for (int64_t first = 0; first < all.rows; first += MOST_ROWS) {
+hipError_t launch_rows(const RowsArgs& all, int64_t most, int esz, F&& kernel, hipStream_t st) {
+    const Shape shape = shape_of(all.units, all.c.blocks);
+    for (int64_t first = 0; first < all.rows; first += most) {
         RowsArgs a = all;
-        a.rows = (int32_t)(all.rows - first < MOST_ROWS ? all.rows - first : MOST_ROWS);
+        a.rows = (int32_t)(all.rows - first < most ? all.rows - first : most);
         a.k = static_cast<char*>(all.k) + first * all.k_stride * esz;
         a.v = static_cast<char*>(all.v) + first * all.v_stride * esz;
         a.slots = all.slots + first;
-        a.group = step_rows * (a.rows > 1024 ? (step_rows > 4 ? 2 : 8) : 1);
-        const dim3 grid((unsigned)((a.rows + a.group - 1) / a.group), (unsigned)((a.units + 255) / 256));
+        a.group = shape.together * (a.rows > 1024 ? BATCH : 1);
+        const dim3 grid((unsigned)((a.rows + a.group - 1) / a.group), (unsigned)shape.columns);
         const hipError_t e = qs_host::launch_kernel(kernel, grid, dim3(256), 0, st, a);
         if (e != hipSuccess) return e;
     }
@@ -348,7 +400,7 @@ int qs_kv_write(const qs_kv_cache* cache, int src_type, const void* k, int64_t k
     const auto kernel = src_type == QS_SRC_F32   ? k_kv_write<qs::SRC_F32>
                         : src_type == QS_SRC_F16 ? k_kv_write<qs::SRC_F16>
                                                  : k_kv_write<qs::SRC_BF16>;
-    const hipError_t e = launch_rows(a, esz, kernel, static_cast<hipStream_t>(hip_stream));
+    const hipError_t e = launch_rows(a, MOST_ROWS, esz, kernel, static_cast<hipStream_t>(hip_stream));
     if (e != hipSuccess) return fail(QS_EIO, "kv_write: launch failed: %s", hipGetErrorString(e));
     return 0;
 }
@@ -374,7 +426,7 @@ int qs_kv_read(const qs_kv_cache* cache, const int32_t* slots, int64_t rows, int
     const auto kernel = dst_type == QS_SRC_F32   ? k_kv_read<qs::SRC_F32>
                         : dst_type == QS_SRC_F16 ? k_kv_read<qs::SRC_F16>
                                                  : k_kv_read<qs::SRC_BF16>;
-    const hipError_t e = launch_rows(a, esz, kernel, static_cast<hipStream_t>(hip_stream));
+    const hipError_t e = launch_rows(a, kMaxRows, esz, kernel, static_cast<hipStream_t>(hip_stream));
     if (e != hipSuccess) return fail(QS_EIO, "kv_read: launch failed: %s", hipGetErrorString(e));
     return 0;
 }
