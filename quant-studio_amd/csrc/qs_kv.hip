@@ -2,6 +2,8 @@
 // (declarations: include/quant_studio.h; the layout: qs_kv.h).
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "qs_host.h"
 #include "qs_kernels.h"
 #include "qs_kv.h"
@@ -57,6 +59,10 @@ QS_DEV Place place_of(const Cache& c, const Unit& u, int slot) {
 // at most 256 and a multiple of a head's units) on one row, `together` rows at a
 // time, BATCH times over.
 constexpr int BATCH = 4, MOST_GROUP = 4 * 16;
+// rows of a launch that writes: what a workgroup looks its slots up among
+constexpr int64_t MOST_ROWS = 8192;
+// calls of no more rows take one at a time: more workgroups
+constexpr int FEW_ROWS = 1024;
 struct Shape {
     int wide, together, columns;    // columns: workgroups for a row
 };
@@ -103,9 +109,9 @@ QS_DEV float codes_of(const float (&x)[8], int bits, int quarter, uint32_t (&cod
 // largest magnitude, then eight codes each, in the order of the cache's rows.
 // Of rows with the same slot the last is written: every workgroup looks its rows'
 // slots up among all later ones, which a launch's few rows make cheap.
-template <int SRC>
+template <int SRC, bool MANY>
 __global__ __launch_bounds__(256) void k_kv_write(RowsArgs a) {
-    __shared__ int mine[MOST_GROUP];
+    __shared__ int mine[MOST_GROUP], replaced[MOST_GROUP];
     const Shape shape = shape_of(a.units, a.c.blocks);
     const int first = (int)blockIdx.x * a.group;
     const int count = a.rows - first < a.group ? a.rows - first : a.group;
@@ -118,41 +124,53 @@ __global__ __launch_bounds__(256) void k_kv_write(RowsArgs a) {
     const int64_t stride = u.value ? a.v_stride : a.k_stride;
     const int64_t from = (int64_t)u.head * 32 * a.c.blocks + 32 * u.block + 8 * u.quarter;
     const int bits = u.value ? a.c.v_bits : a.c.k_bits;
-    // every row's values are on their way before anything waits
-    Eight<SRC> in[BATCH];
+    // The slots of the workgroup's rows and of all later ones, which a launch has few
+    // enough of for one turn, then the rows' values: all are on their way before
+    // anything waits, and the slots are compared meanwhile.
+    const int s0 = (int)threadIdx.x < count ? a.slots[first + threadIdx.x] : -1;
+    constexpr int TIMES = MANY ? BATCH : 1, TURNS = MANY ? (int)(MOST_ROWS / FEW_ROWS) : 1;
+    int later[TURNS][4];
 #pragma unroll
-    for (int i = 0; i < BATCH; i++) {
+    for (int j = 0; j < TURNS; j++) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) later[j][e] = -1;
+        if (first + count + FEW_ROWS * j >= a.rows) continue;       // the same for all
+        const int r = first + count + FEW_ROWS * j + 4 * (int)threadIdx.x;
+        if (r + 3 < a.rows) __builtin_memcpy(later[j], a.slots + r, 16);
+        else
+#pragma unroll
+            for (int e = 0; e < 3; e++)
+                if (r + e < a.rows) later[j][e] = a.slots[r + e];
+    }
+    Eight<SRC> in[TIMES];
+#pragma unroll
+    for (int i = 0; i < TIMES; i++) {
         const int row = sub + i * shape.together;
-        if (live && row < count) load8<SRC>(src, (first + row) * stride + from, in[i]);
+        if (live && row < count) load8_once<SRC>(src, (first + row) * stride + from, in[i]);
     }
     if ((int)threadIdx.x < count) {
-        const int s = a.slots[first + threadIdx.x];
-        mine[threadIdx.x] = (unsigned)s < (unsigned)slots ? s : -1;
+        mine[threadIdx.x] = (unsigned)s0 < (unsigned)slots ? s0 : -1;
+        replaced[threadIdx.x] = 0;
     }
     __syncthreads();
     if (a.rows - first > 1) {
-        // slots of later rows, eight to a thread at a time
-        for (int r0 = first + 1; r0 < a.rows; r0 += 8 * 256) {
-            int s[8];
+        for (int i = 0; i < count; i++) {
+            const int m = mine[i];
+            bool same = (int)threadIdx.x > i && s0 == m;
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const int r = r0 + 256 * j + (int)threadIdx.x;
-                s[j] = r < a.rows ? a.slots[r] : -1;
-            }
-            for (int i = 0; i < count; i++) {
-                const int m = mine[i];
-                bool same = false;
+            for (int j = 0; j < TURNS; j++) {
+                if (first + count + FEW_ROWS * j >= a.rows) break;
 #pragma unroll
-                for (int j = 0; j < 8; j++) same |= s[j] == m && first + i < r0 + 256 * j + (int)threadIdx.x;
-                if (same) mine[i] = -1;         // one that reads it meanwhile has nothing to add
+                for (int e = 0; e < 4; e++) same |= later[j][e] == m;
             }
+            if (same) replaced[i] = 1;
         }
         __syncthreads();
     }
 #pragma unroll
-    for (int i = 0; i < BATCH; i++) {
+    for (int i = 0; i < TIMES; i++) {
         const int row = sub + i * shape.together;
-        const int slot = live && row < count ? mine[row] : -1;
+        const int slot = live && row < count && !replaced[row] ? mine[row] : -1;
         if (slot < 0) continue;     // the same for the four threads of a block
         float x[8];
 #pragma unroll
@@ -188,8 +206,9 @@ __global__ __launch_bounds__(256) void k_kv_write(RowsArgs a) {
 
 // The values of some slots' rows; a slot outside the cache gives zeros. Eight to a
 // thread, of BATCH rows at a time.
-template <int DST>
+template <int DST, bool MANY>
 __global__ __launch_bounds__(256) void k_kv_read(RowsArgs a) {
+    constexpr int TIMES = MANY ? BATCH : 1;
     const Shape shape = shape_of(a.units, a.c.blocks);
     const int64_t first = (int64_t)blockIdx.x * a.group;
     const int count = (int)(a.rows - first < a.group ? a.rows - first : a.group);
@@ -201,16 +220,16 @@ __global__ __launch_bounds__(256) void k_kv_read(RowsArgs a) {
     void* dst = u.value ? a.v : a.k;
     const int64_t stride = u.value ? a.v_stride : a.k_stride;
     const int bits = u.value ? a.c.v_bits : a.c.k_bits;
-    int slot[BATCH];
+    int slot[TIMES];
 #pragma unroll
-    for (int i = 0; i < BATCH; i++) {
+    for (int i = 0; i < TIMES; i++) {
         const int row = sub + i * shape.together;
         slot[i] = row < count ? a.slots[first + row] : -1;
     }
-    uint32_t w[BATCH][4];       // keys: their words; values: a unit each
-    uint16_t step[BATCH];
+    uint32_t w[TIMES][4];       // keys: their words; values: a unit each
+    uint16_t step[TIMES];
 #pragma unroll
-    for (int i = 0; i < BATCH; i++) {
+    for (int i = 0; i < TIMES; i++) {
         w[i][0] = w[i][1] = w[i][2] = w[i][3] = 0;
         step[i] = 0;
         if ((unsigned)slot[i] >= (unsigned)slots) continue;
@@ -233,7 +252,7 @@ __global__ __launch_bounds__(256) void k_kv_read(RowsArgs a) {
         }
     }
 #pragma unroll
-    for (int i = 0; i < BATCH; i++) {
+    for (int i = 0; i < TIMES; i++) {
         const int row = sub + i * shape.together;
         if (row >= count) break;
         float x[8] = {};
@@ -247,15 +266,12 @@ __global__ __launch_bounds__(256) void k_kv_read(RowsArgs a) {
                 x[j] = (bits == 8 ? qskv::code8(c) : qskv::code4(c)) * d;
             }
         }
-        store8<DST>(dst, (first + row) * stride + (int64_t)u.head * 32 * a.c.blocks + 32 * u.block + 8 * u.quarter, x);
+        store8<DST, true>(dst, (first + row) * stride + (int64_t)u.head * 32 * a.c.blocks + 32 * u.block + 8 * u.quarter, x);
     }
 }
 
-// Rows of a launch that writes: what a workgroup looks its slots up among.
-constexpr int64_t MOST_ROWS = 8192;
-
 template <typename F>
-hipError_t launch_rows(const RowsArgs& all, int64_t most, int esz, F&& kernel, hipStream_t st) {
+hipError_t launch_rows(const RowsArgs& all, int64_t most, int esz, F&& few, F&& many, hipStream_t st) {
     const Shape shape = shape_of(all.units, all.c.blocks);
     for (int64_t first = 0; first < all.rows; first += most) {
         RowsArgs a = all;
@@ -263,9 +279,9 @@ hipError_t launch_rows(const RowsArgs& all, int64_t most, int esz, F&& kernel, h
         a.k = static_cast<char*>(all.k) + first * all.k_stride * esz;
         a.v = static_cast<char*>(all.v) + first * all.v_stride * esz;
         a.slots = all.slots + first;
-        a.group = shape.together * (a.rows > 1024 ? BATCH : 1);
+        a.group = shape.together * (a.rows > FEW_ROWS ? BATCH : 1);
         const dim3 grid((unsigned)((a.rows + a.group - 1) / a.group), (unsigned)shape.columns);
-        const hipError_t e = qs_host::launch_kernel(kernel, grid, dim3(256), 0, st, a);
+        const hipError_t e = qs_host::launch_kernel(a.rows > FEW_ROWS ? many : few, grid, dim3(256), 0, st, a);
         if (e != hipSuccess) return e;
     }
     return hipSuccess;
@@ -397,10 +413,14 @@ int qs_kv_write(const qs_kv_cache* cache, int src_type, const void* k, int64_t k
     a.slots = slots;
     a.rows = (int32_t)rows;
     a.units = 8 * a.c.heads * a.c.blocks;
-    const auto kernel = src_type == QS_SRC_F32   ? k_kv_write<qs::SRC_F32>
-                        : src_type == QS_SRC_F16 ? k_kv_write<qs::SRC_F16>
-                                                 : k_kv_write<qs::SRC_BF16>;
-    const hipError_t e = launch_rows(a, MOST_ROWS, esz, kernel, static_cast<hipStream_t>(hip_stream));
+    hipStream_t st = static_cast<hipStream_t>(hip_stream);
+    const auto launch = [&](auto type) {
+        constexpr int T = decltype(type)::value;
+        return launch_rows(a, MOST_ROWS, esz, k_kv_write<T, false>, k_kv_write<T, true>, st);
+    };
+    const hipError_t e = src_type == QS_SRC_F32   ? launch(std::integral_constant<int, qs::SRC_F32>{})
+                         : src_type == QS_SRC_F16 ? launch(std::integral_constant<int, qs::SRC_F16>{})
+                                                  : launch(std::integral_constant<int, qs::SRC_BF16>{});
     if (e != hipSuccess) return fail(QS_EIO, "kv_write: launch failed: %s", hipGetErrorString(e));
     return 0;
 }
@@ -423,10 +443,14 @@ int qs_kv_read(const qs_kv_cache* cache, const int32_t* slots, int64_t rows, int
     a.slots = slots;
     a.rows = (int32_t)rows;
     a.units = 8 * a.c.heads * a.c.blocks;
-    const auto kernel = dst_type == QS_SRC_F32   ? k_kv_read<qs::SRC_F32>
-                        : dst_type == QS_SRC_F16 ? k_kv_read<qs::SRC_F16>
-                                                 : k_kv_read<qs::SRC_BF16>;
-    const hipError_t e = launch_rows(a, kMaxRows, esz, kernel, static_cast<hipStream_t>(hip_stream));
+    hipStream_t st = static_cast<hipStream_t>(hip_stream);
+    const auto launch = [&](auto type) {
+        constexpr int T = decltype(type)::value;
+        return launch_rows(a, kMaxRows, esz, k_kv_read<T, false>, k_kv_read<T, true>, st);
+    };
+    const hipError_t e = dst_type == QS_SRC_F32   ? launch(std::integral_constant<int, qs::SRC_F32>{})
+                         : dst_type == QS_SRC_F16 ? launch(std::integral_constant<int, qs::SRC_F16>{})
+                                                  : launch(std::integral_constant<int, qs::SRC_BF16>{});
     if (e != hipSuccess) return fail(QS_EIO, "kv_read: launch failed: %s", hipGetErrorString(e));
     return 0;
 }

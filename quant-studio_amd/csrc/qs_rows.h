@@ -18,6 +18,13 @@ QS_DEV void load8(const void* p, int64_t at, Eight<SRC>& o) {
     o.w[0] = s[0];
     if constexpr (SRC == qs::SRC_F32) o.w[1] = s[1];
 }
+// values that are read or written once: around the caches' other contents
+template <int SRC>
+QS_DEV void load8_once(const void* p, int64_t at, Eight<SRC>& o) {
+    const u32x4* s = reinterpret_cast<const u32x4*>(static_cast<const char*>(p) + at * (SRC == qs::SRC_F32 ? 4 : 2));
+    o.w[0] = __builtin_nontemporal_load(s);
+    if constexpr (SRC == qs::SRC_F32) o.w[1] = __builtin_nontemporal_load(s + 1);
+}
 template <int SRC>
 QS_DEV float value8(const Eight<SRC>& o, int i) {
     if constexpr (SRC == qs::SRC_F32) return __uint_as_float(o.w[i >> 2][i & 3]);
@@ -37,17 +44,21 @@ QS_DEV uint32_t bits16(float f) {
     qs::keep_in_register(f);
     return (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)f);
 }
-template <int DST>
+template <int DST, bool ONCE = false>
 QS_DEV void store8(void* p, int64_t at, const float (&v)[8]) {
     u32x4* d = reinterpret_cast<u32x4*>(static_cast<char*>(p) + at * (DST == qs::SRC_F32 ? 4 : 2));
+    const auto put = [&](int i, const u32x4& o) {
+        if constexpr (ONCE) __builtin_nontemporal_store(o, d + i);
+        else d[i] = o;
+    };
     if constexpr (DST == qs::SRC_F32) {
-        d[0] = u32x4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
-        d[1] = u32x4{__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7])};
+        put(0, u32x4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])});
+        put(1, u32x4{__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7])});
     } else {
         u32x4 o;
 #pragma unroll
         for (int i = 0; i < 4; i++) o[i] = bits16<DST>(v[2 * i]) | (bits16<DST>(v[2 * i + 1]) << 16);
-        d[0] = o;
+        put(0, o);
     }
 }
 
