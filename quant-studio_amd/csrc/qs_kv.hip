@@ -92,9 +92,12 @@ QS_DEV float codes_of(const float (&x)[8], int bits, int quarter, uint32_t (&cod
         const float id = d != 0.0f ? 1.0f / d : 0.0f;
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            // -128 comes of steps below f16's smallest only, where the value is 0
-            const int q = max(qs::code_of(x[j], id), -127);
-            code[j] = q < 0 ? 128u - (uint32_t)q : (uint32_t)q;
+            // Half away from zero, of the magnitude: m + the largest f32 below 0.5 passes
+            // a whole number exactly where m + 0.5 does (m + 0.5 itself would also take
+            // 0.5's predecessor to 1). Over 127 only with steps below f16's smallest,
+            // which are 0.
+            const uint32_t m = (uint32_t)fminf(fabsf(x[j] * id) + 0x1.fffffep-2f, 127.0f);
+            code[j] = m | (__float_as_uint(x[j]) >> 31) << 7;
         }
         return d;
     }
