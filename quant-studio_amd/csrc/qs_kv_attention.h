@@ -44,7 +44,7 @@ struct Split {
     int32_t groups;                 // workgroups
     bool whole;                     // each takes one segment as a whole, and nothing is joined
     // of each workgroup, first for a segment that begins before it, then for one that goes on after it
-    float* parts;                   // [groups][2][COLUMNS][head size], relative to R
+    float* parts;                   // [groups][2][COLUMNS][head size], 2^-24 of a sum relative to R
     float2* stats;                  // [groups][2][COLUMNS]: R, sum of p
     int4* segments;                 // [groups]: sequence, head and column tile, last workgroup of the segment
                                     // that begins here and goes on, or -1 for none
@@ -66,8 +66,7 @@ QS_DEV int64_t row_of(const AttentionArgs& a, int seq, int head, int column) {
     return ((((int64_t)seq * a.fresh + token) * a.c.heads + head) * a.group + column - token * a.group) * (32 * a.c.blocks);
 }
 
-// unit: what a result of 1 is in the parts
-hipError_t launch_join(const AttentionArgs& a, const Split& split, float unit, hipStream_t st);
+hipError_t launch_join(const AttentionArgs& a, const Split& split, hipStream_t st);
 
 template <int K_BITS, int V_BITS>
 hipError_t launch_attention(const AttentionArgs& a, const Split& split, hipStream_t st);

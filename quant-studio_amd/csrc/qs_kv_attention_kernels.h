@@ -10,17 +10,17 @@
 //            block's dimensions, with P = p step (the step runs along the sum)
 //
 // The scores' D has its slots where the values' P wants them (a lane: one query,
-// slots 4 g .. 4 g + 3 of both sixteens), so nothing moves between lanes. Eight-bit
-// codes go to f16 without a conversion, as subnormal numbers (c 2^-24), which the
-// matrix units multiply exactly; four-bit ones by a multiply-add that takes their
-// offset off (left on, it would have to come off the sums, and these would cancel).
-// P is held to 22 bits: a query has two of the 16
-// columns, one takes f16(P), the other f16(P - f16(P)). So that the second does
-// not fall below f16's range, p is relative to R = m - s, with m the running
-// maximum and 2^s the power of two that takes the largest step so far to 2^14 ..
-// 2^15: what is lost is under 2^-39 of the largest P. q is rounded to f16 after its
-// row is scaled to 2^14 .. 2^15 in the same way: all of a bf16 or f16 q down to
-// 2^-39 of the row's largest; an f32 q takes two products, 22 bits.
+// slots 4 g .. 4 g + 3 of both sixteens), so nothing moves between lanes. Codes go to
+// f16 without a conversion, as subnormal numbers (c 2^-24), which the matrix units
+// multiply exactly; from four-bit ones an addition takes their offset of 8 (left on, it
+// would have to come off the sums, and these would cancel).
+// P is held to 21 bits or more: a query has two of the 16 columns, one takes f16(P),
+// the other f16(P - f16(P)). So that the second does not fall below f16's range, p is
+// relative to R = m - s, with m the running maximum and 2^s a power of two that takes
+// the largest step so far to just below 2^15: what is lost is under 2^-24 of the
+// largest P, mostly far under. q is rounded to f16 after its row is scaled to 2^14 ..
+// 2^15 in the same way: all of a bf16 or f16 q down to 2^-35 of the row's largest; an
+// f32 q takes two products, 22 bits.
 #pragma once
 
 #include "qs_kv_attention.h"
@@ -102,15 +102,12 @@ QS_DEV uint32_t sign_and_magnitude(uint32_t w, uint32_t pick) {
     return __builtin_amdgcn_perm(0u, w, pick) & 0x807f807fu;
 }
 
-// the four-bit codes `i` and i + 4 of a word, less 8, as f16: 1024 + u or 1024 + 16 u
-// by its bits, which an exact multiply-add takes to u - 8
+// The four-bit codes i and i + 4 of a word as f16, less 8: a subnormal number too,
+// c 2^-24 or (odd i, whose bits are not shifted down) c 2^-20.
 QS_DEV uint32_t four_bits(uint32_t w, int i) {
-    w = i & 2 ? w >> 8 : w;
-    const uint32_t bits = (w & (i & 1 ? 0x00f000f0u : 0x000f000fu)) | 0x64006400u;
-    const half2_t h = __builtin_bit_cast(half2_t, bits);
-    const half2_t v = i & 1 ? __builtin_elementwise_fma(h, half2_t{(_Float16)0.0625f, (_Float16)0.0625f}, half2_t{(_Float16)-72.0f, (_Float16)-72.0f})
-                            : h + half2_t{(_Float16)-1032.0f, (_Float16)-1032.0f};
-    return __builtin_bit_cast(uint32_t, v);
+    w = (i & 2 ? w >> 8 : w) & (i & 1 ? 0x00f000f0u : 0x000f000fu);
+    const _Float16 eight = i & 1 ? (_Float16)-0x1p-17f : (_Float16)-0x1p-21f;
+    return __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2_t, w) + half2_t{eight, eight});
 }
 
 // eight codes of a key's block as f16
@@ -141,12 +138,17 @@ QS_DEV uint32_t value_pair(const Codes<N>& x, const Codes<N>& y, int n) {
     }
 }
 
-// Two values as f16: to nearest for f32 results, else by the one instruction that
-// cuts off (a bit less of P)
+// Two P as the lane's column takes them: f16(P), cut off, in the first (second = 0); in
+// the second (0xffffe000, what of an f32 an f16 has) what that leaves of it, cut off as
+// well, which one instruction does for both, or to nearest for f32 results.
 template <bool NEAREST>
-QS_DEV half2_t two_halves(float x, float y) {
-    if constexpr (NEAREST) return half2_t{(_Float16)x, (_Float16)y};
-    else return __builtin_bit_cast(half2_t, __builtin_amdgcn_cvt_pkrtz(x, y));
+QS_DEV uint32_t two_halves(float x, float y, uint32_t second) {
+    const auto cut = [](float v, uint32_t mask) { return __uint_as_float(__float_as_uint(v) & mask); };
+    if constexpr (NEAREST) {
+        const float u = cut(x, 0xffffe000u), v = cut(y, 0xffffe000u);
+        return __builtin_bit_cast(uint32_t, half2_t{(_Float16)(second ? x - u : u), (_Float16)(second ? y - v : v)});
+    }
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x - cut(x, second), y - cut(y, second)));
 }
 
 // the queries of a wave, as the scores' products take them
@@ -200,7 +202,8 @@ QS_DEV void load_queries(const AttentionArgs& a, int seq, int head, int tile, in
             half2_t h, l;
 #pragma unroll
             for (int j = 0; j < 2; j++) {
-                const float v = __builtin_ldexpf(x[b][2 * i + j], e);
+                // where a four-bit key's code counts 16 times
+                const float v = __builtin_ldexpf(x[b][2 * i + j], K_BITS == 4 && i & 1 ? e - 4 : e);
                 h[j] = (_Float16)v;
                 if constexpr (WIDE) l[j] = (_Float16)(v - (float)h[j]);
             }
@@ -209,7 +212,7 @@ QS_DEV void load_queries(const AttentionArgs& a, int seq, int head, int tile, in
         }
     }
     o.scale = a.scale * LOG2E;
-    o.up = (K_BITS == 8 ? 24 : 0) - e;
+    o.up = 24 - e;
     o.last = length - a.fresh + 1 + token;
     o.first = a.window > 0 && o.last > a.window ? o.last - a.window : 0;
 }
@@ -219,7 +222,7 @@ template <int BLOCKS>
 struct Sums {
     f32x4 acc[BLOCKS][2];               // dims 32 block + 8 g + 2 r + e at [block][e][r]
     float top, ref, total;              // running maximum, R, sum of p
-    int step;                           // bits of the largest step so far
+    uint32_t step;                      // the bits of all steps so far, or'ed
 };
 template <int BLOCKS>
 QS_DEV void clear(Sums<BLOCKS>& o) {
@@ -318,8 +321,6 @@ QS_DEV void load_values(const AttentionArgs& a, const Place& at, Tile<K_BITS, V_
     }
 }
 
-typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
-
 // One step: the slots start .. start + 31, in `t`. The next step's keys and values
 // (at `next`) are loaded into the registers of this one's as soon as these are done
 // with, and arrive while the other half is computed.
@@ -368,20 +369,21 @@ QS_DEV void attend(const AttentionArgs& a, int start, bool edge, int held, const
     }
     // the running maximum and R
     float top = sums.top;
-    u16x2 most{0, 0};
+    uint32_t steps = 0;
 #pragma unroll
     for (int s = 0; s < 2; s++) {
 #pragma unroll
         for (int r = 0; r < 4; r++) top = fmaxf(top, x[s][r]);
 #pragma unroll
-        for (int i = 0; i < STEPS; i++)     // eight-bit steps are not negative
-            most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, V_BITS == 8 ? t.vs[s].w[i] : t.vs[s].w[i] & 0x7fff7fffu));
+        for (int i = 0; i < STEPS; i++) steps |= t.vs[s].w[i];
     }
     top = max_over_slots(top);
-    const uint32_t big = over_slots(most[0] > most[1] ? most[0] : most[1], [](uint32_t u, uint32_t v) { return max(u, v); });
-    sums.step = max(sums.step, (int)big);
-    // 2^s takes the largest step to 2^14 .. 2^15; a subnormal one, or none, counts as 2^-14
-    const int s = 29 - max(sums.step >> 10, 1);
+    steps = over_slots(steps, [](uint32_t u, uint32_t v) { return u | v; });
+    sums.step |= steps | steps >> 16;
+    // 2^s takes every step below 2^15. Or'ed exponents bound them all, and are over the
+    // largest by 15 at most, by 7 for steps below 2, which takes that much off 39 bits; a
+    // subnormal step, or none, counts as 2^-14.
+    const int exponent = (int)(sums.step >> 10 & 31), s = 29 - (exponent > 1 ? exponent : 1);
     const float ref = top > -__builtin_inff() ? top - (float)s : -__builtin_inff();
     const float base = top > -__builtin_inff() ? ref : 0.0f;
     const float shrink = __builtin_amdgcn_exp2f(sums.ref - base);   // 0 where nothing was seen yet
@@ -403,23 +405,16 @@ QS_DEV void attend(const AttentionArgs& a, int start, bool edge, int held, const
 #pragma unroll
                 for (int r = 0; r < 4; r++) sums.acc[b][e][r] *= shrink;
     }
-    const float second = lane & 8 ? -1.0f : 0.0f;
+    const uint32_t second = lane & 8 ? 0xffffe000u : 0u;
 #pragma unroll
     for (int b = 0; b < BLOCKS; b++) {
         u32x4 w;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            float v[2];
-#pragma unroll
-            for (int j = 0; j < 2; j++) {
-                const int n = 2 * i + j;
-                // + 0 makes it one instruction that takes the step as f16
-                v[j] = __builtin_fmaf(p[n], step_of(t.vs[n >> 2], n & 3, b), 0.0f);
-            }
-            // both columns round alike: the first to f16(P), the second what that leaves
-            const half2_t h = two_halves<WIDE>(v[0], v[1]);
-            w[i] = __builtin_bit_cast(uint32_t, two_halves<WIDE>(__builtin_fmaf((float)h[0], second, v[0]),
-                                                                 __builtin_fmaf((float)h[1], second, v[1])));
+            const int n = 2 * i;
+            const float d0 = step_of(t.vs[n >> 2], n & 3, b), d1 = step_of(t.vs[n >> 2], (n & 3) + 1, b);
+            // + 0 makes it one instruction that takes the step as f16
+            w[i] = two_halves<WIDE>(__builtin_fmaf(p[n], d0, 0.0f), __builtin_fmaf(p[n + 1], d1, 0.0f), second);
         }
 #pragma unroll
         for (int e = 0; e < 2; e++) {
@@ -436,8 +431,9 @@ QS_DEV void attend(const AttentionArgs& a, int start, bool edge, int held, const
     load_values(a, next, t);
 }
 
-// The wave's sums as one: the four lanes of a query's slots, and its two columns.
-template <int BLOCKS>
+// The wave's sums as one: the four lanes of a query's slots, and its two columns;
+// four-bit codes that count 16 times.
+template <int V_BITS, int BLOCKS>
 QS_DEV void finish(Sums<BLOCKS>& o) {
     o.total = sum_over_slots(o.total);
 #pragma unroll
@@ -445,7 +441,10 @@ QS_DEV void finish(Sums<BLOCKS>& o) {
 #pragma unroll
         for (int e = 0; e < 2; e++)
 #pragma unroll
-            for (int r = 0; r < 4; r++) o.acc[b][e][r] += other_column(o.acc[b][e][r]);
+            for (int r = 0; r < 4; r++) {
+                const float v = o.acc[b][e][r] + other_column(o.acc[b][e][r]);
+                o.acc[b][e][r] = V_BITS == 4 && e ? v * 0.0625f : v;
+            }
 }
 
 QS_DEV int length_of(const AttentionArgs& a, int seq) {
@@ -616,7 +615,7 @@ void k_kv_attention(AttentionArgs a, Split split) {
                 attend(a, start, start < span.all_first || start + TILE > span.all_last || held != 3, held, at, q, t, sums);
             }
         }
-        finish(sums);
+        finish<V_BITS>(sums);
         if (!(lane & 8)) {
 #pragma unroll
             for (int b = 0; b < BLOCKS; b++)
@@ -641,7 +640,7 @@ void k_kv_attention(AttentionArgs a, Split split) {
         const bool whole = from == 0 && to == steps.count;
         const int64_t row = row_of(a, seq, head, tile * COLUMNS + column);
         const int64_t slot = ((int64_t)blockIdx.x * 2 + (from == 0)) * COLUMNS + column;
-        const float inverse = total != 0.0f ? (V_BITS == 8 ? 0x1p24f : 1.0f) / total : 0.0f;    // 0: it sees nothing
+        const float inverse = total != 0.0f ? 0x1p24f / total : 0.0f;    // 0: it sees nothing
 #pragma unroll
         for (int i = 0; i < BLOCKS / 2; i++) {
             float2 v{0, 0};
@@ -673,7 +672,7 @@ hipError_t launch_blocks(const AttentionArgs& a, const Split& split, hipStream_t
     const auto kernel = a.type == QS_SRC_F32 ? k_kv_attention<K_BITS, V_BITS, BLOCKS, true>
                                              : k_kv_attention<K_BITS, V_BITS, BLOCKS, false>;
     const hipError_t e = qs_host::launch_kernel(kernel, dim3((unsigned)split.groups), dim3(64 * WAVES), 0, st, a, split);
-    return e != hipSuccess || split.whole ? e : launch_join(a, split, V_BITS == 8 ? 0x1p24f : 1.0f, st);
+    return e != hipSuccess || split.whole ? e : launch_join(a, split, st);
 }
 
 template <int K_BITS, int V_BITS>

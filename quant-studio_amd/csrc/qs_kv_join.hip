@@ -10,7 +10,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 // grid (workgroups, columns). D / 4 threads take a part's row, the others the next
 // parts; every thread keeps a running maximum, and LDS joins them in a fixed order.
 template <int BLOCKS>
-__global__ __launch_bounds__(256) void k_kv_join(AttentionArgs a, Split split, float unit) {
+__global__ __launch_bounds__(256) void k_kv_join(AttentionArgs a, Split split) {
     const int4 s = split.segments[blockIdx.x];
     if (s.z < 0) return;
     constexpr int D = 32 * BLOCKS, LANES = D / 4, ROWS = 256 / LANES;
@@ -55,15 +55,15 @@ __global__ __launch_bounds__(256) void k_kv_join(AttentionArgs a, Split split, f
 #pragma unroll
         for (int j = 0; j < 4; j++) sum[j] = __builtin_fmaf(acc[i][lane][j], is, sum[j]);
     }
-    const float inverse = total != 0.0f ? unit / total : 0.0f;
+    const float inverse = total != 0.0f ? 0x1p24f / total : 0.0f;
     store_two(a, row + 4 * lane, sum[0] * inverse, sum[1] * inverse);
     store_two(a, row + 4 * lane + 2, sum[2] * inverse, sum[3] * inverse);
 }
 
-hipError_t launch_join(const AttentionArgs& a, const Split& split, float unit, hipStream_t st) {
+hipError_t launch_join(const AttentionArgs& a, const Split& split, hipStream_t st) {
     const int columns = a.group * a.fresh < COLUMNS ? a.group * a.fresh : COLUMNS;
     const auto kernel = a.c.blocks == 2 ? k_kv_join<2> : a.c.blocks == 4 ? k_kv_join<4> : a.c.blocks == 6 ? k_kv_join<6> : k_kv_join<8>;
-    return qs_host::launch_kernel(kernel, dim3((unsigned)split.groups, (unsigned)columns), dim3(256), 0, st, a, split, unit);
+    return qs_host::launch_kernel(kernel, dim3((unsigned)split.groups, (unsigned)columns), dim3(256), 0, st, a, split);
 }
 
 }  // namespace qskv
