@@ -357,20 +357,30 @@ int cache_of(const qs_kv_cache* cache, Cache& c) {
 }
 
 Split split_of(const AttentionArgs& a, void* workspace) {
-    // As many workgroups as the GPU holds at a time; fewer where even the longest
-    // sequences would not give each a step for every wave. Sequences of a few steps at
-    // most are not split. The workspace is the same for every type.
+    // As many workgroups as the GPU holds at a time, unless even the longest sequences
+    // would not give each a step for every wave. Sequences of a few steps at most are
+    // not split; those of one are in equal parts, which each workgroup knows before it
+    // knows the length; more of them are in equal runs of all their steps, since the
+    // longest may be of any share. The workspace is the same for every type.
     constexpr int64_t CUS = 256, FEW = 8;
-    const int64_t full = CUS * resident(a.c.blocks, a.type == QS_SRC_F32);
     const int64_t heads = (int64_t)a.c.heads * column_tiles(a);
     const int64_t steps = ((int64_t)a.pages_each * a.c.page + TILE - 1) / TILE;
     Split s{};
     if (a.batch == 0 || a.fresh == 0) return s;
-    s.whole = steps <= FEW;
-    const int64_t most = (a.batch * heads * (steps + OPENING) + WAVES - 1) / WAVES;
-    s.groups = (int32_t)(s.whole ? a.batch * heads : most < full ? most : full);
-    if (s.whole) return s;
-    const int64_t room = most < CUS * resident(a.c.blocks, false) ? most : CUS * resident(a.c.blocks, false);
+    const auto groups = [&](bool wide) {
+        const int64_t full = CUS * resident(a.c.blocks, wide), most = (a.batch * heads * (steps + OPENING) + WAVES - 1) / WAVES;
+        return most < full ? most : full;
+    };
+    s.groups = (int32_t)groups(a.type == QS_SRC_F32);
+    if (steps <= FEW) {
+        s.share = 1;
+    } else if (a.batch == 1) {
+        const int64_t most = (steps + WAVES - 1) / WAVES, share = s.groups / heads;
+        s.share = (int32_t)(share < 1 ? 1 : share < most ? share : most);
+    }
+    if (s.share) s.groups = (int32_t)(a.batch * heads * s.share);
+    if (s.share == 1) return s;
+    const int64_t room = groups(false);
     const int64_t parts = round_up(room * 2 * COLUMNS * 32 * a.c.blocks * 4, 256);
     const int64_t stats = round_up(room * 2 * COLUMNS * 8, 256);
     uint8_t* base = static_cast<uint8_t*>(workspace);
@@ -463,6 +473,7 @@ int64_t qs_kv_attention_workspace(const qs_kv_cache* cache, int64_t batch, int64
     qs_host::clear_error();
     qskv::AttentionArgs a{};
     const int bad = attention_sizes(cache, batch, new_tokens, query_heads, pages_each, a);
+    a.type = QS_SRC_BF16;       // whose calls split no less than f32's
     return bad ? bad : qskv::split_of(a, nullptr).bytes;
 }
 

@@ -26,6 +26,7 @@
 #include "qs_kv_attention.h"
 #include "qs_launch_kernel.h"
 #include "qs_rows.h"
+#include "qs_wave.h"
 
 namespace qskv {
 
@@ -160,38 +161,40 @@ struct Queries {
     int first, last;                        // slots that the lane's query sees: first .. last - 1
 };
 
-template <int K_BITS, int BLOCKS, bool WIDE>
-QS_DEV void load_queries(const AttentionArgs& a, int seq, int head, int tile, int length,
-                         Queries<BLOCKS, WIDE>& o) {
+// as they are in memory, eight of every block to a lane
+template <int BLOCKS, bool WIDE>
+struct RawQueries {
+    qsr::Eight<WIDE ? qs::SRC_F32 : qs::SRC_BF16> b[BLOCKS];
+};
+template <int BLOCKS, bool WIDE>
+QS_DEV void load_queries(const AttentionArgs& a, int seq, int head, int tile, RawQueries<BLOCKS, WIDE>& o) {
     const int lane = threadIdx.x & 63, g = lane >> 4, column = tile * COLUMNS + (lane & 7);
     const bool live = column < a.group * a.fresh;
     const int token = live ? column / a.group : 0, mine = live ? column - token * a.group : 0;
     const int64_t at = ((int64_t)seq * a.fresh + token) * a.q_stride + (int64_t)(head * a.group + mine) * 32 * BLOCKS;
+#pragma unroll
+    for (int b = 0; b < BLOCKS; b++) qsr::load8<WIDE ? qs::SRC_F32 : qs::SRC_BF16>(a.q, at + 32 * b + 8 * g, o.b[b]);
+}
+template <int K_BITS, int BLOCKS, bool WIDE>
+QS_DEV void prepare_queries(const AttentionArgs& a, int tile, int length, const RawQueries<BLOCKS, WIDE>& raw,
+                            Queries<BLOCKS, WIDE>& o) {
+    const int lane = threadIdx.x & 63, column = tile * COLUMNS + (lane & 7);
+    const bool live = column < a.group * a.fresh, bf16 = a.type == QS_SRC_BF16;
+    const int token = live ? column / a.group : 0;
     float x[BLOCKS][8];
     float top = 0.0f;
 #pragma unroll
-    for (int b = 0; b < BLOCKS; b++) {
-        if constexpr (WIDE) {
-            qsr::Eight<qs::SRC_F32> e;
-            qsr::load8<qs::SRC_F32>(a.q, at + 32 * b + 8 * g, e);
-#pragma unroll
-            for (int i = 0; i < 8; i++) x[b][i] = qsr::value8<qs::SRC_F32>(e, i);
-        } else {
-            qsr::Eight<qs::SRC_BF16> e;
-            qsr::load8<qs::SRC_BF16>(a.q, at + 32 * b + 8 * g, e);
-            const bool bf16 = a.type == QS_SRC_BF16;
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const uint32_t h = e.w[0][i >> 1] >> (16 * (i & 1));
-                x[b][i] = bf16 ? __uint_as_float(h << 16) : half_of(h);
-            }
-        }
+    for (int b = 0; b < BLOCKS; b++)
 #pragma unroll
         for (int i = 0; i < 8; i++) {
+            if constexpr (WIDE) x[b][i] = qsr::value8<qs::SRC_F32>(raw.b[b], i);
+            else {
+                const uint32_t h = raw.b[b].w[0][i >> 1] >> (16 * (i & 1));
+                x[b][i] = bf16 ? __uint_as_float(h << 16) : half_of(h);
+            }
             x[b][i] = live ? x[b][i] : 0.0f;
             top = fmaxf(top, fabsf(x[b][i]));
         }
-    }
     top = max_over_slots(top);
     const bool scaled = top > 0.0f && top < __builtin_inff();
     const int e = scaled ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;     // top 2^e in 2^14 .. 2^15
@@ -476,68 +479,34 @@ struct Deal {
     int seq, base;
 };
 constexpr int64_t LEAST = WAVES;        // steps of a workgroup
-QS_DEV int wave_sum(int v) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
-    return v;
+QS_DEV int64_t quotient(int64_t a, int64_t b) {     // of numbers from 0 on
+    return (a | b) >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);
 }
-QS_DEV int wave_scan(int v) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int w = __shfl_up(v, o);
-        v += lane >= o ? w : 0;
-    }
-    return v;
-}
+QS_DEV int units_of(const AttentionArgs& a, int seq) { return OPENING + steps_of(a, length_of(a, seq)).count; }
 QS_DEV Deal deal(const AttentionArgs& a, int groups, int heads) {
-    __shared__ int sums[WAVES], found[2];
-    const int wave = threadIdx.x >> 6;
-    constexpr int THREADS = 64 * WAVES;
-    Deal d;
-    const int first = (int)threadIdx.x < a.batch ? OPENING + steps_of(a, length_of(a, threadIdx.x)).count : 0;
-    if (a.batch == 1) {
-        d.total = (int64_t)(OPENING + steps_of(a, length_of(a, 0)).count) * heads;
-        d.seq = d.base = 0;
-    } else {
-        int n = first;
-        for (int i = threadIdx.x + THREADS; i < a.batch; i += THREADS) n += OPENING + steps_of(a, length_of(a, i)).count;
-        n = wave_sum(n);
-        if ((threadIdx.x & 63) == 0) sums[wave] = n;
-        __syncthreads();
-        int all = 0;
-#pragma unroll
-        for (int i = 0; i < WAVES; i++) all += sums[i];
-        all = __builtin_amdgcn_readfirstlane(all);
-        d.total = (int64_t)all * heads;
+    // every wave by itself: a lane adds up a run of sequences, and these sums are added along the lanes
+    const int lane = threadIdx.x & 63, each_lane = (a.batch + 63) >> 6;
+    int sum = 0;
+#pragma unroll 4
+    for (int i = 0; i < each_lane; i++) {
+        const int seq = lane * each_lane + i;
+        sum += seq < a.batch ? units_of(a, seq) : 0;
     }
-    d.each = (d.total + groups - 1) / groups;
+    const int scan = qs::wave_incl_scan(sum);
+    Deal d;
+    d.total = (int64_t)__builtin_amdgcn_readlane(scan, 63) * heads;
+    d.each = quotient(d.total + groups - 1, groups);
     d.each = d.each < LEAST ? LEAST : d.each;
-    if (a.batch == 1) return d;
     const int64_t begin = blockIdx.x * d.each;
     if (begin >= d.total) return d;
-    const int at = (int)(begin / heads);
-    int before = 0;
-    for (int i = 0;; i += THREADS) {        // one of them holds `at`, which is below their sum
-        const int mine = i + (int)threadIdx.x;
-        const int n = i == 0 ? first : mine < a.batch ? OPENING + steps_of(a, length_of(a, mine)).count : 0;
-        const int scan = wave_scan(n);
-        __syncthreads();
-        if ((threadIdx.x & 63) == 63) sums[wave] = scan;
-        if (threadIdx.x == 0) found[0] = -1;
-        __syncthreads();
-        int end = before + scan;
-#pragma unroll
-        for (int w = 0; w < WAVES; w++) {
-            end += w < wave ? sums[w] : 0;
-            before += sums[w];
-        }
-        if (at >= end - n && at < end) found[0] = mine, found[1] = end - n;
-        __syncthreads();
-        if (found[0] >= 0) break;
+    const int at = (int)quotient(begin, heads);
+    const int run = __builtin_ctzll(__ballot(at < scan));       // the lane whose run it is in
+    d.seq = run * each_lane;
+    d.base = __builtin_amdgcn_readlane(scan - sum, run);
+    for (int n = units_of(a, d.seq); at >= d.base + n; n = units_of(a, d.seq)) {
+        d.base += n;
+        d.seq++;
     }
-    d.seq = __builtin_amdgcn_readfirstlane(found[0]);
-    d.base = __builtin_amdgcn_readfirstlane(found[1]);
     return d;
 }
 
@@ -557,9 +526,10 @@ void k_kv_attention(AttentionArgs a, Split split) {
     int seq, base = 0, which = -1, from = 0;        // which: head and column tile
     int64_t each = 0;
     int4 going{0, 0, -1, 0};
-    if (split.whole) {
-        seq = (int)blockIdx.x / heads;
-        which = (int)blockIdx.x - seq * heads;
+    if (split.share) {
+        const int segment = (int)blockIdx.x / split.share;
+        seq = segment / heads;
+        which = segment - seq * heads;
         at = 0;
         end = 1;
     } else {
@@ -575,10 +545,14 @@ void k_kv_attention(AttentionArgs a, Split split) {
         const int length = length_of(a, seq);
         const Steps steps = steps_of(a, length);
         int to = steps.count;                       // from .. to - 1 of them
-        if (!split.whole) {
+        if (split.share) {
+            const int part = (int)blockIdx.x % split.share, some = steps.count / split.share, more = steps.count % split.share;
+            from = part * some + (part < more ? part : more);
+            to = from + some + (part < more);
+        } else {
             if (which < 0) {
                 const int64_t rel = at - (int64_t)base * heads;
-                which = (int)(rel / (OPENING + steps.count));
+                which = (int)quotient(rel, OPENING + steps.count);
                 at -= rel - (int64_t)which * (OPENING + steps.count);
                 from = (int)(begin - at) - OPENING;
             }
@@ -588,6 +562,8 @@ void k_kv_attention(AttentionArgs a, Split split) {
             if (to <= from) break;                  // it ends before they do
         }
         const int head = which / tiles, tile = which - head * tiles;
+        RawQueries<BLOCKS, WIDE> raw;
+        load_queries(a, seq, head, tile, raw);
         const Span span = span_of(a, tile, length);
         Sums<BLOCKS> sums;
         clear(sums);
@@ -607,7 +583,7 @@ void k_kv_attention(AttentionArgs a, Split split) {
             load_keys(a, at, t);
             load_values(a, at, t);
             Queries<BLOCKS, WIDE> q;
-            load_queries<K_BITS, BLOCKS, WIDE>(a, seq, head, tile, length, q);
+            prepare_queries<K_BITS>(a, tile, length, raw, q);
             for (; i < stop; i += WAVES) {
                 const int start = start_of(i), held = at.held;
                 at = place_of(a, ahead, head, start_of(i + WAVES));
@@ -655,8 +631,11 @@ void k_kv_attention(AttentionArgs a, Split split) {
         }
         if (!whole && sub == 0) split.stats[slot] = float2{ref, total};
         __syncthreads();
-        if (split.whole) break;
-        if (from == 0 && !whole) going = int4{seq, which, (int)((at + OPENING + steps.count - 1) / each), 0};
+        if (split.share) {
+            if (from == 0 && !whole) going = int4{seq, which, (int)blockIdx.x + split.share - 1, 0};
+            break;
+        }
+        if (from == 0 && !whole) going = int4{seq, which, (int)quotient(at + OPENING + steps.count - 1, each), 0};
         at += OPENING + steps.count;
         from = 0;
         if (++which == heads) {         // only the last segment ends before its steps do
@@ -664,7 +643,7 @@ void k_kv_attention(AttentionArgs a, Split split) {
             seq++;
         }
     }
-    if (!split.whole && threadIdx.x == 0) split.segments[blockIdx.x] = going;
+    if (split.share != 1 && threadIdx.x == 0) split.segments[blockIdx.x] = going;
 }
 
 template <int K_BITS, int V_BITS, int BLOCKS>
@@ -672,7 +651,7 @@ hipError_t launch_blocks(const AttentionArgs& a, const Split& split, hipStream_t
     const auto kernel = a.type == QS_SRC_F32 ? k_kv_attention<K_BITS, V_BITS, BLOCKS, true>
                                              : k_kv_attention<K_BITS, V_BITS, BLOCKS, false>;
     const hipError_t e = qs_host::launch_kernel(kernel, dim3((unsigned)split.groups), dim3(64 * WAVES), 0, st, a, split);
-    return e != hipSuccess || split.whole ? e : launch_join(a, split, st);
+    return e != hipSuccess || split.share == 1 ? e : launch_join(a, split, st);
 }
 
 template <int K_BITS, int V_BITS>
