@@ -42,17 +42,13 @@ QS_DEV Unit unit_of(const Cache& c, int u) {
     o.quarter = u & 3;
     return o;
 }
-// the codes of the unit's head and kind in the slot's row, and its step
+// where a slot's page has the unit's head, and the slot in the page
 struct Place {
-    uint8_t* row;
-    uint16_t* step;
+    uint8_t* head;
+    int slot;
 };
 QS_DEV Place place_of(const Cache& c, const Unit& u, int slot) {
-    const int at = slot & (c.page - 1);
-    uint8_t* p = qskv::head_of(c, slot >> c.shift, u.head);
-    const int bits = u.value ? c.v_bits : c.k_bits, row = qskv::row_bytes(bits, c.blocks);
-    if (u.value) p += c.page * (qskv::row_bytes(c.k_bits, c.blocks) + 2 * c.blocks);
-    return {p + at * row, reinterpret_cast<uint16_t*>(p + c.page * row) + at * c.blocks + u.block};
+    return {qskv::head_of(c, slot >> c.shift, u.head), slot & (c.page - 1)};
 }
 
 // How threads are laid over rows: `wide` of them (whole heads' keys or values, so
@@ -183,9 +179,11 @@ __global__ __launch_bounds__(256) void k_kv_write(RowsArgs a) {
         const Place p = place_of(a.c, u, slot);
         // a step that f16 cannot hold, like a NaN or an infinity in the block, stands for no values
         const uint32_t h = qs::f16_bits(d);
-        if (u.quarter == 0) *p.step = (uint16_t)((h & 0x7fffu) < 0x7c00u ? h : 0x7e00u);
+        if (u.quarter == 0)
+            *reinterpret_cast<uint16_t*>(p.head + qskv::step_at(a.c, p.slot, u.value, u.block)) =
+                (uint16_t)((h & 0x7fffu) < 0x7c00u ? h : 0x7e00u);
         if (!u.value) {
-            uint8_t* o = p.row + qskv::k_unit(bits, a.c.blocks, u.quarter, u.block);
+            uint8_t* o = p.head + qskv::k_unit(a.c, p.slot, u.quarter, u.block);
             if (bits == 8) {
                 uint32_t w[2];
                 qs::bytes_of(code, w);
@@ -199,7 +197,7 @@ __global__ __launch_bounds__(256) void k_kv_write(RowsArgs a) {
         } else {
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                uint8_t* o = p.row + qskv::v_unit(bits, a.c.blocks, 4 * u.quarter + j, u.block);
+                uint8_t* o = p.head + qskv::v_unit(a.c, p.slot, 4 * u.quarter + j, u.block);
                 if (bits == 8) *reinterpret_cast<uint16_t*>(o) = (uint16_t)(code[2 * j] | code[2 * j + 1] << 8);
                 else *o = (uint8_t)(code[2 * j] | code[2 * j + 1] << 4);
             }
@@ -237,9 +235,9 @@ __global__ __launch_bounds__(256) void k_kv_read(RowsArgs a) {
         step[i] = 0;
         if ((unsigned)slot[i] >= (unsigned)slots) continue;
         const Place p = place_of(a.c, u, slot[i]);
-        step[i] = *p.step;
+        step[i] = *reinterpret_cast<const uint16_t*>(p.head + qskv::step_at(a.c, p.slot, u.value, u.block));
         if (!u.value) {
-            const uint8_t* o = p.row + qskv::k_unit(bits, a.c.blocks, u.quarter, u.block);
+            const uint8_t* o = p.head + qskv::k_unit(a.c, p.slot, u.quarter, u.block);
             if (bits == 8) {
                 const uint2 c = *reinterpret_cast<const uint2*>(o);
                 w[i][0] = c.x, w[i][1] = c.y;
@@ -249,7 +247,7 @@ __global__ __launch_bounds__(256) void k_kv_read(RowsArgs a) {
         } else {
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                const uint8_t* o = p.row + qskv::v_unit(bits, a.c.blocks, 4 * u.quarter + j, u.block);
+                const uint8_t* o = p.head + qskv::v_unit(a.c, p.slot, 4 * u.quarter + j, u.block);
                 w[i][j] = bits == 8 ? *reinterpret_cast<const uint16_t*>(o) : *o;
             }
         }

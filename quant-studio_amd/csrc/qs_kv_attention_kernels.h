@@ -64,39 +64,32 @@ QS_DEV float other_column(float v) {
     return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), 0x128, 0xF, 0xF, true));
 }
 
-// N bytes of consecutive codes as words
-template <int N>
-struct Codes {
-    uint32_t w[(N + 3) / 4];
-};
-// through a buffer descriptor: a lane's offset `at` stays the same for every step,
-// and where the step is lies in scalar registers
+// N bytes of consecutive codes as words, loaded through a buffer descriptor: a lane's
+// offset `at` stays the same for every step, and where the step is lies in scalar
+// registers
 typedef __amdgpu_buffer_rsrc_t Buffer;
 template <int N>
-QS_DEV void load(Codes<N>& o, Buffer p, int at, int from) {
-    if constexpr (N % 16 == 0) {
+struct Codes {
+    uint32_t w[N / 4];
+};
+template <int N>
+QS_DEV void load_piece(uint32_t* o, Buffer p, int at, int from) {
+    if constexpr (N == 16) {
+        const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(p, at, from, 0);
 #pragma unroll
-        for (int i = 0; i < N / 16; i++) {
-            const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(p, at + 16 * i, from, 0);
-#pragma unroll
-            for (int j = 0; j < 4; j++) o.w[4 * i + j] = v[j];
-        }
-    } else if constexpr (N % 8 == 0) {
-#pragma unroll
-        for (int i = 0; i < N / 8; i++) {
-            const u32x2 v = __builtin_amdgcn_raw_buffer_load_b64(p, at + 8 * i, from, 0);
-            o.w[2 * i] = v[0], o.w[2 * i + 1] = v[1];
-        }
-    } else if constexpr (N % 4 == 0) {
-#pragma unroll
-        for (int i = 0; i < N / 4; i++) o.w[i] = __builtin_amdgcn_raw_buffer_load_b32(p, at + 4 * i, from, 0);
+        for (int j = 0; j < 4; j++) o[j] = v[j];
+    } else if constexpr (N == 8) {
+        const u32x2 v = __builtin_amdgcn_raw_buffer_load_b64(p, at, from, 0);
+        o[0] = v[0], o[1] = v[1];
     } else {
-#pragma unroll
-        for (int i = 0; i < (N + 3) / 4; i++) {
-            o.w[i] = __builtin_amdgcn_raw_buffer_load_b16(p, at + 4 * i, from, 0);
-            if (4 * i + 2 < N) o.w[i] |= (uint32_t)__builtin_amdgcn_raw_buffer_load_b16(p, at + 4 * i + 2, from, 0) << 16;
-        }
+        o[0] = __builtin_amdgcn_raw_buffer_load_b32(p, at, from, 0);
     }
+}
+template <int N>
+QS_DEV void load(Codes<N>& o, Buffer p, int at, int from) {
+    constexpr int PIECE = N % 16 == 0 ? 16 : N % 8 == 0 ? 8 : 4;
+#pragma unroll
+    for (int i = 0; i < N; i += PIECE) load_piece<PIECE>(o.w + i / 4, p, at + i, from);
 }
 
 QS_DEV uint32_t sign_and_magnitude(uint32_t w, uint32_t pick) {
@@ -127,15 +120,18 @@ QS_DEV u32x4 key_block(const Codes<BITS * BLOCKS>& c, int b) {
     }
     return o;
 }
-// code n of two slots as f16
-template <int BITS, int N>
-QS_DEV uint32_t value_pair(const Codes<N>& x, const Codes<N>& y, int n) {
+// code n of the slots 2 i and 2 i + 1 of four as f16
+template <int BITS, int BLOCKS>
+QS_DEV uint32_t value_pair(const Codes<BITS * BLOCKS>& c, int i, int n) {
+    // `run` bytes of each slot one after another: bytes `x` and `y` have the code
+    constexpr int RUN = BITS * BLOCKS / 4;
+    const int x = 2 * i * RUN + n * BITS / 8, y = x + RUN;
     if constexpr (BITS == 8) {
-        const uint32_t at = n & 3;
-        return __builtin_amdgcn_perm(y.w[n >> 2], x.w[n >> 2], at * 0x01010101u + 0x04040000u) & 0x807f807fu;
+        return __builtin_amdgcn_perm(c.w[y >> 2], c.w[x >> 2], (x & 3) * 0x00000101u + (y & 3) * 0x01010000u + 0x04040000u) & 0x807f807fu;
     } else {
-        const uint32_t both = __builtin_amdgcn_perm(y.w[n >> 3], x.w[n >> 3], n & 4 ? 0x07060302u : 0x05040100u);
-        return four_bits(both, n & 3);
+        // the half words that have it; their codes 0 .. 3 are those from n & ~3 on
+        const uint32_t hx = x & 2 ? 0x0302u : 0x0100u, hy = y & 2 ? 0x07060000u : 0x05040000u;
+        return four_bits(__builtin_amdgcn_perm(c.w[y >> 2], c.w[x >> 2], hx | hy), n & 3);
     }
 }
 
@@ -256,15 +252,16 @@ QS_DEV Span span_of(const AttentionArgs& a, int tile, int length) {
 typedef const __attribute__((address_space(4))) int32_t* Ints;
 QS_DEV Ints constant(const int32_t* p) { return (Ints)(uintptr_t)p; }
 
-// A step's codes and steps (of quantisation) in registers. Both sixteens of slots lie
-// in one page each. A lane has, of each sixteen: a quarter of key m's codes, of the
-// slots 4 g .. 4 g + 3 the values' codes of two dims of every block, and their steps.
+// What a lane loads of a step's 32 slots, both sixteens of which lie in one page each:
+// of each sixteen a quarter of key m's codes, and of the slots 4 g .. 4 g + 3 the values'
+// codes of two dims of every block. The steps (of quantisation) are wanted by sixteen
+// lanes each: one loads them, and LDS gives them to all.
 template <int K_BITS, int V_BITS, int BLOCKS>
 struct Tile {
-    static constexpr int KROW = row_bytes(K_BITS, BLOCKS), VROW = row_bytes(V_BITS, BLOCKS), STEPS = 2 * BLOCKS;
-    Codes<KROW / 4> kc[2];
-    Codes<4 * STEPS> ks[2], vs[2];
-    Codes<VROW / 16> vc[2][4];
+    static constexpr int KROW = row_bytes(K_BITS, BLOCKS), VROW = row_bytes(V_BITS, BLOCKS);
+    Codes<KROW / 4> keys[2];
+    Codes<VROW / 4> values[2];          // of one slot after another
+    Codes<2 * BLOCKS> steps;
 };
 // where they are: the same for the whole wave
 struct Place {
@@ -301,27 +298,28 @@ template <int K_BITS, int V_BITS, int BLOCKS>
 QS_DEV void load_keys(const AttentionArgs& a, const Place& at, Tile<K_BITS, V_BITS, BLOCKS>& t) {
     typedef Tile<K_BITS, V_BITS, BLOCKS> T;
     const int lane = threadIdx.x & 63, g = lane >> 4, m = lane & 15;
+    constexpr int RUN = T::KROW / 4, PIECES = RUN / 16 * 16;
 #pragma unroll
     for (int s = 0; s < 2; s++) {
         const Buffer p = buffer_of<K_BITS, V_BITS, BLOCKS>(a, s ? at.head1 : at.head0);
-        const int slot = s ? at.slot1 : at.slot0;
-        load(t.kc[s], p, m * T::KROW + g * (T::KROW / 4), slot * T::KROW);
-        load(t.ks[s], p, 4 * T::STEPS * g, a.c.page * T::KROW + slot * T::STEPS);
+        const int from = (s ? at.slot1 : at.slot0) * T::KROW;
+#pragma unroll
+        for (int i = 0; i < PIECES; i += 16) load_piece<16>(t.keys[s].w + i / 4, p, m * T::KROW + 16 * g + 4 * i, from);
+        if constexpr (RUN > PIECES) load_piece<8>(t.keys[s].w + PIECES / 4, p, m * T::KROW + 8 * g + 4 * PIECES, from);
     }
+    // half a wave takes a sixteen's
+    const int codes = a.c.page * (T::KROW + T::VROW);
+    const uint8_t* p = lane < 32 ? at.head0 + (codes + at.slot0 * 4 * BLOCKS) : at.head1 + (codes + at.slot1 * 4 * BLOCKS);
+    __builtin_memcpy(t.steps.w, __builtin_assume_aligned(p + (lane & 31) * 2 * BLOCKS, 4), 2 * BLOCKS);
 }
 template <int K_BITS, int V_BITS, int BLOCKS>
 QS_DEV void load_values(const AttentionArgs& a, const Place& at, Tile<K_BITS, V_BITS, BLOCKS>& t) {
     typedef Tile<K_BITS, V_BITS, BLOCKS> T;
     const int lane = threadIdx.x & 63, g = lane >> 4, m = lane & 15;
 #pragma unroll
-    for (int s = 0; s < 2; s++) {
-        const Buffer p = buffer_of<K_BITS, V_BITS, BLOCKS>(a, s ? at.head1 : at.head0);
-        const int slot = s ? at.slot1 : at.slot0, codes = a.c.page * (T::KROW + T::STEPS);
-        load(t.vs[s], p, 4 * T::STEPS * g, codes + a.c.page * T::VROW + slot * T::STEPS);
-#pragma unroll
-        for (int r = 0; r < 4; r++)
-            load(t.vc[s][r], p, 4 * T::VROW * g + m * (T::VROW / 16) + T::VROW * r, codes + slot * T::VROW);
-    }
+    for (int s = 0; s < 2; s++)
+        load(t.values[s], buffer_of<K_BITS, V_BITS, BLOCKS>(a, s ? at.head1 : at.head0), 4 * T::VROW * g + m * (T::VROW / 4),
+             a.c.page * T::KROW + (s ? at.slot1 : at.slot0) * T::VROW);
 }
 
 // One step: the slots start .. start + 31, in `t`. The next step's keys and values
@@ -331,32 +329,51 @@ QS_DEV void load_values(const AttentionArgs& a, const Place& at, Tile<K_BITS, V_
 // whatever they hold, since a lane's scores and steps are its query's own copies.
 template <bool WIDE, int K_BITS, int V_BITS, int BLOCKS>
 QS_DEV void attend(const AttentionArgs& a, int start, bool edge, int held, const Place& next,
-                   const Queries<BLOCKS, WIDE>& q, Tile<K_BITS, V_BITS, BLOCKS>& t, Sums<BLOCKS>& sums) {
-    constexpr int STEPS = 2 * BLOCKS;
+                   const Queries<BLOCKS, WIDE>& q, uint32_t* lds, Tile<K_BITS, V_BITS, BLOCKS>& t, Sums<BLOCKS>& sums) {
     const int lane = threadIdx.x & 63, g = lane >> 4;
-    const auto step_of = [](const Codes<4 * STEPS>& c, int r, int b) {
+    // steps of four slots, and one of them
+    typedef Codes<8 * BLOCKS> Steps4;
+    const auto steps_from = [&](int s, bool value, Steps4& o) {
+        const uint32_t* p = lds + (s * 16 + 4 * g) * BLOCKS + (value ? 2 * BLOCKS : 0);
+#pragma unroll
+        for (int i = 0; i < 2 * BLOCKS; i += 4) {
+            const u32x4 v = *reinterpret_cast<const u32x4*>(p + i);
+#pragma unroll
+            for (int j = 0; j < 4; j++) o.w[i + j] = v[j];
+        }
+    };
+    const auto step_of = [](const Steps4& c, int r, int b) {
         const int n = r * BLOCKS + b;
         return half_of(c.w[n >> 1] >> (16 * (n & 1)));
     };
+    // lane after lane they are the two sixteens' steps as they lie in their pages
+#pragma unroll
+    for (int i = 0; i < BLOCKS / 2; i++) lds[lane * (BLOCKS / 2) + i] = t.steps.w[i];
+    qs::wave_sync<true>();
     // scores, in powers of two
     float x[2][4];
 #pragma unroll
     for (int s = 0; s < 2; s++) {
 #pragma unroll
         for (int r = 0; r < 4; r++) x[s][r] = 0.0f;
+        Steps4 ks;
+        steps_from(s, false, ks);
 #pragma unroll
         for (int b = 0; b < BLOCKS; b++) {
-            const u32x4 k = key_block<K_BITS, BLOCKS>(t.kc[s], b);
+            const u32x4 k = key_block<K_BITS, BLOCKS>(t.keys[s], b);
             f32x4 d = mfma(k, q.q[b], f32x4{0, 0, 0, 0});
             if constexpr (WIDE) d = mfma(k, q.lo[b], d);
 #pragma unroll
-            for (int r = 0; r < 4; r++) x[s][r] = __builtin_fmaf(d[r], step_of(t.ks[s], r, b), x[s][r]);
+            for (int r = 0; r < 4; r++) x[s][r] = __builtin_fmaf(d[r], step_of(ks, r, b), x[s][r]);
         }
 #pragma unroll
         for (int r = 0; r < 4; r++) x[s][r] = __builtin_ldexpf(x[s][r] * q.scale, q.up);
     }
     __builtin_amdgcn_sched_barrier(0);      // loads that move up would need registers of their own
     load_keys(a, next, t);
+    Steps4 vs[2];
+    steps_from(0, true, vs[0]);
+    steps_from(1, true, vs[1]);
     if (edge) {
 #pragma unroll
         for (int s = 0; s < 2; s++)
@@ -366,7 +383,7 @@ QS_DEV void attend(const AttentionArgs& a, int start, bool edge, int held, const
                 if (!((held >> s & 1) && p >= q.first && p < q.last)) {
                     x[s][r] = -__builtin_inff();
 #pragma unroll
-                    for (int i = 0; i < BLOCKS / 2; i++) t.vs[s].w[r * (BLOCKS / 2) + i] = 0;
+                    for (int i = 0; i < BLOCKS / 2; i++) vs[s].w[r * (BLOCKS / 2) + i] = 0;
                 }
             }
     }
@@ -378,7 +395,7 @@ QS_DEV void attend(const AttentionArgs& a, int start, bool edge, int held, const
 #pragma unroll
         for (int r = 0; r < 4; r++) top = fmaxf(top, x[s][r]);
 #pragma unroll
-        for (int i = 0; i < STEPS; i++) steps |= t.vs[s].w[i];
+        for (int i = 0; i < 2 * BLOCKS; i++) steps |= vs[s].w[i];
     }
     top = max_over_slots(top);
     steps = over_slots(steps, [](uint32_t u, uint32_t v) { return u | v; });
@@ -415,7 +432,7 @@ QS_DEV void attend(const AttentionArgs& a, int start, bool edge, int held, const
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const int n = 2 * i;
-            const float d0 = step_of(t.vs[n >> 2], n & 3, b), d1 = step_of(t.vs[n >> 2], (n & 3) + 1, b);
+            const float d0 = step_of(vs[n >> 2], n & 3, b), d1 = step_of(vs[n >> 2], (n & 3) + 1, b);
             // + 0 makes it one instruction that takes the step as f16
             w[i] = two_halves<WIDE>(__builtin_fmaf(p[n], d0, 0.0f), __builtin_fmaf(p[n + 1], d1, 0.0f), second);
         }
@@ -424,8 +441,7 @@ QS_DEV void attend(const AttentionArgs& a, int start, bool edge, int held, const
             u32x4 c;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const int n = 2 * i;
-                c[i] = value_pair<V_BITS>(t.vc[n >> 2][n & 3], t.vc[n >> 2][(n & 3) + 1], 2 * b + e);
+                c[i] = value_pair<V_BITS, BLOCKS>(t.values[i >> 1], i & 1, 2 * b + e);
             }
             sums.acc[b][e] = mfma(c, w, sums.acc[b][e]);
         }
@@ -520,6 +536,7 @@ void k_kv_attention(AttentionArgs a, Split split) {
     constexpr int D = 32 * BLOCKS, ROW = D + 4;     // 4: the eight columns' words in other banks
     __shared__ __attribute__((aligned(16))) float acc[WAVES][COLUMNS][ROW];
     __shared__ float2 stats[WAVES][COLUMNS];
+    __shared__ __attribute__((aligned(16))) uint32_t steps_lds[WAVES][TILE * BLOCKS];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane >> 4;
     const int tiles = column_tiles(a), heads = a.c.heads * tiles;
     int64_t at, end;
@@ -588,7 +605,7 @@ void k_kv_attention(AttentionArgs a, Split split) {
                 const int start = start_of(i), held = at.held;
                 at = place_of(a, ahead, head, start_of(i + WAVES));
                 ahead = pages_of(a, table, start_of(i + 2 * WAVES));
-                attend(a, start, start < span.all_first || start + TILE > span.all_last || held != 3, held, at, q, t, sums);
+                attend(a, start, start < span.all_first || start + TILE > span.all_last || held != 3, held, at, q, steps_lds[wave], t, sums);
             }
         }
         finish<V_BITS>(sums);
