@@ -385,6 +385,7 @@ Split split_of(const AttentionArgs& a, void* workspace) {
     s.parts = reinterpret_cast<float*>(base);
     s.stats = reinterpret_cast<float2*>(base + parts);
     s.segments = reinterpret_cast<int4*>(base + parts + stats);
+    s.listed = (int32_t)(a.batch * heads <= s.groups ? a.batch * heads : 0);
     s.bytes = parts + stats + room * 16;
     return s;
 }

@@ -47,8 +47,11 @@ struct Split {
     // of each workgroup, first for a segment that begins before it, then for one that goes on after it
     float* parts;                   // [groups][2][COLUMNS][head size], 2^-24 of a sum relative to R
     float2* stats;                  // [groups][2][COLUMNS]: R, sum of p
-    int4* segments;                 // [groups]: sequence, head and column tile, last workgroup of the segment
-                                    // that begins here and goes on, or -1 for none
+    // Of runs: segments that more than one workgroup has, as sequence, head and column tile, first and last
+    // workgroup (-1: it is one's alone). One entry for each head and column tile of a sequence where these
+    // are no more than workgroups (`listed`), else one for that which goes on after each workgroup.
+    int4* segments;
+    int32_t listed;
     int64_t bytes;                  // of the workspace
 };
 Split split_of(const AttentionArgs& a, void* workspace);

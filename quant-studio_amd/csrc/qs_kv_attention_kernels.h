@@ -466,10 +466,11 @@ QS_DEV void finish(Sums<BLOCKS>& o) {
             }
 }
 
-QS_DEV int length_of(const AttentionArgs& a, int seq) {
-    const int most = a.pages_each << a.c.shift, n = constant(a.lengths)[seq];
+QS_DEV int cut_length(const AttentionArgs& a, int n) {
+    const int most = a.pages_each << a.c.shift;
     return n < 0 ? 0 : n > most ? most : n;
 }
+QS_DEV int length_of(const AttentionArgs& a, int seq) { return cut_length(a, constant(a.lengths)[seq]); }
 // Steps of a sequence for any of its queries, from step `begin` on: at least one,
 // so that queries that see nothing get their zeros.
 struct Steps {
@@ -530,7 +531,9 @@ QS_DEV Deal deal(const AttentionArgs& a, int groups, int heads) {
 // the workgroup has of one head's and column tile's steps of a sequence) and join
 // their sums through LDS. A segment that is a whole one is written as the result,
 // else as a part that k_kv_join takes.
-template <int K_BITS, int V_BITS, int BLOCKS, bool WIDE>
+// SHARE: its segment is the steps that it has of the split's `share`, dealt to their
+// waves in turn.
+template <int K_BITS, int V_BITS, int BLOCKS, bool WIDE, bool SHARE>
 __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(resident(BLOCKS, WIDE))))
 void k_kv_attention(AttentionArgs a, Split split) {
     constexpr int D = 32 * BLOCKS, ROW = D + 4;     // 4: the eight columns' words in other banks
@@ -539,16 +542,14 @@ void k_kv_attention(AttentionArgs a, Split split) {
     __shared__ __attribute__((aligned(16))) uint32_t steps_lds[WAVES][TILE * BLOCKS];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane >> 4;
     const int tiles = column_tiles(a), heads = a.c.heads * tiles;
-    int64_t at, end;
+    int64_t at = 0, end = 1, each = 0;
     int seq, base = 0, which = -1, from = 0;        // which: head and column tile
-    int64_t each = 0;
-    int4 going{0, 0, -1, 0};
-    if (split.share) {
+    int4 going{0, 0, 0, -1};
+    if constexpr (SHARE) {
         const int segment = (int)blockIdx.x / split.share;
         seq = segment / heads;
         which = segment - seq * heads;
-        at = 0;
-        end = 1;
+        from = (int)blockIdx.x - segment * split.share;     // which part
     } else {
         const Deal d = deal(a, split.groups, heads);
         each = d.each;
@@ -559,14 +560,12 @@ void k_kv_attention(AttentionArgs a, Split split) {
     }
     const int64_t begin = at;
     while (at < end) {
-        const int length = length_of(a, seq);
-        const Steps steps = steps_of(a, length);
-        int to = steps.count;                       // from .. to - 1 of them
-        if (split.share) {
-            const int part = (int)blockIdx.x % split.share, some = steps.count / split.share, more = steps.count % split.share;
-            from = part * some + (part < more ? part : more);
-            to = from + some + (part < more);
-        } else {
+        int length = constant(a.lengths)[seq];
+        Steps steps{};
+        int to = 0;                                 // from .. to - 1 of them
+        if constexpr (!SHARE) {
+            length = cut_length(a, length);
+            steps = steps_of(a, length);
             if (which < 0) {
                 const int64_t rel = at - (int64_t)base * heads;
                 which = (int)quotient(rel, OPENING + steps.count);
@@ -574,38 +573,56 @@ void k_kv_attention(AttentionArgs a, Split split) {
                 from = (int)(begin - at) - OPENING;
             }
             // `at`: where the head's begin, `from` below 0 where they do in this workgroup
-            to = to < end - at - OPENING ? to : (int)(end - at) - OPENING;
+            to = steps.count < end - at - OPENING ? steps.count : (int)(end - at) - OPENING;
             from = from < 0 ? 0 : from;
             if (to <= from) break;                  // it ends before they do
         }
         const int head = which / tiles, tile = which - head * tiles;
         RawQueries<BLOCKS, WIDE> raw;
         load_queries(a, seq, head, tile, raw);
-        const Span span = span_of(a, tile, length);
         Sums<BLOCKS> sums;
         clear(sums);
         const Ints table = constant(a.tables + seq * a.table_stride);
-        // of them, those that this column tile's queries see
-        const int low = span.first / TILE - steps.begin, high = (span.last + TILE - 1) / TILE - steps.begin;
-        const int stop = high < to ? high : to;
-        int i = (low > from ? low : from) + wave;
-        if (i < stop) {
+        // The wave's steps i, i + stride, ... before `stop`, counted from the sequence's
+        // start, of those that this column tile's queries see. The first one's codes are
+        // asked for as soon as it is known which it is: a part's first step depends on
+        // the length only with a window.
+        constexpr bool RUN = !SHARE;
+        const int stride = RUN ? WAVES : split.share * WAVES, most = ((a.pages_each << a.c.shift) + TILE - 1) / TILE;
+        const bool early = SHARE && a.window == 0;
+        Span span{};
+        int i = RUN ? steps.begin + from + wave : from * WAVES + wave, stop = RUN ? steps.begin + to : most;
+        const auto see = [&] {
+            if (SHARE) length = cut_length(a, length);
+            span = span_of(a, tile, length);
+            const int low = span.first / TILE, high = (span.last + TILE - 1) / TILE;
+            stop = high < stop ? high : stop;
+            if (!early) i = RUN ? (low > steps.begin + from ? low + wave : i) : low + i;
+        };
+        if (!early) see();
+        Place place;
+        Pages ahead;
+        Tile<K_BITS, V_BITS, BLOCKS> t;
+        const bool any = i < stop;
+        if (any) {
+            place = place_of(a, pages_of(a, table, i * TILE), head, i * TILE);
+            ahead = pages_of(a, table, (i + stride < stop ? i + stride : i) * TILE);
+            load_keys(a, place, t);
+            load_values(a, place, t);
+        }
+        if (early) see();
+        if (any && i < stop) {
             // The pages of a step are asked for two steps ahead, its codes one ahead; after
             // the last step it is that step's again, whose codes are in the caches.
-            const int final = i + (stop - 1 - i) / WAVES * WAVES;
-            const auto start_of = [&](int n) { return (steps.begin + (n < final ? n : final)) * TILE; };
-            Place at = place_of(a, pages_of(a, table, start_of(i)), head, start_of(i));
-            Pages ahead = pages_of(a, table, start_of(i + WAVES));
-            Tile<K_BITS, V_BITS, BLOCKS> t;
-            load_keys(a, at, t);
-            load_values(a, at, t);
+            const int final = i + (stop - 1 - i) / stride * stride;
+            const auto start_of = [&](int n) { return (n < final ? n : final) * TILE; };
             Queries<BLOCKS, WIDE> q;
             prepare_queries<K_BITS>(a, tile, length, raw, q);
-            for (; i < stop; i += WAVES) {
-                const int start = start_of(i), held = at.held;
-                at = place_of(a, ahead, head, start_of(i + WAVES));
-                ahead = pages_of(a, table, start_of(i + 2 * WAVES));
-                attend(a, start, start < span.all_first || start + TILE > span.all_last || held != 3, held, at, q, steps_lds[wave], t, sums);
+            for (; i < stop; i += stride) {
+                const int start = i * TILE, held = place.held;
+                place = place_of(a, ahead, head, start_of(i + stride));
+                ahead = pages_of(a, table, start_of(i + 2 * stride));
+                attend(a, start, start < span.all_first || start + TILE > span.all_last || held != 3, held, place, q, steps_lds[wave], t, sums);
             }
         }
         finish<V_BITS>(sums);
@@ -630,7 +647,7 @@ void k_kv_attention(AttentionArgs a, Split split) {
             part[w] = s.x > -__builtin_inff() ? __builtin_amdgcn_exp2f(s.x - ref) : s.y;    // s.y: 0, or NaN
             total = __builtin_fmaf(s.y, part[w], total);
         }
-        const bool whole = from == 0 && to == steps.count;
+        const bool whole = SHARE ? split.share == 1 : from == 0 && to == steps.count;
         const int64_t row = row_of(a, seq, head, tile * COLUMNS + column);
         const int64_t slot = ((int64_t)blockIdx.x * 2 + (from == 0)) * COLUMNS + column;
         const float inverse = total != 0.0f ? 0x1p24f / total : 0.0f;    // 0: it sees nothing
@@ -648,11 +665,11 @@ void k_kv_attention(AttentionArgs a, Split split) {
         }
         if (!whole && sub == 0) split.stats[slot] = float2{ref, total};
         __syncthreads();
-        if (split.share) {
-            if (from == 0 && !whole) going = int4{seq, which, (int)blockIdx.x + split.share - 1, 0};
-            break;
+        if constexpr (SHARE) return;
+        if (from == 0) {
+            if (!whole) going = int4{seq, which, (int)blockIdx.x, (int)quotient(at + OPENING + steps.count - 1, each)};
+            if (split.listed && threadIdx.x == 0) split.segments[seq * heads + which] = whole ? int4{0, 0, 0, -1} : going;
         }
-        if (from == 0 && !whole) going = int4{seq, which, (int)quotient(at + OPENING + steps.count - 1, each), 0};
         at += OPENING + steps.count;
         from = 0;
         if (++which == heads) {         // only the last segment ends before its steps do
@@ -660,13 +677,14 @@ void k_kv_attention(AttentionArgs a, Split split) {
             seq++;
         }
     }
-    if (split.share != 1 && threadIdx.x == 0) split.segments[blockIdx.x] = going;
+    if (!split.listed && threadIdx.x == 0) split.segments[blockIdx.x] = going;
 }
 
 template <int K_BITS, int V_BITS, int BLOCKS>
 hipError_t launch_blocks(const AttentionArgs& a, const Split& split, hipStream_t st) {
-    const auto kernel = a.type == QS_SRC_F32 ? k_kv_attention<K_BITS, V_BITS, BLOCKS, true>
-                                             : k_kv_attention<K_BITS, V_BITS, BLOCKS, false>;
+    const auto kernel =
+        a.type == QS_SRC_F32 ? (split.share ? k_kv_attention<K_BITS, V_BITS, BLOCKS, true, true> : k_kv_attention<K_BITS, V_BITS, BLOCKS, true, false>)
+                             : (split.share ? k_kv_attention<K_BITS, V_BITS, BLOCKS, false, true> : k_kv_attention<K_BITS, V_BITS, BLOCKS, false, false>);
     const hipError_t e = qs_host::launch_kernel(kernel, dim3((unsigned)split.groups), dim3(64 * WAVES), 0, st, a, split);
     return e != hipSuccess || split.share == 1 ? e : launch_join(a, split, st);
 }
