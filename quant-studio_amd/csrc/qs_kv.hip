@@ -355,37 +355,44 @@ int cache_of(const qs_kv_cache* cache, Cache& c) {
 }
 
 Split split_of(const AttentionArgs& a, void* workspace) {
-    // As many workgroups as the GPU holds at a time, unless even the longest sequences
-    // would not give each a step for every wave. Sequences of a few steps at most are
-    // not split; those of one are in equal parts, which each workgroup knows before it
-    // knows the length; more of them are in equal runs of all their steps, since the
-    // longest may be of any share. The workspace is the same for every type.
+    // As many workgroups of four waves as the GPU holds at a time, unless even the
+    // longest sequences would not give each a step for every wave. Sequences of a few
+    // steps at most are not split; those of one are in equal parts, which each workgroup
+    // knows before it knows the length; more of them are in equal runs of all their
+    // steps, since the longest may be of any share. Where there are more segments than
+    // workgroups, waves take them by themselves: opening one is most of what a short one
+    // takes.
     constexpr int64_t CUS = 256, FEW = 8;
-    const int64_t heads = (int64_t)a.c.heads * column_tiles(a);
+    const int64_t segments = (int64_t)a.batch * a.c.heads * column_tiles(a);
     const int64_t steps = ((int64_t)a.pages_each * a.c.page + TILE - 1) / TILE;
     Split s{};
     if (a.batch == 0 || a.fresh == 0) return s;
-    const auto groups = [&](bool wide) {
-        const int64_t full = CUS * resident(a.c.blocks, wide), most = (a.batch * heads * (steps + OPENING) + WAVES - 1) / WAVES;
-        return most < full ? most : full;
+    const auto plan = [&](bool wide) {
+        const int64_t full = CUS * resident(a.c.blocks, wide);
+        Split p{};
+        p.waves = segments > (steps <= FEW ? 1 : 2) * full && a.batch > 1 ? 1 : 4;
+        if (steps <= FEW) {
+            p.share = 1;
+        } else if (a.batch == 1) {
+            const int64_t share = full / segments, most = (steps + p.waves - 1) / p.waves;
+            p.share = (int32_t)(share < 1 ? 1 : share < most ? share : most);
+        }
+        const int64_t held = full * (4 / p.waves), most = segments * (steps / p.waves + 1 + OPENING);
+        p.groups = (int32_t)(p.share ? segments * p.share : most < held ? most : held);
+        return p;
     };
-    s.groups = (int32_t)groups(a.type == QS_SRC_F32);
-    if (steps <= FEW) {
-        s.share = 1;
-    } else if (a.batch == 1) {
-        const int64_t most = (steps + WAVES - 1) / WAVES, share = s.groups / heads;
-        s.share = (int32_t)(share < 1 ? 1 : share < most ? share : most);
-    }
-    if (s.share) s.groups = (int32_t)(a.batch * heads * s.share);
+    s = plan(a.type == QS_SRC_F32);
     if (s.share == 1) return s;
-    const int64_t room = groups(false);
+    // the workspace is the same for every type
+    const Split narrow = plan(false), wide = plan(true);
+    const int64_t room = narrow.groups > wide.groups ? narrow.groups : wide.groups;
     const int64_t parts = round_up(room * 2 * COLUMNS * 32 * a.c.blocks * 4, 256);
     const int64_t stats = round_up(room * 2 * COLUMNS * 8, 256);
     uint8_t* base = static_cast<uint8_t*>(workspace);
     s.parts = reinterpret_cast<float*>(base);
     s.stats = reinterpret_cast<float2*>(base + parts);
     s.segments = reinterpret_cast<int4*>(base + parts + stats);
-    s.listed = (int32_t)(a.batch * heads <= s.groups ? a.batch * heads : 0);
+    s.listed = (int32_t)(segments <= s.groups ? segments : 0);
     s.bytes = parts + stats + room * 16;
     return s;
 }
@@ -472,8 +479,14 @@ int64_t qs_kv_attention_workspace(const qs_kv_cache* cache, int64_t batch, int64
     qs_host::clear_error();
     qskv::AttentionArgs a{};
     const int bad = attention_sizes(cache, batch, new_tokens, query_heads, pages_each, a);
-    a.type = QS_SRC_BF16;       // whose calls split no less than f32's
-    return bad ? bad : qskv::split_of(a, nullptr).bytes;
+    if (bad) return bad;
+    int64_t most = 0;           // of any type
+    for (int type : {QS_SRC_F32, QS_SRC_BF16}) {
+        a.type = type;
+        const int64_t n = qskv::split_of(a, nullptr).bytes;
+        most = n > most ? n : most;
+    }
+    return most;
 }
 
 int qs_kv_attention(const qs_kv_cache* cache, int type, const void* q, int64_t q_token_stride_bytes, int64_t batch,

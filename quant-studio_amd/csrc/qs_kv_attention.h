@@ -34,14 +34,13 @@ inline __host__ __device__ int column_tiles(const AttentionArgs& a) {
 
 // How a call's work is split, and where its workgroups leave what is joined.
 constexpr int TILE = 32;            // slots of a wave's step
-constexpr int WAVES = 4;            // of a workgroup, a step each in turn
-constexpr int OPENING = 8;          // steps that beginning with another segment takes as long as
+constexpr int OPENING = 2;          // steps of its waves that a workgroup takes as long to begin with another segment
 // workgroups that a CU holds, by the registers of a wave
 __host__ __device__ constexpr int resident(int blocks, bool wide) {
-    return blocks == 2 ? 4 : blocks == 4 ? (wide ? 2 : 3) : blocks == 6 ? 2 : wide ? 1 : 2;
+    return blocks == 2 ? 4 : blocks == 4 ? (wide ? 2 : 3) : wide ? 1 : 2;
 }
 struct Split {
-    int32_t groups;                 // workgroups
+    int32_t groups, waves;          // workgroups, waves in each: 4, which take steps in turn, or 1
     int32_t share;                  // workgroups of a head's and column tile's steps of a sequence, 1: they take all;
                                     // 0: they take equal runs of all steps of the call
     // of each workgroup, first for a segment that begins before it, then for one that goes on after it

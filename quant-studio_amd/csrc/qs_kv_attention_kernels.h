@@ -488,55 +488,55 @@ QS_DEV Steps steps_of(const AttentionArgs& a, int length) {
 // The call's steps in a row (by sequence, head, tile of columns, then along the
 // sequence), dealt to the workgroups in equal runs: `total` of them, `each` to a
 // workgroup, this one's first one in sequence `seq`, whose own begin at `base` of one
-// head's. A head's steps count OPENING more than they are, which comes first: what
+// head's. A head's steps count `opening` more than they are, which comes first: what
 // beginning with another one takes. The lengths are on the device, so every workgroup
 // adds them up.
 struct Deal {
     int64_t total, each;
     int seq, base;
 };
-constexpr int64_t LEAST = WAVES;        // steps of a workgroup
 QS_DEV int64_t quotient(int64_t a, int64_t b) {     // of numbers from 0 on
     return (a | b) >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);
 }
-QS_DEV int units_of(const AttentionArgs& a, int seq) { return OPENING + steps_of(a, length_of(a, seq)).count; }
-QS_DEV Deal deal(const AttentionArgs& a, int groups, int heads) {
+QS_DEV int units_of(const AttentionArgs& a, int opening, int seq) { return opening + steps_of(a, length_of(a, seq)).count; }
+QS_DEV Deal deal(const AttentionArgs& a, int groups, int waves, int opening, int heads) {
     // every wave by itself: a lane adds up a run of sequences, and these sums are added along the lanes
     const int lane = threadIdx.x & 63, each_lane = (a.batch + 63) >> 6;
     int sum = 0;
 #pragma unroll 4
     for (int i = 0; i < each_lane; i++) {
         const int seq = lane * each_lane + i;
-        sum += seq < a.batch ? units_of(a, seq) : 0;
+        sum += seq < a.batch ? units_of(a, opening, seq) : 0;
     }
     const int scan = qs::wave_incl_scan(sum);
     Deal d;
     d.total = (int64_t)__builtin_amdgcn_readlane(scan, 63) * heads;
     d.each = quotient(d.total + groups - 1, groups);
-    d.each = d.each < LEAST ? LEAST : d.each;
+    d.each = d.each < waves ? waves : d.each;
     const int64_t begin = blockIdx.x * d.each;
     if (begin >= d.total) return d;
     const int at = (int)quotient(begin, heads);
     const int run = __builtin_ctzll(__ballot(at < scan));       // the lane whose run it is in
     d.seq = run * each_lane;
     d.base = __builtin_amdgcn_readlane(scan - sum, run);
-    for (int n = units_of(a, d.seq); at >= d.base + n; n = units_of(a, d.seq)) {
+    for (int n = units_of(a, opening, d.seq); at >= d.base + n; n = units_of(a, opening, d.seq)) {
         d.base += n;
         d.seq++;
     }
     return d;
 }
 
-// A workgroup of four waves, which take a segment's steps in turn (a segment: what
-// the workgroup has of one head's and column tile's steps of a sequence) and join
+// A workgroup of four waves or one, which take a segment's steps in turn (a segment:
+// what the workgroup has of one head's and column tile's steps of a sequence) and join
 // their sums through LDS. A segment that is a whole one is written as the result,
 // else as a part that k_kv_join takes.
 // SHARE: its segment is the steps that it has of the split's `share`, dealt to their
 // waves in turn.
-template <int K_BITS, int V_BITS, int BLOCKS, bool WIDE, bool SHARE>
+template <int K_BITS, int V_BITS, int BLOCKS, bool WIDE, int WAVES, bool SHARE>
 __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(resident(BLOCKS, WIDE))))
 void k_kv_attention(AttentionArgs a, Split split) {
     constexpr int D = 32 * BLOCKS, ROW = D + 4;     // 4: the eight columns' words in other banks
+    constexpr int OPENING = qskv::OPENING * WAVES;
     __shared__ __attribute__((aligned(16))) float acc[WAVES][COLUMNS][ROW];
     __shared__ float2 stats[WAVES][COLUMNS];
     __shared__ __attribute__((aligned(16))) uint32_t steps_lds[WAVES][TILE * BLOCKS];
@@ -551,7 +551,7 @@ void k_kv_attention(AttentionArgs a, Split split) {
         which = segment - seq * heads;
         from = (int)blockIdx.x - segment * split.share;     // which part
     } else {
-        const Deal d = deal(a, split.groups, heads);
+        const Deal d = deal(a, split.groups, WAVES, OPENING, heads);
         each = d.each;
         at = blockIdx.x * d.each;
         end = at + d.each < d.total ? at + d.each : d.total;
@@ -636,34 +636,37 @@ void k_kv_attention(AttentionArgs a, Split split) {
             if (g == 0) stats[wave][lane & 7] = float2{sums.ref, sums.total};
         }
         __syncthreads();
-        // thread: a column, two dims of every 64
-        const int column = threadIdx.x >> 5, sub = threadIdx.x & 31;
-        float ref = -__builtin_inff(), total = 0.0f, part[WAVES];
-#pragma unroll
-        for (int w = 0; w < WAVES; w++) ref = fmaxf(ref, stats[w][column].x);
-#pragma unroll
-        for (int w = 0; w < WAVES; w++) {
-            const float2 s = stats[w][column];
-            part[w] = s.x > -__builtin_inff() ? __builtin_amdgcn_exp2f(s.x - ref) : s.y;    // s.y: 0, or NaN
-            total = __builtin_fmaf(s.y, part[w], total);
-        }
         const bool whole = SHARE ? split.share == 1 : from == 0 && to == steps.count;
-        const int64_t row = row_of(a, seq, head, tile * COLUMNS + column);
-        const int64_t slot = ((int64_t)blockIdx.x * 2 + (from == 0)) * COLUMNS + column;
-        const float inverse = total != 0.0f ? 0x1p24f / total : 0.0f;    // 0: it sees nothing
+        // thread: two dims of every 64 of a column, or of one after another
+        const int sub = threadIdx.x & 31;
 #pragma unroll
-        for (int i = 0; i < BLOCKS / 2; i++) {
-            float2 v{0, 0};
+        for (int column = threadIdx.x >> 5; column < COLUMNS; column += 2 * WAVES) {
+            float ref = -__builtin_inff(), total = 0.0f, part[WAVES];
+#pragma unroll
+            for (int w = 0; w < WAVES; w++) ref = fmaxf(ref, stats[w][column].x);
 #pragma unroll
             for (int w = 0; w < WAVES; w++) {
-                const float2 u = *reinterpret_cast<const float2*>(&acc[w][column][64 * i + 2 * sub]);
-                v.x = __builtin_fmaf(u.x, part[w], v.x);
-                v.y = __builtin_fmaf(u.y, part[w], v.y);
+                const float2 s = stats[w][column];
+                part[w] = s.x > -__builtin_inff() ? __builtin_amdgcn_exp2f(s.x - ref) : s.y;    // s.y: 0, or NaN
+                total = __builtin_fmaf(s.y, part[w], total);
             }
-            if (!whole) *reinterpret_cast<float2*>(split.parts + slot * D + 64 * i + 2 * sub) = v;
-            else if (row >= 0) store_two(a, row + 64 * i + 2 * sub, v.x * inverse, v.y * inverse);
+            const int64_t row = row_of(a, seq, head, tile * COLUMNS + column);
+            const int64_t slot = ((int64_t)blockIdx.x * 2 + (from == 0)) * COLUMNS + column;
+            const float inverse = total != 0.0f ? 0x1p24f / total : 0.0f;    // 0: it sees nothing
+#pragma unroll
+            for (int i = 0; i < BLOCKS / 2; i++) {
+                float2 v{0, 0};
+#pragma unroll
+                for (int w = 0; w < WAVES; w++) {
+                    const float2 u = *reinterpret_cast<const float2*>(&acc[w][column][64 * i + 2 * sub]);
+                    v.x = __builtin_fmaf(u.x, part[w], v.x);
+                    v.y = __builtin_fmaf(u.y, part[w], v.y);
+                }
+                if (!whole) *reinterpret_cast<float2*>(split.parts + slot * D + 64 * i + 2 * sub) = v;
+                else if (row >= 0) store_two(a, row + 64 * i + 2 * sub, v.x * inverse, v.y * inverse);
+            }
+            if (!whole && sub == 0) split.stats[slot] = float2{ref, total};
         }
-        if (!whole && sub == 0) split.stats[slot] = float2{ref, total};
         __syncthreads();
         if constexpr (SHARE) return;
         if (from == 0) {
@@ -680,13 +683,17 @@ void k_kv_attention(AttentionArgs a, Split split) {
     if (!split.listed && threadIdx.x == 0) split.segments[blockIdx.x] = going;
 }
 
+template <int K_BITS, int V_BITS, int BLOCKS, bool WIDE>
+hipError_t launch_typed(const AttentionArgs& a, const Split& split, hipStream_t st) {
+    const auto kernel = split.waves == 4 ? (split.share ? k_kv_attention<K_BITS, V_BITS, BLOCKS, WIDE, 4, true> : k_kv_attention<K_BITS, V_BITS, BLOCKS, WIDE, 4, false>)
+                                         : (split.share ? k_kv_attention<K_BITS, V_BITS, BLOCKS, WIDE, 1, true> : k_kv_attention<K_BITS, V_BITS, BLOCKS, WIDE, 1, false>);
+    const hipError_t e = qs_host::launch_kernel(kernel, dim3((unsigned)split.groups), dim3((unsigned)(64 * split.waves)), 0, st, a, split);
+    return e != hipSuccess || split.share == 1 ? e : launch_join(a, split, st);
+}
 template <int K_BITS, int V_BITS, int BLOCKS>
 hipError_t launch_blocks(const AttentionArgs& a, const Split& split, hipStream_t st) {
-    const auto kernel =
-        a.type == QS_SRC_F32 ? (split.share ? k_kv_attention<K_BITS, V_BITS, BLOCKS, true, true> : k_kv_attention<K_BITS, V_BITS, BLOCKS, true, false>)
-                             : (split.share ? k_kv_attention<K_BITS, V_BITS, BLOCKS, false, true> : k_kv_attention<K_BITS, V_BITS, BLOCKS, false, false>);
-    const hipError_t e = qs_host::launch_kernel(kernel, dim3((unsigned)split.groups), dim3(64 * WAVES), 0, st, a, split);
-    return e != hipSuccess || split.share == 1 ? e : launch_join(a, split, st);
+    return a.type == QS_SRC_F32 ? launch_typed<K_BITS, V_BITS, BLOCKS, true>(a, split, st)
+                                : launch_typed<K_BITS, V_BITS, BLOCKS, false>(a, split, st);
 }
 
 template <int K_BITS, int V_BITS>
