@@ -361,39 +361,32 @@ Split split_of(const AttentionArgs& a, void* workspace) {
     // knows before it knows the length; more of them are in equal runs of all their
     // steps, since the longest may be of any share. Where there are more segments than
     // workgroups, waves take them by themselves: opening one is most of what a short one
-    // takes.
+    // takes; and as a whole, where the longest cannot take much longer than all together.
     constexpr int64_t CUS = 256, FEW = 8;
-    const int64_t segments = (int64_t)a.batch * a.c.heads * column_tiles(a);
     const int64_t steps = ((int64_t)a.pages_each * a.c.page + TILE - 1) / TILE;
+    const int64_t segments = (int64_t)a.batch * a.c.heads * column_tiles(a);
+    const int64_t full = CUS * resident(a.c.blocks, columns_of(a), a.type == QS_SRC_F32);
     Split s{};
     if (a.batch == 0 || a.fresh == 0) return s;
-    const auto plan = [&](bool wide) {
-        const int64_t full = CUS * resident(a.c.blocks, wide);
-        Split p{};
-        p.waves = segments > (steps <= FEW ? 1 : 2) * full && a.batch > 1 ? 1 : 4;
-        if (steps <= FEW) {
-            p.share = 1;
-        } else if (a.batch == 1) {
-            const int64_t share = full / segments, most = (steps + p.waves - 1) / p.waves;
-            p.share = (int32_t)(share < 1 ? 1 : share < most ? share : most);
-        }
-        const int64_t held = full * (4 / p.waves), most = segments * (steps / p.waves + 1 + OPENING);
-        p.groups = (int32_t)(p.share ? segments * p.share : most < held ? most : held);
-        return p;
-    };
-    s = plan(a.type == QS_SRC_F32);
+    s.waves = segments > (steps <= FEW ? 1 : 2) * full && a.batch > 1 ? 1 : 4;
+    const int64_t held = full * (4 / s.waves);
+    if (steps <= FEW || (s.waves == 1 && steps <= FEW * (1 + segments / held))) {
+        s.share = 1;
+    } else if (a.batch == 1) {
+        const int64_t share = full / segments, most = (steps + s.waves - 1) / s.waves;
+        s.share = (int32_t)(share < 1 ? 1 : share < most ? share : most);
+    }
+    const int64_t most = segments * (steps / s.waves + 1 + OPENING);
+    s.groups = (int32_t)(s.share ? segments * s.share : most < held ? most : held);
     if (s.share == 1) return s;
-    // the workspace is the same for every type
-    const Split narrow = plan(false), wide = plan(true);
-    const int64_t room = narrow.groups > wide.groups ? narrow.groups : wide.groups;
-    const int64_t parts = round_up(room * 2 * COLUMNS * 32 * a.c.blocks * 4, 256);
-    const int64_t stats = round_up(room * 2 * COLUMNS * 8, 256);
+    const int64_t parts = round_up((int64_t)s.groups * 2 * columns_of(a) * 32 * a.c.blocks * 4, 256);
+    const int64_t stats = round_up((int64_t)s.groups * 2 * columns_of(a) * 8, 256);
     uint8_t* base = static_cast<uint8_t*>(workspace);
     s.parts = reinterpret_cast<float*>(base);
     s.stats = reinterpret_cast<float2*>(base + parts);
     s.segments = reinterpret_cast<int4*>(base + parts + stats);
     s.listed = (int32_t)(segments <= s.groups ? segments : 0);
-    s.bytes = parts + stats + room * 16;
+    s.bytes = parts + stats + (int64_t)s.groups * 16;
     return s;
 }
 

@@ -12,7 +12,6 @@ namespace qskv {
 // checks a cache of the C ABI and fills in `c`; 0, or the error's code
 int cache_of(const qs_kv_cache* cache, Cache& c);
 
-constexpr int COLUMNS = 8;          // queries of a workgroup: a matrix product's 16 columns are two for each
 
 struct AttentionArgs {
     Cache c;
@@ -27,25 +26,30 @@ struct AttentionArgs {
     float scale;
 };
 
-// one workgroup's queries: COLUMNS of a key/value head's group * fresh
+// Queries of a workgroup, of a key/value head's group * fresh: eight, for each of which a
+// matrix product has two of its 16 columns, or twice as many, which read and unpack the
+// head once and not twice, where there are so many and a wave's registers hold them.
+inline __host__ __device__ int columns_of(const AttentionArgs& a) {
+    return a.group * a.fresh > 8 && a.c.blocks <= 4 && a.type != QS_SRC_F32 ? 16 : 8;
+}
 inline __host__ __device__ int column_tiles(const AttentionArgs& a) {
-    return (a.group * a.fresh + COLUMNS - 1) / COLUMNS;
+    return (a.group * a.fresh + columns_of(a) - 1) / columns_of(a);
 }
 
 // How a call's work is split, and where its workgroups leave what is joined.
 constexpr int TILE = 32;            // slots of a wave's step
 constexpr int OPENING = 2;          // steps of its waves that a workgroup takes as long to begin with another segment
-// workgroups that a CU holds, by the registers of a wave
-__host__ __device__ constexpr int resident(int blocks, bool wide) {
-    return blocks == 2 ? 4 : blocks == 4 ? (wide ? 2 : 3) : wide ? 1 : 2;
+// workgroups of four waves that a CU holds, by the registers of a wave
+__host__ __device__ constexpr int resident(int blocks, int columns, bool wide) {
+    return blocks == 2 ? (columns == 16 ? 3 : 4) : blocks == 4 ? (wide || columns == 16 ? 2 : 3) : wide ? 1 : 2;
 }
 struct Split {
     int32_t groups, waves;          // workgroups, waves in each: 4, which take steps in turn, or 1
     int32_t share;                  // workgroups of a head's and column tile's steps of a sequence, 1: they take all;
                                     // 0: they take equal runs of all steps of the call
     // of each workgroup, first for a segment that begins before it, then for one that goes on after it
-    float* parts;                   // [groups][2][COLUMNS][head size], 2^-24 of a sum relative to R
-    float2* stats;                  // [groups][2][COLUMNS]: R, sum of p
+    float* parts;                   // [groups][2][columns][head size], 2^-24 of a sum relative to R
+    float2* stats;                  // [groups][2][columns]: R, sum of p
     // Of runs: segments that more than one workgroup has, as sequence, head and column tile, first and last
     // workgroup (-1: it is one's alone). One entry for each head and column tile of a sequence where these
     // are no more than workgroups (`listed`), else one for that which goes on after each workgroup.

@@ -163,8 +163,8 @@ struct RawQueries {
     qsr::Eight<WIDE ? qs::SRC_F32 : qs::SRC_BF16> b[BLOCKS];
 };
 template <int BLOCKS, bool WIDE>
-QS_DEV void load_queries(const AttentionArgs& a, int seq, int head, int tile, RawQueries<BLOCKS, WIDE>& o) {
-    const int lane = threadIdx.x & 63, g = lane >> 4, column = tile * COLUMNS + (lane & 7);
+QS_DEV void load_queries(const AttentionArgs& a, int seq, int head, int first, RawQueries<BLOCKS, WIDE>& o) {
+    const int lane = threadIdx.x & 63, g = lane >> 4, column = first + (lane & 7);
     const bool live = column < a.group * a.fresh;
     const int token = live ? column / a.group : 0, mine = live ? column - token * a.group : 0;
     const int64_t at = ((int64_t)seq * a.fresh + token) * a.q_stride + (int64_t)(head * a.group + mine) * 32 * BLOCKS;
@@ -172,9 +172,9 @@ QS_DEV void load_queries(const AttentionArgs& a, int seq, int head, int tile, Ra
     for (int b = 0; b < BLOCKS; b++) qsr::load8<WIDE ? qs::SRC_F32 : qs::SRC_BF16>(a.q, at + 32 * b + 8 * g, o.b[b]);
 }
 template <int K_BITS, int BLOCKS, bool WIDE>
-QS_DEV void prepare_queries(const AttentionArgs& a, int tile, int length, const RawQueries<BLOCKS, WIDE>& raw,
+QS_DEV void prepare_queries(const AttentionArgs& a, int first, int length, const RawQueries<BLOCKS, WIDE>& raw,
                             Queries<BLOCKS, WIDE>& o) {
-    const int lane = threadIdx.x & 63, column = tile * COLUMNS + (lane & 7);
+    const int lane = threadIdx.x & 63, column = first + (lane & 7);
     const bool live = column < a.group * a.fresh, bf16 = a.type == QS_SRC_BF16;
     const int token = live ? column / a.group : 0;
     float x[BLOCKS][8];
@@ -237,11 +237,11 @@ QS_DEV void clear(Sums<BLOCKS>& o) {
 struct Span {
     int first, last, all_first, all_last;
 };
-QS_DEV Span span_of(const AttentionArgs& a, int tile, int length) {
-    const int high = min(a.group * a.fresh, (tile + 1) * COLUMNS) - 1;
+QS_DEV Span span_of(const AttentionArgs& a, int first, int columns, int length) {
+    const int high = min(a.group * a.fresh, first + columns) - 1;
     Span s;
     s.last = length - a.fresh + 1 + high / a.group;
-    s.all_last = length - a.fresh + 1 + tile * COLUMNS / a.group;
+    s.all_last = length - a.fresh + 1 + first / a.group;
     s.first = a.window > 0 && s.all_last > a.window ? s.all_last - a.window : 0;
     s.all_first = a.window > 0 && s.last > a.window ? s.last - a.window : 0;
     return s;
@@ -327,9 +327,9 @@ QS_DEV void load_values(const AttentionArgs& a, const Place& at, Tile<K_BITS, V_
 // with, and arrive while the other half is computed.
 // edge: some query does not see all of the slots; to it they count for nothing,
 // whatever they hold, since a lane's scores and steps are its query's own copies.
-template <bool WIDE, int K_BITS, int V_BITS, int BLOCKS>
+template <bool WIDE, int K_BITS, int V_BITS, int BLOCKS, int SETS>
 QS_DEV void attend(const AttentionArgs& a, int start, bool edge, int held, const Place& next,
-                   const Queries<BLOCKS, WIDE>& q, uint32_t* lds, Tile<K_BITS, V_BITS, BLOCKS>& t, Sums<BLOCKS>& sums) {
+                   const Queries<BLOCKS, WIDE> (&q)[SETS], uint32_t* lds, Tile<K_BITS, V_BITS, BLOCKS>& t, Sums<BLOCKS> (&sums)[SETS]) {
     const int lane = threadIdx.x & 63, g = lane >> 4;
     // steps of four slots, and one of them
     typedef Codes<8 * BLOCKS> Steps4;
@@ -351,99 +351,110 @@ QS_DEV void attend(const AttentionArgs& a, int start, bool edge, int held, const
     for (int i = 0; i < BLOCKS / 2; i++) lds[lane * (BLOCKS / 2) + i] = t.steps.w[i];
     qs::wave_sync<true>();
     // scores, in powers of two
-    float x[2][4];
+    float x[SETS][2][4];
 #pragma unroll
     for (int s = 0; s < 2; s++) {
 #pragma unroll
-        for (int r = 0; r < 4; r++) x[s][r] = 0.0f;
+        for (int n = 0; n < 4 * SETS; n++) x[n >> 2][s][n & 3] = 0.0f;
         Steps4 ks;
         steps_from(s, false, ks);
 #pragma unroll
         for (int b = 0; b < BLOCKS; b++) {
             const u32x4 k = key_block<K_BITS, BLOCKS>(t.keys[s], b);
-            f32x4 d = mfma(k, q.q[b], f32x4{0, 0, 0, 0});
-            if constexpr (WIDE) d = mfma(k, q.lo[b], d);
 #pragma unroll
-            for (int r = 0; r < 4; r++) x[s][r] = __builtin_fmaf(d[r], step_of(ks, r, b), x[s][r]);
+            for (int n = 0; n < SETS; n++) {
+                f32x4 d = mfma(k, q[n].q[b], f32x4{0, 0, 0, 0});
+                if constexpr (WIDE) d = mfma(k, q[n].lo[b], d);
+#pragma unroll
+                for (int r = 0; r < 4; r++) x[n][s][r] = __builtin_fmaf(d[r], step_of(ks, r, b), x[n][s][r]);
+            }
         }
 #pragma unroll
-        for (int r = 0; r < 4; r++) x[s][r] = __builtin_ldexpf(x[s][r] * q.scale, q.up);
+        for (int n = 0; n < SETS; n++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) x[n][s][r] = __builtin_ldexpf(x[n][s][r] * q[n].scale, q[n].up);
     }
     __builtin_amdgcn_sched_barrier(0);      // loads that move up would need registers of their own
     load_keys(a, next, t);
-    Steps4 vs[2];
-    steps_from(0, true, vs[0]);
-    steps_from(1, true, vs[1]);
+    Steps4 vs[SETS][2];
+#pragma unroll
+    for (int n = 0; n < SETS; n++)
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+            if (n == 0) steps_from(s, true, vs[0][s]);
+            else vs[n][s] = vs[0][s];
+        }
     if (edge) {
 #pragma unroll
-        for (int s = 0; s < 2; s++)
+        for (int n = 0; n < 8 * SETS; n++) {
+            const int set = n >> 3, s = n >> 2 & 1, r = n & 3, p = start + 16 * s + 4 * g + r;
+            if (!((held >> s & 1) && p >= q[set].first && p < q[set].last)) {
+                x[set][s][r] = -__builtin_inff();
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const int p = start + 16 * s + 4 * g + r;
-                if (!((held >> s & 1) && p >= q.first && p < q.last)) {
-                    x[s][r] = -__builtin_inff();
-#pragma unroll
-                    for (int i = 0; i < BLOCKS / 2; i++) vs[s].w[r * (BLOCKS / 2) + i] = 0;
-                }
+                for (int i = 0; i < BLOCKS / 2; i++) vs[set][s].w[r * (BLOCKS / 2) + i] = 0;
             }
+        }
     }
-    // the running maximum and R
-    float top = sums.top;
-    uint32_t steps = 0;
+    float p[SETS][8];
 #pragma unroll
-    for (int s = 0; s < 2; s++) {
+    for (int n = 0; n < SETS; n++) {
+        // the running maximum and R
+        float top = sums[n].top;
+        uint32_t steps = 0;
 #pragma unroll
-        for (int r = 0; r < 4; r++) top = fmaxf(top, x[s][r]);
+        for (int s = 0; s < 2; s++) {
 #pragma unroll
-        for (int i = 0; i < 2 * BLOCKS; i++) steps |= vs[s].w[i];
-    }
-    top = max_over_slots(top);
-    steps = over_slots(steps, [](uint32_t u, uint32_t v) { return u | v; });
-    sums.step |= steps | steps >> 16;
-    // 2^s takes every step below 2^15. Or'ed exponents bound them all, and are over the
-    // largest by 15 at most, by 7 for steps below 2, which takes that much off 39 bits; a
-    // subnormal step, or none, counts as 2^-14.
-    const int exponent = (int)(sums.step >> 10 & 31), s = 29 - (exponent > 1 ? exponent : 1);
-    const float ref = top > -__builtin_inff() ? top - (float)s : -__builtin_inff();
-    const float base = top > -__builtin_inff() ? ref : 0.0f;
-    const float shrink = __builtin_amdgcn_exp2f(sums.ref - base);   // 0 where nothing was seen yet
-    sums.top = top;
-    sums.ref = ref;
-    float p[8];
-    float total = 0.0f;
+            for (int r = 0; r < 4; r++) top = fmaxf(top, x[n][s][r]);
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        p[i] = __builtin_amdgcn_exp2f(x[i >> 2][i & 3] - base);
-        total += p[i];
-    }
-    sums.total = __builtin_fmaf(sums.total, shrink, total);
-    if (__any(shrink != 1.0f)) {
+            for (int i = 0; i < 2 * BLOCKS; i++) steps |= vs[n][s].w[i];
+        }
+        top = max_over_slots(top);
+        steps = over_slots(steps, [](uint32_t u, uint32_t v) { return u | v; });
+        sums[n].step |= steps | steps >> 16;
+        // 2^s takes every step below 2^15. Or'ed exponents bound them all, and are over the
+        // largest by 15 at most, by 7 for steps below 2, which takes that much off 39 bits; a
+        // subnormal step, or none, counts as 2^-14.
+        const int exponent = (int)(sums[n].step >> 10 & 31), s = 29 - (exponent > 1 ? exponent : 1);
+        const float ref = top > -__builtin_inff() ? top - (float)s : -__builtin_inff();
+        const float base = top > -__builtin_inff() ? ref : 0.0f;
+        const float shrink = __builtin_amdgcn_exp2f(sums[n].ref - base);    // 0 where nothing was seen yet
+        sums[n].top = top;
+        sums[n].ref = ref;
+        float total = 0.0f;
 #pragma unroll
-        for (int b = 0; b < BLOCKS; b++)
+        for (int i = 0; i < 8; i++) {
+            p[n][i] = __builtin_amdgcn_exp2f(x[n][i >> 2][i & 3] - base);
+            total += p[n][i];
+        }
+        sums[n].total = __builtin_fmaf(sums[n].total, shrink, total);
+        if (__any(shrink != 1.0f)) {
 #pragma unroll
-            for (int e = 0; e < 2; e++)
+            for (int b = 0; b < BLOCKS; b++)
 #pragma unroll
-                for (int r = 0; r < 4; r++) sums.acc[b][e][r] *= shrink;
+                for (int e = 0; e < 2; e++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) sums[n].acc[b][e][r] *= shrink;
+        }
     }
     const uint32_t second = lane & 8 ? 0xffffe000u : 0u;
 #pragma unroll
     for (int b = 0; b < BLOCKS; b++) {
-        u32x4 w;
+        u32x4 w[SETS];
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int n = 2 * i;
-            const float d0 = step_of(vs[n >> 2], n & 3, b), d1 = step_of(vs[n >> 2], (n & 3) + 1, b);
+        for (int n = 0; n < 4 * SETS; n++) {
+            const int set = n >> 2, i = 2 * (n & 3);
+            const Steps4& d = vs[set][i >> 2];
             // + 0 makes it one instruction that takes the step as f16
-            w[i] = two_halves<WIDE>(__builtin_fmaf(p[n], d0, 0.0f), __builtin_fmaf(p[n + 1], d1, 0.0f), second);
+            w[set][n & 3] = two_halves<WIDE>(__builtin_fmaf(p[set][i], step_of(d, i & 3, b), 0.0f),
+                                             __builtin_fmaf(p[set][i + 1], step_of(d, (i & 3) + 1, b), 0.0f), second);
         }
 #pragma unroll
         for (int e = 0; e < 2; e++) {
             u32x4 c;
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                c[i] = value_pair<V_BITS, BLOCKS>(t.values[i >> 1], i & 1, 2 * b + e);
-            }
-            sums.acc[b][e] = mfma(c, w, sums.acc[b][e]);
+            for (int i = 0; i < 4; i++) c[i] = value_pair<V_BITS, BLOCKS>(t.values[i >> 1], i & 1, 2 * b + e);
+#pragma unroll
+            for (int n = 0; n < SETS; n++) sums[n].acc[b][e] = mfma(c, w[n], sums[n].acc[b][e]);
         }
     }
     __builtin_amdgcn_sched_barrier(0);
@@ -532,16 +543,16 @@ QS_DEV Deal deal(const AttentionArgs& a, int groups, int waves, int opening, int
 // else as a part that k_kv_join takes.
 // SHARE: its segment is the steps that it has of the split's `share`, dealt to their
 // waves in turn.
-template <int K_BITS, int V_BITS, int BLOCKS, bool WIDE, int WAVES, bool SHARE>
-__global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(resident(BLOCKS, WIDE))))
+template <int K_BITS, int V_BITS, int BLOCKS, bool WIDE, int SETS, int WAVES, bool SHARE>
+__global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(resident(BLOCKS, 8 * SETS, WIDE))))
 void k_kv_attention(AttentionArgs a, Split split) {
-    constexpr int D = 32 * BLOCKS, ROW = D + 4;     // 4: the eight columns' words in other banks
+    constexpr int COLUMNS = 8 * SETS, D = 32 * BLOCKS, ROW = D + 4;     // 4: the eight columns' words in other banks
     constexpr int OPENING = qskv::OPENING * WAVES;
     __shared__ __attribute__((aligned(16))) float acc[WAVES][COLUMNS][ROW];
     __shared__ float2 stats[WAVES][COLUMNS];
     __shared__ __attribute__((aligned(16))) uint32_t steps_lds[WAVES][TILE * BLOCKS];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane >> 4;
-    const int tiles = column_tiles(a), heads = a.c.heads * tiles;
+    const int tiles = (a.group * a.fresh + COLUMNS - 1) / COLUMNS, heads = a.c.heads * tiles;
     int64_t at = 0, end = 1, each = 0;
     int seq, base = 0, which = -1, from = 0;        // which: head and column tile
     int4 going{0, 0, 0, -1};
@@ -577,11 +588,14 @@ void k_kv_attention(AttentionArgs a, Split split) {
             from = from < 0 ? 0 : from;
             if (to <= from) break;                  // it ends before they do
         }
-        const int head = which / tiles, tile = which - head * tiles;
-        RawQueries<BLOCKS, WIDE> raw;
-        load_queries(a, seq, head, tile, raw);
-        Sums<BLOCKS> sums;
-        clear(sums);
+        const int head = which / tiles, first = (which - head * tiles) * COLUMNS;    // its first column
+        RawQueries<BLOCKS, WIDE> raw[SETS];
+        Sums<BLOCKS> sums[SETS];
+#pragma unroll
+        for (int n = 0; n < SETS; n++) {
+            load_queries(a, seq, head, first + 8 * n, raw[n]);
+            clear(sums[n]);
+        }
         const Ints table = constant(a.tables + seq * a.table_stride);
         // The wave's steps i, i + stride, ... before `stop`, counted from the sequence's
         // start, of those that this column tile's queries see. The first one's codes are
@@ -594,7 +608,7 @@ void k_kv_attention(AttentionArgs a, Split split) {
         int i = RUN ? steps.begin + from + wave : from * WAVES + wave, stop = RUN ? steps.begin + to : most;
         const auto see = [&] {
             if (SHARE) length = cut_length(a, length);
-            span = span_of(a, tile, length);
+            span = span_of(a, first, COLUMNS, length);
             const int low = span.first / TILE, high = (span.last + TILE - 1) / TILE;
             stop = high < stop ? high : stop;
             if (!early) i = RUN ? (low > steps.begin + from ? low + wave : i) : low + i;
@@ -616,8 +630,9 @@ void k_kv_attention(AttentionArgs a, Split split) {
             // the last step it is that step's again, whose codes are in the caches.
             const int final = i + (stop - 1 - i) / stride * stride;
             const auto start_of = [&](int n) { return (n < final ? n : final) * TILE; };
-            Queries<BLOCKS, WIDE> q;
-            prepare_queries<K_BITS>(a, tile, length, raw, q);
+            Queries<BLOCKS, WIDE> q[SETS];
+#pragma unroll
+            for (int n = 0; n < SETS; n++) prepare_queries<K_BITS>(a, first + 8 * n, length, raw[n], q[n]);
             for (; i < stop; i += stride) {
                 const int start = i * TILE, held = place.held;
                 place = place_of(a, ahead, head, start_of(i + stride));
@@ -625,15 +640,20 @@ void k_kv_attention(AttentionArgs a, Split split) {
                 attend(a, start, start < span.all_first || start + TILE > span.all_last || held != 3, held, place, q, steps_lds[wave], t, sums);
             }
         }
-        finish<V_BITS>(sums);
-        if (!(lane & 8)) {
+#pragma unroll
+        for (int n = 0; n < SETS; n++) {
+            finish<V_BITS>(sums[n]);
+            if (lane & 8) continue;
+            const int column = 8 * n + (lane & 7);
 #pragma unroll
             for (int b = 0; b < BLOCKS; b++)
 #pragma unroll
-                for (int h = 0; h < 2; h++)
-                    *reinterpret_cast<f32x4*>(&acc[wave][lane & 7][32 * b + 8 * g + 4 * h]) =
-                        f32x4{sums.acc[b][0][2 * h], sums.acc[b][1][2 * h], sums.acc[b][0][2 * h + 1], sums.acc[b][1][2 * h + 1]};
-            if (g == 0) stats[wave][lane & 7] = float2{sums.ref, sums.total};
+                for (int h = 0; h < 2; h++) {
+                    const f32x4(&v)[2] = sums[n].acc[b];
+                    *reinterpret_cast<f32x4*>(&acc[wave][column][32 * b + 8 * g + 4 * h]) =
+                        f32x4{v[0][2 * h], v[1][2 * h], v[0][2 * h + 1], v[1][2 * h + 1]};
+                }
+            if (g == 0) stats[wave][column] = float2{sums[n].ref, sums[n].total};
         }
         __syncthreads();
         const bool whole = SHARE ? split.share == 1 : from == 0 && to == steps.count;
@@ -650,7 +670,7 @@ void k_kv_attention(AttentionArgs a, Split split) {
                 part[w] = s.x > -__builtin_inff() ? __builtin_amdgcn_exp2f(s.x - ref) : s.y;    // s.y: 0, or NaN
                 total = __builtin_fmaf(s.y, part[w], total);
             }
-            const int64_t row = row_of(a, seq, head, tile * COLUMNS + column);
+            const int64_t row = row_of(a, seq, head, first + column);
             const int64_t slot = ((int64_t)blockIdx.x * 2 + (from == 0)) * COLUMNS + column;
             const float inverse = total != 0.0f ? 0x1p24f / total : 0.0f;    // 0: it sees nothing
 #pragma unroll
@@ -683,17 +703,21 @@ void k_kv_attention(AttentionArgs a, Split split) {
     if (!split.listed && threadIdx.x == 0) split.segments[blockIdx.x] = going;
 }
 
-template <int K_BITS, int V_BITS, int BLOCKS, bool WIDE>
-hipError_t launch_typed(const AttentionArgs& a, const Split& split, hipStream_t st) {
-    const auto kernel = split.waves == 4 ? (split.share ? k_kv_attention<K_BITS, V_BITS, BLOCKS, WIDE, 4, true> : k_kv_attention<K_BITS, V_BITS, BLOCKS, WIDE, 4, false>)
-                                         : (split.share ? k_kv_attention<K_BITS, V_BITS, BLOCKS, WIDE, 1, true> : k_kv_attention<K_BITS, V_BITS, BLOCKS, WIDE, 1, false>);
+template <int K_BITS, int V_BITS, int BLOCKS, bool WIDE, int SETS>
+hipError_t launch_sets(const AttentionArgs& a, const Split& split, hipStream_t st) {
+    const auto kernel = split.waves == 4 ? (split.share ? k_kv_attention<K_BITS, V_BITS, BLOCKS, WIDE, SETS, 4, true>
+                                                        : k_kv_attention<K_BITS, V_BITS, BLOCKS, WIDE, SETS, 4, false>)
+                                         : (split.share ? k_kv_attention<K_BITS, V_BITS, BLOCKS, WIDE, SETS, 1, true>
+                                                        : k_kv_attention<K_BITS, V_BITS, BLOCKS, WIDE, SETS, 1, false>);
     const hipError_t e = qs_host::launch_kernel(kernel, dim3((unsigned)split.groups), dim3((unsigned)(64 * split.waves)), 0, st, a, split);
     return e != hipSuccess || split.share == 1 ? e : launch_join(a, split, st);
 }
 template <int K_BITS, int V_BITS, int BLOCKS>
 hipError_t launch_blocks(const AttentionArgs& a, const Split& split, hipStream_t st) {
-    return a.type == QS_SRC_F32 ? launch_typed<K_BITS, V_BITS, BLOCKS, true>(a, split, st)
-                                : launch_typed<K_BITS, V_BITS, BLOCKS, false>(a, split, st);
+    if (a.type == QS_SRC_F32) return launch_sets<K_BITS, V_BITS, BLOCKS, true, 1>(a, split, st);
+    if constexpr (BLOCKS <= 4)
+        if (columns_of(a) == 16) return launch_sets<K_BITS, V_BITS, BLOCKS, false, 2>(a, split, st);
+    return launch_sets<K_BITS, V_BITS, BLOCKS, false, 1>(a, split, st);
 }
 
 template <int K_BITS, int V_BITS>

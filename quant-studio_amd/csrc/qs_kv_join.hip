@@ -19,7 +19,7 @@ __global__ __launch_bounds__(THREADS) void k_kv_join(AttentionArgs a, Split spli
     constexpr int D = 32 * BLOCKS, LANES = D / 4, ROWS = THREADS / LANES, TIMES = 4;
     __shared__ f32x4 acc[ROWS][LANES];
     __shared__ float2 stats[ROWS];
-    const int tiles = column_tiles(a), column = (int)blockIdx.y;
+    const int tiles = column_tiles(a), columns = columns_of(a), column = (int)blockIdx.y;
     int4 s;
     if (split.share) {
         const int heads = a.c.heads * tiles, seq = (int)blockIdx.x / heads, first = (int)blockIdx.x * split.share;
@@ -29,7 +29,7 @@ __global__ __launch_bounds__(THREADS) void k_kv_join(AttentionArgs a, Split spli
         if (s.w < 0) return;
     }
     const int head = s.y / tiles;
-    const int64_t row = row_of(a, s.x, head, (s.y - head * tiles) * COLUMNS + column);
+    const int64_t row = row_of(a, s.x, head, (s.y - head * tiles) * columns + column);
     if (row < 0) return;
     const int mine = (int)threadIdx.x / LANES, lane = (int)threadIdx.x - mine * LANES;
     const int count = s.w - s.z + 1;
@@ -45,7 +45,7 @@ __global__ __launch_bounds__(THREADS) void k_kv_join(AttentionArgs a, Split spli
                 part[j] = float2{-__builtin_inff(), 0.0f};
                 v[j] = f32x4{0, 0, 0, 0};
                 if (n < count) {
-                    const int64_t slot = ((int64_t)(s.z + n) * 2 + (n == 0)) * COLUMNS + column;
+                    const int64_t slot = ((int64_t)(s.z + n) * 2 + (n == 0)) * columns + column;
                     part[j] = split.stats[slot];
                     v[j] = *reinterpret_cast<const f32x4*>(split.parts + slot * D + 4 * lane);
                 }
@@ -91,7 +91,7 @@ __global__ __launch_bounds__(THREADS) void k_kv_join(AttentionArgs a, Split spli
 
 template <int BLOCKS>
 hipError_t launch_blocks(const AttentionArgs& a, const Split& split, hipStream_t st) {
-    const int columns = a.group * a.fresh < COLUMNS ? a.group * a.fresh : COLUMNS;
+    const int columns = a.group * a.fresh < columns_of(a) ? a.group * a.fresh : columns_of(a);
     const int segments = split.share ? split.groups / split.share : split.listed ? split.listed : split.groups;
     const bool many = split.groups > 48 * segments;        // parts of a segment
     return qs_host::launch_kernel(many ? k_kv_join<BLOCKS, 1024> : k_kv_join<BLOCKS, 256>, dim3((unsigned)segments, (unsigned)columns),
