@@ -97,7 +97,7 @@ class KVCache:
 
 def _rows(what: str, name: str, x, cache: KVCache):
     """(x, its row stride in bytes): rows of heads * head_dim values in a layout the C call takes."""
-    t, width, esz = x.shape[0], cache.heads * cache.head_dim, x.element_size()
+    width, esz = cache.heads * cache.head_dim, x.element_size()
     if x.dim() == 3:
         if x.shape[1] != cache.heads or x.shape[2] != cache.head_dim:
             raise ValueError(f"{what}: {name} must be (t, {cache.heads}, {cache.head_dim}), got {tuple(x.shape)}")
@@ -105,17 +105,18 @@ def _rows(what: str, name: str, x, cache: KVCache):
         raise ValueError(f"{what}: {name} must be (t, {cache.heads}, {cache.head_dim}) or (t, {width}), got {tuple(x.shape)}")
     if x.is_contiguous() and x.data_ptr() % 16 == 0:
         return x, width * esz
+    t = x.shape[0]
     dense = x.stride(-1) == 1 and (x.dim() == 2 or x.shape[1] == 1 or x.stride(1) == cache.head_dim)
     if not dense or x.data_ptr() % 16 or (t > 1 and (x.stride(0) < width or x.stride(0) * esz % 16)):
         x = torch.empty(x.shape, dtype=x.dtype, device=x.device).copy_(x)
     return x, (x.stride(0) if t > 1 else width) * esz
 
 
-def _slots(what: str, slots, dev: int):
-    if slots.dtype != torch.int32 or slots.dim() != 1:
-        raise ValueError(f"{what}: slots must be int32 (t,), got {slots.dtype} {tuple(slots.shape)}")
-    _same_device(dev, what, "slots", slots)
-    return slots if slots.is_contiguous() else slots.contiguous()
+def _ints(what: str, name: str, x, dims: int, dev: int):
+    if x.dtype != torch.int32 or x.dim() != dims:
+        raise ValueError(f"{what}: {name} must be int32 with {dims} dimension(s), got {x.dtype} {tuple(x.shape)}")
+    if x.get_device() != dev:
+        _same_device(dev, what, name, x)
 
 
 def kv_write(cache: KVCache, k, v, slots) -> None:
@@ -128,19 +129,27 @@ def kv_write(cache: KVCache, k, v, slots) -> None:
     step over float16's largest number makes the values of its block of 32 NaN."""
     lib = _lib()
     src = _type_id(k.dtype, "kv_write")
-    _no_gradient("kv_write", "k", k)
-    _no_gradient("kv_write", "v", v)
+    if k.requires_grad or v.requires_grad:
+        _no_gradient("kv_write", "k", k)
+        _no_gradient("kv_write", "v", v)
     dev = cache._dev
-    _same_device(dev, "kv_write", "k", k)
-    _same_device(dev, "kv_write", "v", v)
-    if k.dtype != v.dtype or k.dim() == 0 or v.dim() == 0 or k.shape[0] != v.shape[0]:
-        raise ValueError(f"kv_write: k and v must be alike, got {k.dtype} {tuple(k.shape)} and {v.dtype} {tuple(v.shape)}")
-    k, k_stride = _rows("kv_write", "k", k, cache)
-    v, v_stride = _rows("kv_write", "v", v, cache)
-    slots = _slots("kv_write", slots, dev)
-    t = k.shape[0]
-    if slots.shape[0] != t:
-        raise ValueError(f"kv_write: {slots.shape[0]} slots for {t} rows")
+    if k.get_device() != dev or v.get_device() != dev:
+        _same_device(dev, "kv_write", "k", k)
+        _same_device(dev, "kv_write", "v", v)
+    if k.dtype != v.dtype:
+        raise ValueError(f"kv_write: k and v must be alike, got {k.dtype} and {v.dtype}")
+    _ints("kv_write", "slots", slots, 1, dev)
+    t = slots.shape[0]
+    if k.shape != (t, cache.heads, cache.head_dim) or v.shape != k.shape or not k.is_contiguous() or not v.is_contiguous() \
+            or (k.data_ptr() | v.data_ptr()) % 16:
+        k, k_stride = _rows("kv_write", "k", k, cache)
+        v, v_stride = _rows("kv_write", "v", v, cache)
+        if k.shape[0] != t or v.shape[0] != t:
+            raise ValueError(f"kv_write: {k.shape[0]} and {v.shape[0]} rows for {t} slots")
+    else:
+        k_stride = v_stride = cache.heads * cache.head_dim * k.element_size()
+    if not slots.is_contiguous():
+        slots = slots.contiguous()
     _call(dev, lib.qs_kv_write, cache._ref, src, k.data_ptr(), k_stride, v.data_ptr(), v_stride, slots.data_ptr(), t)
 
 
@@ -151,8 +160,10 @@ def kv_read(cache: KVCache, slots, dtype=None):
     dtype = torch.bfloat16 if dtype is None else dtype
     dst = _type_id(dtype, "kv_read")
     dev = cache._dev
-    slots = _slots("kv_read", slots, dev)
-    t = slots.shape[0]
+    _ints("kv_read", "slots", slots, 1, dev)
+    if not slots.is_contiguous():
+        slots = slots.contiguous()
+    t = len(slots)
     k = cache.data.new_empty((t, cache.heads, cache.head_dim), dtype=dtype)
     v = torch.empty_like(k)
     _call(dev, lib.qs_kv_read, cache._ref, slots.data_ptr(), t, dst, k.data_ptr(), v.data_ptr())
@@ -189,27 +200,28 @@ def kv_attention(q, cache: KVCache, tables, lengths, scale: float | None = None,
     out: a contiguous tensor of q's shape and type to write instead of a new one."""
     lib = _lib()
     kind = _type_id(q.dtype, "kv_attention")
-    _no_gradient("kv_attention", "q", q)
+    if q.requires_grad:
+        _no_gradient("kv_attention", "q", q)
     dev, d = cache._dev, cache.head_dim
-    _same_device(dev, "kv_attention", "q", q)
+    if q.get_device() != dev:
+        _same_device(dev, "kv_attention", "q", q)
     shape = q.shape
     if len(shape) == 3:
-        b, heads = shape[0], shape[1]
+        b, heads, width = shape
         n = 1
     elif len(shape) == 4:
-        b, n, heads = shape[0], shape[1], shape[2]
+        b, n, heads, width = shape
     else:
         raise ValueError(f"kv_attention: q must be (b, heads, {d}) or (b, n, heads, {d}), got {tuple(shape)}")
-    if shape[-1] != d or heads == 0 or heads % cache.heads:
-        raise ValueError(f"kv_attention: q has {heads} heads of {shape[-1]} values, the cache {cache.heads} of {d}")
+    if width != d or heads == 0 or heads % cache.heads:
+        raise ValueError(f"kv_attention: q has {heads} heads of {width} values, the cache {cache.heads} of {d}")
     if n > 16:
         raise ValueError(f"kv_attention: {n} new tokens of a sequence, at most 16")
-    if tables.dtype != torch.int32 or tables.dim() != 2 or tables.shape[0] != b:
-        raise ValueError(f"kv_attention: tables must be int32 ({b}, m), got {tables.dtype} {tuple(tables.shape)}")
-    if lengths.dtype != torch.int32 or lengths.dim() != 1 or lengths.shape[0] != b:
-        raise ValueError(f"kv_attention: lengths must be int32 ({b},), got {lengths.dtype} {tuple(lengths.shape)}")
-    _same_device(dev, "kv_attention", "tables", tables)
-    _same_device(dev, "kv_attention", "lengths", lengths)
+    _ints("kv_attention", "tables", tables, 2, dev)
+    _ints("kv_attention", "lengths", lengths, 1, dev)
+    rows, m = tables.shape
+    if rows != b or len(lengths) != b:
+        raise ValueError(f"kv_attention: {rows} tables and {len(lengths)} lengths for {b} sequences")
     if window < 0:
         raise ValueError(f"kv_attention: window {window} < 0")
     esz = q.element_size()
@@ -222,10 +234,14 @@ def kv_attention(q, cache: KVCache, tables, lengths, scale: float | None = None,
             q = torch.empty(shape, dtype=q.dtype, device=q.device).copy_(q)
         else:
             stride = between
-    m = tables.shape[1]
-    if m > 1 and tables.stride(1) != 1 or b > 1 and tables.stride(0) < m:
-        tables = tables.contiguous()
-    lengths = lengths if lengths.is_contiguous() else lengths.contiguous()
+    table_stride = m
+    if not tables.is_contiguous():
+        if (m > 1 and tables.stride(1) != 1) or (b > 1 and tables.stride(0) < m):
+            tables = tables.contiguous()
+        elif b > 1:
+            table_stride = tables.stride(0)
+    if not lengths.is_contiguous():
+        lengths = lengths.contiguous()
     key = (b, n, heads, m)
     need = cache._work.get(key)
     if need is None:
@@ -235,12 +251,12 @@ def kv_attention(q, cache: KVCache, tables, lengths, scale: float | None = None,
         work = cache.data.new_empty((need,))
         work_ptr = work.data_ptr()
     if out is None:
-        out = q.new_empty(shape)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.dtype != q.dtype or out.shape != shape or not out.is_contiguous() or not out.is_cuda or out.get_device() != dev:
         raise ValueError(f"kv_attention: out must be contiguous {q.dtype} {tuple(shape)} on cuda:{dev}")
     else:
         _no_gradient("kv_attention", "out", out)
     _call(dev, lib.qs_kv_attention, cache._ref, kind, q.data_ptr(), stride * esz, b, n, heads, tables.data_ptr(), m,
-          tables.stride(0) if b > 1 else m, lengths.data_ptr(), 1 / math.sqrt(d) if scale is None else scale, window,
+          table_stride, lengths.data_ptr(), 1 / math.sqrt(d) if scale is None else scale, window,
           out.data_ptr(), out.numel() * esz, work_ptr, need)
     return out

@@ -5,6 +5,7 @@ of these values in 64 bits."""
 from __future__ import annotations
 
 import math
+import threading
 
 import pytest
 import torch
@@ -186,6 +187,39 @@ def test_batches(qs, batch):
     attend(qs, qs.KVCache(sum(-(-n // 16) for n in lengths) + 1, 16, 1, 64, "q8_0", "q4_0"), lengths, 3, 1, torch.bfloat16, 5)
 
 
+@pytest.mark.parametrize("batch,heads,d,longest", [(300, 8, 64, 200), (300, 8, 128, 2500), (600, 8, 64, 900), (100, 24, 64, 700)])
+def test_many_segments(qs, batch, heads, d, longest):
+    """More heads of sequences than workgroups: whole ones to a wave each, and long ones among them split."""
+    g = torch.Generator().manual_seed(batch)
+    lengths = torch.randint(0, 25, (batch,), generator=g).tolist()
+    lengths[0], lengths[batch // 3], lengths[-1] = longest, longest // 2 + 1, 0
+    attend(qs, qs.KVCache(sum(-(-n // 32) for n in lengths) + 1, 32, heads, d, "q8_0", "q4_0"), lengths, heads * 2, 1, torch.bfloat16, 14)
+
+
+@pytest.mark.parametrize("length", [1, 100, 257, 1000, 4097])
+@pytest.mark.parametrize("window", [0, 40, 600])
+@pytest.mark.parametrize("table", [0, 50])
+def test_a_lone_sequence(qs, length, window, table):
+    """Its tables as wide as it needs, and far wider."""
+    cache = qs.KVCache(100, 64, 2, 128, "q4_0", "q8_0")
+    tables, rows = ref.fill(qs, cache, [length], torch.float16, 15, poison=True)
+    wide = torch.full((1, tables.shape[1] + table), -1, dtype=torch.int32, device=DEV)
+    wide[:, :tables.shape[1]] = tables
+    q = torch.randn((1, 2, 10, 128), generator=torch.Generator().manual_seed(15)).to(DEV, torch.float16)
+    y = qs.kv_attention(q, cache, wide, ints(length), window=window)
+    want, far = ref.attention64(q, rows, window=window)
+    ref.check(y, want, far)
+
+
+def test_out_may_be_q(qs):
+    cache = qs.KVCache(80, 16, 2, 64, "q8_0")
+    lengths = [400, 3, 0, 700]
+    tables, _ = ref.fill(qs, cache, lengths, torch.bfloat16, 16)
+    q = torch.randn((4, 3, 12, 64), generator=torch.Generator().manual_seed(16)).to(DEV, torch.bfloat16)
+    want = qs.kv_attention(q, cache, tables, ints(*lengths))
+    assert qs.kv_attention(q, cache, tables, ints(*lengths), out=q) is q and torch.equal(q, want)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("spread", [1e-30, 1e-4, 30.0, 2e4])
 def test_large_and_small_queries(qs, dtype, spread):
@@ -284,6 +318,74 @@ def test_over_four_gigabytes(qs):
     ref.check(qs.kv_attention(q, cache, tables, ints(2500, 70)), want, far)
     slots = cache.slots(tables[:1], torch.arange(2500, device=DEV)[None])[0]
     assert torch.equal(qs.kv_read(cache, slots, dtype=torch.float32)[0].cpu().double(), rows[0][0])
+
+
+def test_python_refuses(qs):
+    """Types, shapes, places and gradients."""
+    cache = qs.KVCache(2, 16, 2, 64)
+    x, slots, q = torch.ones((3, 2, 64), device=DEV), ints(0, 1, 2), torch.ones((1, 4, 64), device=DEV)
+    tables, lengths = ints(0, 1).view(1, 2), ints(3)
+    write = lambda k=x, v=x, s=slots: qs.kv_write(cache, k, v, s)  # noqa: E731
+    for call, word in ((lambda: write(k=x.double()), "dtype"), (lambda: write(v=x.half()), "alike"), (lambda: write(k=x[:2]), "rows"),
+                       (lambda: write(s=slots[:2]), "rows"), (lambda: write(s=slots.long()), "int32"), (lambda: write(k=x.cpu()), "is on cpu"),
+                       (lambda: write(s=slots.cpu()), "is on cpu"), (lambda: write(v=x[:, :1]), "must be"), (lambda: write(k=x[0]), "must be"),
+                       (lambda: write(k=x.clone().requires_grad_()), "requires a gradient"),
+                       (lambda: write(v=x.clone().requires_grad_()), "requires a gradient"), (lambda: qs.kv_read(cache, slots.long()), "int32"),
+                       (lambda: qs.kv_read(cache, slots.cpu()), "is on cpu"), (lambda: qs.kv_read(cache, slots, dtype=torch.int8), "dtype")):
+        with pytest.raises(ValueError, match=word):
+            call()
+    attend = lambda q=q, t=tables, n=lengths, **k: qs.kv_attention(q, cache, t, n, **k)  # noqa: E731
+    for call, word in ((lambda: attend(q=q.double()), "dtype"), (lambda: attend(q=q[0]), "q must be"), (lambda: attend(q=q[:, :3]), "heads"),
+                       (lambda: attend(q=q[:, :0]), "heads"), (lambda: attend(q=torch.ones((1, 4, 128), device=DEV)), "heads"),
+                       (lambda: attend(q=torch.ones((1, 17, 4, 64), device=DEV)), "at most 16"), (lambda: attend(q=q.cpu()), "is on cpu"),
+                       (lambda: attend(t=tables.long()), "int32"), (lambda: attend(t=tables[0]), "int32"), (lambda: attend(t=tables.cpu()), "is on cpu"),
+                       (lambda: attend(n=lengths.long()), "int32"), (lambda: attend(n=ints(1, 2)), "1 sequences"),
+                       (lambda: attend(t=tables.view(2, 1)), "1 sequences"), (lambda: attend(window=-1), "window"),
+                       (lambda: attend(out=torch.ones((1, 4, 64), device=DEV).half()), "out must be"),
+                       (lambda: attend(out=torch.ones((1, 4, 128), device=DEV)[..., :64]), "out must be"),
+                       (lambda: attend(q=q.clone().requires_grad_()), "requires a gradient"),
+                       (lambda: attend(out=q.clone().requires_grad_()), "requires a gradient")):
+        with pytest.raises(ValueError, match=word):
+            call()
+    with pytest.raises(qs.QuantSpecError, match="query heads"):
+        attend(q=torch.ones((1, 258, 64), device=DEV))
+    with torch.no_grad():
+        write(k=x.clone().requires_grad_())
+        attend(q=q.clone().requires_grad_())
+
+
+def test_threads_share_a_cache(qs):
+    """Reads from several threads at once, each on a stream of its own: the bits of a call alone."""
+    cache = qs.KVCache(60, 16, 2, 64, "q8_0", "q4_0")
+    calls = []
+    for i, lengths in enumerate(([300], [20, 40], [5] * 8, [400, 1, 7])):
+        tables = torch.randint(0, 60, (len(lengths), 30), generator=torch.Generator().manual_seed(i)).to(DEV, torch.int32)
+        q = torch.randn((len(lengths), 6, 64), generator=torch.Generator().manual_seed(i)).to(DEV, torch.bfloat16)
+        calls.append((q, tables, ints(*lengths)))
+    k, v = ref.keys_values(960, 2, 64, torch.bfloat16, 17)
+    qs.kv_write(cache, k, v, torch.arange(960, dtype=torch.int32, device=DEV))
+    wants = [qs.kv_attention(q, cache, t, n) for q, t, n in calls]
+    torch.cuda.synchronize()
+    faults = []
+
+    def work(i):
+        try:
+            q, t, n = calls[i]
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    y = qs.kv_attention(q, cache, t, n)
+                    torch.cuda.current_stream().synchronize()
+                    if not torch.equal(y, wants[i]):
+                        faults.append(i)
+        except BaseException as e:          # noqa: BLE001 - shown by the test's own thread
+            faults.append(repr(e))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(calls))]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join(60)
+    assert not any(th.is_alive() for th in threads) and not faults, faults
 
 
 # ---- streams and graphs ----
