@@ -36,6 +36,11 @@ inline __host__ __device__ int column_tiles(const AttentionArgs& a) {
     return (a.group * a.fresh + columns_of(a) - 1) / columns_of(a);
 }
 
+// A code c of the matrix products is c 2^-code_power, for f32 queries at other bits than
+// for those of 16 bits; `once_of` times a sum of products with values' codes is the sum.
+__host__ __device__ constexpr int code_power(int bits, bool wide) { return bits == 8 ? (wide ? 21 : 24) : wide ? 18 : 22; }
+__host__ __device__ constexpr float once_of(int v_bits, bool wide) { return (float)(1 << code_power(v_bits, wide)); }
+
 // How a call's work is split, and where its workgroups leave what is joined.
 constexpr int TILE = 32;            // slots of a wave's step
 constexpr int OPENING = 2;          // steps of its waves that a workgroup takes as long to begin with another segment
@@ -48,8 +53,8 @@ struct Split {
     int32_t share;                  // workgroups of a head's and column tile's steps of a sequence, 1: they take all;
                                     // 0: they take equal runs of all steps of the call
     // of each workgroup, first for a segment that begins before it, then for one that goes on after it
-    float* parts;                   // [groups][2][columns][head size], 2^-24 of a sum relative to R
-    float2* stats;                  // [groups][2][columns]: R, sum of p
+    float* parts;                   // [groups][2][columns][head size], sums relative to the maximum, in units of once_of
+    float2* stats;                  // [groups][2][columns]: maximum, sum of p
     // Of runs: segments that more than one workgroup has, as sequence, head and column tile, first and last
     // workgroup (-1: it is one's alone). One entry for each head and column tile of a sequence where these
     // are no more than workgroups (`listed`), else one for that which goes on after each workgroup.

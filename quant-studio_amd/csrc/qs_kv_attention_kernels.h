@@ -11,16 +11,15 @@
 //
 // The scores' D has its slots where the values' P wants them (a lane: one query,
 // slots 4 g .. 4 g + 3 of both sixteens), so nothing moves between lanes. Codes go to
-// f16 without a conversion, as subnormal numbers (c 2^-24), which the matrix units
-// multiply exactly; from four-bit ones an addition takes their offset of 8 (left on, it
-// would have to come off the sums, and these would cancel).
+// f16 without a conversion, as subnormal numbers, which the matrix units take;
+// from four-bit ones an addition takes their offset of 8 (left on, it would have to come
+// off the sums, and these would cancel).
 // P is held to 21 bits or more: a query has two of the 16 columns, one takes f16(P),
-// the other f16(P - f16(P)). So that the second does not fall below f16's range, p is
-// relative to R = m - s, with m the running maximum and 2^s a power of two that takes
-// the largest step so far to just below 2^15: what is lost is under 2^-24 of the
-// largest P, mostly far under. q is rounded to f16 after its row is scaled to 2^14 ..
-// 2^15 in the same way: all of a bf16 or f16 q down to 2^-35 of the row's largest; an
-// f32 q takes two products, 22 bits.
+// the other f16(P - f16(P)). So that the second does not fall below f16's range, p counts
+// 2^s times, a power of two that takes the largest step so far to just below 2^15: what
+// is lost is under 2^-24 of the largest P, mostly far under. q is rounded to f16 after
+// its row is scaled to 2^14 .. 2^15 in the same way: all of a bf16 or f16 q down to 2^-35
+// of the row's largest; an f32 q takes two products, 22 bits.
 #pragma once
 
 #include "qs_kv_attention.h"
@@ -92,46 +91,50 @@ QS_DEV void load(Codes<N>& o, Buffer p, int at, int from) {
     for (int i = 0; i < N; i += PIECE) load_piece<PIECE>(o.w + i / 4, p, at + i, from);
 }
 
-QS_DEV uint32_t sign_and_magnitude(uint32_t w, uint32_t pick) {
-    return __builtin_amdgcn_perm(0u, w, pick) & 0x807f807fu;
+// Codes as f16, two at a time. What lies far below 2^-14 in a subnormal factor is lost in
+// the matrix units' sums, as if they took its bits where they are: with c 2^-24 for
+// four-bit codes and 2^-20 for every second, log p was off by 2.6e-6 (32 slots of 128
+// values), and 131,071 values' average by 1.4e-4 of itself. So the bits lie higher, at the
+// cost of a shift; and FINE (f32 queries) as high as they can, at that of one to two
+// instructions for each pair, where log p is off by 1.5e-7 as with an f32 product.
+template <bool FINE>
+QS_DEV uint32_t sign_and_magnitude(uint32_t twice) {        // a byte beside itself in each half
+    return FINE ? (twice & 0x80008000u) | ((twice << 3) & 0x03f803f8u) : twice & 0x807f807fu;
 }
-
-// The four-bit codes i and i + 4 of a word as f16, less 8: a subnormal number too,
-// c 2^-24 or (odd i, whose bits are not shifted down) c 2^-20.
+// the four-bit codes i and i + 4 of a word, less 8; not FINE, those of odd i count 16 times
+template <bool FINE>
 QS_DEV uint32_t four_bits(uint32_t w, int i) {
-    w = (i & 2 ? w >> 8 : w) & (i & 1 ? 0x00f000f0u : 0x000f000fu);
-    const _Float16 eight = i & 1 ? (_Float16)-0x1p-17f : (_Float16)-0x1p-21f;
+    if constexpr (FINE) w = (i == 0 ? w << 6 : i == 1 ? w << 2 : i == 2 ? w >> 2 : w >> 6) & 0x03c003c0u;
+    else w = (i & 2 ? w >> 6 : w << 2) & (i & 1 ? 0x03c003c0u : 0x003c003cu);
+    const _Float16 eight = FINE || i & 1 ? (_Float16)-0x1p-15f : (_Float16)-0x1p-19f;
     return __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2_t, w) + half2_t{eight, eight});
 }
 
-// eight codes of a key's block as f16
-template <int BITS, int BLOCKS>
+// eight codes of a key's block
+template <bool FINE, int BITS, int BLOCKS>
 QS_DEV u32x4 key_block(const Codes<BITS * BLOCKS>& c, int b) {
     u32x4 o;
-    if constexpr (BITS == 8) {
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-            o[2 * i] = sign_and_magnitude(c.w[2 * b + i], 0x01010000u);
-            o[2 * i + 1] = sign_and_magnitude(c.w[2 * b + i], 0x03030202u);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; i++) o[i] = four_bits(c.w[b], i);
+    for (int i = 0; i < 4; i++) {
+        if constexpr (BITS == 8)
+            o[i] = sign_and_magnitude<FINE>(__builtin_amdgcn_perm(0u, c.w[2 * b + (i >> 1)], i & 1 ? 0x03030202u : 0x01010000u));
+        else o[i] = four_bits<FINE>(c.w[b], i);
     }
     return o;
 }
-// code n of the slots 2 i and 2 i + 1 of four as f16
-template <int BITS, int BLOCKS>
+// code n of the slots 2 i and 2 i + 1 of four
+template <bool FINE, int BITS, int BLOCKS>
 QS_DEV uint32_t value_pair(const Codes<BITS * BLOCKS>& c, int i, int n) {
     // `run` bytes of each slot one after another: bytes `x` and `y` have the code
     constexpr int RUN = BITS * BLOCKS / 4;
     const int x = 2 * i * RUN + n * BITS / 8, y = x + RUN;
     if constexpr (BITS == 8) {
-        return __builtin_amdgcn_perm(c.w[y >> 2], c.w[x >> 2], (x & 3) * 0x00000101u + (y & 3) * 0x01010000u + 0x04040000u) & 0x807f807fu;
+        return sign_and_magnitude<FINE>(
+            __builtin_amdgcn_perm(c.w[y >> 2], c.w[x >> 2], (x & 3) * 0x00000101u + (y & 3) * 0x01010000u + 0x04040000u));
     } else {
         // the half words that have it; their codes 0 .. 3 are those from n & ~3 on
         const uint32_t hx = x & 2 ? 0x0302u : 0x0100u, hy = y & 2 ? 0x07060000u : 0x05040000u;
-        return four_bits(__builtin_amdgcn_perm(c.w[y >> 2], c.w[x >> 2], hx | hy), n & 3);
+        return four_bits<FINE>(__builtin_amdgcn_perm(c.w[y >> 2], c.w[x >> 2], hx | hy), n & 3);
     }
 }
 
@@ -202,7 +205,7 @@ QS_DEV void prepare_queries(const AttentionArgs& a, int first, int length, const
 #pragma unroll
             for (int j = 0; j < 2; j++) {
                 // where a four-bit key's code counts 16 times
-                const float v = __builtin_ldexpf(x[b][2 * i + j], K_BITS == 4 && i & 1 ? e - 4 : e);
+                const float v = __builtin_ldexpf(x[b][2 * i + j], K_BITS == 4 && !WIDE && i & 1 ? e - 4 : e);
                 h[j] = (_Float16)v;
                 if constexpr (WIDE) l[j] = (_Float16)(v - (float)h[j]);
             }
@@ -211,7 +214,7 @@ QS_DEV void prepare_queries(const AttentionArgs& a, int first, int length, const
         }
     }
     o.scale = a.scale * LOG2E;
-    o.up = 24 - e;
+    o.up = code_power(K_BITS, WIDE) - e;
     o.last = length - a.fresh + 1 + token;
     o.first = a.window > 0 && o.last > a.window ? o.last - a.window : 0;
 }
@@ -220,15 +223,17 @@ QS_DEV void prepare_queries(const AttentionArgs& a, int first, int length, const
 template <int BLOCKS>
 struct Sums {
     f32x4 acc[BLOCKS][2];               // dims 32 block + 8 g + 2 r + e at [block][e][r]
-    float top, ref, total;              // running maximum, R, sum of p
+    float top, total;                   // running maximum, sum of p; p and P count 2^power times
+    int power;
     uint32_t step;                      // the bits of all steps so far, or'ed
 };
 template <int BLOCKS>
 QS_DEV void clear(Sums<BLOCKS>& o) {
 #pragma unroll
     for (int b = 0; b < BLOCKS; b++) o.acc[b][0] = o.acc[b][1] = f32x4{0, 0, 0, 0};
-    o.top = o.ref = -__builtin_inff();
+    o.top = -__builtin_inff();
     o.total = 0.0f;
+    o.power = 0;
     o.step = 0;
 }
 
@@ -360,7 +365,7 @@ QS_DEV void attend(const AttentionArgs& a, int start, bool edge, int held, const
         steps_from(s, false, ks);
 #pragma unroll
         for (int b = 0; b < BLOCKS; b++) {
-            const u32x4 k = key_block<K_BITS, BLOCKS>(t.keys[s], b);
+            const u32x4 k = key_block<WIDE, K_BITS, BLOCKS>(t.keys[s], b);
 #pragma unroll
             for (int n = 0; n < SETS; n++) {
                 f32x4 d = mfma(k, q[n].q[b], f32x4{0, 0, 0, 0});
@@ -398,7 +403,7 @@ QS_DEV void attend(const AttentionArgs& a, int start, bool edge, int held, const
     float p[SETS][8];
 #pragma unroll
     for (int n = 0; n < SETS; n++) {
-        // the running maximum and R
+        // the running maximum and the power of two
         float top = sums[n].top;
         uint32_t steps = 0;
 #pragma unroll
@@ -415,15 +420,17 @@ QS_DEV void attend(const AttentionArgs& a, int start, bool edge, int held, const
         // largest by 15 at most, by 7 for steps below 2, which takes that much off 39 bits; a
         // subnormal step, or none, counts as 2^-14.
         const int exponent = (int)(sums[n].step >> 10 & 31), s = 29 - (exponent > 1 ? exponent : 1);
-        const float ref = top > -__builtin_inff() ? top - (float)s : -__builtin_inff();
-        const float base = top > -__builtin_inff() ? ref : 0.0f;
-        const float shrink = __builtin_amdgcn_exp2f(sums[n].ref - base);    // 0 where nothing was seen yet
+        const float base = top > -__builtin_inff() ? top : 0.0f;
+        // 0 where nothing was seen yet
+        const float shrink = __builtin_ldexpf(__builtin_amdgcn_exp2f(sums[n].top - base), s - sums[n].power);
         sums[n].top = top;
-        sums[n].ref = ref;
+        sums[n].power = s;
+        // 2^s multiplies p: in the exponent it would take bits of what is there
+        const float power = __uint_as_float((uint32_t)(127 + s) << 23);
         float total = 0.0f;
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            p[n][i] = __builtin_amdgcn_exp2f(x[n][i >> 2][i & 3] - base);
+            p[n][i] = __builtin_amdgcn_exp2f(x[n][i >> 2][i & 3] - base) * power;
             total += p[n][i];
         }
         sums[n].total = __builtin_fmaf(sums[n].total, shrink, total);
@@ -452,7 +459,7 @@ QS_DEV void attend(const AttentionArgs& a, int start, bool edge, int held, const
         for (int e = 0; e < 2; e++) {
             u32x4 c;
 #pragma unroll
-            for (int i = 0; i < 4; i++) c[i] = value_pair<V_BITS, BLOCKS>(t.values[i >> 1], i & 1, 2 * b + e);
+            for (int i = 0; i < 4; i++) c[i] = value_pair<WIDE, V_BITS, BLOCKS>(t.values[i >> 1], i & 1, 2 * b + e);
 #pragma unroll
             for (int n = 0; n < SETS; n++) sums[n].acc[b][e] = mfma(c, w[n], sums[n].acc[b][e]);
         }
@@ -462,10 +469,11 @@ QS_DEV void attend(const AttentionArgs& a, int start, bool edge, int held, const
 }
 
 // The wave's sums as one: the four lanes of a query's slots, and its two columns;
-// four-bit codes that count 16 times.
-template <int V_BITS, int BLOCKS>
+// four-bit codes that count 16 times, and p that counts 2^power times.
+template <bool SIXTEEN, int BLOCKS>
 QS_DEV void finish(Sums<BLOCKS>& o) {
-    o.total = sum_over_slots(o.total);
+    const float once = __builtin_ldexpf(1.0f, -o.power);
+    o.total = sum_over_slots(o.total) * once;
 #pragma unroll
     for (int b = 0; b < BLOCKS; b++)
 #pragma unroll
@@ -473,7 +481,7 @@ QS_DEV void finish(Sums<BLOCKS>& o) {
 #pragma unroll
             for (int r = 0; r < 4; r++) {
                 const float v = o.acc[b][e][r] + other_column(o.acc[b][e][r]);
-                o.acc[b][e][r] = V_BITS == 4 && e ? v * 0.0625f : v;
+                o.acc[b][e][r] = v * (SIXTEEN && e ? 0.0625f * once : once);
             }
 }
 
@@ -642,7 +650,7 @@ void k_kv_attention(AttentionArgs a, Split split) {
         }
 #pragma unroll
         for (int n = 0; n < SETS; n++) {
-            finish<V_BITS>(sums[n]);
+            finish<V_BITS == 4 && !WIDE>(sums[n]);
             if (lane & 8) continue;
             const int column = 8 * n + (lane & 7);
 #pragma unroll
@@ -653,7 +661,7 @@ void k_kv_attention(AttentionArgs a, Split split) {
                     *reinterpret_cast<f32x4*>(&acc[wave][column][32 * b + 8 * g + 4 * h]) =
                         f32x4{v[0][2 * h], v[1][2 * h], v[0][2 * h + 1], v[1][2 * h + 1]};
                 }
-            if (g == 0) stats[wave][column] = float2{sums[n].ref, sums[n].total};
+            if (g == 0) stats[wave][column] = float2{sums[n].top, sums[n].total};
         }
         __syncthreads();
         const bool whole = SHARE ? split.share == 1 : from == 0 && to == steps.count;
@@ -672,7 +680,7 @@ void k_kv_attention(AttentionArgs a, Split split) {
             }
             const int64_t row = row_of(a, seq, head, first + column);
             const int64_t slot = ((int64_t)blockIdx.x * 2 + (from == 0)) * COLUMNS + column;
-            const float inverse = total != 0.0f ? 0x1p24f / total : 0.0f;    // 0: it sees nothing
+            const float inverse = total != 0.0f ? once_of(V_BITS, WIDE) / total : 0.0f;    // 0: it sees nothing
 #pragma unroll
             for (int i = 0; i < BLOCKS / 2; i++) {
                 float2 v{0, 0};
