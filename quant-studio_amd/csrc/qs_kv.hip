@@ -317,6 +317,10 @@ int attention_sizes(const qs_kv_cache* cache, int64_t batch, int64_t fresh, int6
         return fail(QS_EINVAL, "tables of %lld pages of %d slots: negative, or over 2^30 slots", (long long)pages_each, a.c.page);
     if (batch * pages_each * a.c.page > INT64_C(1) << 34)
         return fail(QS_EINVAL, "%lld tables of %lld pages of %d slots: over 2^34 slots", (long long)batch, (long long)pages_each, a.c.page);
+    // workgroups may be as many: a launch has under 2^32 threads
+    if (batch * a.c.heads * ((query_heads / a.c.heads * fresh + 7) / 8) > INT64_C(1) << 25)
+        return fail(QS_EINVAL, "%lld sequences of %d heads with %lld queries each: over 2^25 eights of queries", (long long)batch,
+                    a.c.heads, (long long)(query_heads / a.c.heads * fresh));
     a.batch = (int32_t)batch;
     a.fresh = (int32_t)fresh;
     a.group = (int32_t)(query_heads / a.c.heads);

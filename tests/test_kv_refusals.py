@@ -74,13 +74,22 @@ def test_read_refuses(qs, bad, word):
 @pytest.mark.parametrize("bad,word", [
     (dict(t=5), b"query type"), (dict(b=-1), b"sequences"), (dict(b=(1 << 14) + 1), b"sequences"), (dict(n=17), b"new tokens"),
     (dict(n=-1), b"new tokens"), (dict(hq=3), b"query heads"), (dict(hq=0), b"query heads"), (dict(hq=258), b"query heads"),
-    (dict(m=-1), b"tables"), (dict(m=1 << 27, ts=1 << 27), b"2^30"), (dict(b=1 << 12, m=1 << 20, ts=1 << 20), b"2^34"), (dict(window=-1), b"window"), (dict(q=None), b"null"),
+    (dict(m=-1), b"tables"), (dict(m=1 << 27, ts=1 << 27), b"2^30"), (dict(b=1 << 12, m=1 << 20, ts=1 << 20), b"2^34"), (dict(b=1 << 14, hq=256, n=16), b"2^25"),
+    (dict(window=-1), b"window"), (dict(q=None), b"null"),
     (dict(tables=None), b"null"), (dict(lengths=None), b"null"), (dict(out=None), b"null"), (dict(q=72), b"aligned"),
     (dict(out=72), b"aligned"), (dict(tables=66), b"aligned"), (dict(qs=496), b"token stride"), (dict(qs=520), b"token stride"),
     (dict(qs=1 << 62), b"2^62-byte span"), (dict(ts=2), b"table stride"), (dict(ts=1 << 60), b"2^62-byte span"), (dict(size=1023), b"out holds")])
 def test_attention_refuses(qs, bad, word):
     L = qs.library()
     assert attention(L, cache(), **bad) == -22 and word in L.qs_last_error(), L.qs_last_error()
+
+
+def test_attention_refuses_more_workgroups_than_a_launch_has(qs):
+    L = qs.library()
+    c = cache(heads=1024)
+    assert attention(L, c, hq=4096, b=1 << 14, n=16, qs=1 << 20) == -22 and b"2^25" in L.qs_last_error()
+    assert L.qs_kv_attention_workspace(c, 1 << 14, 16, 4096, 3) == -22
+    assert L.qs_kv_attention_workspace(c, 1 << 14, 2, 4096, 3) == 0
 
 
 def test_attention_refuses_workspaces(qs):
