@@ -538,7 +538,7 @@ QS_DEV Deal deal(const AttentionArgs& a, int groups, int waves, int opening, int
     const int run = __builtin_ctzll(__ballot(at < scan));       // the lane whose run it is in
     d.seq = run * each_lane;
     d.base = __builtin_amdgcn_readlane(scan - sum, run);
-    for (int n = units_of(a, opening, d.seq); at >= d.base + n; n = units_of(a, opening, d.seq)) {
+    for (int n = units_of(a, opening, d.seq); at >= d.base + n && d.seq + 1 < a.batch; n = units_of(a, opening, d.seq)) {
         d.base += n;
         d.seq++;
     }
@@ -578,7 +578,7 @@ void k_kv_attention(AttentionArgs a, Split split) {
         base = d.base;
     }
     const int64_t begin = at;
-    while (at < end) {
+    while (at < end && seq < a.batch) {
         int length = constant(a.lengths)[seq];
         Steps steps{};
         int to = 0;                                 // from .. to - 1 of them

@@ -25,8 +25,9 @@ __global__ __launch_bounds__(THREADS) void k_kv_join(AttentionArgs a, Split spli
         const int heads = a.c.heads * tiles, seq = (int)blockIdx.x / heads, first = (int)blockIdx.x * split.share;
         s = int4{seq, (int)blockIdx.x - seq * heads, first, first + split.share - 1};
     } else {
+        // all of them within bounds, unless lengths changed meanwhile
         s = split.segments[blockIdx.x];
-        if (s.w < 0) return;
+        if ((unsigned)s.x >= (unsigned)a.batch || (unsigned)s.y >= (unsigned)(a.c.heads * tiles) || s.z < 0 || s.w < s.z || s.w >= split.groups) return;
     }
     const int head = s.y / tiles;
     const int64_t row = row_of(a, s.x, head, (s.y - head * tiles) * columns + column);
