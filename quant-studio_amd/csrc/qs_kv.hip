@@ -360,13 +360,25 @@ int cache_of(const qs_kv_cache* cache, Cache& c) {
 
 Split split_of(const AttentionArgs& a, void* workspace) {
     // As many workgroups of four waves as the GPU holds at a time, unless even the
-    // longest sequences would not give each a step for every wave. Sequences of a few
-    // steps at most are not split; those of one are in equal parts, which each workgroup
-    // knows before it knows the length; more of them are in equal runs of all their
-    // steps, since the longest may be of any share. Where there are more segments than
-    // workgroups, waves take them by themselves: opening one is most of what a short one
-    // takes; and as a whole, where the longest cannot take much longer than all together.
+    // longest sequences would not give each a step for every wave.
+    //
+    // Sequences of `whole` steps at most are not split: one segment to a workgroup, so that
+    // nothing is joined. Of 8 heads of 128 in 8 bits: 8 sequences of 600 slots take 10.9 us,
+    // 13.0 split, 40 take 17.8, 23.7 split, 150 take 47, 56 split (ragged ones 36, 33 split);
+    // of 900 slots 40 ragged ones 16.0 and 20.5, but 150 take 48.6 and 38.2. A lone one of
+    // 290 slots takes 7.7, 8.2 split, of 420 slots 8.9 and 8.6.
+    //
+    // A lone sequence is in equal parts, which each workgroup knows before it knows the
+    // length; more of them are in equal runs of all their steps, since the longest may be of
+    // any share.
+    //
+    // Where there are more segments than workgroups, waves take them by themselves: opening
+    // one is most of what a short one takes (700 ragged sequences of 250 slots: 43.7 us, 56.8
+    // with four waves to each; 8 of 500 slots, with fewer: 13.8, and 12.5 with four). They
+    // take them as a whole, where the longest cannot take much longer than all together (600
+    // of 1,200 slots: 319 us, 356 split).
     constexpr int64_t CUS = 256, FEW = 8;
+    const int64_t whole = a.batch > 1 ? 24 : 12;
     const int64_t steps = ((int64_t)a.pages_each * a.c.page + TILE - 1) / TILE;
     const int64_t segments = (int64_t)a.batch * a.c.heads * column_tiles(a);
     const int64_t full = CUS * resident(a.c.blocks, columns_of(a), a.type == QS_SRC_F32);
@@ -374,7 +386,7 @@ Split split_of(const AttentionArgs& a, void* workspace) {
     if (a.batch == 0 || a.fresh == 0) return s;
     s.waves = segments > (steps <= FEW ? 1 : 2) * full && a.batch > 1 ? 1 : 4;
     const int64_t held = full * (4 / s.waves);
-    if (steps <= FEW || (s.waves == 1 && steps <= FEW * (1 + segments / held))) {
+    if (steps <= whole || (s.waves == 1 && steps <= whole * (1 + segments / held))) {
         s.share = 1;
     } else if (a.batch == 1) {
         const int64_t share = full / segments, most = (steps + s.waves - 1) / s.waves;
