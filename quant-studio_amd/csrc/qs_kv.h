@@ -61,13 +61,6 @@ QS_DEV int step_at(const Cache& c, int slot, bool value, int block) {
            2 * (((slot >> 2) * 8 + (value ? 4 : 0) + (slot & 3)) * c.blocks + block);
 }
 
-// the f32 value of an eight-bit code (sign and magnitude) and of a four-bit one
-QS_DEV float code8(uint32_t b) {
-    const float m = (float)(b & 127u);
-    return b & 128u ? -m : m;
-}
-QS_DEV float code4(uint32_t n) { return (float)((int)(n & 15u) - 8); }
-
 QS_DEV float half_of(uint32_t bits) { return (float)__builtin_bit_cast(_Float16, (uint16_t)bits); }
 
 }  // namespace qskv

@@ -28,8 +28,11 @@ struct RowsArgs {
 
 // the eight values of a thread: a quarter of a block, keys or values
 struct Unit {
-    int head, block, quarter;
+    int head, block, quarter, bits;
     bool value;
+    int codes, step;            // bytes in a page of the first slot's: its codes, its step
+    int four, one, step_four;   // bytes to the slot four on, to the next of four
+    int pair;                   // values: bytes between its four units of two codes
 };
 QS_DEV Unit unit_of(const Cache& c, int u) {
     const int per_head = 4 * c.blocks;
@@ -40,15 +43,28 @@ QS_DEV Unit unit_of(const Cache& c, int u) {
     u -= o.head * per_head;
     o.block = u >> 2;
     o.quarter = u & 3;
+    o.bits = o.value ? c.v_bits : c.k_bits;
+    const int head = (int)__umul24(o.head, c.page * qskv::slot_bytes(c.k_bits, c.v_bits, c.blocks));
+    const auto at = [&](int slot) {
+        return o.value ? qskv::v_unit(c, slot, 4 * o.quarter, o.block) : qskv::k_unit(c, slot, o.quarter, o.block);
+    };
+    o.codes = head + at(0);
+    o.four = at(4) - at(0);
+    o.one = at(1) - at(0);
+    o.pair = qskv::v_unit(c, 0, 1, 0) - qskv::v_unit(c, 0, 0, 0);
+    o.step = head + qskv::step_at(c, 0, o.value, o.block);
+    o.step_four = qskv::step_at(c, 4, false, 0) - qskv::step_at(c, 0, false, 0);
     return o;
 }
-// where a slot's page has the unit's head, and the slot in the page
+// where the unit of a slot has its codes and its step
 struct Place {
-    uint8_t* head;
-    int slot;
+    uint8_t *codes, *step;
 };
 QS_DEV Place place_of(const Cache& c, const Unit& u, int slot) {
-    return {qskv::head_of(c, slot >> c.shift, u.head), slot & (c.page - 1)};
+    uint8_t* page = c.data + (uint64_t)(uint32_t)(slot >> c.shift) * (uint32_t)c.page_bytes;
+    const uint32_t in = (uint32_t)slot & (uint32_t)(c.page - 1), fours = in >> 2, rest = in & 3;
+    return {page + (u.codes + __umul24(fours, u.four) + __umul24(rest, u.one)),
+            page + (u.step + __umul24(fours, u.step_four) + __umul24(rest, 2 * c.blocks))};
 }
 
 // How threads are laid over rows: `wide` of them (whole heads' keys or values, so
@@ -71,36 +87,100 @@ __host__ __device__ inline Shape shape_of(int units, int blocks) {
     return s;
 }
 
-// codes of eight values as the cache holds them, their block's step; four threads hold a block
-QS_DEV float codes_of(const float (&x)[8], int bits, int quarter, uint32_t (&code)[8]) {
-    if (bits == 8) {
-        float top = 0.0f;
+// a byte of a word from the whole part of f: 0 of a negative one and of NaN, 255 above
+template <int AT>
+QS_DEV uint32_t byte_of(float f, uint32_t w) {
+    return __builtin_amdgcn_cvt_pk_u8_f32(__builtin_truncf(f), AT, w);
+}
+// 1 / d of a step that f16 holds, correctly rounded: one step of Newton's method on the
+// hardware's reciprocal, which is as good from 2^-60 to 2^60 (every f32 of them compared
+// with the division, which takes twice the instructions). The codes of smaller steps
+// stand for zeros, those of larger ones for no values, whatever they are.
+QS_DEV float inverse_of(float d) {
+    const float y = __builtin_amdgcn_rcpf(d);
+    return __builtin_fmaf(__builtin_fmaf(-d, y, 1.0f), y, y);
+}
+// m / 127, correctly rounded (compared likewise): the product with 1 / 127 and what it is off by
+QS_DEV float of_127(float m) {
+    const float q = m * (1.0f / 127.0f);
+    return __builtin_fmaf(__builtin_fmaf(-127.0f, q, m), 1.0f / 127.0f, q);
+}
+
+// largest magnitude of a block as f32 bits, a NaN above all
+template <int SRC>
+QS_DEV float top_of(const Eight<SRC>& in, const float (&x)[8]) {
+    uint32_t m;
+    if constexpr (SRC == qs::SRC_F32) {
+        m = 0;
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const float m = fabsf(x[j]);
-            top = m > top || m != m ? m : top;      // keeps a NaN
-        }
-        const float m1 = qs::quad_xor<1>(top);
-        top = m1 > top || m1 != m1 ? m1 : top;
-        const float m2 = qs::quad_xor<2>(top);
-        top = m2 > top || m2 != m2 ? m2 : top;
-        const float d = top / 127.0f;
-        const float id = d != 0.0f ? 1.0f / d : 0.0f;
+        for (int j = 0; j < 8; j++) m = max(m, __float_as_uint(x[j]) & 0x7fffffffu);
+    } else {
+        // the order of the 16-bit types' magnitudes is that of their bits
+        using u16x2 = uint16_t __attribute__((ext_vector_type(2)));
+        u16x2 h = __builtin_bit_cast(u16x2, in.w[0][0] & 0x7fff7fffu);
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            // Half away from zero, of the magnitude: m + the largest f32 below 0.5 passes
-            // a whole number exactly where m + 0.5 does (m + 0.5 itself would also take
-            // 0.5's predecessor to 1). Over 127 only with steps below f16's smallest,
-            // which are 0.
-            const uint32_t m = (uint32_t)fminf(fabsf(x[j] * id) + 0x1.fffffep-2f, 127.0f);
-            code[j] = m | (__float_as_uint(x[j]) >> 31) << 7;
-        }
+        for (int j = 1; j < 4; j++) h = __builtin_elementwise_max(h, __builtin_bit_cast(u16x2, in.w[0][j] & 0x7fff7fffu));
+        m = max((uint32_t)h[0], (uint32_t)h[1]);
+    }
+    m = max(m, qs::quad_xor<1>(m));
+    m = max(m, qs::quad_xor<2>(m));
+    if constexpr (SRC == qs::SRC_F16) return (float)__builtin_bit_cast(_Float16, (uint16_t)m);
+    return __uint_as_float(SRC == qs::SRC_BF16 ? m << 16 : m);
+}
+// the value of the largest magnitude, the first of them, a NaN above all
+template <int SRC>
+QS_DEV float peak_of(const float (&x)[8], int quarter) {
+    if constexpr (SRC == qs::SRC_F32) return qs::quad_absmax_first(x, quarter);
+    // The f32 bits of 16-bit types end in 13 zeros at least: turned left by one, the
+    // sign is last, and between it and the magnitude is room for the place, first ones above.
+    const uint32_t place = (uint32_t)(31 - 8 * quarter) << 1;
+    uint32_t key = 0;
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        const uint32_t b = __float_as_uint(x[j]);
+        key = max(key, __builtin_rotateleft32(b, 1) | (place - 2 * j));
+    }
+    key = max(key, qs::quad_xor<1>(key));
+    key = max(key, qs::quad_xor<2>(key));
+    return __uint_as_float(__builtin_rotateright32(key & ~0x3eu, 1));
+}
+
+// Codes of eight values as the cache holds them, and their block's step, which four
+// threads find together: eight bits as two words of four codes each; four bits as a
+// word of four pairs, a key's (0, 2) (4, 6) (1, 3) (5, 7), a value's (0, 1) (2, 3) ...
+template <int SRC>
+QS_DEV float codes_of(const Eight<SRC>& in, const Unit& u, uint32_t (&code)[2]) {
+    float x[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) x[j] = value8<SRC>(in, j);
+    if (u.bits == 8) {
+        const float d = of_127(top_of<SRC>(in, x)), id = inverse_of(d);
+        // Half away from zero, of the magnitude: m + the largest f32 below 0.5 passes a
+        // whole number exactly where m + 0.5 does (m + 0.5 itself would also take 0.5's
+        // predecessor to 1). Over 127 only where the codes do not matter.
+        const auto four = [&](int j) {
+            const auto of = [&](int e) { return fabsf(x[j + e] * id) + 0x1.fffffep-2f; };
+            const uint32_t w = byte_of<3>(of(3), byte_of<2>(of(2), byte_of<1>(of(1), byte_of<0>(of(0), 0))));
+            const auto high = [&](int e) { return __float_as_uint(x[j + e]); };
+            const uint32_t low2 = __builtin_amdgcn_perm(high(1), high(0), 0x0c0c0703u);
+            const uint32_t signs = __builtin_amdgcn_perm(high(3), high(2), 0x07030c0cu) | low2;
+            return w | (signs & 0x80808080u);
+        };
+        code[0] = four(0);
+        code[1] = four(4);
         return d;
     }
-    const float d = qs::quad_absmax_first(x, quarter) * -0.125f;
-    const float id = d != 0.0f ? 1.0f / d : 0.0f;
-#pragma unroll
-    for (int j = 0; j < 8; j++) code[j] = qs::level_of(x[j], id, 8.5f, 15.5f);
+    const float d = peak_of<SRC>(x, u.quarter) * -0.125f, id = inverse_of(d);
+    const auto level = [&](int j) { return fminf(x[j] * id + 8.5f, 15.5f); };
+    uint32_t low, high;
+    if (u.value) {
+        low = byte_of<3>(level(6), byte_of<2>(level(4), byte_of<1>(level(2), byte_of<0>(level(0), 0))));
+        high = byte_of<3>(level(7), byte_of<2>(level(5), byte_of<1>(level(3), byte_of<0>(level(1), 0))));
+    } else {
+        low = byte_of<3>(level(5), byte_of<2>(level(1), byte_of<1>(level(4), byte_of<0>(level(0), 0))));
+        high = byte_of<3>(level(7), byte_of<2>(level(3), byte_of<1>(level(6), byte_of<0>(level(2), 0))));
+    }
+    code[0] = low | high << 4;
     return d;
 }
 
@@ -122,7 +202,6 @@ __global__ __launch_bounds__(256) void k_kv_write(RowsArgs a) {
     const void* src = u.value ? a.v : a.k;
     const int64_t stride = u.value ? a.v_stride : a.k_stride;
     const int64_t from = (int64_t)u.head * 32 * a.c.blocks + 32 * u.block + 8 * u.quarter;
-    const int bits = u.value ? a.c.v_bits : a.c.k_bits;
     // The slots of the workgroup's rows and of all later ones, which a launch has few
     // enough of for one turn, then the rows' values: all are on their way before
     // anything waits, and the slots are compared meanwhile.
@@ -153,14 +232,30 @@ __global__ __launch_bounds__(256) void k_kv_write(RowsArgs a) {
     }
     __syncthreads();
     if (a.rows - first > 1) {
+        // most often the later slots are all outside the range of the workgroup's own
+        uint32_t low = ~0u, high = 0, near = ~0u;
+        for (int i = 0; i < count; i++) {
+            const int m = mine[i];
+            low = min(low, (uint32_t)m);
+            high = (uint32_t)max((int)high, m);
+        }
+#pragma unroll
+        for (int j = 0; j < TURNS; j++) {
+            if (first + count + FEW_ROWS * j >= a.rows) break;
+#pragma unroll
+            for (int e = 0; e < 4; e++) near = min(near, (uint32_t)later[j][e] - low);
+        }
+        const bool any = near <= high - low;
         for (int i = 0; i < count; i++) {
             const int m = mine[i];
             bool same = (int)threadIdx.x > i && s0 == m;
+            if (any) {
 #pragma unroll
-            for (int j = 0; j < TURNS; j++) {
-                if (first + count + FEW_ROWS * j >= a.rows) break;
+                for (int j = 0; j < TURNS; j++) {
+                    if (first + count + FEW_ROWS * j >= a.rows) break;
 #pragma unroll
-                for (int e = 0; e < 4; e++) same |= later[j][e] == m;
+                    for (int e = 0; e < 4; e++) same |= later[j][e] == m;
+                }
             }
             if (same) replaced[i] = 1;
         }
@@ -171,36 +266,22 @@ __global__ __launch_bounds__(256) void k_kv_write(RowsArgs a) {
         const int row = sub + i * shape.together;
         const int slot = live && row < count && !replaced[row] ? mine[row] : -1;
         if (slot < 0) continue;     // the same for the four threads of a block
-        float x[8];
-#pragma unroll
-        for (int j = 0; j < 8; j++) x[j] = value8<SRC>(in[i], j);
-        uint32_t code[8];
-        const float d = codes_of(x, bits, u.quarter, code);
+        uint32_t code[2];
+        const float d = codes_of<SRC>(in[i], u, code);
         const Place p = place_of(a.c, u, slot);
         // a step that f16 cannot hold, like a NaN or an infinity in the block, stands for no values
         const uint32_t h = qs::f16_bits(d);
-        if (u.quarter == 0)
-            *reinterpret_cast<uint16_t*>(p.head + qskv::step_at(a.c, p.slot, u.value, u.block)) =
-                (uint16_t)((h & 0x7fffu) < 0x7c00u ? h : 0x7e00u);
+        if (u.quarter == 0) *reinterpret_cast<uint16_t*>(p.step) = (uint16_t)((h & 0x7fffu) < 0x7c00u ? h : 0x7e00u);
         if (!u.value) {
-            uint8_t* o = p.head + qskv::k_unit(a.c, p.slot, u.quarter, u.block);
-            if (bits == 8) {
-                uint32_t w[2];
-                qs::bytes_of(code, w);
-                *reinterpret_cast<uint2*>(o) = uint2{w[0], w[1]};
-            } else {
-                uint32_t w = 0;
+            if (u.bits == 8) *reinterpret_cast<uint2*>(p.codes) = uint2{code[0], code[1]};
+            else *reinterpret_cast<uint32_t*>(p.codes) = code[0];
+        } else if (u.bits == 8) {
 #pragma unroll
-                for (int j = 0; j < 8; j++) w |= code[j] << (4 * (j >> 1) + 16 * (j & 1));
-                *reinterpret_cast<uint32_t*>(o) = w;
-            }
+            for (int j = 0; j < 4; j++)
+                *reinterpret_cast<uint16_t*>(p.codes + j * u.pair) = (uint16_t)(code[j >> 1] >> (16 * (j & 1)));
         } else {
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                uint8_t* o = p.head + qskv::v_unit(a.c, p.slot, 4 * u.quarter + j, u.block);
-                if (bits == 8) *reinterpret_cast<uint16_t*>(o) = (uint16_t)(code[2 * j] | code[2 * j + 1] << 8);
-                else *o = (uint8_t)(code[2 * j] | code[2 * j + 1] << 4);
-            }
+            for (int j = 0; j < 4; j++) p.codes[j * u.pair] = (uint8_t)(code[0] >> (8 * j));
         }
     }
 }
@@ -220,7 +301,6 @@ __global__ __launch_bounds__(256) void k_kv_read(RowsArgs a) {
     const Unit u = unit_of(a.c, at);
     void* dst = u.value ? a.v : a.k;
     const int64_t stride = u.value ? a.v_stride : a.k_stride;
-    const int bits = u.value ? a.c.v_bits : a.c.k_bits;
     int slot[TIMES];
 #pragma unroll
     for (int i = 0; i < TIMES; i++) {
@@ -235,20 +315,19 @@ __global__ __launch_bounds__(256) void k_kv_read(RowsArgs a) {
         step[i] = 0;
         if ((unsigned)slot[i] >= (unsigned)slots) continue;
         const Place p = place_of(a.c, u, slot[i]);
-        step[i] = *reinterpret_cast<const uint16_t*>(p.head + qskv::step_at(a.c, p.slot, u.value, u.block));
+        step[i] = *reinterpret_cast<const uint16_t*>(p.step);
         if (!u.value) {
-            const uint8_t* o = p.head + qskv::k_unit(a.c, p.slot, u.quarter, u.block);
-            if (bits == 8) {
-                const uint2 c = *reinterpret_cast<const uint2*>(o);
+            if (u.bits == 8) {
+                const uint2 c = *reinterpret_cast<const uint2*>(p.codes);
                 w[i][0] = c.x, w[i][1] = c.y;
             } else {
-                w[i][0] = *reinterpret_cast<const uint32_t*>(o);
+                w[i][0] = *reinterpret_cast<const uint32_t*>(p.codes);
             }
         } else {
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                const uint8_t* o = p.head + qskv::v_unit(a.c, p.slot, 4 * u.quarter + j, u.block);
-                w[i][j] = bits == 8 ? *reinterpret_cast<const uint16_t*>(o) : *o;
+                const uint8_t* o = p.codes + j * u.pair;
+                w[i][j] = u.bits == 8 ? *reinterpret_cast<const uint16_t*>(o) : *o;
             }
         }
     }
@@ -256,16 +335,24 @@ __global__ __launch_bounds__(256) void k_kv_read(RowsArgs a) {
     for (int i = 0; i < TIMES; i++) {
         const int row = sub + i * shape.together;
         if (row >= count) break;
-        float x[8] = {};
-        if ((unsigned)slot[i] < (unsigned)slots) {
-            const float d = qskv::half_of(step[i]);
+        // Codes go through f16 two at a time, as subnormals c 2^-24, and c d is exact in
+        // f32: a magnitude of 7 bits times a step of 11. Of a slot outside all is 0.
+        const float d = qskv::half_of(step[i]), large = d * 0x1p24f;
+        const float less = u.bits == 8 ? 0.0f : -8.0f * d;
+        float x[8];
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const uint32_t c = u.value ? w[i][j >> 1] >> (bits * (j & 1))
-                                   : bits == 8 ? w[i][j >> 2] >> (8 * (j & 3))
-                                               : w[i][0] >> (4 * (j >> 1) + 16 * (j & 1));
-                x[j] = (bits == 8 ? qskv::code8(c) : qskv::code4(c)) * d;
+        for (int j = 0; j < 4; j++) {
+            uint32_t two;
+            if (u.bits == 8) {
+                const uint32_t c = u.value ? w[i][j] : w[i][j >> 1];
+                two = __builtin_amdgcn_perm(0, c, u.value || j % 2 == 0 ? 0x01010000u : 0x03030202u) & 0x807f807fu;
+            } else {
+                two = (u.value ? w[i][j] | w[i][j] << 12 : w[i][0] >> (4 * j)) & 0x000f000fu;
             }
+            using f16x2 = _Float16 __attribute__((ext_vector_type(2)));
+            const f16x2 h = __builtin_bit_cast(f16x2, two);
+            x[2 * j] = __builtin_fmaf((float)h[0], large, less);
+            x[2 * j + 1] = __builtin_fmaf((float)h[1], large, less);
         }
         store8<DST, true>(dst, (first + row) * stride + (int64_t)u.head * 32 * a.c.blocks + 32 * u.block + 8 * u.quarter, x);
     }

@@ -36,6 +36,12 @@ QS_DEV float value8(const Eight<SRC>& o, int i) {
 QS_DEV uint32_t bf16_bits(float f) {
     return (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)f);
 }
+// two of them, the first in the low half: one instruction
+QS_DEV uint32_t bf16_pair(float lo, float hi) {
+    using f32x2 = float __attribute__((ext_vector_type(2)));
+    using bf16x2 = __bf16 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{lo, hi}, bf16x2));
+}
 template <int DST>
 QS_DEV uint32_t bits16(float f) {
     if constexpr (DST == qs::SRC_BF16) return bf16_bits(f);
@@ -57,7 +63,10 @@ QS_DEV void store8(void* p, int64_t at, const float (&v)[8]) {
     } else {
         u32x4 o;
 #pragma unroll
-        for (int i = 0; i < 4; i++) o[i] = bits16<DST>(v[2 * i]) | (bits16<DST>(v[2 * i + 1]) << 16);
+        for (int i = 0; i < 4; i++) {
+            if constexpr (DST == qs::SRC_BF16) o[i] = bf16_pair(v[2 * i], v[2 * i + 1]);
+            else o[i] = bits16<DST>(v[2 * i]) | (bits16<DST>(v[2 * i + 1]) << 16);
+        }
         put(0, o);
     }
 }
