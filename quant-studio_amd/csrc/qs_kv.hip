@@ -23,7 +23,9 @@ struct RowsArgs {
     int64_t k_stride, v_stride;     // between rows, in values
     const int32_t* slots;
     int32_t rows, units;            // units: of eight values in a row's keys and values
-    int32_t group;                  // rows of a workgroup
+    int32_t group;                  // rows of a workgroup at a time
+    int32_t wide, together;         // threads on a row, rows at a time
+    uint32_t per_wide, per_block;   // 2^20 / wide and 2^18 / blocks, rounded up: threads and units divide by them
 };
 
 // the eight values of a thread: a quarter of a block, keys or values
@@ -34,27 +36,39 @@ struct Unit {
     int four, one, step_four;   // bytes to the slot four on, to the next of four
     int pair;                   // values: bytes between its four units of two codes
 };
-QS_DEV Unit unit_of(const Cache& c, int u) {
-    const int per_head = 4 * c.blocks;
+QS_DEV Unit unit_of(const RowsArgs& a, uint32_t u) {
+    const Cache& c = a.c;
+    const uint32_t blocks = (uint32_t)c.blocks, of_keys = __umul24(4 * blocks, c.heads);
     Unit o;
-    o.value = u >= per_head * c.heads;
-    u -= o.value ? per_head * c.heads : 0;
-    o.head = u / per_head;
-    u -= o.head * per_head;
-    o.block = u >> 2;
-    o.quarter = u & 3;
+    o.value = u >= of_keys;
+    u -= o.value ? of_keys : 0;
+    o.quarter = (int)(u & 3);
+    o.head = (int)(__umul24(u >> 2, a.per_block) >> 18);
+    o.block = (int)((u >> 2) - __umul24(o.head, blocks));
     o.bits = o.value ? c.v_bits : c.k_bits;
-    const int head = (int)__umul24(o.head, c.page * qskv::slot_bytes(c.k_bits, c.v_bits, c.blocks));
-    const auto at = [&](int slot) {
-        return o.value ? qskv::v_unit(c, slot, 4 * o.quarter, o.block) : qskv::k_unit(c, slot, o.quarter, o.block);
-    };
-    o.codes = head + at(0);
-    o.four = at(4) - at(0);
-    o.one = at(1) - at(0);
-    o.pair = qskv::v_unit(c, 0, 1, 0) - qskv::v_unit(c, 0, 0, 0);
-    o.step = head + qskv::step_at(c, 0, o.value, o.block);
-    o.step_four = qskv::step_at(c, 4, false, 0) - qskv::step_at(c, 0, false, 0);
+    const uint32_t head = __umul24(o.head, c.page * qskv::slot_bytes(c.k_bits, c.v_bits, c.blocks));
+    // the layout's distances: a slot's keys take 4 runs and its values one of a quarter of theirs
+    const uint32_t run = __umul24(blocks, o.bits);
+    o.codes = (int)head + (o.value ? qskv::v_unit(c, 0, 4 * o.quarter, o.block) : qskv::k_unit(c, 0, o.quarter, o.block));
+    o.four = 16 * run;
+    o.one = o.value ? run >> 2 : 4 * run;
+    o.pair = (int)run;
+    o.step = (int)head + qskv::step_at(c, 0, o.value, o.block);
+    o.step_four = 16 * blocks;
     return o;
+}
+// The rows of keys or of values. Both are read first: the compiler would choose
+// between their addresses, and load what it chose with a wait of its own.
+struct Side {
+    void* data;
+    int64_t stride;
+};
+QS_DEV Side side_of(const RowsArgs& a, bool value) {
+    using Global = __attribute__((address_space(1))) void*;
+    Global k = (Global)a.k, v = (Global)a.v;
+    int64_t k_stride = a.k_stride, v_stride = a.v_stride;
+    asm("" : "+s"(k), "+s"(v), "+s"(k_stride), "+s"(v_stride));
+    return {(void*)(value ? v : k), value ? v_stride : k_stride};
 }
 // where the unit of a slot has its codes and its step
 struct Place {
@@ -67,22 +81,23 @@ QS_DEV Place place_of(const Cache& c, const Unit& u, int slot) {
             page + (u.step + __umul24(fours, u.step_four) + __umul24(rest, 2 * c.blocks))};
 }
 
-// How threads are laid over rows: `wide` of them (whole heads' keys or values, so
-// at most 256 and a multiple of a head's units) on one row, `together` rows at a
-// time, BATCH times over.
-constexpr int BATCH = 4, MOST_GROUP = 4 * 16;
-// rows of a launch that writes: what a workgroup looks its slots up among
-constexpr int64_t MOST_ROWS = 8192;
+// How threads are laid over rows: `wide` of them (whole heads' keys or values, so at
+// most all and a multiple of a head's units) on one row, `together` rows at a time,
+// BATCH times over.
+constexpr int BATCH = 4;
 // calls of no more rows take one at a time: more workgroups
 constexpr int FEW_ROWS = 1024;
+// rows of a launch that writes: what a workgroup looks its slots up among, a turn of four for each thread
+constexpr int64_t MOST_ROWS = 8192;
+constexpr int WRITERS = 1024;       // threads of a workgroup that writes many rows
 struct Shape {
     int wide, together, columns;    // columns: workgroups for a row
 };
-__host__ __device__ inline Shape shape_of(int units, int blocks) {
-    const int most = 256 / (4 * blocks) * (4 * blocks);
+__host__ __device__ inline Shape shape_of(int units, int blocks, int threads) {
+    const int most = threads / (4 * blocks) * (4 * blocks);
     Shape s;
     s.wide = units < most ? units : most;
-    s.together = 256 / s.wide;
+    s.together = threads / s.wide;
     s.columns = (units + s.wide - 1) / s.wide;
     return s;
 }
@@ -189,31 +204,34 @@ QS_DEV float codes_of(const Eight<SRC>& in, const Unit& u, uint32_t (&code)[2]) 
 // Of rows with the same slot the last is written: every workgroup looks its rows'
 // slots up among all later ones, which a launch's few rows make cheap.
 template <int SRC, bool MANY>
-__global__ __launch_bounds__(256) void k_kv_write(RowsArgs a) {
-    __shared__ int mine[MOST_GROUP], replaced[MOST_GROUP];
-    const Shape shape = shape_of(a.units, a.c.blocks);
+__global__ __launch_bounds__(MANY ? WRITERS : 256) void k_kv_write(RowsArgs a) {
+    constexpr int THREADS = MANY ? WRITERS : 256, TIMES = MANY ? BATCH : 1;
+    constexpr int TURN = 4 * THREADS, TURNS = MANY ? (int)(MOST_ROWS / TURN) : FEW_ROWS / TURN;
+    constexpr int MOST_GROUP = TIMES * THREADS / 16;       // a row has 16 units at least
+    __shared__ __attribute__((aligned(16))) int mine[MOST_GROUP];
+    __shared__ int replaced[MOST_GROUP];
     const int first = (int)blockIdx.x * a.group;
     const int count = a.rows - first < a.group ? a.rows - first : a.group;
     const int slots = a.c.pages << a.c.shift;
-    const int sub = (int)threadIdx.x / shape.wide;
-    const int at = (int)blockIdx.y * shape.wide + ((int)threadIdx.x - sub * shape.wide);
-    const bool live = sub < shape.together && at < a.units;
-    const Unit u = unit_of(a.c, live ? at : 0);
-    const void* src = u.value ? a.v : a.k;
-    const int64_t stride = u.value ? a.v_stride : a.k_stride;
-    const int64_t from = (int64_t)u.head * 32 * a.c.blocks + 32 * u.block + 8 * u.quarter;
+    const int sub = (int)(__umul24(threadIdx.x, a.per_wide) >> 20);
+    const int at = (int)blockIdx.y * a.wide + ((int)threadIdx.x - (int)__umul24(sub, a.wide));
+    const bool live = sub < a.together && at < a.units;
+    const Unit u = unit_of(a, live ? at : 0);
+    const Side src = side_of(a, u.value);
+    const int64_t from = first * src.stride + (__umul24(u.head, 32 * a.c.blocks) + 32 * u.block + 8 * u.quarter);
+    const int64_t next = a.together * src.stride;
+    int64_t from_row = from + sub * src.stride;
     // The slots of the workgroup's rows and of all later ones, which a launch has few
     // enough of for one turn, then the rows' values: all are on their way before
     // anything waits, and the slots are compared meanwhile.
     const int s0 = (int)threadIdx.x < count ? a.slots[first + threadIdx.x] : -1;
-    constexpr int TIMES = MANY ? BATCH : 1, TURNS = MANY ? (int)(MOST_ROWS / FEW_ROWS) : 1;
     int later[TURNS][4];
 #pragma unroll
     for (int j = 0; j < TURNS; j++) {
 #pragma unroll
         for (int e = 0; e < 4; e++) later[j][e] = -1;
-        if (first + count + FEW_ROWS * j >= a.rows) continue;       // the same for all
-        const int r = first + count + FEW_ROWS * j + 4 * (int)threadIdx.x;
+        if (first + count + TURN * j >= a.rows) continue;       // the same for all
+        const int r = first + count + TURN * j + 4 * (int)threadIdx.x;
         if (r + 3 < a.rows) __builtin_memcpy(later[j], a.slots + r, 16);
         else
 #pragma unroll
@@ -223,10 +241,12 @@ __global__ __launch_bounds__(256) void k_kv_write(RowsArgs a) {
     Eight<SRC> in[TIMES];
 #pragma unroll
     for (int i = 0; i < TIMES; i++) {
-        const int row = sub + i * shape.together;
-        if (live && row < count) load8_once<SRC>(src, (first + row) * stride + from, in[i]);
+        const int row = sub + i * a.together;
+        // others' rows are the first one's, so that no load waits in a branch
+        load8_once<SRC>(src.data, live && row < count ? from_row : from, in[i]);
+        from_row += next;
     }
-    if ((int)threadIdx.x < count) {
+    if ((int)threadIdx.x < MOST_GROUP) {
         mine[threadIdx.x] = (unsigned)s0 < (unsigned)slots ? s0 : -1;
         replaced[threadIdx.x] = 0;
     }
@@ -234,14 +254,14 @@ __global__ __launch_bounds__(256) void k_kv_write(RowsArgs a) {
     if (a.rows - first > 1) {
         // most often the later slots are all outside the range of the workgroup's own
         uint32_t low = ~0u, high = 0, near = ~0u;
-        for (int i = 0; i < count; i++) {
-            const int m = mine[i];
-            low = min(low, (uint32_t)m);
-            high = (uint32_t)max((int)high, m);
+        for (int i = 0; i < count; i += 4) {
+            const int4 m = *reinterpret_cast<const int4*>(mine + i);
+            low = min(min(min(low, (uint32_t)m.x), min((uint32_t)m.y, (uint32_t)m.z)), (uint32_t)m.w);
+            high = (uint32_t)max(max(max((int)high, m.x), max(m.y, m.z)), m.w);
         }
 #pragma unroll
         for (int j = 0; j < TURNS; j++) {
-            if (first + count + FEW_ROWS * j >= a.rows) break;
+            if (first + count + TURN * j >= a.rows) break;
 #pragma unroll
             for (int e = 0; e < 4; e++) near = min(near, (uint32_t)later[j][e] - low);
         }
@@ -252,7 +272,7 @@ __global__ __launch_bounds__(256) void k_kv_write(RowsArgs a) {
             if (any) {
 #pragma unroll
                 for (int j = 0; j < TURNS; j++) {
-                    if (first + count + FEW_ROWS * j >= a.rows) break;
+                    if (first + count + TURN * j >= a.rows) break;
 #pragma unroll
                     for (int e = 0; e < 4; e++) same |= later[j][e] == m;
                 }
@@ -263,7 +283,7 @@ __global__ __launch_bounds__(256) void k_kv_write(RowsArgs a) {
     }
 #pragma unroll
     for (int i = 0; i < TIMES; i++) {
-        const int row = sub + i * shape.together;
+        const int row = sub + i * a.together;
         const int slot = live && row < count && !replaced[row] ? mine[row] : -1;
         if (slot < 0) continue;     // the same for the four threads of a block
         uint32_t code[2];
@@ -291,53 +311,60 @@ __global__ __launch_bounds__(256) void k_kv_write(RowsArgs a) {
 template <int DST, bool MANY>
 __global__ __launch_bounds__(256) void k_kv_read(RowsArgs a) {
     constexpr int TIMES = MANY ? BATCH : 1;
-    const Shape shape = shape_of(a.units, a.c.blocks);
-    const int64_t first = (int64_t)blockIdx.x * a.group;
-    const int count = (int)(a.rows - first < a.group ? a.rows - first : a.group);
     const int slots = a.c.pages << a.c.shift;
-    const int sub = (int)threadIdx.x / shape.wide;
-    const int at = (int)blockIdx.y * shape.wide + ((int)threadIdx.x - sub * shape.wide);
-    if (sub >= shape.together || at >= a.units) return;
-    const Unit u = unit_of(a.c, at);
-    void* dst = u.value ? a.v : a.k;
-    const int64_t stride = u.value ? a.v_stride : a.k_stride;
+    const int sub = (int)(__umul24(threadIdx.x, a.per_wide) >> 20);
+    const int at = (int)blockIdx.y * a.wide + ((int)threadIdx.x - (int)__umul24(sub, a.wide));
+    if (sub >= a.together || at >= a.units) return;
+    const Unit u = unit_of(a, at);
+    const Side dst = side_of(a, u.value);
+    const int first = (int)blockIdx.x * a.group;
+    const int64_t next = a.together * dst.stride;
+    int64_t to = (first + sub) * dst.stride + (__umul24(u.head, 32 * a.c.blocks) + 32 * u.block + 8 * u.quarter);
+    const int count = a.rows - first < a.group ? a.rows - first : a.group;
     int slot[TIMES];
 #pragma unroll
     for (int i = 0; i < TIMES; i++) {
-        const int row = sub + i * shape.together;
-        slot[i] = row < count ? a.slots[first + row] : -1;
+        const int row = sub + i * a.together;
+        slot[i] = a.slots[first + (row < count ? row : 0)];
     }
     uint32_t w[TIMES][4];       // keys: their words; values: a unit each
     uint16_t step[TIMES];
+    const uint8_t* codes[TIMES];
 #pragma unroll
     for (int i = 0; i < TIMES; i++) {
-        w[i][0] = w[i][1] = w[i][2] = w[i][3] = 0;
-        step[i] = 0;
-        if ((unsigned)slot[i] >= (unsigned)slots) continue;
-        const Place p = place_of(a.c, u, slot[i]);
+        // a slot outside is read as the first, and its step as 0
+        const Place p = place_of(a.c, u, (unsigned)slot[i] < (unsigned)slots ? slot[i] : 0);
         step[i] = *reinterpret_cast<const uint16_t*>(p.step);
-        if (!u.value) {
-            if (u.bits == 8) {
-                const uint2 c = *reinterpret_cast<const uint2*>(p.codes);
-                w[i][0] = c.x, w[i][1] = c.y;
-            } else {
-                w[i][0] = *reinterpret_cast<const uint32_t*>(p.codes);
-            }
-        } else {
+        codes[i] = p.codes;
+    }
+    // one branch around all rows' loads: none waits for another
+    if (u.value && u.bits == 8) {
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const uint8_t* o = p.codes + j * u.pair;
-                w[i][j] = u.bits == 8 ? *reinterpret_cast<const uint16_t*>(o) : *o;
-            }
+        for (int i = 0; i < TIMES; i++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) w[i][j] = *reinterpret_cast<const uint16_t*>(codes[i] + j * u.pair);
+    } else if (u.value) {
+#pragma unroll
+        for (int i = 0; i < TIMES; i++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) w[i][j] = codes[i][j * u.pair];
+    } else if (u.bits == 8) {
+#pragma unroll
+        for (int i = 0; i < TIMES; i++) {
+            const uint2 c = *reinterpret_cast<const uint2*>(codes[i]);
+            w[i][0] = c.x, w[i][1] = c.y;
         }
+    } else {
+#pragma unroll
+        for (int i = 0; i < TIMES; i++) w[i][0] = *reinterpret_cast<const uint32_t*>(codes[i]);
     }
 #pragma unroll
     for (int i = 0; i < TIMES; i++) {
-        const int row = sub + i * shape.together;
+        const int row = sub + i * a.together;
         if (row >= count) break;
         // Codes go through f16 two at a time, as subnormals c 2^-24, and c d is exact in
-        // f32: a magnitude of 7 bits times a step of 11. Of a slot outside all is 0.
-        const float d = qskv::half_of(step[i]), large = d * 0x1p24f;
+        // f32: a magnitude of 7 bits times a step of 11.
+        const float d = (unsigned)slot[i] < (unsigned)slots ? qskv::half_of(step[i]) : 0.0f, large = d * 0x1p24f;
         const float less = u.bits == 8 ? 0.0f : -8.0f * d;
         float x[8];
 #pragma unroll
@@ -354,22 +381,28 @@ __global__ __launch_bounds__(256) void k_kv_read(RowsArgs a) {
             x[2 * j] = __builtin_fmaf((float)h[0], large, less);
             x[2 * j + 1] = __builtin_fmaf((float)h[1], large, less);
         }
-        store8<DST, true>(dst, (first + row) * stride + (int64_t)u.head * 32 * a.c.blocks + 32 * u.block + 8 * u.quarter, x);
+        store8<DST, true>(dst.data, to, x);
+        to += next;
     }
 }
 
 template <typename F>
-hipError_t launch_rows(const RowsArgs& all, int64_t most, int esz, F&& few, F&& many, hipStream_t st) {
-    const Shape shape = shape_of(all.units, all.c.blocks);
+hipError_t launch_rows(const RowsArgs& all, int64_t most, int threads, int esz, F&& few, F&& many, hipStream_t st) {
     for (int64_t first = 0; first < all.rows; first += most) {
         RowsArgs a = all;
         a.rows = (int32_t)(all.rows - first < most ? all.rows - first : most);
         a.k = static_cast<char*>(all.k) + first * all.k_stride * esz;
         a.v = static_cast<char*>(all.v) + first * all.v_stride * esz;
         a.slots = all.slots + first;
-        a.group = shape.together * (a.rows > FEW_ROWS ? BATCH : 1);
+        const bool much = a.rows > FEW_ROWS;
+        const Shape shape = shape_of(all.units, all.c.blocks, much ? threads : 256);
+        a.group = shape.together * (much ? BATCH : 1);
+        a.wide = shape.wide;
+        a.together = shape.together;
+        a.per_wide = (uint32_t)(((1 << 20) + shape.wide - 1) / shape.wide);
+        a.per_block = (uint32_t)(((1 << 18) + a.c.blocks - 1) / a.c.blocks);
         const dim3 grid((unsigned)((a.rows + a.group - 1) / a.group), (unsigned)shape.columns);
-        const hipError_t e = qs_host::launch_kernel(a.rows > FEW_ROWS ? many : few, grid, dim3(256), 0, st, a);
+        const hipError_t e = qs_host::launch_kernel(much ? many : few, grid, dim3(much ? threads : 256), 0, st, a);
         if (e != hipSuccess) return e;
     }
     return hipSuccess;
@@ -531,7 +564,7 @@ int qs_kv_write(const qs_kv_cache* cache, int src_type, const void* k, int64_t k
     hipStream_t st = static_cast<hipStream_t>(hip_stream);
     const auto launch = [&](auto type) {
         constexpr int T = decltype(type)::value;
-        return launch_rows(a, MOST_ROWS, esz, k_kv_write<T, false>, k_kv_write<T, true>, st);
+        return launch_rows(a, MOST_ROWS, WRITERS, esz, k_kv_write<T, false>, k_kv_write<T, true>, st);
     };
     const hipError_t e = src_type == QS_SRC_F32   ? launch(std::integral_constant<int, qs::SRC_F32>{})
                          : src_type == QS_SRC_F16 ? launch(std::integral_constant<int, qs::SRC_F16>{})
@@ -561,7 +594,7 @@ int qs_kv_read(const qs_kv_cache* cache, const int32_t* slots, int64_t rows, int
     hipStream_t st = static_cast<hipStream_t>(hip_stream);
     const auto launch = [&](auto type) {
         constexpr int T = decltype(type)::value;
-        return launch_rows(a, kMaxRows, esz, k_kv_read<T, false>, k_kv_read<T, true>, st);
+        return launch_rows(a, kMaxRows, 256, esz, k_kv_read<T, false>, k_kv_read<T, true>, st);
     };
     const hipError_t e = dst_type == QS_SRC_F32   ? launch(std::integral_constant<int, qs::SRC_F32>{})
                          : dst_type == QS_SRC_F16 ? launch(std::integral_constant<int, qs::SRC_F16>{})
