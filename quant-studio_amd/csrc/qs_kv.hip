@@ -89,7 +89,7 @@ constexpr int BATCH = 4;
 constexpr int FEW_ROWS = 1024;
 // rows of a launch that writes: what a workgroup looks its slots up among, a turn of four for each thread
 constexpr int64_t MOST_ROWS = 8192;
-constexpr int WRITERS = 1024;       // threads of a workgroup that writes many rows
+constexpr int WRITERS = 512;      // threads of a workgroup that writes many rows
 struct Shape {
     int wide, together, columns;    // columns: workgroups for a row
 };
@@ -209,7 +209,7 @@ __global__ __launch_bounds__(MANY ? WRITERS : 256) void k_kv_write(RowsArgs a) {
     constexpr int TURN = 4 * THREADS, TURNS = MANY ? (int)(MOST_ROWS / TURN) : FEW_ROWS / TURN;
     constexpr int MOST_GROUP = TIMES * THREADS / 16;       // a row has 16 units at least
     __shared__ __attribute__((aligned(16))) int mine[MOST_GROUP];
-    __shared__ int replaced[MOST_GROUP];
+    __shared__ int replaced[MOST_GROUP], chain[MOST_GROUP], heads[THREADS];
     const int first = (int)blockIdx.x * a.group;
     const int count = a.rows - first < a.group ? a.rows - first : a.group;
     const int slots = a.c.pages << a.c.shift;
@@ -246,12 +246,17 @@ __global__ __launch_bounds__(MANY ? WRITERS : 256) void k_kv_write(RowsArgs a) {
         load8_once<SRC>(src.data, live && row < count ? from_row : from, in[i]);
         from_row += next;
     }
+    // The workgroup's rows by their slots: chains from a table of as many heads as threads.
+    const auto place_in = [&](int slot) { return ((uint32_t)slot * 0x9e3779b1u) / (0x80000000u / THREADS * 2); };
+    const bool held = (unsigned)s0 < (unsigned)slots;
+    heads[threadIdx.x] = -1;
     if ((int)threadIdx.x < MOST_GROUP) {
-        mine[threadIdx.x] = (unsigned)s0 < (unsigned)slots ? s0 : -1;
+        mine[threadIdx.x] = held ? s0 : -1;
         replaced[threadIdx.x] = 0;
     }
     __syncthreads();
     if (a.rows - first > 1) {
+        if (held) chain[threadIdx.x] = atomicExch(&heads[place_in(s0)], (int)threadIdx.x);
         // most often the later slots are all outside the range of the workgroup's own
         uint32_t low = ~0u, high = 0, near = ~0u;
         for (int i = 0; i < count; i += 4) {
@@ -259,25 +264,26 @@ __global__ __launch_bounds__(MANY ? WRITERS : 256) void k_kv_write(RowsArgs a) {
             low = min(min(min(low, (uint32_t)m.x), min((uint32_t)m.y, (uint32_t)m.z)), (uint32_t)m.w);
             high = (uint32_t)max(max(max((int)high, m.x), max(m.y, m.z)), m.w);
         }
+        __syncthreads();
+        // a row's slot is in a later one: of the workgroup's own, or behind them
+        const auto look_up = [&](int slot, int before) {
+            for (int i = heads[place_in(slot)]; i >= 0; i = chain[i])
+                if (i < before && mine[i] == slot) replaced[i] = 1;
+        };
+        if (held) look_up(s0, (int)threadIdx.x);
 #pragma unroll
         for (int j = 0; j < TURNS; j++) {
             if (first + count + TURN * j >= a.rows) break;
 #pragma unroll
             for (int e = 0; e < 4; e++) near = min(near, (uint32_t)later[j][e] - low);
         }
-        const bool any = near <= high - low;
-        for (int i = 0; i < count; i++) {
-            const int m = mine[i];
-            bool same = (int)threadIdx.x > i && s0 == m;
-            if (any) {
+        if (near <= high - low) {
 #pragma unroll
-                for (int j = 0; j < TURNS; j++) {
-                    if (first + count + TURN * j >= a.rows) break;
+            for (int j = 0; j < TURNS; j++) {
+                if (first + count + TURN * j >= a.rows) break;
 #pragma unroll
-                    for (int e = 0; e < 4; e++) same |= later[j][e] == m;
-                }
+                for (int e = 0; e < 4; e++) look_up(later[j][e], count);
             }
-            if (same) replaced[i] = 1;
         }
         __syncthreads();
     }
