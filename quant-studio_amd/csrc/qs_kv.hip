@@ -201,8 +201,18 @@ QS_DEV float codes_of(const Eight<SRC>& in, const Unit& u, uint32_t (&code)[2]) 
 
 // A thread takes eight values, four threads a block of 32: its step from their
 // largest magnitude, then eight codes each, in the order of the cache's rows.
-// Of rows with the same slot the last is written: every workgroup looks its rows'
-// slots up among all later ones, which a launch's few rows make cheap.
+// Of rows with the same slot the last is written: every workgroup looks all later
+// slots up in a table of its own rows' (16,383 rows of one head of 64 in any order take
+// 27.6 us; 82 with every own slot compared with every later one). With MANY rows a
+// workgroup has WRITERS threads, which share that work among more rows: 8,191 rows of
+// eight heads of 128 in any order take 29.9 us, 35.4 with 256 threads, 29.4 with 1,024;
+// 1,025 rows 10.2, 9.9 and 12.0.
+//
+// 8,191 such rows in order, bf16 to keys of 8 and values of 4 bits, are 47 MB and take
+// 25.4 us, 1.85 TB/s; a copy of as many bytes takes 11.3. All rows are on their way at
+// once, so that reading (15.7 us without the rest), the codes' 700 instructions a wave and
+// the scattered stores (8 us) overlap little. Staging the values' codes in LDS for wide stores took 1.4 us
+// more, a row or two at a time instead of BATCH 0.4 to 8 us more.
 template <int SRC, bool MANY>
 __global__ __launch_bounds__(MANY ? WRITERS : 256) void k_kv_write(RowsArgs a) {
     constexpr int THREADS = MANY ? WRITERS : 256, TIMES = MANY ? BATCH : 1;
@@ -313,7 +323,9 @@ __global__ __launch_bounds__(MANY ? WRITERS : 256) void k_kv_write(RowsArgs a) {
 }
 
 // The values of some slots' rows; a slot outside the cache gives zeros. Eight to a
-// thread, of BATCH rows at a time.
+// thread, of BATCH rows at a time, whose loads are all on their way before the first
+// is waited for. Bound by HBM: 65,535 rows of eight heads of 128, 8 bits to bf16, 411 MB,
+// take 78.6 us, 5.2 TB/s, as fast as a large copy.
 template <int DST, bool MANY>
 __global__ __launch_bounds__(256) void k_kv_read(RowsArgs a) {
     constexpr int TIMES = MANY ? BATCH : 1;
@@ -511,11 +523,17 @@ Split split_of(const AttentionArgs& a, void* workspace) {
     Split s{};
     if (a.batch == 0 || a.fresh == 0) return s;
     s.waves = segments > (steps <= FEW ? 1 : 2) * full && a.batch > 1 ? 1 : 4;
-    const int64_t held = full * (4 / s.waves);
+    // Where loads are all that bounds it, eight-bit codes of heads of 128 or 256 for eight
+    // 16-bit queries, one workgroup less on each CU streams better: 8 sequences of 32,767
+    // slots 114.2 and 116.7 us, of heads of 256 and 16,000 slots 115 and 121; four-bit ones
+    // of 128 take 45.6, 44.2 with all, heads of 64 with 8 bits 35.6 and 35.1.
+    const bool lean = s.waves == 4 && a.c.k_bits + a.c.v_bits == 16 && a.c.blocks % 4 == 0 && columns_of(a) == 8 &&
+                      a.type != QS_SRC_F32;
+    const int64_t held = s.waves == 4 ? full - lean * CUS : 4 * full;
     if (steps <= whole || (s.waves == 1 && steps <= whole * (1 + segments / held))) {
         s.share = 1;
     } else if (a.batch == 1) {
-        const int64_t share = full / segments, most = (steps + s.waves - 1) / s.waves;
+        const int64_t share = held / segments, most = (steps + s.waves - 1) / s.waves;
         s.share = (int32_t)(share < 1 ? 1 : share < most ? share : most);
     }
     const int64_t most = segments * (steps / s.waves + 1 + OPENING);

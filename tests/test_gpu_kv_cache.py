@@ -214,6 +214,26 @@ def test_a_lone_sequence(qs, length, window, table):
     ref.check(y, want, far)
 
 
+@pytest.mark.parametrize("heads,d,length", [(1, 64, 30000), (1, 256, 20001), (2, 128, 70001)])
+def test_a_head_of_many_parts(qs, heads, d, length):
+    attend(qs, qs.KVCache(-(-length // 256) + 1, 256, heads, d, "q8_0", "q4_0"), [length], 3 * heads, 2, torch.bfloat16, 17)
+
+
+@pytest.mark.parametrize("heads,d,t", [(1, 64, 1500), (1, 256, 5000), (3, 192, 1030), (33, 64, 1100)])
+@pytest.mark.parametrize("slots", [40, 100000])
+def test_many_rows_of_few_and_of_many_slots(qs, heads, d, t, slots):
+    """Most of them again and again, and in any order; the last row of a slot stays."""
+    cache = qs.KVCache(-(-slots // 1024), 1024, heads, d, "q4_0", "q8_0")
+    k, v = ref.keys_values(t, heads, d, torch.float16, 18)
+    at = torch.randint(-3, slots, (t,), generator=torch.Generator().manual_seed(t)).to(torch.int32)
+    last = {s: i for i, s in enumerate(at.tolist()) if s >= 0}
+    qs.kv_write(cache, k, v, at.to(DEV))
+    rows = torch.tensor(list(last.values()))
+    got = qs.kv_read(cache, at[rows].to(DEV), dtype=torch.float32)
+    for x, kind, y in ((k, "q4_0", got[0]), (v, "q8_0", got[1])):
+        assert torch.equal(y.cpu().double(), ref.values64(qs, kind, x[rows.to(DEV)]))
+
+
 def test_out_may_be_q(qs):
     cache = qs.KVCache(80, 16, 2, 64, "q8_0")
     lengths = [400, 3, 0, 700]
