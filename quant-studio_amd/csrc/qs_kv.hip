@@ -85,8 +85,10 @@ QS_DEV Place place_of(const Cache& c, const Unit& u, int slot) {
 // most all and a multiple of a head's units) on one row, `together` rows at a time,
 // BATCH times over.
 constexpr int BATCH = 4;
-// calls of no more rows take one at a time: more workgroups
-constexpr int FEW_ROWS = 1024;
+// Calls of no more rows, and no more workgroups than the GPU holds at a time, take one row
+// at a time: 1,000 rows of eight heads of 128 read in 4.2 us, 4.4 in batches; 4,000 of one
+// head 3.6 and 4.4; but 2,100 of eight heads 6.1 and 5.1.
+constexpr int FEW_ROWS = 4096, HELD = 2048;
 // rows of a launch that writes: what a workgroup looks its slots up among, a turn of four for each thread
 constexpr int64_t MOST_ROWS = 8192;
 constexpr int WRITERS = 512;      // threads of a workgroup that writes many rows
@@ -202,17 +204,17 @@ QS_DEV float codes_of(const Eight<SRC>& in, const Unit& u, uint32_t (&code)[2]) 
 // A thread takes eight values, four threads a block of 32: its step from their
 // largest magnitude, then eight codes each, in the order of the cache's rows.
 // Of rows with the same slot the last is written: every workgroup looks all later
-// slots up in a table of its own rows' (16,383 rows of one head of 64 in any order take
-// 27.6 us; 82 with every own slot compared with every later one). With MANY rows a
-// workgroup has WRITERS threads, which share that work among more rows: 8,191 rows of
-// eight heads of 128 in any order take 29.9 us, 35.4 with 256 threads, 29.4 with 1,024;
-// 1,025 rows 10.2, 9.9 and 12.0.
+// slots up in a table of its own rows' (16,383 rows of one head of 64 in any order, written
+// and read back, take 27.6 us; 82 with every own slot compared with every later one). With
+// MANY rows a workgroup has WRITERS threads, which share that work among more rows: 8,191
+// rows of eight heads of 128 in any order, written and read back, take 29.9 us, 35.4 with
+// 256 threads, 29.4 with 1,024; 1,025 rows 10.2, 9.9 and 12.0.
 //
 // 8,191 such rows in order, bf16 to keys of 8 and values of 4 bits, are 47 MB and take
-// 25.4 us, 1.85 TB/s; a copy of as many bytes takes 11.3. All rows are on their way at
-// once, so that reading (15.7 us without the rest), the codes' 700 instructions a wave and
-// the scattered stores (8 us) overlap little. Staging the values' codes in LDS for wide stores took 1.4 us
-// more, a row or two at a time instead of BATCH 0.4 to 8 us more.
+// 15 us, 3.1 TB/s; a copy of as many bytes takes 11.3. All rows are on their way at once,
+// so that reading, 600 instructions a wave for the codes (2.5 us of it) and the
+// scattered stores (5 us of it) overlap little. Staging the values' codes in LDS for wide stores
+// took 1.4 us more, a row or two at a time instead of BATCH 0.4 to 8 us more.
 template <int SRC, bool MANY>
 __global__ __launch_bounds__(MANY ? WRITERS : 256) void k_kv_write(RowsArgs a) {
     constexpr int THREADS = MANY ? WRITERS : 256, TIMES = MANY ? BATCH : 1;
@@ -412,8 +414,9 @@ hipError_t launch_rows(const RowsArgs& all, int64_t most, int threads, int esz, 
         a.k = static_cast<char*>(all.k) + first * all.k_stride * esz;
         a.v = static_cast<char*>(all.v) + first * all.v_stride * esz;
         a.slots = all.slots + first;
-        const bool much = a.rows > FEW_ROWS;
-        const Shape shape = shape_of(all.units, all.c.blocks, much ? threads : 256);
+        Shape shape = shape_of(all.units, all.c.blocks, 256);
+        const bool much = a.rows > FEW_ROWS || (int64_t)a.rows * shape.columns > HELD * shape.together;
+        if (much) shape = shape_of(all.units, all.c.blocks, threads);
         a.group = shape.together * (much ? BATCH : 1);
         a.wide = shape.wide;
         a.together = shape.together;

@@ -48,7 +48,8 @@ class KVCache:
 
     data: uint8 (pages, bytes of a page), zeros at first, or a tensor to use as it
     is. A page may be copied to another (data[j] = data[i]), of a cache of the same
-    sizes too; the order of a page's bytes is the library's own."""
+    sizes too; the order of a page's bytes is the library's own. What a cache is does
+    not change: its attributes cannot be set."""
 
     __slots__ = ("pages", "page_size", "heads", "head_dim", "k_type", "v_type", "data", "_c", "_ref", "_dev", "_work")
 
@@ -81,6 +82,11 @@ class KVCache:
         self._c = _Cache(_TYPES[k_type], _TYPES[v_type], heads, head_dim, page_size, pages, data.data_ptr())
         self._ref = ctypes.byref(self._c)
         self._work = {}         # (sequences, new tokens, query heads, table columns) -> workspace bytes
+
+    def __setattr__(self, name, value):
+        if hasattr(self, "_work"):      # the last one set
+            raise AttributeError(f"KVCache: {name} cannot be set: the calls would go on with what it was")
+        object.__setattr__(self, name, value)
 
     def slots(self, tables, positions):
         """int32 slots of positions (b, n) of sequences whose pages are tables

@@ -377,6 +377,13 @@ def test_python_refuses(qs):
         attend(q=q.clone().requires_grad_())
 
 
+def test_a_cache_stays_what_it_is(qs):
+    cache = qs.KVCache(2, 16, 1, 64)
+    for name in ("data", "pages", "page_size", "heads", "k_type"):
+        with pytest.raises(AttributeError, match=name):
+            setattr(cache, name, getattr(cache, name))
+
+
 def test_threads_share_a_cache(qs):
     """Reads from several threads at once, each on a stream of its own: the bits of a call alone."""
     cache = qs.KVCache(60, 16, 2, 64, "q8_0", "q4_0")
