@@ -231,8 +231,9 @@ __global__ __launch_bounds__(MANY ? WRITERS : 256) void k_kv_write(RowsArgs a) {
     const Unit u = unit_of(a, live ? at : 0);
     const Side src = side_of(a, u.value);
     const int64_t from = first * src.stride + (__umul24(u.head, 32 * a.c.blocks) + 32 * u.block + 8 * u.quarter);
-    const int64_t next = a.together * src.stride;
-    int64_t from_row = from + sub * src.stride;
+    // unsigned: behind the last row, where nothing is read, it may pass 2^63
+    const uint64_t next = (uint64_t)src.stride * a.together;
+    uint64_t from_row = from + (uint64_t)src.stride * sub;
     // The slots of the workgroup's rows and of all later ones, which a launch has few
     // enough of for one turn, then the rows' values: all are on their way before
     // anything waits, and the slots are compared meanwhile.
@@ -255,7 +256,7 @@ __global__ __launch_bounds__(MANY ? WRITERS : 256) void k_kv_write(RowsArgs a) {
     for (int i = 0; i < TIMES; i++) {
         const int row = sub + i * a.together;
         // others' rows are the first one's, so that no load waits in a branch
-        load8_once<SRC>(src.data, live && row < count ? from_row : from, in[i]);
+        load8_once<SRC>(src.data, live && row < count ? (int64_t)from_row : from, in[i]);
         from_row += next;
     }
     // The workgroup's rows by their slots: chains from a table of as many heads as threads.

@@ -263,6 +263,6 @@ def kv_attention(q, cache: KVCache, tables, lengths, scale: float | None = None,
     else:
         _no_gradient("kv_attention", "out", out)
     _call(dev, lib.qs_kv_attention, cache._ref, kind, q.data_ptr(), stride * esz, b, n, heads, tables.data_ptr(), m,
-          table_stride, lengths.data_ptr(), 1 / math.sqrt(d) if scale is None else scale, window,
+          table_stride, lengths.data_ptr(), 1 / math.sqrt(d) if scale is None else scale, min(window, 1 << 62),
           out.data_ptr(), out.numel() * esz, work_ptr, need)
     return out

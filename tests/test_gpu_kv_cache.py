@@ -253,6 +253,17 @@ def test_large_and_small_queries(qs, dtype, spread):
     attend(qs, qs.KVCache(20, 16, 2, 128, "q4_0", "q4_0"), [200, 50], 4, 1, dtype, 6, spread=spread, scale=-0.02)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("spread,scale", [(0.0, 0.1), (1.0, 0.0), (1.0, -3.0), (1e-20, 1e20)])
+def test_scales_and_queries_of_zeros(qs, dtype, spread, scale):
+    attend(qs, qs.KVCache(70, 16, 2, 64, "q8_0", "q4_0"), [300, 1, 0, 700], 6, 2, dtype, 19, spread=spread, scale=scale)
+
+
+@pytest.mark.parametrize("window", [2 ** 31 - 2, 2 ** 31, 2 ** 63, 2 ** 64 + 1])
+def test_windows_longer_than_all(qs, window):
+    attend(qs, qs.KVCache(70, 16, 2, 64, "q8_0", "q4_0"), [300, 1, 0, 700], 6, 2, torch.bfloat16, 20, window=window)
+
+
 @pytest.mark.parametrize("size", [1e-6, 1e-3, 1e3])
 @pytest.mark.parametrize("kind", TYPES)
 def test_large_and_small_values(qs, size, kind):
