@@ -49,6 +49,29 @@ def test_rows_are_the_quantizers(qs, d, k_type, v_type, dtype, heads, t, page):
             assert torch.equal(x.to(out), y)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("power", [-20, -6, 0, 7])
+def test_ties_are_the_quantizers(qs, dtype, kind, power):
+    """Bit for bit: largest magnitudes of either sign in a block, codes half way between two."""
+    g = torch.Generator().manual_seed(power + 30)
+    x = torch.randint(-255, 256, (1200, 2, 64), generator=g).float() / 2
+    x[:400] = torch.randint(-2, 3, (400, 2, 64), generator=g).float()
+    x[400:600] = (x[400:600] / 16).round() * 8.5
+    x[600:800, :, ::7] = 127.0
+    x[800:1000, :, 5::32] = -127.0
+    x[1100:] = 0.0
+    x[1150:, 0, 3] = -0.0
+    x = (x * 2.0 ** power).to(DEV, dtype)
+    cache = qs.KVCache(5, 256, 2, 64, kind)
+    slots = torch.arange(1200, dtype=torch.int32, device=DEV)
+    for rows in (slots[:700], slots[700:], slots):     # a row or several at a time
+        qs.kv_write(cache, x[rows.long()], x[rows.long()].flip(2).contiguous(), rows)
+        got = qs.kv_read(cache, rows, dtype=torch.float32)
+        for y, z in zip(got, (x, x.flip(2))):
+            assert torch.equal(y.cpu().double(), ref.values64(qs, kind, z[rows.long()].contiguous()))
+
+
 @pytest.mark.parametrize("t", [2, 50, 300, 2000, 9000])
 def test_a_slot_twice_holds_the_last_row(qs, t):
     """Also across the rows of different workgroups and launches."""
