@@ -235,8 +235,8 @@ __global__ __launch_bounds__(MANY ? WRITERS : 256) void k_kv_write(RowsArgs a) {
     const uint64_t next = (uint64_t)src.stride * a.together;
     uint64_t from_row = from + (uint64_t)src.stride * sub;
     // The slots of the workgroup's rows and of all later ones, which a launch has few
-    // enough of for one turn, then the rows' values: all are on their way before
-    // anything waits, and the slots are compared meanwhile.
+    // enough of for four turns, then the rows' values: all are on their way before
+    // anything waits, and the slots are looked up meanwhile.
     const int s0 = (int)threadIdx.x < count ? a.slots[first + threadIdx.x] : -1;
     int later[TURNS][4];
 #pragma unroll
