@@ -37,10 +37,10 @@ inline __host__ __device__ int column_tiles(const AttentionArgs& a) {
     return (a.group * a.fresh + columns_of(a) - 1) / columns_of(a);
 }
 
-// A code c of the matrix products is c 2^-code_power, for f32 queries at other bits than
-// for those of 16 bits; `once_of` times a sum of products with values' codes is the sum.
-__host__ __device__ constexpr int code_power(int bits, bool wide) { return bits == 8 ? (wide ? 21 : 24) : wide ? 18 : 22; }
-__host__ __device__ constexpr float once_of(int v_bits, bool wide) { return (float)(1 << code_power(v_bits, wide)); }
+// A code c of the matrix products is c 2^-CODE_POWER, a normal f16; ONCE times a sum of
+// products with values' codes is the sum.
+constexpr int CODE_POWER = 9;
+constexpr float ONCE = 1 << CODE_POWER;
 
 // How a call's work is split, and where its workgroups leave what is joined.
 constexpr int TILE = 32;            // slots of a wave's step
@@ -58,7 +58,7 @@ struct Split {
     int32_t share;                  // workgroups of a head's and column tile's steps of a sequence, 1: they take all;
                                     // 0: they take equal runs of all steps of the call
     // of each workgroup, first for a segment that begins before it, then for one that goes on after it
-    float* parts;                   // [groups][2][columns][head size], sums relative to the maximum, in units of once_of
+    float* parts;                   // [groups][2][columns][head size], sums relative to the maximum, in units of ONCE
     float2* stats;                  // [groups][2][columns]: maximum, sum of p
     // Of runs: segments that more than one workgroup has, as sequence, head and column tile, first and last
     // workgroup (-1: it is one's alone). One entry for each head and column tile of a sequence where these

@@ -11,9 +11,9 @@
 //
 // The scores' D has its slots where the values' P wants them (a lane: one query,
 // slots 4 g .. 4 g + 3 of both sixteens), so nothing moves between lanes. Codes go to
-// f16 without a conversion, as subnormal numbers, which the matrix units take;
-// from four-bit ones an addition takes their offset of 8 (left on, it would have to come
-// off the sums, and these would cancel).
+// f16 without a conversion: their bits are a subnormal number, which a multiplication by a
+// power of two takes up; from four-bit ones it takes their offset of 8 as well (left on, it
+// would have to come off the sums, and these would cancel).
 // P is held to 21 bits or more: a query has two of the 16 columns, one takes f16(P),
 // the other f16(P - f16(P)). So that the second does not fall below f16's range, p counts
 // 2^s times, a power of two that takes the largest step so far to just below 2^15: what
@@ -99,50 +99,47 @@ QS_DEV void load(Codes<N>& o, Buffer p, int at, int from) {
     for (int i = 0; i < N; i += PIECE) load_piece<PIECE>(o.w + i / 4, p, at + i, from);
 }
 
-// Codes as f16, two at a time. What lies far below 2^-14 in a subnormal factor is lost in
-// the matrix units' sums, as if they took its bits where they are: with c 2^-24 for
-// four-bit codes and 2^-20 for every second, log p was off by 2.6e-6 (32 slots of 128
-// values), and 131,071 values' average by 1.4e-4 of itself. So the bits lie higher, at the
-// cost of a shift; and FINE (f32 queries) as high as they can, at that of one to two
-// instructions for each pair, where log p is off by 1.5e-7 as with an f32 product.
-template <bool FINE>
+// Codes as f16, two at a time: c 2^-CODE_POWER, exactly, and normal numbers. As they come out
+// of the bytes they are subnormal, and the matrix units take a subnormal factor's bits where
+// they are: what lies far below 2^-14 is lost in their sums. With subnormal codes averages of
+// 131,071 slots were off by 1e-4 of their rms (four bits; 3e-5 with eight), now by 3e-7. One
+// packed multiplication a pair takes them up (1 x 131,071 slots of eight bits 60.5 us, 59.3
+// without it), for four-bit codes in the instruction that takes their offset off.
 QS_DEV uint32_t sign_and_magnitude(uint32_t twice) {        // a byte beside itself in each half
-    return FINE ? (twice & 0x80008000u) | ((twice << 3) & 0x03f803f8u) : twice & 0x807f807fu;
+    return __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2_t, twice & 0x807f807fu) * half2_t{(_Float16)0x1p15f, (_Float16)0x1p15f});
 }
-// the four-bit codes i and i + 4 of a word, less 8; not FINE, those of odd i count 16 times
-template <bool FINE>
+// the four-bit codes i and i + 4 of a word, less 8
 QS_DEV uint32_t four_bits(uint32_t w, int i) {
-    if constexpr (FINE) w = (i == 0 ? w << 6 : i == 1 ? w << 2 : i == 2 ? w >> 2 : w >> 6) & 0x03c003c0u;
-    else w = (i & 2 ? w >> 6 : w << 2) & (i & 1 ? 0x03c003c0u : 0x003c003cu);
-    const _Float16 eight = FINE || i & 1 ? (_Float16)-0x1p-15f : (_Float16)-0x1p-19f;
-    return __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2_t, w) + half2_t{eight, eight});
+    const uint32_t two = (i & 2 ? w >> 8 : w) & (i & 1 ? 0x00f000f0u : 0x000f000fu);
+    const _Float16 up = i & 1 ? (_Float16)0x1p11f : (_Float16)0x1p15f, eight = (_Float16)-0x1p-6f;
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(__builtin_bit_cast(half2_t, two), half2_t{up, up}, half2_t{eight, eight}));
 }
 
 // eight codes of a key's block
-template <bool FINE, int BITS, int BLOCKS>
+template <int BITS, int BLOCKS>
 QS_DEV u32x4 key_block(const Codes<BITS * BLOCKS>& c, int b) {
     u32x4 o;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         if constexpr (BITS == 8)
-            o[i] = sign_and_magnitude<FINE>(__builtin_amdgcn_perm(0u, c.w[2 * b + (i >> 1)], i & 1 ? 0x03030202u : 0x01010000u));
-        else o[i] = four_bits<FINE>(c.w[b], i);
+            o[i] = sign_and_magnitude(__builtin_amdgcn_perm(0u, c.w[2 * b + (i >> 1)], i & 1 ? 0x03030202u : 0x01010000u));
+        else o[i] = four_bits(c.w[b], i);
     }
     return o;
 }
 // code n of the slots 2 i and 2 i + 1 of four
-template <bool FINE, int BITS, int BLOCKS>
+template <int BITS, int BLOCKS>
 QS_DEV uint32_t value_pair(const Codes<BITS * BLOCKS>& c, int i, int n) {
     // `run` bytes of each slot one after another: bytes `x` and `y` have the code
     constexpr int RUN = BITS * BLOCKS / 4;
     const int x = 2 * i * RUN + n * BITS / 8, y = x + RUN;
     if constexpr (BITS == 8) {
-        return sign_and_magnitude<FINE>(
+        return sign_and_magnitude(
             __builtin_amdgcn_perm(c.w[y >> 2], c.w[x >> 2], (x & 3) * 0x00000101u + (y & 3) * 0x01010000u + 0x04040000u));
     } else {
         // the half words that have it; their codes 0 .. 3 are those from n & ~3 on
         const uint32_t hx = x & 2 ? 0x0302u : 0x0100u, hy = y & 2 ? 0x07060000u : 0x05040000u;
-        return four_bits<FINE>(__builtin_amdgcn_perm(c.w[y >> 2], c.w[x >> 2], hx | hy), n & 3);
+        return four_bits(__builtin_amdgcn_perm(c.w[y >> 2], c.w[x >> 2], hx | hy), n & 3);
     }
 }
 
@@ -182,7 +179,7 @@ QS_DEV void load_queries(const AttentionArgs& a, int seq, int head, int first, R
 #pragma unroll
     for (int b = 0; b < BLOCKS; b++) qsr::load8<WIDE ? qs::SRC_F32 : qs::SRC_BF16>(a.q, at + 32 * b + 8 * g, o.b[b]);
 }
-template <int K_BITS, int BLOCKS, bool WIDE>
+template <int BLOCKS, bool WIDE>
 QS_DEV void prepare_queries(const AttentionArgs& a, int first, int length, const RawQueries<BLOCKS, WIDE>& raw,
                             Queries<BLOCKS, WIDE>& o) {
     const int lane = threadIdx.x & 63, column = first + (lane & 7);
@@ -212,8 +209,7 @@ QS_DEV void prepare_queries(const AttentionArgs& a, int first, int length, const
             half2_t h, l;
 #pragma unroll
             for (int j = 0; j < 2; j++) {
-                // where a four-bit key's code counts 16 times
-                const float v = __builtin_ldexpf(x[b][2 * i + j], K_BITS == 4 && !WIDE && i & 1 ? e - 4 : e);
+                const float v = __builtin_ldexpf(x[b][2 * i + j], e);
                 h[j] = (_Float16)v;
                 if constexpr (WIDE) l[j] = (_Float16)(v - (float)h[j]);
             }
@@ -222,7 +218,7 @@ QS_DEV void prepare_queries(const AttentionArgs& a, int first, int length, const
         }
     }
     o.scale = a.scale * LOG2E;
-    o.up = code_power(K_BITS, WIDE) - e;
+    o.up = CODE_POWER - e;
     o.last = length - a.fresh + 1 + token;
     o.first = a.window > 0 && o.last > a.window ? o.last - a.window : 0;
 }
@@ -373,7 +369,7 @@ QS_DEV void attend(const AttentionArgs& a, int start, bool edge, int held, const
         steps_from(s, false, ks);
 #pragma unroll
         for (int b = 0; b < BLOCKS; b++) {
-            const u32x4 k = key_block<WIDE, K_BITS, BLOCKS>(t.keys[s], b);
+            const u32x4 k = key_block<K_BITS, BLOCKS>(t.keys[s], b);
 #pragma unroll
             for (int n = 0; n < SETS; n++) {
                 f32x4 d = mfma(k, q[n].q[b], f32x4{0, 0, 0, 0});
@@ -467,7 +463,7 @@ QS_DEV void attend(const AttentionArgs& a, int start, bool edge, int held, const
         for (int e = 0; e < 2; e++) {
             u32x4 c;
 #pragma unroll
-            for (int i = 0; i < 4; i++) c[i] = value_pair<WIDE, V_BITS, BLOCKS>(t.values[i >> 1], i & 1, 2 * b + e);
+            for (int i = 0; i < 4; i++) c[i] = value_pair<V_BITS, BLOCKS>(t.values[i >> 1], i & 1, 2 * b + e);
 #pragma unroll
             for (int n = 0; n < SETS; n++) sums[n].acc[b][e] = mfma(c, w[n], sums[n].acc[b][e]);
         }
@@ -477,8 +473,8 @@ QS_DEV void attend(const AttentionArgs& a, int start, bool edge, int held, const
 }
 
 // The wave's sums as one: the four lanes of a query's slots, and its two columns;
-// four-bit codes that count 16 times, and p that counts 2^power times.
-template <bool SIXTEEN, int BLOCKS>
+// p counts 2^power times.
+template <int BLOCKS>
 QS_DEV void finish(Sums<BLOCKS>& o) {
     const float once = __builtin_ldexpf(1.0f, -o.power);
     o.total = sum_over_slots(o.total) * once;
@@ -487,10 +483,8 @@ QS_DEV void finish(Sums<BLOCKS>& o) {
 #pragma unroll
         for (int e = 0; e < 2; e++)
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const float v = o.acc[b][e][r] + other_column(o.acc[b][e][r]);
-                o.acc[b][e][r] = v * (SIXTEEN && e ? 0.0625f * once : once);
-            }
+            for (int r = 0; r < 4; r++)
+                o.acc[b][e][r] = (o.acc[b][e][r] + other_column(o.acc[b][e][r])) * once;
 }
 
 QS_DEV int cut_length(const AttentionArgs& a, int n) {
@@ -648,7 +642,7 @@ void k_kv_attention(AttentionArgs a, Split split) {
             const auto start_of = [&](int n) { return (n < final ? n : final) * TILE; };
             Queries<BLOCKS, WIDE> q[SETS];
 #pragma unroll
-            for (int n = 0; n < SETS; n++) prepare_queries<K_BITS>(a, first + 8 * n, length, raw[n], q[n]);
+            for (int n = 0; n < SETS; n++) prepare_queries(a, first + 8 * n, length, raw[n], q[n]);
             for (; i < stop; i += stride) {
                 const int start = i * TILE, held = place.held;
                 place = place_of(a, ahead, head, start_of(i + stride));
@@ -658,7 +652,7 @@ void k_kv_attention(AttentionArgs a, Split split) {
         }
 #pragma unroll
         for (int n = 0; n < SETS; n++) {
-            finish<V_BITS == 4 && !WIDE>(sums[n]);
+            finish(sums[n]);
             if (lane & 8) continue;
             const int column = 8 * n + (lane & 7);
 #pragma unroll
@@ -688,7 +682,7 @@ void k_kv_attention(AttentionArgs a, Split split) {
             }
             const int64_t row = row_of(a, seq, head, first + column);
             const int64_t slot = ((int64_t)blockIdx.x * 2 + (from == 0)) * COLUMNS + column;
-            const float inverse = total != 0.0f ? once_of(V_BITS, WIDE) / total : 0.0f;    // 0: it sees nothing
+            const float inverse = total != 0.0f ? ONCE / total : 0.0f;    // 0: it sees nothing
 #pragma unroll
             for (int i = 0; i < BLOCKS / 2; i++) {
                 float2 v{0, 0};
