@@ -14,12 +14,11 @@
 // f16 without a conversion: their bits are a subnormal number, which a multiplication by a
 // power of two takes up; from four-bit ones it takes their offset of 8 as well (left on, it
 // would have to come off the sums, and these would cancel).
-// P is held to 21 bits or more: a query has two of the 16 columns, one takes f16(P),
-// the other f16(P - f16(P)). So that the second does not fall below f16's range, p counts
-// 2^s times, a power of two that takes the largest step so far to just below 2^15: what
-// is lost is under 2^-24 of the largest P, mostly far under. q is rounded to f16 after
-// its row is scaled to 2^14 .. 2^15 in the same way: all of a bf16 or f16 q down to 2^-35
-// of the row's largest; an f32 q takes two products, 22 bits.
+// P is held to 21 bits or more beside the largest of its block of 32 dimensions: a query has
+// two of the 16 columns, one takes f16(P), the other f16(P - f16(P)). So that neither leaves
+// f16's range, P count by a power of two that follows the largest of them (Sums). q is
+// rounded to f16 after its row is scaled to 2^14 .. 2^15 likewise: all of a bf16 or f16 q
+// down to 2^-35 of the row's largest; an f32 q takes two products, 22 bits.
 //
 // What bounds it (heads of 128, bf16 queries, four to a head): eight-bit codes their bytes,
 // 8 sequences of 32,767 slots 570 MB in 114 us with the join, 5.0 TB/s, of which loads
@@ -40,6 +39,8 @@ namespace qskv {
 typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+typedef short i16x2 __attribute__((ext_vector_type(2)));
 
 constexpr float LOG2E = 1.44269504088896341f;
 
@@ -143,17 +144,16 @@ QS_DEV uint32_t value_pair(const Codes<BITS * BLOCKS>& c, int i, int n) {
     }
 }
 
-// Two P as the lane's column takes them: f16(P), cut off, in the first (second = 0); in
-// the second (0xffffe000, what of an f32 an f16 has) what that leaves of it, cut off as
-// well, which one instruction does for both, or to nearest for f32 results.
-template <bool NEAREST>
-QS_DEV uint32_t two_halves(float x, float y, uint32_t second) {
-    const auto cut = [](float v, uint32_t mask) { return __uint_as_float(__float_as_uint(v) & mask); };
-    if constexpr (NEAREST) {
-        const float u = cut(x, 0xffffe000u), v = cut(y, 0xffffe000u);
-        return __builtin_bit_cast(uint32_t, half2_t{(_Float16)(second ? x - u : u), (_Float16)(second ? y - v : v)});
-    }
-    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x - cut(x, second), y - cut(y, second)));
+// Two P as the lane's column takes them: f16(P) in the first (second = 0); in the second (1)
+// what that leaves of it, in f16 as well.
+QS_DEV uint32_t two_halves(float x, float y, float second) {
+    // Both as f32 hold them: the compiler would form the product that x is and its f16 in one
+    // instruction, which rounds once, and where x lies half way the two columns would differ.
+    asm("" : "+v"(x), "+v"(y));
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    const half2_t h = __builtin_convertvector(f32x2{x, y}, half2_t);
+    const half2_t v{(_Float16)__builtin_fmaf((float)h[0], -second, x), (_Float16)__builtin_fmaf((float)h[1], -second, y)};
+    return __builtin_bit_cast(uint32_t, v);
 }
 
 // the queries of a wave, as the scores' products take them
@@ -165,6 +165,10 @@ struct Queries {
     int first, last;                        // slots that the lane's query sees: first .. last - 1
 };
 
+// A column without a query takes the last one. No lane branches off for it: where lanes join
+// again the compiler (ROCm 7.2's) has saved registers for the joined ones alone.
+QS_DEV int column_of(const AttentionArgs& a, int column) { return min(column, a.group * a.fresh - 1); }
+
 // as they are in memory, eight of every block to a lane
 template <int BLOCKS, bool WIDE>
 struct RawQueries {
@@ -172,9 +176,8 @@ struct RawQueries {
 };
 template <int BLOCKS, bool WIDE>
 QS_DEV void load_queries(const AttentionArgs& a, int seq, int head, int first, RawQueries<BLOCKS, WIDE>& o) {
-    const int lane = threadIdx.x & 63, g = lane >> 4, column = first + (lane & 7);
-    const bool live = column < a.group * a.fresh;
-    const int token = live ? column / a.group : 0, mine = live ? column - token * a.group : 0;
+    const int lane = threadIdx.x & 63, g = lane >> 4, column = column_of(a, first + (lane & 7));
+    const int token = column / a.group, mine = column - token * a.group;
     const int64_t at = ((int64_t)seq * a.fresh + token) * a.q_stride + (int64_t)(head * a.group + mine) * 32 * BLOCKS;
 #pragma unroll
     for (int b = 0; b < BLOCKS; b++) qsr::load8<WIDE ? qs::SRC_F32 : qs::SRC_BF16>(a.q, at + 32 * b + 8 * g, o.b[b]);
@@ -182,9 +185,8 @@ QS_DEV void load_queries(const AttentionArgs& a, int seq, int head, int first, R
 template <int BLOCKS, bool WIDE>
 QS_DEV void prepare_queries(const AttentionArgs& a, int first, int length, const RawQueries<BLOCKS, WIDE>& raw,
                             Queries<BLOCKS, WIDE>& o) {
-    const int lane = threadIdx.x & 63, column = first + (lane & 7);
+    const int lane = threadIdx.x & 63, column = first + (lane & 7), token = column_of(a, column) / a.group;
     const bool live = column < a.group * a.fresh, bf16 = a.type == QS_SRC_BF16;
-    const int token = live ? column / a.group : 0;
     float x[BLOCKS][8];
     float top = 0.0f;
 #pragma unroll
@@ -223,22 +225,51 @@ QS_DEV void prepare_queries(const AttentionArgs& a, int first, int length, const
     o.first = a.window > 0 && o.last > a.window ? o.last - a.window : 0;
 }
 
-// what a wave has summed up of its slots
+// What a wave has summed up of its slots. P count by 2^power, which follows the largest |P| of
+// the query so far: 2^(TARGET - 1) or more as it counts when the power is chosen, by up to
+// 2^SLACK less while the running maximum rises, and never 2^LIMIT. A block whose own largest
+// is then below 2^(FLOOR - 1), where the second of two f16 would come to lose bits of it,
+// counts by a power of its own. (One power for the largest step seen, whatever its p and its
+// block, left blocks of small values and those beside large ones of no weight 6 to 17 bits:
+// errors up to 1e-2.) The running maximum is a whole number, so that what it takes off is a
+// power of two as well.
+//
+// What a wave pays: the powers are chosen on its first step of a segment, 0.4 us (1 of 17
+// slots 5.4 to 5.8 us, 61 ragged ones 30.2 to 32.2, 16 of 8,191 with four bits 46.3 to 47.6),
+// and seldom again: a step asks for it where the maximum rose by more than is left of the
+// slack, or a value's step could take a P to 2^LIMIT. Looking at every P of every step took
+// 16 of 8,191 slots to 52 us, choosing anew wherever the maximum rises to 55.
+constexpr int LIMIT = 15, TARGET = 11, FLOOR = 3, SLACK = 6, MOST = 60;
 template <int BLOCKS>
 struct Sums {
     f32x4 acc[BLOCKS][2];               // dims 32 block + 8 g + 2 r + e at [block][e][r]
-    float top, total;                   // running maximum, sum of p; p and P count 2^power times
-    int power;
-    uint32_t step;                      // the bits of all steps so far, or'ed
+    float top, total;                   // the running maximum, rounded up to a whole number; sum of p
+    float up;                           // 2^power
+    int slack;                          // what is left of SLACK
 };
+// When the power was chosen, each block's largest |P| was below 2^(size - 126). Few steps need
+// that: it lies in LDS, a lane's own copy 64 words apart.
+QS_DEV i16x2 size_at(const uint32_t* sizes, int i) { return __builtin_bit_cast(i16x2, sizes[64 * i]); }
 template <int BLOCKS>
-QS_DEV void clear(Sums<BLOCKS>& o) {
+QS_DEV void clear(Sums<BLOCKS>& o, uint32_t* sizes) {
 #pragma unroll
     for (int b = 0; b < BLOCKS; b++) o.acc[b][0] = o.acc[b][1] = f32x4{0, 0, 0, 0};
     o.top = -__builtin_inff();
     o.total = 0.0f;
-    o.power = 0;
-    o.step = 0;
+    o.up = (float)(INT64_C(1) << MOST);
+    o.slack = 0;
+#pragma unroll
+    for (int i = 0; i < BLOCKS / 2; i++) sizes[64 * i] = 0;
+}
+QS_DEV i16x2 both(int v) { return i16x2{(short)v, (short)v}; }
+QS_DEV i16x2 larger(i16x2 a, i16x2 b) { return __builtin_elementwise_max(a, b); }
+QS_DEV int larger_of(i16x2 v) { return max((int)v[0], (int)v[1]); }
+QS_DEV int power_of(float up) { return (int)(__float_as_uint(up) >> 23) - 127; }
+// which blocks count by their own powers, all bits, and what blocks count by
+QS_DEV i16x2 own(i16x2 size, int power) { return (i16x2)(size < both(FLOOR + 126 - power)); }
+QS_DEV i16x2 powers(i16x2 size, int power) {
+    const i16x2 m = own(size, power), alone = __builtin_elementwise_min(both(TARGET + 126) - size, both(power + MOST));
+    return (alone & m) | (both(power) & ~m);
 }
 
 // What the queries of a wave see: any of them slots first .. last - 1 at most, all of
@@ -331,33 +362,121 @@ QS_DEV void load_values(const AttentionArgs& a, const Place& at, Tile<K_BITS, V_
              a.c.page * T::KROW + (s ? at.slot1 : at.slot0) * T::VROW);
 }
 
+// The running maximum rose by `fall`, which takes as much off all earlier P; `by`: the powers
+// of two that the blocks' sums have to be multiplied by.
+template <int BLOCKS>
+QS_DEV void lower(Sums<BLOCKS>& o, int fall, i16x2 (&by)[BLOCKS / 2]) {
+    o.total = __builtin_ldexpf(o.total, -fall);
+    o.slack -= fall;
+#pragma unroll
+    for (int i = 0; i < BLOCKS / 2; i++) by[i] = both(-fall);
+}
+// The same, and chooses the powers anew where that is more than the slack or a P reaches
+// LIMIT. For other queries nothing else changes: none depends on what another one sees.
+// first: there are no sums yet.
+template <int BLOCKS, typename F>
+QS_DEV void settle(Sums<BLOCKS>& o, uint32_t* sizes, bool first, int fall, const float (&p)[8], F&& step, i16x2 (&by)[BLOCKS / 2]) {
+    const int was = power_of(o.up);
+    i16x2 now[BLOCKS / 2], most = both(0);
+#pragma unroll
+    for (int i = 0; i < BLOCKS / 2; i++) {
+        uint32_t e[2];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            float f = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; j++) f = fmaxf(f, fabsf(__builtin_fmaf(p[j], step(j, 2 * i + h), 0.0f)));
+            e[h] = __float_as_uint(f) >> 23;
+        }
+        now[i] = __builtin_bit_cast(i16x2, over_slots(e[0] | e[1] << 16, [](uint32_t u, uint32_t v) {
+            return __builtin_bit_cast(uint32_t, larger(__builtin_bit_cast(i16x2, u), __builtin_bit_cast(i16x2, v)));
+        }));
+    }
+    bool anew = true;
+    if (!first) {
+#pragma unroll
+        for (int i = 0; i < BLOCKS / 2; i++) most = larger(most, now[i] + powers(size_at(sizes, i), was));
+        anew = fall > o.slack || larger_of(most) > LIMIT + 126;
+        most = both(0);
+#pragma unroll
+        for (int i = 0; i < BLOCKS / 2; i++) {
+            const i16x2 then = size_at(sizes, i);
+            now[i] = anew ? larger(then - both(SLACK - o.slack + fall), now[i]) : then;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < BLOCKS / 2; i++) most = larger(most, now[i]);
+    const int power = anew ? min(TARGET + 126 - larger_of(most), MOST) : was;
+    if (!first) {
+        o.total = __builtin_ldexpf(o.total, -fall);
+#pragma unroll
+        for (int i = 0; i < BLOCKS / 2; i++)
+            by[i] = larger(powers(now[i], power) - powers(size_at(sizes, i), was) - both(fall), both(-126));
+    }
+#pragma unroll
+    for (int i = 0; i < BLOCKS / 2; i++) sizes[64 * i] = __builtin_bit_cast(uint32_t, now[i]);
+    o.up = __builtin_ldexpf(1.0f, power);
+    o.slack = anew ? SLACK : o.slack - fall;
+}
+// The f16 bits of the least step of a value that could take a P of the wave to LIMIT, 0
+// where a block of a query counts by a power of its own: then each step settles.
+template <int BLOCKS, int SETS>
+QS_DEV uint32_t steep_of(const Sums<BLOCKS> (&sums)[SETS], const uint32_t* sizes) {
+    float up = 0.0f;
+    bool uneven = false;
+#pragma unroll
+    for (int n = 0; n < SETS; n++) {
+        i16x2 any = both(0);
+#pragma unroll
+        for (int i = 0; i < BLOCKS / 2; i++) any |= own(size_at(sizes, n * (BLOCKS / 2) + i), power_of(sums[n].up));
+        const bool seen = sums[n].top > -__builtin_inff();
+        up = fmaxf(up, seen ? sums[n].up : 0.0f);
+        uneven |= seen & (__builtin_bit_cast(uint32_t, any) != 0);
+    }
+    // over the eight queries: lanes ^ 1, ^ 2 and, four being alike, ^ 7
+    uint32_t u = __float_as_uint(up);
+    u = max(u, qs::quad_xor<1>(u));
+    u = max(u, qs::quad_xor<2>(u));
+    u = max(u, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)u, 0x141, 0xF, 0xF, true));
+    const float least = __uint_as_float(((uint32_t)(254 + LIMIT) << 23) - u);       // 2^LIMIT / up
+    return __any(uneven) ? 0 : __builtin_amdgcn_readfirstlane(__builtin_bit_cast(uint16_t, (_Float16)least));
+}
+
 // One step: the slots start .. start + 31, in `t`. The next step's keys and values
 // (at `next`) are loaded into the registers of this one's as soon as these are done
 // with, and arrive while the other half is computed.
 // edge: some query does not see all of the slots; to it they count for nothing,
 // whatever they hold, since a lane's scores and steps are its query's own copies.
+// first: of the segment's steps of the wave.
 template <bool WIDE, int K_BITS, int V_BITS, int BLOCKS, int SETS>
-QS_DEV void attend(const AttentionArgs& a, int start, bool edge, int held, const Place& next,
-                   const Queries<BLOCKS, WIDE> (&q)[SETS], uint32_t* lds, Tile<K_BITS, V_BITS, BLOCKS>& t, Sums<BLOCKS> (&sums)[SETS]) {
+QS_DEV void attend(const AttentionArgs& a, int start, bool first, bool edge, int held, const Place& next,
+                   const Queries<BLOCKS, WIDE> (&q)[SETS], uint32_t* lds, Tile<K_BITS, V_BITS, BLOCKS>& t,
+                   Sums<BLOCKS> (&sums)[SETS], uint32_t* sizes, uint32_t& least) {
     const int lane = threadIdx.x & 63, g = lane >> 4;
     // steps of four slots, and one of them
-    typedef Codes<8 * BLOCKS> Steps4;
+    struct Steps4 {
+        u32x4 w[BLOCKS / 2];
+    };
     const auto steps_from = [&](int s, bool value, Steps4& o) {
         const uint32_t* p = lds + (s * 16 + 4 * g) * BLOCKS + (value ? 2 * BLOCKS : 0);
 #pragma unroll
-        for (int i = 0; i < 2 * BLOCKS; i += 4) {
-            const u32x4 v = *reinterpret_cast<const u32x4*>(p + i);
-#pragma unroll
-            for (int j = 0; j < 4; j++) o.w[i + j] = v[j];
-        }
+        for (int i = 0; i < BLOCKS / 2; i++) o.w[i] = *reinterpret_cast<const u32x4*>(p + 4 * i);
     };
-    const auto step_of = [](const Steps4& c, int r, int b) {
-        const int n = r * BLOCKS + b;
-        return half_of(c.w[n >> 1] >> (16 * (n & 1)));
+    const auto two_of = [](const Steps4& c, int r, int b) {
+        const int n = (r * BLOCKS + b) >> 1;
+        return c.w[n >> 2][n & 3];
     };
-    // lane after lane they are the two sixteens' steps as they lie in their pages
+    const auto step_of = [&](const Steps4& c, int r, int b) { return half_of(two_of(c, r, b) >> (16 * (b & 1))); };
+    // lane after lane they are the two sixteens' steps as they lie in their pages, four keys', then four values'
+    u16x2 large{0, 0};
 #pragma unroll
-    for (int i = 0; i < BLOCKS / 2; i++) lds[lane * (BLOCKS / 2) + i] = t.steps.w[i];
+    for (int i = 0; i < BLOCKS / 2; i++) {
+        lds[lane * (BLOCKS / 2) + i] = t.steps.w[i];
+        large = __builtin_elementwise_max(large, __builtin_bit_cast(u16x2, t.steps.w[i] & 0x7fff7fffu));
+    }
+    uint32_t largest = lane & 4 ? max((uint32_t)large[0], (uint32_t)large[1]) : 0;
+    asm volatile("" : "+v"(largest));   // from here on, in place of what it comes from
+    bool steep = largest >= least;
     qs::wave_sync<true>();
     // scores, in powers of two
     float x[SETS][2][4];
@@ -395,69 +514,93 @@ QS_DEV void attend(const AttentionArgs& a, int start, bool edge, int held, const
         }
     if (edge) {
 #pragma unroll
-        for (int n = 0; n < 8 * SETS; n++) {
-            const int set = n >> 3, s = n >> 2 & 1, r = n & 3, p = start + 16 * s + 4 * g + r;
-            if (!((held >> s & 1) && p >= q[set].first && p < q[set].last)) {
-                x[set][s][r] = -__builtin_inff();
+        for (int n = 0; n < 2 * SETS; n++) {
+            const int set = n >> 1, s = n & 1;
+            uint32_t keep[4];
 #pragma unroll
-                for (int i = 0; i < BLOCKS / 2; i++) vs[set][s].w[r * (BLOCKS / 2) + i] = 0;
+            for (int r = 0; r < 4; r++) {
+                const int p = start + 16 * s + 4 * g + r;
+                const bool sees = (bool)(held >> s & 1) & (p >= q[set].first) & (p < q[set].last);      // lanes do not branch
+                x[set][s][r] = sees ? x[set][s][r] : -__builtin_inff();
+                keep[r] = sees ? ~0u : 0u;
+            }
+#pragma unroll
+            for (int i = 0; i < BLOCKS / 2; i++) {
+                constexpr int ROW = BLOCKS / 2;     // words of a slot
+                vs[set][s].w[i] &= u32x4{keep[4 * i / ROW], keep[(4 * i + 1) / ROW], keep[(4 * i + 2) / ROW], keep[(4 * i + 3) / ROW]};
             }
         }
     }
     float p[SETS][8];
+    int fall[SETS];         // the running maximum rose by so much
+    bool rose = false;
 #pragma unroll
     for (int n = 0; n < SETS; n++) {
-        // the running maximum and the power of two
-        float top = sums[n].top;
-        uint32_t steps = 0;
+        const float was = sums[n].top;
+        float top = -__builtin_inff();
 #pragma unroll
-        for (int s = 0; s < 2; s++) {
-#pragma unroll
-            for (int r = 0; r < 4; r++) top = fmaxf(top, x[n][s][r]);
-#pragma unroll
-            for (int i = 0; i < 2 * BLOCKS; i++) steps |= vs[n][s].w[i];
-        }
-        top = max_over_slots(top);
-        steps = over_slots(steps, [](uint32_t u, uint32_t v) { return u | v; });
-        sums[n].step |= steps | steps >> 16;
-        // 2^s takes every step below 2^15. Or'ed exponents bound them all, and are over the
-        // largest by 15 at most, by 7 for steps below 2, which takes that much off 39 bits; a
-        // subnormal step, or none, counts as 2^-14.
-        const int exponent = (int)(sums[n].step >> 10 & 31), s = 29 - (exponent > 1 ? exponent : 1);
+        for (int i = 0; i < 8; i++) top = fmaxf(top, x[n][i >> 2][i & 3]);
+        top = fmaxf(was, __builtin_ceilf(max_over_slots(top)));
         const float base = top > -__builtin_inff() ? top : 0.0f;
-        // 0 where nothing was seen yet
-        const float shrink = __builtin_ldexpf(__builtin_amdgcn_exp2f(sums[n].top - base), s - sums[n].power);
+#pragma unroll
+        for (int i = 0; i < 8; i++) p[n][i] = __builtin_amdgcn_exp2f(x[n][i >> 2][i & 3] - base);
+        fall[n] = top != was ? (int)fminf(top - was, 1000.0f) : 0;      // 1000: nothing was seen yet
+        rose |= fall[n] != 0;
+        steep |= fall[n] > sums[n].slack;
         sums[n].top = top;
-        sums[n].power = s;
-        // 2^s multiplies p: in the exponent it would take bits of what is there
-        const float power = __uint_as_float((uint32_t)(127 + s) << 23);
+    }
+    const bool moves = __any(steep | rose), moved = moves && !first;
+    i16x2 by[SETS][BLOCKS / 2];
+    if (moves) {
+        if (__any(steep)) {
+#pragma unroll
+            for (int n = 0; n < SETS; n++)
+                settle(sums[n], sizes + 32 * BLOCKS * n, first, fall[n], p[n], [&](int i, int b) {
+                    // a copy: the compiler would keep all steps as f32 for what follows
+                    uint32_t two = two_of(vs[n][i >> 2], i & 3, b);
+                    asm volatile("" : "+v"(two));
+                    return half_of(two >> (16 * (b & 1)));
+                }, by[n]);
+            least = steep_of(sums, sizes);
+        } else {
+#pragma unroll
+            for (int n = 0; n < SETS; n++) lower(sums[n], fall[n], by[n]);
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < SETS; n++) {
         float total = 0.0f;
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            p[n][i] = __builtin_amdgcn_exp2f(x[n][i >> 2][i & 3] - base) * power;
             total += p[n][i];
+            p[n][i] *= sums[n].up;
         }
-        sums[n].total = __builtin_fmaf(sums[n].total, shrink, total);
-        if (__any(shrink != 1.0f)) {
-#pragma unroll
-            for (int b = 0; b < BLOCKS; b++)
-#pragma unroll
-                for (int e = 0; e < 2; e++)
-#pragma unroll
-                    for (int r = 0; r < 4; r++) sums[n].acc[b][e][r] *= shrink;
-        }
+        sums[n].total += total;
     }
-    const uint32_t second = lane & 8 ? 0xffffe000u : 0u;
+    const float second = lane & 8 ? 1.0f : 0.0f;
 #pragma unroll
     for (int b = 0; b < BLOCKS; b++) {
         u32x4 w[SETS];
 #pragma unroll
-        for (int n = 0; n < 4 * SETS; n++) {
-            const int set = n >> 2, i = 2 * (n & 3);
-            const Steps4& d = vs[set][i >> 2];
+        for (int n = 0; n < SETS; n++) {
+            if (moved) {
+                const float f = __builtin_ldexpf(1.0f, by[n][b >> 1][b & 1]);
+#pragma unroll
+                for (int i = 0; i < 8; i++) sums[n].acc[b][i >> 2][i & 3] *= f;
+            }
+            if (__builtin_expect(least == 0, 0)) {      // p goes on to this block's power
+                const int power = power_of(sums[n].up);
+                const auto at = [&](int b) { return b < 0 ? power : powers(size_at(sizes, (n * BLOCKS + b) >> 1), power)[b & 1]; };
+                const float f = __builtin_ldexpf(1.0f, at(b) - at(b - 1));
+#pragma unroll
+                for (int i = 0; i < 8; i++) p[n][i] *= f;
+            }
+            float u[8];
             // + 0 makes it one instruction that takes the step as f16
-            w[set][n & 3] = two_halves<WIDE>(__builtin_fmaf(p[set][i], step_of(d, i & 3, b), 0.0f),
-                                             __builtin_fmaf(p[set][i + 1], step_of(d, (i & 3) + 1, b), 0.0f), second);
+#pragma unroll
+            for (int i = 0; i < 8; i++) u[i] = __builtin_fmaf(p[n][i], step_of(vs[n][i >> 2], i & 3, b), 0.0f);
+#pragma unroll
+            for (int i = 0; i < 4; i++) w[n][i] = two_halves(u[2 * i], u[2 * i + 1], second);
         }
 #pragma unroll
         for (int e = 0; e < 2; e++) {
@@ -472,19 +615,19 @@ QS_DEV void attend(const AttentionArgs& a, int start, bool edge, int held, const
     load_values(a, next, t);
 }
 
-// The wave's sums as one: the four lanes of a query's slots, and its two columns;
-// p counts 2^power times.
+// The wave's sums as one: the four lanes of a query's slots, and its two columns; what
+// P count by.
 template <int BLOCKS>
-QS_DEV void finish(Sums<BLOCKS>& o) {
-    const float once = __builtin_ldexpf(1.0f, -o.power);
-    o.total = sum_over_slots(o.total) * once;
+QS_DEV void finish(Sums<BLOCKS>& o, const uint32_t* sizes) {
+    o.total = sum_over_slots(o.total);
 #pragma unroll
-    for (int b = 0; b < BLOCKS; b++)
+    for (int b = 0; b < BLOCKS; b++) {
+        const float once = __builtin_ldexpf(1.0f, -powers(size_at(sizes, b >> 1), power_of(o.up))[b & 1]);
 #pragma unroll
         for (int e = 0; e < 2; e++)
 #pragma unroll
-            for (int r = 0; r < 4; r++)
-                o.acc[b][e][r] = (o.acc[b][e][r] + other_column(o.acc[b][e][r])) * once;
+            for (int r = 0; r < 4; r++) o.acc[b][e][r] = (o.acc[b][e][r] + other_column(o.acc[b][e][r])) * once;
+    }
 }
 
 QS_DEV int cut_length(const AttentionArgs& a, int n) {
@@ -561,7 +704,9 @@ void k_kv_attention(AttentionArgs a, Split split) {
     __shared__ __attribute__((aligned(16))) float acc[WAVES][COLUMNS][ROW];
     __shared__ float2 stats[WAVES][COLUMNS];
     __shared__ __attribute__((aligned(16))) uint32_t steps_lds[WAVES][TILE * BLOCKS];
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane >> 4;
+    __shared__ uint32_t sizes[WAVES][SETS * BLOCKS / 2][64];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const auto sizes_of = [&](int n) { return &sizes[wave][n * (BLOCKS / 2)][threadIdx.x & 63]; };
     const int tiles = (a.group * a.fresh + COLUMNS - 1) / COLUMNS, heads = a.c.heads * tiles;
     int64_t at = 0, end = 1, each = 0;
     int seq, base = 0, which = -1, from = 0;        // which: head and column tile
@@ -604,7 +749,7 @@ void k_kv_attention(AttentionArgs a, Split split) {
 #pragma unroll
         for (int n = 0; n < SETS; n++) {
             load_queries(a, seq, head, first + 8 * n, raw[n]);
-            clear(sums[n]);
+            clear(sums[n], sizes_of(n));
         }
         const Ints table = constant(a.tables + seq * a.table_stride);
         // The wave's steps i, i + stride, ... before `stop`, counted from the sequence's
@@ -641,18 +786,24 @@ void k_kv_attention(AttentionArgs a, Split split) {
             const int final = i + (stop - 1 - i) / stride * stride;
             const auto start_of = [&](int n) { return (n < final ? n : final) * TILE; };
             Queries<BLOCKS, WIDE> q[SETS];
+            uint32_t least = 0;
 #pragma unroll
             for (int n = 0; n < SETS; n++) prepare_queries(a, first + 8 * n, length, raw[n], q[n]);
-            for (; i < stop; i += stride) {
+            for (bool opens = true; i < stop; i += stride, opens = false) {
                 const int start = i * TILE, held = place.held;
                 place = place_of(a, ahead, head, start_of(i + stride));
                 ahead = pages_of(a, table, start_of(i + 2 * stride));
-                attend(a, start, start < span.all_first || start + TILE > span.all_last || held != 3, held, place, q, steps_lds[wave], t, sums);
+                const bool edge = start < span.all_first || start + TILE > span.all_last || held != 3;
+                attend(a, start, opens, edge, held, place, q, steps_lds[wave], t, sums, sizes_of(0), least);
             }
         }
+        // anew from here, so that no step holds registers for the addresses of what follows
+        int thread = (int)threadIdx.x;
+        asm volatile("" : "+v"(thread));
+        const int lane = thread & 63, g = lane >> 4;
 #pragma unroll
         for (int n = 0; n < SETS; n++) {
-            finish(sums[n]);
+            finish(sums[n], &sizes[wave][n * (BLOCKS / 2)][lane]);
             if (lane & 8) continue;
             const int column = 8 * n + (lane & 7);
 #pragma unroll
@@ -668,9 +819,10 @@ void k_kv_attention(AttentionArgs a, Split split) {
         __syncthreads();
         const bool whole = SHARE ? split.share == 1 : from == 0 && to == steps.count;
         // thread: two dims of every 64 of a column, or of one after another
-        const int sub = threadIdx.x & 31;
+        const int sub = thread & 31;
 #pragma unroll
-        for (int column = threadIdx.x >> 5; column < COLUMNS; column += 2 * WAVES) {
+        for (int k = 0; k < COLUMNS; k += 2 * WAVES) {
+            const int column = k + (thread >> 5);
             float ref = -__builtin_inff(), total = 0.0f, part[WAVES];
 #pragma unroll
             for (int w = 0; w < WAVES; w++) ref = fmaxf(ref, stats[w][column].x);

@@ -97,3 +97,118 @@ def test_small_terms_of_scores_beside_large_ones(qs, dtype, kind, below, d):
     want, size = (p * v).sum(0), (p * v.abs()).sum(0)
     far = (2 * (2 * e_s + 4 * U)[:, None] + 2.0 ** -21 + 2 * (2 + 96) * U) * size
     ref.check(y[0, 0], want, far + half_spacing(want.abs() + far, dtype))
+
+
+def weighted(qs, cache, scores, v, queries, dtype, length=None, batch=2):
+    """Attention over rows whose keys are one value, so that a score is one product: sequences of the same rows, the
+    `queries` of a head 1, 1/2, 1/4 ... in the key's place. Returns y and the result in 64 bits with what an
+    f32 computation may be off by: a score by four roundings, the rest as in ref.attention64; a slot's P to 2^-21."""
+    n, heads, d = v.shape
+    k = torch.zeros((n, heads, d))
+    k[:, :, 0] = scores if scores.dim() == 2 else scores[:, None]
+    rows, table = held(qs, cache, k, v)
+    q = torch.zeros((batch, 1, heads * queries, d))
+    q[..., 0] = 2.0 ** -torch.arange(queries).repeat(heads)
+    length = n if length is None else length
+    y = qs.kv_attention(q.to(DEV, dtype), cache, table.expand(batch, -1), ints(*[length] * batch), scale=1.0)
+    s = (rows[0][0][:length, :, None, :1] * q[0, 0].view(heads, queries, d)[None, :, :, :1].double())[..., 0]
+    far = 2 * (2 * 4 * U * s.abs().amax(0) + 4 * U) + 2.0 ** -21 + 2 * (length / 32 + 96) * U
+    p = torch.softmax(s, 0)
+    vv = rows[0][1][:length, :, None]
+    want, size = (p[..., None] * vv).sum(0), (p[..., None] * vv.abs()).sum(0)
+    want, far = want.view(heads * queries, d), (far[..., None] * size).view(heads * queries, d)
+    return y[:, 0], want.expand(batch, -1, -1), (far + half_spacing(want.abs() + far, dtype)).expand(batch, -1, -1)
+
+
+@pytest.mark.parametrize("kind", ["q8_0", "q4_0"])
+@pytest.mark.parametrize("seed", range(4))
+def test_two_slots_of_many_heads(qs, kind, seed):
+    """So many P that some of them round to half way between two f16: both parts of such a one belong together."""
+    scores = torch.randn((2, 512), generator=torch.Generator().manual_seed(seed)) * 2
+    ref.check(*weighted(qs, qs.KVCache(1, 16, 512, 64, "q8_0", kind), scores, positive(2, 512, 64, seed), 8, torch.float32, batch=1))
+
+
+def positive(n, heads, d, seed):
+    return torch.randn((n, heads, d), generator=torch.Generator().manual_seed(seed)).abs() + 0.1
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kind", ["q8_0", "q4_0"])
+@pytest.mark.parametrize("d", [64, 128, 192, 256])
+@pytest.mark.parametrize("large,small", [(60.0, 1.0), (100.0, 0.02), (1e4, 1e-2)])
+def test_blocks_of_other_sizes(qs, dtype, kind, d, large, small):
+    """A block of small values is as exact as if there were no large ones beside it."""
+    v = positive(760, 2, d, 1)
+    v[..., 32:] *= small
+    v[..., :32] *= large
+    scores = torch.randn(760, generator=torch.Generator().manual_seed(2)) * 2
+    ref.check(*weighted(qs, qs.KVCache(48, 16, 2, d, "q8_0", kind), scores, v, 4, dtype))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kind", ["q8_0", "q4_0"])
+@pytest.mark.parametrize("queries", [4, 12])
+@pytest.mark.parametrize("at", [(7, 500), (0, 1), (758, 759)])
+@pytest.mark.parametrize("times", [5e3, 1e6])
+def test_large_values_of_no_weight(qs, dtype, kind, queries, at, times):
+    """Two slots whose scores are 60 below the others' do not show, however large their values."""
+    v = positive(760, 2, 128, 3) * 0.02
+    scores = torch.randn(760, generator=torch.Generator().manual_seed(4))
+    for i in at:
+        v[i] *= times
+        scores[i] = -60.0
+    ref.check(*weighted(qs, qs.KVCache(48, 16, 2, 128, "q8_0", kind), scores, v, 1 if queries == 4 else queries, dtype))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kind", ["q8_0", "q4_0"])
+@pytest.mark.parametrize("d", [64, 128, 192, 256])
+@pytest.mark.parametrize("queries", [3, 13])
+@pytest.mark.parametrize("slope", [-40.0, -8.0, 0.0, 8.0, 40.0])
+def test_sizes_that_change_along_a_sequence(qs, dtype, kind, d, queries, slope):
+    """Scores that rise or fall, and blocks whose values rise, fall, or are nothing for a while, over six steps of
+    each wave, and over one."""
+    n = 760
+    v = positive(n, 2, d, 5)
+    along = torch.linspace(-1, 1, n)[:, None, None]
+    for b in range(d // 32):
+        part = v[..., 32 * b:32 * b + 32]
+        part *= (10.0 ** (2 * along), 10.0 ** (-2 * along), torch.ones_like(along), (along > 0.3).float(), (along < -0.3).float(),
+                 torch.zeros_like(along), 10.0 ** (3 * along.abs() - 3), (along.abs() < 0.001).float())[(b + 3) % 8]
+    scores = torch.linspace(0, 1, n) * slope + torch.randn(n, generator=torch.Generator().manual_seed(6))
+    cache = qs.KVCache(48, 16, 2, d, "q8_0", kind)
+    for length in (n, 130):
+        ref.check(*weighted(qs, cache, scores, v, queries, dtype, length))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kind", ["q8_0", "q4_0"])
+@pytest.mark.parametrize("d", [64, 128, 192, 256])
+def test_a_block_of_nan_beside_numbers(qs, dtype, kind, d):
+    """A NaN in a value that a query sees makes its block of the result NaN, and nothing of the others less exact."""
+    v = positive(300, 2, d, 7) * 0.05
+    v[100, :, 3] = math.nan
+    scores = torch.randn(300, generator=torch.Generator().manual_seed(8)) * 3
+    y, want, far = weighted(qs, qs.KVCache(20, 16, 2, d, "q8_0", kind), scores, v, 4, dtype)
+    assert y[..., :32].isnan().all()
+    ref.check(y[..., 32:], want[..., 32:], far[..., 32:])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("bad", [math.nan, 3e4])
+def test_what_another_query_sees_does_not_matter(qs, dtype, bad):
+    """Bit for bit: keys and values of the last new tokens, of a window's slots before an earlier one's, of nothing."""
+    cache = qs.KVCache(9, 16, 2, 128, "q8_0", "q8_0")
+    k, v = ref.keys_values(100, 2, 128, torch.float32, 9)
+    rows, table = held(qs, cache, k, v)
+    q = torch.randn((1, 4, 6, 128), generator=torch.Generator().manual_seed(10)).to(DEV, dtype)
+    for window in (0, 20):
+        y = qs.kv_attention(q, cache, table, ints(100), window=window)
+        kept = cache.data.clone()
+        at = [98, 99, 100, 120] + ([0, 60, 76] if window else [])       # the first one sees those above 96 - window
+        x = torch.full((len(at), 2, 128), bad, device=DEV)
+        qs.kv_write(cache, x, x, ints(*at))
+        z = qs.kv_attention(q, cache, table, ints(100), window=window)
+        assert torch.equal(z[:, :2], y[:, :2])
+        assert not torch.equal(z[:, 2:], y[:, 2:])
+        cache.data.copy_(kept)
