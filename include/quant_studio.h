@@ -296,7 +296,8 @@ int64_t qs_kv_attention_workspace(const qs_kv_cache *cache, int64_t batch, int64
  *   workspace: qs_kv_attention_workspace() bytes, 256-byte aligned, used by this
  *              call alone until it is done; may be NULL where that is 0
  * Tables and lengths must not change until the call's work is done.
- * A query that sees no position gives zeros; what lies at positions that it does
+ * A query that sees no position gives zeros, one whose scores are all -infinity (its
+ * own infinities, or sums out of f32's range) NaN; what lies at positions that it does
  * not see does not matter, whatever it is. Sums and statistics are f32; q is held to
  * 22 bits or more beside its row's largest value, p times a step of V to 21
  * beside the largest of its block of 32 values of the head. The result does not depend on timing; in the last bits of f32 it

@@ -42,6 +42,13 @@ inline __host__ __device__ int column_tiles(const AttentionArgs& a) {
 constexpr int CODE_POWER = 9;
 constexpr float ONCE = 1 << CODE_POWER;
 
+// A running maximum is -infinity where a query sees nothing, else LOWEST or more. What its sums
+// are to be multiplied by: nothing seen gives zeros, scores of -infinity alone give no values.
+constexpr float LOWEST = -0x1.fffffep127f;
+QS_DEV float inverse_of(float top, float total) {
+    return total != 0.0f ? ONCE / total : top >= LOWEST ? __builtin_nanf("") : 0.0f;
+}
+
 // How a call's work is split, and where its workgroups leave what is joined.
 constexpr int TILE = 32;            // slots of a wave's step
 // Steps of its waves that a workgroup takes as long to begin with another segment: 61 ragged

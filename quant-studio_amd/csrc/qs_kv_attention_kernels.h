@@ -512,7 +512,12 @@ QS_DEV void attend(const AttentionArgs& a, int start, bool first, bool edge, int
             if (n == 0) steps_from(s, true, vs[0][s]);
             else vs[n][s] = vs[0][s];
         }
+    float lowest[SETS];     // of a maximum over slots of which some are seen: scores may all be -infinity
+#pragma unroll
+    for (int n = 0; n < SETS; n++) lowest[n] = LOWEST;
     if (edge) {
+#pragma unroll
+        for (int n = 0; n < SETS; n++) lowest[n] = -__builtin_inff();
 #pragma unroll
         for (int n = 0; n < 2 * SETS; n++) {
             const int set = n >> 1, s = n & 1;
@@ -523,6 +528,7 @@ QS_DEV void attend(const AttentionArgs& a, int start, bool first, bool edge, int
                 const bool sees = (bool)(held >> s & 1) & (p >= q[set].first) & (p < q[set].last);      // lanes do not branch
                 x[set][s][r] = sees ? x[set][s][r] : -__builtin_inff();
                 keep[r] = sees ? ~0u : 0u;
+                lowest[set] = sees ? LOWEST : lowest[set];
             }
 #pragma unroll
             for (int i = 0; i < BLOCKS / 2; i++) {
@@ -537,7 +543,7 @@ QS_DEV void attend(const AttentionArgs& a, int start, bool first, bool edge, int
 #pragma unroll
     for (int n = 0; n < SETS; n++) {
         const float was = sums[n].top;
-        float top = -__builtin_inff();
+        float top = lowest[n];
 #pragma unroll
         for (int i = 0; i < 8; i++) top = fmaxf(top, x[n][i >> 2][i & 3]);
         top = fmaxf(was, __builtin_ceilf(max_over_slots(top)));
@@ -834,7 +840,7 @@ void k_kv_attention(AttentionArgs a, Split split) {
             }
             const int64_t row = row_of(a, seq, head, first + column);
             const int64_t slot = ((int64_t)blockIdx.x * 2 + (from == 0)) * COLUMNS + column;
-            const float inverse = total != 0.0f ? ONCE / total : 0.0f;    // 0: it sees nothing
+            const float inverse = inverse_of(ref, total);
 #pragma unroll
             for (int i = 0; i < BLOCKS / 2; i++) {
                 float2 v{0, 0};

@@ -87,7 +87,7 @@ __global__ __launch_bounds__(THREADS) void k_kv_join(AttentionArgs a, Split spli
 #pragma unroll
         for (int e = 0; e < 4; e++) sum[e] = __builtin_fmaf(acc[i][threadIdx.x][e], is, sum[e]);
     }
-    const float inverse = total != 0.0f ? ONCE / total : 0.0f;
+    const float inverse = inverse_of(ref, total);
     store_two(a, row + 4 * threadIdx.x, sum[0] * inverse, sum[1] * inverse);
     store_two(a, row + 4 * threadIdx.x + 2, sum[2] * inverse, sum[3] * inverse);
 }

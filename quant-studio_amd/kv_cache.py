@@ -200,8 +200,8 @@ def kv_attention(q, cache: KVCache, tables, lengths, scale: float | None = None,
     a page that is not in the cache, such as -1, are seen by no query.
     lengths: (b,) int32, the new tokens counted, cut to 0 .. m * page_size. Token i of
     n is at position P = length - n + i and sees positions up to P, with a window those
-    above P - window; one that sees none gives zeros. What lies at other positions
-    does not matter, whatever it is.
+    above P - window; one that sees none gives zeros, one whose scores are all
+    -infinity NaN. What lies at other positions does not matter, whatever it is.
     scale: 1 / sqrt(head_dim) by default.
     out: a contiguous tensor of q's shape and type to write instead of a new one."""
     lib = _lib()

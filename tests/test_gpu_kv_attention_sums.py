@@ -195,6 +195,29 @@ def test_a_block_of_nan_beside_numbers(qs, dtype, kind, d):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("length,columns", [(2, 1), (40, 3), (40, 70), (700, 70)])
+@pytest.mark.parametrize("value,scale", [(-math.inf, 0.1), (math.inf, -0.1), (-2.0, math.inf), (2.0, -math.inf), (-2e38, 1e3)])
+def test_scores_that_are_all_minus_infinity(qs, dtype, length, columns, value, scale):
+    """NaN, as the softmax of them is, and zeros only where a query sees nothing: the first of three new tokens of two."""
+    if dtype == torch.float16 and abs(value) > 1e30 and value > -math.inf and value < math.inf:
+        pytest.skip("no such f16")
+    cache = qs.KVCache(70, 16, 2, 64, "q8_0", "q4_0")
+    k, v = torch.zeros((length, 2, 64)), torch.randn((length, 2, 64), generator=torch.Generator().manual_seed(1))
+    k[..., 0] = torch.rand((length, 2), generator=torch.Generator().manual_seed(2)) + 1
+    if abs(value) == math.inf:      # a zero of a key would make the score NaN
+        k += 1
+    qs.kv_write(cache, k.to(DEV), v.to(DEV), torch.arange(length, dtype=torch.int32, device=DEV))
+    q = torch.zeros((1, 3, 4, 64))
+    q[..., 0] = value
+    q[:, :, 3, 0] = 0.5 if abs(scale) < 1e3 else value
+    y = qs.kv_attention(q.to(DEV, dtype), cache, torch.arange(columns, dtype=torch.int32, device=DEV)[None], ints(length), scale=scale)
+    sees = torch.arange(3) >= 3 - length
+    assert torch.equal(y.isnan().all(3).cpu()[0, :, :3], sees[:, None].expand(3, 3)) and not y[:, ~sees].any()
+    if abs(scale) < 1e3:
+        assert not y[:, :, 3].isnan().any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("bad", [math.nan, 3e4])
 def test_what_another_query_sees_does_not_matter(qs, dtype, bad):
     """Bit for bit: keys and values of the last new tokens, of a window's slots before an earlier one's, of nothing."""
