@@ -219,8 +219,9 @@ QS_DEV void prepare_queries(const AttentionArgs& a, int first, int length, const
             if constexpr (WIDE) o.lo[b][i] = __builtin_bit_cast(uint32_t, l);
         }
     }
-    o.scale = a.scale * LOG2E;
-    o.up = CODE_POWER - e;
+    // a mantissa and a power of two: scale log2(e) itself may pass f32's range where no score does
+    o.scale = __builtin_amdgcn_frexp_mantf(a.scale) * LOG2E;
+    o.up = CODE_POWER - e + __builtin_amdgcn_frexp_expf(a.scale);
     o.last = length - a.fresh + 1 + token;
     o.first = a.window > 0 && o.last > a.window ? o.last - a.window : 0;
 }

@@ -217,6 +217,19 @@ def test_scores_that_are_all_minus_infinity(qs, dtype, length, columns, value, s
         assert not y[:, :, 3].isnan().any()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("power", [127, 120, -120, -130])
+def test_scales_near_the_ends_of_f32(qs, dtype, power):
+    """Where scale log2(e) is out of range, and where scale is subnormal, scores of usual sizes are right."""
+    cache = qs.KVCache(13, 16, 2, 64, "q8_0", "q4_0")
+    k, v = ref.keys_values(200, 2, 64, torch.float32, 11)
+    rows, table = held(qs, cache, k, v)
+    q = (torch.randn((1, 2, 6, 64), generator=torch.Generator().manual_seed(12)) * 2.0 ** (-power - 3)).to(DEV, dtype)
+    scale = 1.5 * 2.0 ** power
+    want, far = bound(q, rows, scale)
+    ref.check(qs.kv_attention(q, cache, table, ints(200), scale=scale), want, far)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("bad", [math.nan, 3e4])
 def test_what_another_query_sees_does_not_matter(qs, dtype, bad):
