@@ -11,7 +11,7 @@ The reference ends at the GGUF file and has none of this. Every function is one
 call into the gfx950 library (C ABI in include/quant_studio.h) on torch's current
 stream; nothing is synchronised, and every failure raises. These are serving
 forms: codes carry no gradient, and a tensor that requires one is refused while
-gradients are recorded.
+gradients are recorded, one with a tangent of forward mode always.
 """
 
 from __future__ import annotations
@@ -23,13 +23,13 @@ from . import packed
 from .packed import _call, _device_of, _fail, _no_gradient, _same_device, _type_id
 
 _TYPES = {"q8_0": 8, "q4_0": 2}         # QS_TYPE_* of include/quant_studio.h
-torch = None
+torch = forward_ad = None
 
 
 def _lib():
-    global torch
+    global torch, forward_ad
     lib = packed._lib()
-    torch = packed.torch
+    torch, forward_ad = packed.torch, packed.forward_ad
     return lib
 
 
@@ -135,7 +135,7 @@ def kv_write(cache: KVCache, k, v, slots) -> None:
     step over float16's largest number makes the values of its block of 32 NaN."""
     lib = _lib()
     src = _type_id(k.dtype, "kv_write")
-    if k.requires_grad or v.requires_grad:
+    if k.requires_grad or v.requires_grad or forward_ad._current_level >= 0:
         _no_gradient("kv_write", "k", k)
         _no_gradient("kv_write", "v", v)
     dev = cache._dev
@@ -206,7 +206,7 @@ def kv_attention(q, cache: KVCache, tables, lengths, scale: float | None = None,
     out: a contiguous tensor of q's shape and type to write instead of a new one."""
     lib = _lib()
     kind = _type_id(q.dtype, "kv_attention")
-    if q.requires_grad:
+    if q.requires_grad or forward_ad._current_level >= 0:
         _no_gradient("kv_attention", "q", q)
     dev, d = cache._dev, cache.head_dim
     if q.get_device() != dev:

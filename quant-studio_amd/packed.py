@@ -10,7 +10,8 @@ The reference ends at the GGUF file and has none of this. Every function is
 calls into the gfx950 library (C ABI in include/quant_studio.h) on torch's
 current stream; nothing is synchronised, and every failure raises. These are
 serving forms: 8-bit rows and packed weights carry no gradient, and a tensor that
-requires one is refused while gradients are recorded.
+requires one is refused while gradients are recorded, one with a tangent of forward
+mode always.
 
 A decode step makes hundreds of these calls, each a few microseconds of GPU
 work, so what Python does per call counts as much: devices are compared as
@@ -22,19 +23,21 @@ from __future__ import annotations
 import ctypes
 
 torch = None            # imported with the library when a function is first called
+forward_ad = None       # torch's forward mode, likewise
 _L = None
 _TYPE_ID: dict = {}     # dtype -> source type id of the C ABI
 _EXACT = 0x100          # QS_EXACT of include/quant_studio.h
 
 
 def _lib():
-    global torch, _L
+    global torch, forward_ad, _L
     if _L is None:
         import torch as t
+        from torch.autograd import forward_ad as f
         from . import library
         lib = library()
         _TYPE_ID.update({t.float32: 0, t.float16: 1, t.bfloat16: 30})
-        torch, _L = t, lib
+        torch, forward_ad, _L = t, f, lib
     return _L
 
 
@@ -65,6 +68,9 @@ def _no_gradient(what: str, name: str, x) -> None:
     if x.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{what}: {name} requires a gradient and there is no gradient through 8-bit rows: "
                          "detach it, or call under torch.no_grad()")
+    # a tangent is carried whether gradients are recorded or not; outside of forward mode there are none
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(x).tangent is not None:
+        raise ValueError(f"{what}: {name} has a tangent and there is no gradient through 8-bit rows: detach it")
 
 
 def _call(dev: int, fn, *args) -> None:
