@@ -125,22 +125,6 @@ QS_DEV void quad_store_nibbles(const uint32_t (&w)[2], int q, uint8_t* o) {
     }
 }
 
-// level of a value of Q4_0 (offset 8.5, top 15.5) or Q5_0 (16.5, 31.5):
-// clamp(floor(t), 0, top) == trunc(clamp(t, 0, top + 0.5)): truncation is floor
-// on [0, top + 0.5] (NaN clamps to 0 either way)
-QS_DEV uint32_t level_of(float x, float id, float offset, float top) {
-    float t = x * id;
-    t = t + offset;
-    return (uint32_t)clampf(t, 0.0f, top);
-}
-// code of a value of Q8_0: round half away from zero (C roundf). Where 1/d
-// overflowed (d below 127 * 2^-128) x * id is infinite or NaN: saturate to
-// [-128, 127], NaN to 0, instead of an undefined conversion
-QS_DEV int code_of(float x, float id) {
-    const float r = roundf(x * id);
-    return r == r ? (int)clampf(r, -128.0f, 127.0f) : 0;
-}
-
 // one block, four lanes: lane quarter q holds values 8q..8q+7 and writes its
 // share of the block's bytes at o (LDS, block start, 2-byte aligned)
 template <B32 T>
@@ -156,7 +140,11 @@ QS_DEV void b32_block(const float (&x)[8], int q, uint8_t* o) {
         uint32_t l[8], w[2], h5 = 0;
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            l[i] = level_of(x[i], id, OFF, TOP);
+            float t = x[i] * id;
+            t = t + OFF;
+            // clamp(floor(t), 0, top) == trunc(clamp(t, 0, top + 0.5)): truncation
+            // is floor on [0, top + 0.5] (NaN clamps to 0 either way)
+            l[i] = (uint32_t)clampf(t, 0.0f, TOP);
             if constexpr (T == B32::Q5_0) h5 |= (l[i] >> 4) << i;
         }
         bytes_of(l, w);
@@ -206,7 +194,12 @@ QS_DEV void b32_block(const float (&x)[8], int q, uint8_t* o) {
         uint32_t w[2] = {0u, 0u};
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            w[i >> 2] |= ((uint32_t)code_of(x[i], id) & 0xffu) << (8 * (i & 3));
+            // where 1/d overflowed (d below 127 * 2^-128) x * id is infinite or
+            // NaN: saturate to [-128, 127], NaN to 0, instead of an undefined
+            // conversion
+            const float r = roundf(x[i] * id);
+            const int v = r == r ? (int)clampf(r, -128.0f, 127.0f) : 0;
+            w[i >> 2] |= ((uint32_t)v & 0xffu) << (8 * (i & 3));
         }
         if (q == 0) o16[0] = (uint16_t)f16_bits(d);
         uint16_t* p = reinterpret_cast<uint16_t*>(o + 2 + 8 * q);

@@ -165,6 +165,8 @@ QS_DEV float peak_of(const float (&x)[8], int quarter) {
 // Codes of eight values as the cache holds them, and their block's step, which four
 // threads find together: eight bits as two words of four codes each; four bits as a
 // word of four pairs, a key's (0, 2) (4, 6) (1, 3) (5, 7), a value's (0, 1) (2, 3) ...
+// The steps and roundings are those of the quantizers' b32_block, in other instructions; the
+// tests compare them bit for bit, at ties too.
 template <int SRC>
 QS_DEV float codes_of(const Eight<SRC>& in, const Unit& u, uint32_t (&code)[2]) {
     float x[8];
