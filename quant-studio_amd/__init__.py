@@ -383,7 +383,8 @@ from .packed import (AdapterBank, PackedWeight, Q8Rows, packed_linear, q8_rows, 
 # a quantised key-value cache and the attention over it
 from .kv_cache import KVCache, kv_attention, kv_read, kv_write  # noqa: E402
 
-__all__ = ["KVCache", "kv_attention", "kv_read", "kv_write", "AdapterBank", "PackedWeight", "Q8Rows", "packed_linear", "q8_rows", "rms_norm_q8",
+__all__ = ["KVCache", "kv_attention", "kv_read", "kv_write",
+           "AdapterBank", "PackedWeight", "Q8Rows", "packed_linear", "q8_rows", "rms_norm_q8",
            "QUANT_TYPES", "ALL_SPECS", "QuantSpec", "QuantSpecError", "TORCH_DTYPES",
            "GGMLQuantizationType", "LlamaFileType", "library", "quantize", "row_bytes", "init",
            "set_sqrt_rounding", "sqrt_rounding"]

@@ -26,7 +26,7 @@ namespace qskv {
 using qs::u32x2;
 using qs::u32x4;
 
-// a cache as the kernels see it; `row` of K or V: code bytes of a slot's row
+// a cache as the kernels see it
 struct Cache {
     uint8_t* data;
     int64_t page_bytes;

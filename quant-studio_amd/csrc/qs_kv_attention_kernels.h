@@ -680,7 +680,7 @@ QS_DEV Deal deal(const AttentionArgs& a, int groups, int waves, int opening, int
         sum += seq < a.batch ? units_of(a, opening, seq) : 0;
     }
     const int scan = qs::wave_incl_scan(sum);
-    Deal d;
+    Deal d{};
     d.total = (int64_t)__builtin_amdgcn_readlane(scan, 63) * heads;
     d.each = quotient(d.total + groups - 1, groups);
     d.each = d.each < waves ? waves : d.each;
