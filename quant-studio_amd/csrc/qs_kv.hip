@@ -89,7 +89,11 @@ constexpr int BATCH = 4;
 // at a time: 1,000 rows of eight heads of 128 read in 4.2 us, 4.4 in batches; 4,000 of one
 // head 3.6 and 4.4; but 2,100 of eight heads 6.1 and 5.1.
 constexpr int FEW_ROWS = 4096, HELD = 2048;
-// rows of a launch that writes: what a workgroup looks its slots up among, a turn of four for each thread
+// Rows of a launch that writes: what a workgroup looks its slots up among, a turn of four for
+// each thread. Twice as many are better for narrow rows and worse for wide ones, which have
+// more threads that look: 65,535 rows of one head of 64, written and read back, 101 us, 121
+// with 4,096 and 76 with 16,384; 8,191 of eight heads of 128 30.1, 34.3 and 33.0, 32,767
+// 119, 128 and 122.
 constexpr int64_t MOST_ROWS = 8192;
 constexpr int WRITERS = 512;      // threads of a workgroup that writes many rows
 struct Shape {
@@ -507,20 +511,23 @@ Split split_of(const AttentionArgs& a, void* workspace) {
     // longest sequences would not give each a step for every wave.
     //
     // Sequences of `whole` steps at most are not split: one segment to a workgroup, so that
-    // nothing is joined. Of 8 heads of 128 in 8 bits: 8 sequences of 600 slots take 10.9 us,
-    // 13.0 split, 40 take 17.8, 23.7 split, 150 take 47, 56 split (ragged ones 36, 33 split);
-    // of 900 slots 40 ragged ones 16.0 and 20.5, but 150 take 48.6 and 38.2. A lone one of
-    // 290 slots takes 7.7, 8.2 split, of 420 slots 8.9 and 8.6.
+    // nothing is joined. Of 8 heads of 128 in 8 bits: 8 sequences of 600 slots take 13.0 us,
+    // 13.9 split, 40 take 19.9, 25.0 split, 150 take 45.4, 56.8 split (ragged ones 28.2, 36.7
+    // split); but 8 of 900 slots 17.3 and 16.3, ragged ones 16.4 and 13.4. A lone one of
+    // 290 slots takes 9.0, 9.1 split, of 420 slots 10.7 and 9.4. Longer ones are whole where
+    // there are so many that the longest cannot take much longer than all together: 40 of 900
+    // slots 25.5, 29.4 split (ragged ones 18.4, 21.6 split), 150 of 1,500 slots 97 and 111
+    // (ragged 49 and 54), 600 of 1,200 slots 304 and 347; 65 ragged ones of 1,300 30.8 and 29.4.
     //
     // A lone sequence is in equal parts, which each workgroup knows before it knows the
     // length; more of them are in equal runs of all their steps, since the longest may be of
     // any share.
     //
     // Where there are more segments than workgroups, waves take them by themselves: opening
-    // one is most of what a short one takes (700 ragged sequences of 250 slots: 43.7 us, 56.8
-    // with four waves to each; 8 of 500 slots, with fewer: 13.8, and 12.5 with four). They
-    // take them as a whole, where the longest cannot take much longer than all together (600
-    // of 1,200 slots: 319 us, 356 split).
+    // one is most of what a short one takes (700 ragged sequences of 250 slots: 49.3 us, 65.9
+    // with four waves to each; 8 of 500 slots, with fewer: 27.4, and 11.4 with four). Those of
+    // more than FEW steps only where every wave has one (700 ragged ones of 500 slots: 78.9,
+    // 85.2 with four; 200: 40.3, and 32.4 with four).
     constexpr int64_t CUS = 256, FEW = 8;
     const int64_t whole = a.batch > 1 ? 24 : 12;
     const int64_t steps = ((int64_t)a.pages_each * a.c.page + TILE - 1) / TILE;
@@ -528,15 +535,15 @@ Split split_of(const AttentionArgs& a, void* workspace) {
     const int64_t full = CUS * resident(a.c.blocks, columns_of(a), a.type == QS_SRC_F32);
     Split s{};
     if (a.batch == 0 || a.fresh == 0) return s;
-    s.waves = segments > (steps <= FEW ? 1 : 2) * full && a.batch > 1 ? 1 : 4;
+    s.waves = segments > (steps <= FEW ? 1 : 4) * full && a.batch > 1 ? 1 : 4;
     // Where loads are all that bounds it, eight-bit codes of heads of 128 or 256 for eight
     // 16-bit queries, one workgroup less on each CU streams better: 8 sequences of 32,767
-    // slots 114.2 and 116.7 us, of heads of 256 and 16,000 slots 115 and 121; four-bit ones
-    // of 128 take 45.6, 44.2 with all, heads of 64 with 8 bits 35.6 and 35.1.
+    // slots 116.2 and 118.1 us, of heads of 256 and 16,000 slots 121 and 129; four-bit ones
+    // of 128 take 48.0, 45.3 with all, heads of 64 with 8 bits 38.0 and 39.0.
     const bool lean = s.waves == 4 && a.c.k_bits + a.c.v_bits == 16 && a.c.blocks % 4 == 0 && columns_of(a) == 8 &&
                       a.type != QS_SRC_F32;
     const int64_t held = s.waves == 4 ? full - lean * CUS : 4 * full;
-    if (steps <= whole || (s.waves == 1 && steps <= whole * (1 + segments / held))) {
+    if (steps <= whole + (a.batch > 1 ? whole * segments / held : 0)) {
         s.share = 1;
     } else if (a.batch == 1) {
         const int64_t share = held / segments, most = (steps + s.waves - 1) / s.waves;

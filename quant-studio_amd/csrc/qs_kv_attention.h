@@ -29,7 +29,7 @@ struct AttentionArgs {
 // Queries of a workgroup, of a key/value head's group * fresh: eight, for each of which a
 // matrix product has two of its 16 columns, or twice as many, which read and unpack the
 // head once and not twice, where there are so many and a wave's registers hold them (8
-// sequences of 8,000 slots, 12 queries of each head: 42.8 us, 50.7 in eights).
+// sequences of 8,000 slots, 12 queries of each head: 49.7 us, 56.3 in eights).
 inline __host__ __device__ int columns_of(const AttentionArgs& a) {
     return a.group * a.fresh > 8 && a.c.blocks <= 4 && a.type != QS_SRC_F32 ? 16 : 8;
 }
@@ -52,11 +52,14 @@ QS_DEV float inverse_of(float top, float total) {
 // How a call's work is split, and where its workgroups leave what is joined.
 constexpr int TILE = 32;            // slots of a wave's step
 // Steps of its waves that a workgroup takes as long to begin with another segment: 61 ragged
-// sequences of up to 2,047 slots take 69 us with 0, 29.5 with 2, 33 with 8.
+// sequences of up to 2,047 slots take 77 us with 0, 32.3 with 2, 35.6 with 8.
 constexpr int OPENING = 2;
 // Workgroups of four waves that a CU holds, by the registers of a wave. More workgroups than
-// these would wait for others to end (8 sequences of 16,000 slots 63.7 us, one more 65.9; of
-// 64-value heads 34.8 and 40.0).
+// these would wait for others to end (8 sequences of 16,000 slots 61.9 us, one more 64.0; of
+// 64-value heads 38.9 and 43.8), and fewer registers for more of them would not do: heads of
+// 64 65 us, 79 with one more and 66 with one less, sixteen queries of them 55, 102 and 55; of
+// 128 63, 89 and 63, sixteen 52, 139 and 59, f32 68, 71 and 71; of 192 42, 64 and 45, f32
+// 44.5 and 45.4 with one more. f32 ones of 256 need some 350 registers.
 __host__ __device__ constexpr int resident(int blocks, int columns, bool wide) {
     return blocks == 2 ? (columns == 16 ? 3 : 4) : blocks == 4 ? (wide || columns == 16 ? 2 : 3) : wide ? 1 : 2;
 }

@@ -13,9 +13,9 @@ QS_DEV float power(float part, float top, float total) {    // total: of a part 
 // Grid (segments, columns). D / 4 threads take a part's row, the others the next parts,
 // four of them at a time, and LDS joins what they have in a fixed order. Latency is
 // all there is to it, 3.7 to 5.5 us of a call. Of more than 128 parts of a segment 1,024
-// threads have nearly all on their way at once: one sequence of 100,000 slots takes 22.6 us
-// with one head (384 parts or more; 30.2 with 256 threads) and 29.8 with four (192; 30.4),
-// but 14.7 and 13.6 of 8,000 slots with eight heads (63), 24.9 and 24.5 of 40,000 (96).
+// threads have nearly all on their way at once: one sequence of 100,000 slots takes 21.4 us
+// with one head (384 parts or more; 25.8 with 256 threads) and 31.4 with four (192; 31.3),
+// but 16.0 and 14.8 of 8,000 slots with eight heads (63), 26.1 and 25.3 of 40,000 (96).
 template <int BLOCKS, int THREADS>
 __global__ __launch_bounds__(THREADS) void k_kv_join(AttentionArgs a, Split split) {
     constexpr int D = 32 * BLOCKS, LANES = D / 4, ROWS = THREADS / LANES, TIMES = 4;

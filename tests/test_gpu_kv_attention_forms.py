@@ -27,16 +27,16 @@ def workspace(qs, cache, b, n, heads, m):
 @pytest.mark.parametrize("v_type", TYPES)
 @pytest.mark.parametrize("d", [64, 128, 192, 256])
 def test_a_wave_to_a_segment(qs, dtype, k_type, v_type, d):
-    """2,400 heads of sequences are more than twice the workgroups that any form has at a time: a wave takes one
-    after another, whole ones where tables are narrow, runs of all steps where they are wide. One query of a head and
-    more than 8, more than 16 in columns of 8 or 16, several new tokens, and a window."""
-    batch, heads, page = 100, 24, 32
+    """4,800 heads of sequences are more than all waves that any form has at a time: a wave takes one after another,
+    whole ones where tables are narrow, runs of all steps where they are wide. One query of a head and more than 8,
+    more than 16 in columns of 8 or 16, several new tokens, and a window."""
+    batch, heads, page = 100, 48, 32
     g = torch.Generator().manual_seed(d)
     lengths = torch.randint(0, 40, (batch,), generator=g).tolist()
     lengths[3], lengths[50], lengths[-1] = 200, 97, 0
     cache = qs.KVCache(sum(-(-n // page) for n in lengths) + 1, page, heads, d, k_type, v_type)
     tables, rows = ref.fill(qs, cache, lengths, dtype, d, poison=True)
-    wide = torch.full((batch, 200), -1, dtype=torch.int32, device=DEV)
+    wide = torch.full((batch, 400), -1, dtype=torch.int32, device=DEV)
     wide[:, :tables.shape[1]] = tables
     for group, n, window in ((1, 1, 0), (2, 5, 7), (17, 1, 30)):
         q = torch.randn((batch, n, heads * group, d), generator=g).to(DEV, dtype)
