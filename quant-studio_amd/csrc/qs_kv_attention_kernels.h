@@ -239,7 +239,9 @@ QS_DEV void prepare_queries(const AttentionArgs& a, int first, int length, const
 // slots 5.4 to 5.8 us, 61 ragged ones 30.2 to 32.2, 16 of 8,191 with four bits 46.3 to 47.6),
 // and seldom again: a step asks for it where the maximum rose by more than is left of the
 // slack, or a value's step could take a P to 2^LIMIT. Looking at every P of every step took
-// 16 of 8,191 slots to 52 us, choosing anew wherever the maximum rises to 55.
+// 16 of 8,191 slots to 52 us, choosing anew wherever the maximum rises to 55. Where a block has
+// a power of its own, values a thousandth of the others', those take 47.0 us for 42.1; a block
+// of zeros costs nothing.
 constexpr int LIMIT = 15, TARGET = 11, FLOOR = 3, SLACK = 6, MOST = 60;
 template <int BLOCKS>
 struct Sums {
@@ -266,8 +268,8 @@ QS_DEV i16x2 both(int v) { return i16x2{(short)v, (short)v}; }
 QS_DEV i16x2 larger(i16x2 a, i16x2 b) { return __builtin_elementwise_max(a, b); }
 QS_DEV int larger_of(i16x2 v) { return max((int)v[0], (int)v[1]); }
 QS_DEV int power_of(float up) { return (int)(__float_as_uint(up) >> 23) - 127; }
-// which blocks count by their own powers, all bits, and what blocks count by
-QS_DEV i16x2 own(i16x2 size, int power) { return (i16x2)(size < both(FLOOR + 126 - power)); }
+// which blocks count by their own powers, all bits, and what blocks count by; size 0: nothing but zeros so far
+QS_DEV i16x2 own(i16x2 size, int power) { return (i16x2)(size < both(FLOOR + 126 - power)) & (i16x2)(size > both(0)); }
 QS_DEV i16x2 powers(i16x2 size, int power) {
     const i16x2 m = own(size, power), alone = __builtin_elementwise_min(both(TARGET + 126) - size, both(power + MOST));
     return (alone & m) | (both(power) & ~m);
@@ -372,8 +374,9 @@ QS_DEV void lower(Sums<BLOCKS>& o, int fall, i16x2 (&by)[BLOCKS / 2]) {
 #pragma unroll
     for (int i = 0; i < BLOCKS / 2; i++) by[i] = both(-fall);
 }
-// The same, and chooses the powers anew where that is more than the slack or a P reaches
-// LIMIT. For other queries nothing else changes: none depends on what another one sees.
+// The same, and chooses the powers anew where that is more than the slack, a P reaches LIMIT
+// or a block has its first P. For other queries nothing else changes: none depends on what
+// another one sees.
 // first: there are no sums yet.
 template <int BLOCKS, typename F>
 QS_DEV void settle(Sums<BLOCKS>& o, uint32_t* sizes, bool first, int fall, const float (&p)[8], F&& step, i16x2 (&by)[BLOCKS / 2]) {
@@ -395,9 +398,14 @@ QS_DEV void settle(Sums<BLOCKS>& o, uint32_t* sizes, bool first, int fall, const
     }
     bool anew = true;
     if (!first) {
+        i16x2 begins = both(0);
 #pragma unroll
-        for (int i = 0; i < BLOCKS / 2; i++) most = larger(most, now[i] + powers(size_at(sizes, i), was));
-        anew = fall > o.slack || larger_of(most) > LIMIT + 126;
+        for (int i = 0; i < BLOCKS / 2; i++) {
+            const i16x2 then = size_at(sizes, i);
+            most = larger(most, now[i] + powers(then, was));
+            begins |= (i16x2)(then == both(0)) & now[i];
+        }
+        anew = fall > o.slack || larger_of(most) > LIMIT + 126 || __builtin_bit_cast(uint32_t, begins) != 0;
         most = both(0);
 #pragma unroll
         for (int i = 0; i < BLOCKS / 2; i++) {
@@ -419,28 +427,40 @@ QS_DEV void settle(Sums<BLOCKS>& o, uint32_t* sizes, bool first, int fall, const
     o.up = __builtin_ldexpf(1.0f, power);
     o.slack = anew ? SLACK : o.slack - fall;
 }
-// The f16 bits of the least step of a value that could take a P of the wave to LIMIT, 0
-// where a block of a query counts by a power of its own: then each step settles.
+// What a wave goes on by: whether a block of a query counts by a power of its own, and the f16
+// bits of the least steps of values, block by block, that could take a P to LIMIT or begin a
+// block of zeros, less one.
+template <int BLOCKS>
+struct Pace {
+    bool uneven;
+    uint32_t under[BLOCKS / 2];
+};
 template <int BLOCKS, int SETS>
-QS_DEV uint32_t steep_of(const Sums<BLOCKS> (&sums)[SETS], const uint32_t* sizes) {
-    float up = 0.0f;
+QS_DEV Pace<BLOCKS> pace_of(const Sums<BLOCKS> (&sums)[SETS], const uint32_t* sizes) {
+    Pace<BLOCKS> o;
     bool uneven = false;
 #pragma unroll
-    for (int n = 0; n < SETS; n++) {
-        i16x2 any = both(0);
+    for (int i = 0; i < BLOCKS / 2; i++) {
+        i16x2 up = both(-32768);
 #pragma unroll
-        for (int i = 0; i < BLOCKS / 2; i++) any |= own(size_at(sizes, n * (BLOCKS / 2) + i), power_of(sums[n].up));
-        const bool seen = sums[n].top > -__builtin_inff();
-        up = fmaxf(up, seen ? sums[n].up : 0.0f);
-        uneven |= seen & (__builtin_bit_cast(uint32_t, any) != 0);
+        for (int n = 0; n < SETS; n++) {
+            const int power = power_of(sums[n].up);
+            const bool seen = sums[n].top > -__builtin_inff();
+            const i16x2 size = size_at(sizes, n * (BLOCKS / 2) + i), zero = (i16x2)(size == both(0));
+            uneven |= seen & (__builtin_bit_cast(uint32_t, own(size, power)) != 0);
+            up = seen ? larger(up, (powers(size, power) & ~zero) | (both(1000) & zero)) : up;
+        }
+        // over the eight queries: lanes ^ 1, ^ 2 and, four being alike, ^ 7
+        const auto with = [&](uint32_t other) { up = larger(up, __builtin_bit_cast(i16x2, other)); };
+        with(qs::quad_xor<1>(__builtin_bit_cast(uint32_t, up)));
+        with(qs::quad_xor<2>(__builtin_bit_cast(uint32_t, up)));
+        with((uint32_t)__builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, up), 0x141, 0xF, 0xF, true));
+        const half2_t least{(_Float16)__builtin_ldexpf(1.0f, LIMIT - up[0]), (_Float16)__builtin_ldexpf(1.0f, LIMIT - up[1])};
+        const u16x2 under = __builtin_elementwise_sub_sat(__builtin_bit_cast(u16x2, least), u16x2{1, 1});
+        o.under[i] = (uint32_t)__builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, under));
     }
-    // over the eight queries: lanes ^ 1, ^ 2 and, four being alike, ^ 7
-    uint32_t u = __float_as_uint(up);
-    u = max(u, qs::quad_xor<1>(u));
-    u = max(u, qs::quad_xor<2>(u));
-    u = max(u, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)u, 0x141, 0xF, 0xF, true));
-    const float least = __uint_as_float(((uint32_t)(254 + LIMIT) << 23) - u);       // 2^LIMIT / up
-    return __any(uneven) ? 0 : __builtin_amdgcn_readfirstlane(__builtin_bit_cast(uint16_t, (_Float16)least));
+    o.uneven = __any(uneven);
+    return o;
 }
 
 // One step: the slots start .. start + 31, in `t`. The next step's keys and values
@@ -452,8 +472,13 @@ QS_DEV uint32_t steep_of(const Sums<BLOCKS> (&sums)[SETS], const uint32_t* sizes
 template <bool WIDE, int K_BITS, int V_BITS, int BLOCKS, int SETS>
 QS_DEV void attend(const AttentionArgs& a, int start, bool first, bool edge, int held, const Place& next,
                    const Queries<BLOCKS, WIDE> (&q)[SETS], uint32_t* lds, Tile<K_BITS, V_BITS, BLOCKS>& t,
-                   Sums<BLOCKS> (&sums)[SETS], uint32_t* sizes, uint32_t& least) {
-    const int lane = threadIdx.x & 63, g = lane >> 4;
+                   Sums<BLOCKS> (&sums)[SETS], uint32_t* wave_sizes, Pace<BLOCKS>& pace) {
+    // Where registers are scarce, what comes of the lane's number is worked out anew in each step
+    // (16 sequences of 2,048 slots, heads of 256: 43.0 us without, 40.1).
+    int lane = threadIdx.x & 63;
+    if constexpr (!WIDE && BLOCKS * SETS == 8) asm volatile("" : "+v"(lane));
+    const int g = lane >> 4;
+    uint32_t* const sizes = wave_sizes + lane;
     // steps of four slots, and one of them
     struct Steps4 {
         u32x4 w[BLOCKS / 2];
@@ -469,15 +494,17 @@ QS_DEV void attend(const AttentionArgs& a, int start, bool first, bool edge, int
     };
     const auto step_of = [&](const Steps4& c, int r, int b) { return half_of(two_of(c, r, b) >> (16 * (b & 1))); };
     // lane after lane they are the two sixteens' steps as they lie in their pages, four keys', then four values'
-    u16x2 large{0, 0};
+    uint32_t over = 0;
 #pragma unroll
     for (int i = 0; i < BLOCKS / 2; i++) {
-        lds[lane * (BLOCKS / 2) + i] = t.steps.w[i];
-        large = __builtin_elementwise_max(large, __builtin_bit_cast(u16x2, t.steps.w[i] & 0x7fff7fffu));
+        const uint32_t two = t.steps.w[i];
+        lds[lane * (BLOCKS / 2) + i] = two;
+        over |= __builtin_bit_cast(uint32_t, __builtin_elementwise_sub_sat(__builtin_bit_cast(u16x2, two & 0x7fff7fffu),
+                                                                           __builtin_bit_cast(u16x2, pace.under[i])));
     }
-    uint32_t largest = lane & 4 ? max((uint32_t)large[0], (uint32_t)large[1]) : 0;
-    asm volatile("" : "+v"(largest));   // from here on, in place of what it comes from
-    bool steep = largest >= least;
+    over = lane & 4 ? over : 0;
+    asm volatile("" : "+v"(over));      // from here on, in place of what it comes from
+    bool steep = over != 0;
     qs::wave_sync<true>();
     // scores, in powers of two
     float x[SETS][2][4];
@@ -568,7 +595,7 @@ QS_DEV void attend(const AttentionArgs& a, int start, bool first, bool edge, int
                     asm volatile("" : "+v"(two));
                     return half_of(two >> (16 * (b & 1)));
                 }, by[n]);
-            least = steep_of(sums, sizes);
+            pace = pace_of(sums, sizes);
         } else {
 #pragma unroll
             for (int n = 0; n < SETS; n++) lower(sums[n], fall[n], by[n]);
@@ -595,7 +622,7 @@ QS_DEV void attend(const AttentionArgs& a, int start, bool first, bool edge, int
 #pragma unroll
                 for (int i = 0; i < 8; i++) sums[n].acc[b][i >> 2][i & 3] *= f;
             }
-            if (__builtin_expect(least == 0, 0)) {      // p goes on to this block's power
+            if (__builtin_expect(pace.uneven, 0)) {     // p goes on to this block's power
                 const int power = power_of(sums[n].up);
                 const auto at = [&](int b) { return b < 0 ? power : powers(size_at(sizes, (n * BLOCKS + b) >> 1), power)[b & 1]; };
                 const float f = __builtin_ldexpf(1.0f, at(b) - at(b - 1));
@@ -713,7 +740,6 @@ void k_kv_attention(AttentionArgs a, Split split) {
     __shared__ __attribute__((aligned(16))) uint32_t steps_lds[WAVES][TILE * BLOCKS];
     __shared__ uint32_t sizes[WAVES][SETS * BLOCKS / 2][64];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const auto sizes_of = [&](int n) { return &sizes[wave][n * (BLOCKS / 2)][threadIdx.x & 63]; };
     const int tiles = (a.group * a.fresh + COLUMNS - 1) / COLUMNS, heads = a.c.heads * tiles;
     int64_t at = 0, end = 1, each = 0;
     int seq, base = 0, which = -1, from = 0;        // which: head and column tile
@@ -756,7 +782,7 @@ void k_kv_attention(AttentionArgs a, Split split) {
 #pragma unroll
         for (int n = 0; n < SETS; n++) {
             load_queries(a, seq, head, first + 8 * n, raw[n]);
-            clear(sums[n], sizes_of(n));
+            clear(sums[n], &sizes[wave][n * (BLOCKS / 2)][threadIdx.x & 63]);
         }
         const Ints table = constant(a.tables + seq * a.table_stride);
         // The wave's steps i, i + stride, ... before `stop`, counted from the sequence's
@@ -793,7 +819,7 @@ void k_kv_attention(AttentionArgs a, Split split) {
             const int final = i + (stop - 1 - i) / stride * stride;
             const auto start_of = [&](int n) { return (n < final ? n : final) * TILE; };
             Queries<BLOCKS, WIDE> q[SETS];
-            uint32_t least = 0;
+            Pace<BLOCKS> pace{};
 #pragma unroll
             for (int n = 0; n < SETS; n++) prepare_queries(a, first + 8 * n, length, raw[n], q[n]);
             for (bool opens = true; i < stop; i += stride, opens = false) {
@@ -801,7 +827,7 @@ void k_kv_attention(AttentionArgs a, Split split) {
                 place = place_of(a, ahead, head, start_of(i + stride));
                 ahead = pages_of(a, table, start_of(i + 2 * stride));
                 const bool edge = start < span.all_first || start + TILE > span.all_last || held != 3;
-                attend(a, start, opens, edge, held, place, q, steps_lds[wave], t, sums, sizes_of(0), least);
+                attend(a, start, opens, edge, held, place, q, steps_lds[wave], t, sums, sizes[wave][0], pace);
             }
         }
         // anew from here, so that no step holds registers for the addresses of what follows
