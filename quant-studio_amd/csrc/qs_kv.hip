@@ -517,7 +517,11 @@ Split split_of(const AttentionArgs& a, void* workspace) {
     // 290 slots takes 9.0, 9.1 split, of 420 slots 10.7 and 9.4. Longer ones are whole where
     // there are so many that the longest cannot take much longer than all together: 40 of 900
     // slots 25.5, 29.4 split (ragged ones 18.4, 21.6 split), 150 of 1,500 slots 97 and 111
-    // (ragged 49 and 54), 600 of 1,200 slots 304 and 347; 65 ragged ones of 1,300 30.8 and 29.4.
+    // (ragged 49 and 54), 600 of 1,200 slots 304 and 347; 65 ragged ones of 1,300 30.8 and
+    // 29.4. Up to twice `whole` for workgroups of four waves, since lengths may be far below
+    // the tables' width but for a few: 190 of 3,000 slots are 257 us split, 244 whole, but
+    // ragged ones 99 and 107, and one such with 189 of 17 slots 32 and 40 (39 of 17 slots and
+    // one of 900: 12.5, 16.2 whole).
     //
     // A lone sequence is in equal parts, which each workgroup knows before it knows the
     // length; more of them are in equal runs of all their steps, since the longest may be of
@@ -527,7 +531,10 @@ Split split_of(const AttentionArgs& a, void* workspace) {
     // one is most of what a short one takes (700 ragged sequences of 250 slots: 49.3 us, 65.9
     // with four waves to each; 8 of 500 slots, with fewer: 27.4, and 11.4 with four). Those of
     // more than FEW steps only where every wave has one (700 ragged ones of 500 slots: 78.9,
-    // 85.2 with four; 200: 40.3, and 32.4 with four).
+    // 85.2 with four; 200: 40.3, and 32.4 with four); in tables wider than `whole`, where most
+    // may be short all the same, with half as many, in runs (300 of 17 slots in tables for
+    // 3,000: 20 us, with four waves 32 in runs and 25 whole, and where one has 3,000 23, 39 and
+    // 46; ragged ones up to tables of 1,200: 77, 81 and 70).
     constexpr int64_t CUS = 256, FEW = 8;
     const int64_t whole = a.batch > 1 ? 24 : 12;
     const int64_t steps = ((int64_t)a.pages_each * a.c.page + TILE - 1) / TILE;
@@ -535,7 +542,7 @@ Split split_of(const AttentionArgs& a, void* workspace) {
     const int64_t full = CUS * resident(a.c.blocks, columns_of(a), a.type == QS_SRC_F32);
     Split s{};
     if (a.batch == 0 || a.fresh == 0) return s;
-    s.waves = segments > (steps <= FEW ? 1 : 4) * full && a.batch > 1 ? 1 : 4;
+    s.waves = segments > (steps <= FEW ? 1 : steps <= whole ? 4 : 2) * full && a.batch > 1 ? 1 : 4;
     // Where loads are all that bounds it, eight-bit codes of heads of 128 or 256 for eight
     // 16-bit queries, one workgroup less on each CU streams better: 8 sequences of 32,767
     // slots 116.2 and 118.1 us, of heads of 256 and 16,000 slots 121 and 129; four-bit ones
@@ -543,7 +550,8 @@ Split split_of(const AttentionArgs& a, void* workspace) {
     const bool lean = s.waves == 4 && a.c.k_bits + a.c.v_bits == 16 && a.c.blocks % 4 == 0 && columns_of(a) == 8 &&
                       a.type != QS_SRC_F32;
     const int64_t held = s.waves == 4 ? full - lean * CUS : 4 * full;
-    if (steps <= whole + (a.batch > 1 ? whole * segments / held : 0)) {
+    const int64_t more = whole * segments / held;
+    if (steps <= whole + (a.batch == 1 ? 0 : s.waves == 4 ? (more < whole ? more : whole) : segments < held ? 0 : more)) {
         s.share = 1;
     } else if (a.batch == 1) {
         const int64_t share = held / segments, most = (steps + s.waves - 1) / s.waves;
