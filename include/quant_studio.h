@@ -300,9 +300,9 @@ int64_t qs_kv_attention_workspace(const qs_kv_cache *cache, int64_t batch, int64
  * own infinities, or sums out of f32's range) NaN; what lies at positions that it does
  * not see does not matter, whatever it is. Sums and statistics are f32; q is held to
  * 22 bits or more beside its row's largest value, p times a step of V to 21
- * beside the largest of its block of 32 values of the head. The result does not depend on timing; in the last bits of f32 it
- * may depend on the call's other sequences and on pages_each (another split of the
- * sum). batch is at most 2^14, new_tokens 16, query_heads / heads a whole number up
+ * beside the largest of its block of 32 values of the head. The result does not
+ * depend on timing; in the last bits of f32 it may depend on the call's other
+ * sequences and on pages_each (another split of the sum). batch is at most 2^14, new_tokens 16, query_heads / heads a whole number up
  * to 128, pages_each * page_size 2^30, batch times that 2^34, and batch * heads times
  * the eights of a head's queries 2^25. */
 int qs_kv_attention(const qs_kv_cache *cache, int type, const void *q, int64_t q_token_stride_bytes, int64_t batch,

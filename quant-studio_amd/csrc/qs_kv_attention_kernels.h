@@ -21,12 +21,13 @@
 // down to 2^-35 of the row's largest; an f32 q takes two products, 22 bits.
 //
 // What bounds it (heads of 128, bf16 queries, four to a head): eight-bit codes their bytes,
-// 8 sequences of 32,767 slots 570 MB in 114 us with the join, 5.0 TB/s, of which loads
-// alone take 111 (a large copy reaches 5.2 TB/s; matrix units 0.08 of the cycles, vector
-// units 0.5); four-bit ones, at half the bytes for as many codes, loads and the vector
-// instructions that unpack them and make P, which overlap in part: 16 of 8,191 slots 151 MB
-// in 46 us, 3.3 TB/s, loads alone 38. Small calls wait for memory one read after another:
-// lengths, pages, codes, then the join, 11 to 12 us of split calls, 5 of one of 17 slots.
+// 8 sequences of 32,767 slots 570 MB in 116 us with the join, 4.9 TB/s, of which loads
+// alone take 111 (a large copy reaches 5.2 TB/s; matrix units 0.07 of the cycles, vector
+// units 0.54); four-bit ones, at half the bytes for as many codes, loads and the vector
+// instructions that unpack them and make P (0.7), which overlap in part: 16 of 8,191 slots
+// 151 MB in 48 us, 3.1 TB/s, loads alone 38. Small calls wait for memory one read after
+// another: lengths, pages, codes, then the join, 12 to 13 us of split calls, 6 of one of 17
+// slots.
 #pragma once
 
 #include "qs_kv_attention.h"
@@ -230,7 +231,7 @@ QS_DEV void prepare_queries(const AttentionArgs& a, int first, int length, const
 // the query so far: 2^(TARGET - 1) or more as it counts when the power is chosen, by up to
 // 2^SLACK less while the running maximum rises, and never 2^LIMIT. A block whose own largest
 // is then below 2^(FLOOR - 1), where the second of two f16 would come to lose bits of it,
-// counts by a power of its own. (One power for the largest step seen, whatever its p and its
+// counts by a power of its own, 2^MOST times the others' at most. (One power for the largest step seen, whatever its p and its
 // block, left blocks of small values and those beside large ones of no weight 6 to 17 bits:
 // errors up to 1e-2.) The running maximum is a whole number, so that what it takes off is a
 // power of two as well.

